@@ -274,6 +274,97 @@ int delrec_readout_sum_backward(int T, int B, int N, int C, const float* ysum, c
  * (x_binary above); no counterpart in the reference, whose projections are fp32 GEMMs. */
 int delrec_count_nonbinary(const float* x, size_t n, unsigned int* count, void* stream);
 
+/* ---- sequence operators ------------------------------------------------------------ */
+/* Gated linear recurrence, norms around a block, 8-bit activation checkpoints: no
+ * counterpart in the reference.  Tensors are fp32, bf16 or fp16 (dtype), time-major
+ * (T,B,N) with element strides for T and B and contiguous channels; states, weights,
+ * statistics and their gradients are fp32.  lengths (B), int32 or int64
+ * (lengths_wide != 0), NULL for full rows: positions t >= lengths[b] are not read, their
+ * outputs and gradients are written as 0.  Outputs do not overlap inputs unless stated. */
+#define DELREC_F32 0
+#define DELREC_BF16 1
+#define DELREC_F16 2
+#define DELREC_GATE_NONE 0
+#define DELREC_GATE_SIGMOID 1
+#define DELREC_GATE_SILU 2
+
+typedef struct delrec_scan {
+  int32_t T, B, N;
+  int32_t G;             /* gates per position; N = G * D, gate g serves channels gD .. gD+D-1 */
+  int32_t dtype;
+  int32_t decay_input;   /* 1: z enters as (1 - a) z, 0: as z */
+  int32_t lengths_wide;
+  int32_t reserved;
+  int64_t z_t, z_b, f_t, f_b;       /* strides of z (T,B,N) and f (T,B,G) */
+  int64_t h_t, h_b;                 /* of h */
+  int64_t gh_t, gh_b;               /* of the gradient of h */
+  int64_t dz_t, dz_b, df_t, df_b;   /* of dz and df */
+} delrec_scan;
+
+/* h_t = sigmoid(f_t) h_{t-1} + c_t z_t from h0 (B,N) (NULL: 0); resets (T,B) bytes or NULL:
+ * nonzero drops h_{t-1} at that step.  Writes h, hT (B,N) (the state after the last
+ * position; NULL to skip) and, for the backward, states (ceil(T/16), B, N): the state before
+ * every 16th step (NULL to skip).  qz, ez, qf, ef (all or none, G = N): also writes z and f
+ * in 8 bits (delrec_pack8's form). */
+int delrec_gated_scan_forward(const delrec_scan* scan, const void* z, const void* f, const float* h0,
+                              const void* lengths, const uint8_t* resets, void* h, float* hT, float* states,
+                              int8_t* qz, uint8_t* ez, int8_t* qf, uint8_t* ef, void* stream);
+/* Gradients from gh (NULL: 0) and ghT (NULL: 0): dz, df, dh0, any NULL to skip.  With qz
+ * and ez, z is their restored value; with qf and ef, f is (z or f may then be NULL).
+ * h_{t-1} is recomputed from states. */
+size_t delrec_gated_scan_backward_workspace(const delrec_scan* scan);
+int delrec_gated_scan_backward(const delrec_scan* scan, const void* z, const void* f, const int8_t* qz,
+                               const uint8_t* ez, const int8_t* qf, const uint8_t* ef, const void* lengths,
+                               const uint8_t* resets, const float* states, const void* gh, const float* ghT,
+                               void* dz, void* df, float* dh0, void* workspace, size_t workspace_bytes,
+                               void* stream);
+/* One step (T is 1): h (B,N) and next (B,N) from z, f and state (B,N) (NULL: 0); next may be
+ * state itself.  active (B) bytes or NULL: a row with 0 keeps its state and writes h = 0. */
+int delrec_gated_step(const delrec_scan* scan, const void* z, const void* f, const float* state,
+                      const uint8_t* active, void* h, float* next, void* stream);
+
+typedef struct delrec_block {
+  int32_t T, B, N;
+  int32_t dtype;
+  int32_t gate;          /* DELREC_GATE_* */
+  int32_t lengths_wide;
+  float eps;             /* > 0 */
+  int32_t reserved;
+  int64_t x_t, x_b, y_t, y_b, u_t, u_b;         /* strides of x, y, u */
+  int64_t o_t, o_b, n_t, n_b;                   /* of the outputs x' and n */
+  int64_t gx_t, gx_b, gn_t, gn_b;               /* of their gradients */
+  int64_t dx_t, dx_b, dy_t, dy_b, du_t, du_b;   /* of dx, dy, du */
+} delrec_block;
+
+/* out = x + scale * act(u) * (y / rms(y) * w) and n = out / rms(out) * next_w, rms(v) =
+ * sqrt(mean v^2 + eps) over the channels.  y NULL: n is x's norm, out is not written.  n
+ * NULL: no next norm.  w, scale, next_w (N), NULL: ones.  ry, rx (T,B), NULL to skip: the
+ * 1/rms of y and of out, kept for the backward.  N <= 16384. */
+int delrec_block_norm_forward(const delrec_block* block, const void* x, const void* y, const void* u,
+                              const float* w, const float* scale, const float* next_w, const void* lengths,
+                              void* out, void* n, float* ry, float* rx, void* stream);
+/* Gradients from gx (of out) and gn (of n), either NULL: 0.  Outputs NULL to skip. */
+size_t delrec_block_norm_backward_workspace(const delrec_block* block);
+int delrec_block_norm_backward(const delrec_block* block, const void* x, const void* y, const void* u,
+                               const float* w, const float* scale, const float* next_w, const void* lengths,
+                               const float* ry, const float* rx, const void* gx, const void* gn, void* dx,
+                               void* dy, void* du, float* dw, float* dscale, float* dnext_w, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* 8-bit form of x (rows, N), contiguous: q (rows, N) and e (rows, ceil(N/32)).  Channels
+ * go in groups of 32; x is q * 2^(e-127), the scale the smallest power of two >= 2^-126
+ * with max |x| <= 126 * scale over the group's finite values, q = x / scale rounded to
+ * nearest even (at the scale 2^122 at most 63 in magnitude); q = 127 is +inf, -127 -inf,
+ * -128 NaN.  Restored to fp16 it saturates at fp16's largest value. */
+int delrec_pack8(long long rows, int N, int dtype, const void* x, int8_t* q, uint8_t* e, void* stream);
+int delrec_unpack8(long long rows, int N, int dtype, const int8_t* q, const uint8_t* e, void* x, void* stream);
+/* delrec_linear_backward with x (M,K) in 8 bits: its values have 7 significant bits, so one
+ * bf16 piece carries each exactly and dW takes three piece products.  Same workspace as
+ * delrec_linear_backward with x_binary = 1. */
+int delrec_linear_backward8(int M, int K, int N, const int8_t* q, const uint8_t* e, const float* W,
+                            const float* gout, float* dx, float* dW, float* dbias, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ---- device status word ------------------------------------------------------------ */
 /* Kernels record internal inconsistencies (an out-of-range lag or index that was
  * skipped) in a device status word instead of trapping.  Reading it synchronizes. */

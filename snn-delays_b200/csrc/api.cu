@@ -45,7 +45,7 @@ static inline int pow2_at_least(int x) {
       return DELREC_ERR_CUDA;                                              \
     }                                                                      \
   } while (0)
-static unsigned long long g_launches = 0;  // kernels issued by this library (host counter)
+unsigned long long g_launches = 0;  // kernels issued by this library (host counter; sequence.cu adds its own)
 
 // Optional timing of the reverse-scan kernels: CUDA events recorded on the launching
 // stream around each scan launch while enabled (delrec_scan_timing).
@@ -913,9 +913,12 @@ static int run_linear_forward(int M, int K, int N, const float* x, const float* 
   return gemm_run(A, Bw, g, 1, gemm_pick_bn(N), part, st, &g_launches);
 }
 
+// x as fp32 (M,K), or in 8 bits (q8, e8; xb = 1: one exact piece per value)
 static int run_linear_backward(int M, int K, int N, const float* x, const float* W, const float* gout, int xb,
-                               float* dx, float* dW, float* dbias, void* ws, size_t wsb, cudaStream_t st) {
-  if (M <= 0 || K <= 0 || N <= 0 || !gout || (dx && !W) || ((dW || dbias) && !x)) return DELREC_ERR_ARG;
+                               float* dx, float* dW, float* dbias, void* ws, size_t wsb, cudaStream_t st,
+                               const int8_t* q8 = nullptr, const uint8_t* e8 = nullptr) {
+  if (M <= 0 || K <= 0 || N <= 0 || !gout || (dx && !W) || ((dW || dbias) && !x && !(q8 && e8)))
+    return DELREC_ERR_ARG;
   if (((uintptr_t)ws & 255) != 0 || wsb < linear_bwd_ws(M, K, N, xb)) return DELREC_ERR_WORKSPACE;
   const LinPlan p = plan_linear(K, N, xb);
   Carve c(ws, wsb);
@@ -953,8 +956,11 @@ static int run_linear_backward(int M, int K, int N, const float* x, const float*
     if (rc) return rc;
   }
   if (dW || dbias) {
-    k_pack_rows<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, x, K, nullptr, 1, p.nbx,
-                                                                     kPatDistinct3, xb, X);
+    if (q8)
+      k_pack_rows8<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, q8, e8, X);
+    else
+      k_pack_rows<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, x, K, nullptr, 1, p.nbx,
+                                                                       kPatDistinct3, xb, X);
     DR_LAUNCHED();
     // D[c][k'] (+)= sum_m G'[m][c] X_a[m][k'] over the M rows, c < (3-a) Np
     for (int a = 0; a < p.nbx; ++a) {
@@ -1793,6 +1799,13 @@ int delrec_linear_backward(int M, int K, int N, const float* x, const float* W, 
                            float* dx, float* dW, float* dbias, void* ws, size_t wsb, void* stream) {
   return run_linear_backward(M, K, N, x, W, gout, x_binary ? 1 : 0, dx, dW, dbias, ws, wsb,
                              (cudaStream_t)stream);
+}
+
+int delrec_linear_backward8(int M, int K, int N, const int8_t* q, const uint8_t* e, const float* W,
+                            const float* gout, float* dx, float* dW, float* dbias, void* ws, size_t wsb,
+                            void* stream) {
+  if ((dW || dbias) && !(q && e)) return DELREC_ERR_ARG;
+  return run_linear_backward(M, K, N, nullptr, W, gout, 1, dx, dW, dbias, ws, wsb, (cudaStream_t)stream, q, e);
 }
 
 int delrec_hybrid_delay_grad(int N, int LM, const float* C, const float* W, const float* d, float sigma,

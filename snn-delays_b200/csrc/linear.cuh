@@ -25,6 +25,7 @@
 
 #include <cuda_bf16.h>
 
+#include "checkpoint8.cuh"
 #include "common.cuh"
 
 namespace delrec {
@@ -249,6 +250,27 @@ __global__ void k_linear_dw_reduce(int N, int K, int Np, int Kp, const float* __
     } else if (dbias) {
       dbias[n] = v;
     }
+  }
+}
+
+// The projections' bf16 operand rows from x (R, K) in 8 bits: out[r][c] = x (c < K), 1 (c ==
+// K: the bias column), 0 (K < c < Wd).  Exact: 7 significant bits.  Wd is a multiple of 8; a
+// thread writes 8 columns, all of one group.
+__global__ void k_pack_rows8(int R, int K, int Wd, const int8_t* __restrict__ q, const uint8_t* __restrict__ e,
+                             __nv_bfloat16* __restrict__ out) {
+  const int chunks = Wd >> 3, gpr = (K + kQGroup - 1) / kQGroup;
+  const size_t total = (size_t)R * chunks;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
+    const size_t r = i / chunks;
+    const int c0 = (int)(i - r * chunks) * 8;
+    const float s = c0 < K ? q_scale(e[r * gpr + c0 / kQGroup]) : 1.f;
+    __align__(16) __nv_bfloat16 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = c0 + j;
+      v[j] = __float2bfloat16_rn(c < K ? q_decode(q[r * K + c], s) : (c == K ? 1.f : 0.f));
+    }
+    *(uint4*)(out + r * Wd + c0) = *(const uint4*)v;
   }
 }
 

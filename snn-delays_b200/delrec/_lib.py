@@ -43,6 +43,23 @@ class Grads(ctypes.Structure):
                 ("dd", ctypes.c_void_p), ("ds", ctypes.c_void_p)]
 
 
+def _i64(*names):
+    return [(n, ctypes.c_int64) for n in names]
+
+
+class Scan(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("T", "B", "N", "G", "dtype", "decay_input", "lengths_wide",
+                                              "reserved")] \
+        + _i64("z_t", "z_b", "f_t", "f_b", "h_t", "h_b", "gh_t", "gh_b", "dz_t", "dz_b", "df_t", "df_b")
+
+
+class Block(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("T", "B", "N", "dtype", "gate", "lengths_wide")] \
+        + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)] \
+        + _i64("x_t", "x_b", "y_t", "y_b", "u_t", "u_b", "o_t", "o_b", "n_t", "n_b", "gx_t", "gx_b", "gn_t",
+               "gn_b", "dx_t", "dx_b", "dy_t", "dy_b", "du_t", "du_b")
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
@@ -91,6 +108,16 @@ _SIGS = {
     "delrec_readout_sum_backward": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
     "delrec_exchange_floor_workspace": (_S, [_P]),
     "delrec_exchange_floor": (_I, [_P, _P, _S, _P]),
+    "delrec_gated_scan_forward": (_I, [_P] * 14),
+    "delrec_gated_scan_backward_workspace": (_S, [_P]),
+    "delrec_gated_scan_backward": (_I, [_P] * 16 + [_S, _P]),
+    "delrec_gated_step": (_I, [_P] * 8),
+    "delrec_block_norm_forward": (_I, [_P] * 13),
+    "delrec_block_norm_backward_workspace": (_S, [_P]),
+    "delrec_block_norm_backward": (_I, [_P] * 19 + [_S, _P]),
+    "delrec_pack8": (_I, [ctypes.c_longlong, _I, _I, _P, _P, _P, _P]),
+    "delrec_unpack8": (_I, [ctypes.c_longlong, _I, _I, _P, _P, _P, _P]),
+    "delrec_linear_backward8": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
 }
 
 _lib = None
@@ -140,6 +167,66 @@ def require_cuda(*tensors):
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+# ---- sequence operators (gated, block_norm, checkpoint8) ---------------------------------
+
+SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def require_sequence(*tensors):
+    """The dtype code of the first tensor; raises unless all are CUDA tensors of a type the
+    sequence operators take."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError("delrec_b200 runs on CUDA tensors only (there is no CPU path)")
+        if t.dtype not in SEQ_DTYPES:
+            raise RuntimeError(f"delrec_b200 expects float32, bfloat16 or float16 tensors, got {t.dtype}")
+    return SEQ_DTYPES[tensors[0].dtype]
+
+
+def require_lengths(lengths, B, device):
+    if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64) or lengths.device != device \
+            or not lengths.is_contiguous():
+        raise RuntimeError(f"delrec_b200: lengths must be contiguous int32 or int64 ({B},) on {device}")
+
+
+def rows(t):
+    """t with contiguous channels (the last dimension); a copy where they are strided."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def empty_rows(like, dtype=None):
+    """An output shaped like ``like`` with contiguous channels: its layout where that is dense."""
+    r = torch.empty_like(like, dtype=dtype)
+    return r if r.stride(-1) == 1 or r.shape[-1] <= 1 else torch.empty(like.shape, dtype=dtype or like.dtype,
+                                                                       device=like.device)
+
+
+def addr(t):
+    return None if t is None else t.data_ptr()
+
+
+class on_device:
+    """Makes a tensor's device current where it is not, for the launches inside."""
+
+    def __init__(self, t):
+        index = t.device.index
+        self.guard = None if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def scratch(nbytes, device):
+    """Scratch of one call, from torch's caching allocator (so that captured graphs and
+    streams never share it); None for 0 bytes.  Its blocks are 512-byte aligned."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 _ws_cache: dict = {}

@@ -16,6 +16,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .checkpoint8 import pack8
 
 
 def _is_binary(x):
@@ -31,7 +32,7 @@ def _is_binary(x):
 
 class LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, binary_input):
+    def forward(ctx, x, weight, bias, binary_input, checkpoint8=False):
         _lib.require_cuda(x, weight, bias)
         K = x.shape[-1]
         N = weight.shape[0]
@@ -50,17 +51,24 @@ class LinearFn(torch.autograd.Function):
             P = _lib.ptr
             _lib.check(lib.delrec_linear_forward(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(ws),
                                                  ws.numel(), _lib.stream_ptr(dev)), "delrec_linear_forward")
-        ctx.save_for_backward(x2, w)
+        ctx.packed = bool(checkpoint8)
+        if ctx.packed:
+            # only the parameter gradients read x
+            keep = pack8(x2) if ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2]) else None
+            ctx.save_for_backward(keep and keep.q, w, keep and keep.e)
+        else:
+            ctx.save_for_backward(x2, w, None)
         ctx.binary = binary
+        ctx.rows = M
         ctx.has_bias = bias is not None
         ctx.xshape = x.shape
         return out.view(*x.shape[:-1], N)
 
     @staticmethod
     def backward(ctx, gout):
-        x2, w = ctx.saved_tensors
-        M, K = x2.shape
-        N = w.shape[0]
+        x2, w, e = ctx.saved_tensors
+        M = ctx.rows
+        N, K = w.shape
         g = gout.reshape(M, N)
         if not g.is_contiguous() or g.dtype != torch.float32:
             g = g.float().contiguous()
@@ -75,12 +83,18 @@ class LinearFn(torch.autograd.Function):
             db = db.zero_() if db is not None else None
         elif need_dx or need_dw or need_db:
             lib = _lib.lib()
-            ws = _lib.workspace(lib.delrec_linear_backward_workspace(M, K, N, int(ctx.binary)), dev)
+            one_piece = ctx.binary or ctx.packed
+            ws = _lib.workspace(lib.delrec_linear_backward_workspace(M, K, N, int(one_piece)), dev)
             P = _lib.ptr
+            if ctx.packed:
+                _lib.check(lib.delrec_linear_backward8(M, K, N, P(x2), P(e), P(w), P(g), P(dx), P(dw), P(db),
+                                                       P(ws), ws.numel(), _lib.stream_ptr(dev)),
+                           "delrec_linear_backward8")
+                return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None
             _lib.check(lib.delrec_linear_backward(M, K, N, P(x2), P(w), P(g), int(ctx.binary), P(dx), P(dw),
                                                   P(db), P(ws), ws.numel(), _lib.stream_ptr(dev)),
                        "delrec_linear_backward")
-        return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None
+        return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None
 
 
 class ReadoutTimeSum(torch.autograd.Function):
@@ -132,17 +146,26 @@ def readout_time_sum(y, weight, bias=None):
     return ReadoutTimeSum.apply(y, weight, bias)
 
 
-class Linear(torch.nn.Linear):
-    """torch.nn.Linear with the tensor-core fp32-accurate projection of this library."""
+def linear(x, weight, bias=None, *, binary_input=None, checkpoint8=False):
+    """x W^T + bias on the library's projection (see the module's description)."""
+    return LinearFn.apply(x, weight, bias, binary_input, checkpoint8)
 
-    def __init__(self, in_features, out_features, bias=True, binary_input=None, device=None, dtype=None):
+
+class Linear(torch.nn.Linear):
+    """torch.nn.Linear with the tensor-core fp32-accurate projection of this library.
+    ``checkpoint8``: keep the input in 8 bits for the weight gradient."""
+
+    def __init__(self, in_features, out_features, bias=True, binary_input=None, device=None, dtype=None,
+                 checkpoint8=False):
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
         self.binary_input = binary_input
+        self.checkpoint8 = checkpoint8
 
     def forward(self, x):
         if not x.is_cuda:
             raise RuntimeError("delrec_b200 runs on CUDA tensors only (there is no CPU path)")
-        return LinearFn.apply(x, self.weight, self.bias, self.binary_input)
+        return LinearFn.apply(x, self.weight, self.bias, self.binary_input, self.checkpoint8)
 
     def extra_repr(self):
-        return super().extra_repr() + f", binary_input={self.binary_input}"
+        r = super().extra_repr() + f", binary_input={self.binary_input}"
+        return r + ", checkpoint8=True" if self.checkpoint8 else r

@@ -85,6 +85,12 @@ def _init_ff(m, config):
             torch.nn.init.normal_(m.weight, mean=0.0, std=0.1)
 
 
+def _linear(config, inputs, outputs, **kw):
+    """A projection of the zoo; the optional ``config.checkpoint8`` keeps its input in 8 bits
+    for the backward pass (exact where that is a spike train)."""
+    return Linear(inputs, outputs, bias=config.bias, checkpoint8=bool(getattr(config, "checkpoint8", False)), **kw)
+
+
 class SNN(torch.nn.Module):
     """Feedforward LIF network: Linear -> Dropout -> LIF -> spike_registrator per layer."""
 
@@ -94,14 +100,14 @@ class SNN(torch.nn.Module):
         self.config = config
         layers, dim = [], config.input_size
         for idx, width in enumerate(config.hidden_layers):
-            layers.append(Linear(dim, width, bias=config.bias, binary_input=_spike_input(config, idx)))
+            layers.append(_linear(config, dim, width, binary_input=_spike_input(config, idx)))
             dim = width
             layers.append(Dropout(config.feedforward_dropout_rate, step_mode="m"))
             layers.append(_lif(config))
             layers.append(spike_registrator())
             if config.use_batch_norm:
                 layers.append(modified_batchnorm(width, step_mode="m"))
-        layers.append(Linear(dim, config.output_size, bias=config.bias,
+        layers.append(_linear(config, dim, config.output_size,
                              binary_input=_spike_input(config, len(config.hidden_layers))))
         self.layers = torch.nn.Sequential(*layers)
         self.init_weights()
@@ -132,7 +138,7 @@ class SNN(torch.nn.Module):
 def _recurrent_stack(config, recurrent_cls):
     layers, dim = [], config.input_size
     for idx, width in enumerate(config.hidden_layers):
-        layers.append(Linear(dim, width, bias=config.bias, binary_input=_spike_input(config, idx)))
+        layers.append(_linear(config, dim, width, binary_input=_spike_input(config, idx)))
         dim = width
         layers.append(Dropout(config.feedforward_dropout_rate, step_mode="m"))
         last = idx == len(config.hidden_layers) - 1
@@ -143,7 +149,7 @@ def _recurrent_stack(config, recurrent_cls):
         layers.append(spike_registrator())
         if config.use_batch_norm:
             layers.append(modified_batchnorm(width, step_mode="m"))
-    layers.append(Linear(dim, config.output_size, bias=config.bias,
+    layers.append(_linear(config, dim, config.output_size,
                          binary_input=_spike_input(config, len(config.hidden_layers))))
     return torch.nn.Sequential(*layers)
 
@@ -263,7 +269,7 @@ class SNN_synaptic_feedforward_delays(SNN):
         layers, dim = [], config.input_size
         for idx, width in enumerate(config.hidden_layers):
             if config.no_delay_in_first_layer and idx == 0:
-                layers.append(Linear(dim, width, bias=config.bias))
+                layers.append(_linear(config, dim, width))
             else:
                 layers.append(dcls_module(config, dim, width, groups=1))
             dim = width
@@ -273,7 +279,7 @@ class SNN_synaptic_feedforward_delays(SNN):
             if config.use_batch_norm:
                 layers.append(modified_batchnorm(width, step_mode="m"))
         if config.no_delay_in_last_layer:
-            layers.append(Linear(dim, config.output_size, bias=config.bias))
+            layers.append(_linear(config, dim, config.output_size))
         else:
             layers.append(dcls_module(config, dim, config.output_size, groups=1))
         self.layers = torch.nn.Sequential(*layers)
@@ -320,11 +326,11 @@ class SNN_axonal_feedforward_delays(SNN_synaptic_feedforward_delays):
 
     def _delay_stage(self, in_dim, out_dim, delayed):
         if not delayed:
-            return [Linear(in_dim, out_dim, bias=self.config.bias)]
+            return [_linear(self.config, in_dim, out_dim)]
         dc = copy(self.config)
         dc.bias = False
         return [dcls_module(dc, in_channels=in_dim, out_channels=in_dim, groups=in_dim),
-                Linear(in_dim, out_dim, bias=self.config.bias)]
+                _linear(self.config, in_dim, out_dim)]
 
     def init_weights(self):
         for m in self.layers:
@@ -348,7 +354,7 @@ class SNN_recurrent_and_feedforward_delays(SNN_synaptic_feedforward_delays, SNN_
         layers, dim = [], config.input_size
         for idx, width in enumerate(config.hidden_layers):
             if config.no_delay_in_first_layer and idx == 0:
-                layers.append(Linear(dim, width, bias=config.bias))
+                layers.append(_linear(config, dim, width))
             else:
                 layers.append(dcls_module(config, dim, width, groups=1))
             dim = width
@@ -358,7 +364,7 @@ class SNN_recurrent_and_feedforward_delays(SNN_synaptic_feedforward_delays, SNN_
             if config.use_batch_norm:
                 layers.append(modified_batchnorm(width, step_mode="m"))
         if config.no_delay_in_last_layer:
-            layers.append(Linear(dim, config.output_size, bias=config.bias))
+            layers.append(_linear(config, dim, config.output_size))
         else:
             layers.append(dcls_module(config, dim, config.output_size, groups=1))
         self.layers = torch.nn.Sequential(*layers)
@@ -406,13 +412,13 @@ class SNN_axonal_recurrent_and_feedforward_delays(SNN_recurrent_and_feedforward_
 
     def _projection(self, inputs, outputs, delayed):
         if not delayed:
-            return [Linear(inputs, outputs, bias=self.config.bias)]
+            return [_linear(self.config, inputs, outputs)]
         if not self.axonal_feedforward:
             return [dcls_module(self.config, inputs, outputs, groups=1)]
         dc = copy(self.config)
         dc.bias = False
         return [dcls_module(dc, inputs, inputs, groups=inputs),
-                Linear(inputs, outputs, bias=self.config.bias)]
+                _linear(self.config, inputs, outputs)]
 
     def init_weights(self):
         SNN_synaptic_feedforward_delays.init_weights(self)

@@ -15,6 +15,8 @@ import torch
 import torch.nn.functional as F
 
 from . import functional as Fn
+from .block_norm import GATES, block_join, block_norm
+from .gated import gated_scan, gated_step
 
 
 class MemoryModule(torch.nn.Module):
@@ -158,3 +160,75 @@ class BatchNorm1d(torch.nn.BatchNorm1d):
             y = super().forward(x.flatten(0, 1))
             return y.view(shp)
         return super().forward(x)
+
+
+class GatedIntegrator(MemoryModule):
+    """A leaky integrator with a learned, input-dependent decay (``gated.gated_scan``), in
+    place of ``LIFNode`` where no spikes are wanted: forward(z, f) with gate logits f.
+
+    Multi-step mode: z (T,B,N), f (T,B,G) -> h (T,B,N) from a zero state, or from the state
+    of the call before with ``keep_state=True``.  Single-step mode ('s'): z (B,N), f (B,G) ->
+    h (B,N), the state moving on from call to call until ``reset`` (``utils.reset_states``);
+    no gradient passes.  ``v`` is the state (B,N) in float32."""
+
+    def __init__(self, decay_input: bool = True, step_mode: str = "m", keep_state: bool = False,
+                 checkpoint8: bool = False):
+        super().__init__()
+        if step_mode not in ("m", "s"):
+            raise ValueError(f"step_mode must be 'm' or 's', got {step_mode!r}")
+        self.decay_input = decay_input
+        self.step_mode = step_mode
+        self.keep_state = keep_state
+        self.checkpoint8 = checkpoint8
+        self.register_memory("v", None)
+
+    def forward(self, z, f, lengths=None, resets=None):
+        if self.step_mode == "s":
+            if lengths is not None or resets is not None:
+                raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
+            h, self.v = gated_step(z, f, self.v, decay_input=self.decay_input)
+            return h
+        h, v = gated_scan(z, f, self.v if self.keep_state else None, lengths=lengths, resets=resets,
+                          decay_input=self.decay_input, checkpoint8=self.checkpoint8)
+        if self.keep_state:
+            self.v = v.detach()
+        return h
+
+    def extra_repr(self):
+        return f"decay_input={self.decay_input}, step_mode={self.step_mode}, checkpoint8={self.checkpoint8}"
+
+
+class BlockNorm(torch.nn.Module):
+    """RMS norm per position before the first block (``block_norm.block_norm``)."""
+
+    def __init__(self, num_features, eps: float = 1e-5):
+        super().__init__()
+        self.eps = eps
+        self.weight = torch.nn.Parameter(torch.ones(num_features))
+
+    def forward(self, x, lengths=None):
+        return block_norm(x, self.weight, eps=self.eps, lengths=lengths)
+
+
+class BlockJoin(torch.nn.Module):
+    """After a block: norm, gate, residual scale and sum, and the next block's norm
+    (``block_norm.block_join``).  forward(x, y, gate=None) -> (x', n), or x' alone with
+    ``next_norm=False`` (after the last block)."""
+
+    def __init__(self, num_features, gate_act: str = "sigmoid", scale_init: float = 1.0, next_norm: bool = True,
+                 eps: float = 1e-5):
+        super().__init__()
+        if gate_act not in GATES:
+            raise ValueError(f"gate_act must be one of {sorted(GATES)}, got {gate_act!r}")
+        self.gate_act, self.eps = gate_act, eps
+        self.weight = torch.nn.Parameter(torch.ones(num_features))
+        self.scale = torch.nn.Parameter(torch.full((num_features,), float(scale_init)))
+        if next_norm:
+            self.next_weight = torch.nn.Parameter(torch.ones(num_features))
+        else:
+            self.register_parameter("next_weight", None)
+
+    def forward(self, x, y, gate=None, lengths=None):
+        r = block_join(x, y, self.weight, gate=gate, gate_act=self.gate_act, scale=self.scale,
+                       next_weight=self.next_weight, eps=self.eps, lengths=lengths)
+        return r if self.next_weight is not None else r[0]
