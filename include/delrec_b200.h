@@ -309,9 +309,9 @@ typedef struct delrec_scan {
 int delrec_gated_scan_forward(const delrec_scan* scan, const void* z, const void* f, const float* h0,
                               const void* lengths, const uint8_t* resets, void* h, float* hT, float* states,
                               int8_t* qz, uint8_t* ez, int8_t* qf, uint8_t* ef, void* stream);
-/* Gradients from gh (NULL: 0) and ghT (NULL: 0): dz, df, dh0, any NULL to skip.  With qz
- * and ez, z is their restored value; with qf and ef, f is (z or f may then be NULL).
- * h_{t-1} is recomputed from states. */
+/* Gradients from gh (NULL: 0) and ghT (NULL: 0): dz, df, dh0, any NULL to skip.  With qz,
+ * ez, qf, ef (all or none, G = N), z and f are what those stand for.  h_{t-1} is recomputed
+ * from states. */
 size_t delrec_gated_scan_backward_workspace(const delrec_scan* scan);
 int delrec_gated_scan_backward(const delrec_scan* scan, const void* z, const void* f, const int8_t* qz,
                                const uint8_t* ez, const int8_t* qf, const uint8_t* ef, const void* lengths,

@@ -45,7 +45,7 @@ static inline int pow2_at_least(int x) {
       return DELREC_ERR_CUDA;                                              \
     }                                                                      \
   } while (0)
-unsigned long long g_launches = 0;  // kernels issued by this library (host counter; sequence.cu adds its own)
+unsigned long long g_launches = 0;  // kernels issued by this library (host counter; gated.cu and sequence.cu add theirs)
 
 // Optional timing of the reverse-scan kernels: CUDA events recorded on the launching
 // stream around each scan launch while enabled (delrec_scan_timing).

@@ -42,11 +42,6 @@ struct NormArgs {
   float* part;                          // (grid, 2, N): Q and dw_next partials
 };
 
-// V consecutive elements as one aligned access
-template <class T, int V>
-struct alignas(sizeof(T) * V) VecOf {
-  T v[V];
-};
 template <class T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float* o) {
   const VecOf<T, V> r = *(const VecOf<T, V>*)p;
@@ -76,9 +71,10 @@ __device__ __forceinline__ float block_sum(float v, float (*red)[32], int& slot)
   return s;
 }
 
+template <class T>
 __device__ __forceinline__ float gate_value(float u, int kind) {
   float sg, so;
-  sigmoid_pair(u, sg, so);
+  sigmoid_pair<Accurate<T>::value>(u, sg, so);
   return kind == GATE_SIGMOID ? sg : u * sg;
 }
 
@@ -129,7 +125,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
       if (p.ry && tid == 0) p.ry[r] = ry;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float g = GATE ? ws[i] * gate_value(u[i], p.kind) : ws[i];
+        const float g = GATE ? ws[i] * gate_value<T>(u[i], p.kind) : ws[i];
         x[i] = live ? fmaf(y[i] * ry, g, x[i]) : 0.f;
       }
 #pragma unroll
@@ -208,7 +204,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        if (p.y) x[i] = fmaf(y[i], GATE ? ws[i] * gate_value(u[i], p.kind) : ws[i], x[i]);
+        if (p.y) x[i] = fmaf(y[i], GATE ? ws[i] * gate_value<T>(u[i], p.kind) : ws[i], x[i]);
         x[i] *= rx;                             // xh
         qn[i] = fmaf(v[i], x[i], qn[i]);
         v[i] *= nw[i];
@@ -236,7 +232,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
       float a = 1.f, da = 0.f;
       if (GATE) {
         float sg, so;
-        sigmoid_pair(u[i], sg, so);
+        sigmoid_pair<Accurate<T>::value>(u[i], sg, so);
         a = p.kind == GATE_SIGMOID ? sg : u[i] * sg;
         da = p.kind == GATE_SIGMOID ? sg * so : sg * fmaf(u[i], so, 1.f);
       }

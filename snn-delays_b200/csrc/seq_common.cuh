@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cstdio>
 
 #include "../../include/delrec_b200.h"
@@ -45,23 +46,64 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-// sg = sigmoid(f), so = 1 - sigmoid(f) = sigmoid(-f), each to a few ulp for every f: from
-// t = exp(-|f|) in [0, 1], 1 / (1 + t) and t / (1 + t); no cancellation, no overflow.
-__device__ __forceinline__ void sigmoid_pair(float f, float& sg, float& so) {
-  const float t = expf(-fabsf(f));
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));   // 1 ulp on [1, 2]
-  const float s = t * r;
-  const bool pos = f >= 0.f;
-  sg = pos ? r : s;
-  so = pos ? s : r;
+// t = exp(-|f|) in [0, 1].  Accurate (2 ulp) for fp32 data; for 16-bit data one product and
+// one ex2 (its argument's rounding adds |f| units of 2^-24 to t, far below a 16-bit step).
+template <bool ACCURATE>
+__device__ __forceinline__ float exp_neg_abs(float f) {
+  if (ACCURATE) return expf(-fabsf(f));
+  float t;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(f) * -1.4426950408889634f));
+  return t;
 }
+// The larger and the smaller of sigmoid(f) and sigmoid(-f): 1 / (1 + t) and t / (1 + t),
+// each to a few ulp for every f (no cancellation, no overflow).
+template <bool ACCURATE>
+__device__ __forceinline__ void sigmoid_parts(float f, float& big, float& small) {
+  const float t = exp_neg_abs<ACCURATE>(f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.f + t));   // 1 ulp on [1, 2]
+  small = t * big;
+}
+// sg = sigmoid(f), so = 1 - sigmoid(f) = sigmoid(-f)
+template <bool ACCURATE>
+__device__ __forceinline__ void sigmoid_pair(float f, float& sg, float& so) {
+  float big, small;
+  sigmoid_parts<ACCURATE>(f, big, small);
+  const bool pos = f >= 0.f;
+  sg = pos ? big : small;
+  so = pos ? small : big;
+}
+template <class T>
+struct Accurate {
+  static constexpr bool value = sizeof(T) == 4;
+};
+
+// V consecutive elements as one aligned access
+template <class T, int V>
+struct alignas(sizeof(T) * V) VecOf {
+  T v[V];
+};
 
 // lengths (B) int32 or int64; NULL: every row is T long
 __device__ __forceinline__ int row_length(const void* lengths, int wide, int b, int T) {
   if (!lengths) return T;
   const long long n = wide ? ((const long long*)lengths)[b] : (long long)((const int*)lengths)[b];
   return n < 0 ? 0 : (n > T ? T : (int)n);
+}
+
+static inline int seq_grid(size_t n, int threads, int per_sm) {
+  const size_t g = (n + threads - 1) / threads;
+  return (int)std::max<size_t>(1, std::min(g, (size_t)kSeqSMs * per_sm));
+}
+
+// calls fn(T()) with the element type
+template <class F>
+static int by_dtype(int dtype, F&& fn) {
+  switch (dtype) {
+    case DELREC_F32: return fn(float());
+    case DELREC_BF16: return fn(__nv_bfloat16());
+    case DELREC_F16: return fn(__half());
+  }
+  return DELREC_ERR_ARG;
 }
 
 }  // namespace delrec

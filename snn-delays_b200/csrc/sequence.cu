@@ -1,93 +1,12 @@
-// extern "C" entry points of the sequence operators: argument checks, kernel variants and
-// launch shapes.  No allocation happens here.
+// extern "C" entry points of the block norms and the 8-bit checkpoints: argument checks, kernel
+// variants and launch shapes.  No allocation happens here.
 #include <algorithm>
 
 #include "block_norm.cuh"
 #include "checkpoint8.cuh"
-#include "gated_scan.cuh"
 #include "seq_common.cuh"
 
 namespace delrec {
-
-static int seq_grid(size_t n, int threads, int per_sm) {
-  const size_t g = (n + threads - 1) / threads;
-  return (int)std::max<size_t>(1, std::min(g, (size_t)kSeqSMs * per_sm));
-}
-
-// calls fn(T()) with the element type
-template <class F>
-static int by_dtype(int dtype, F&& fn) {
-  switch (dtype) {
-    case DELREC_F32: return fn(float());
-    case DELREC_BF16: return fn(__nv_bfloat16());
-    case DELREC_F16: return fn(__half());
-  }
-  return DELREC_ERR_ARG;
-}
-
-// --------------------------------------------------------------------------------
-// gated scan
-// --------------------------------------------------------------------------------
-static int check_scan(const delrec_scan* s) {
-  if (!s || s->T < 1 || s->B < 1 || s->N < 1 || s->G < 1 || s->N % s->G != 0) return DELREC_ERR_ARG;
-  if (s->dtype < DELREC_F32 || s->dtype > DELREC_F16) return DELREC_ERR_ARG;
-  if (s->T > (1 << 30)) return DELREC_ERR_UNSUPPORTED;
-  return DELREC_OK;
-}
-
-struct ScanShape {
-  int P, csize;
-  unsigned grid;
-};
-
-static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh) {
-  p->T = s->T; p->B = s->B; p->N = s->N; p->G = s->G; p->D = s->N / s->G;
-  p->decay_input = s->decay_input; p->wide = s->lengths_wide;
-  if (p->D > 32) {
-    p->tph = (p->D + 31) / 32;
-    p->cpt = 32;
-    p->tiles = p->G * p->tph;
-  } else {
-    p->tph = 0;
-    p->cpt = 32 / p->D * p->D;
-    p->tiles = (p->N + p->cpt - 1) / p->cpt;
-  }
-  const long long items = (long long)p->B * p->tiles;
-  const int segs = (p->T + kSeg - 1) / kSeg;
-  sh->P = segs >= kScanWarps ? kScanWarps : 1;
-  // few rows: the blocks of a cluster share one row's time
-  int c = 1;
-  while (c < kScanCluster && items * c < 2 * kSeqSMs && sh->P * c * 2 <= segs) c *= 2;
-  sh->csize = c;
-  if (items * c > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
-  sh->grid = (unsigned)(items * c);
-  return DELREC_OK;
-}
-
-static int scan_launch(void (*kern)(ScanArgs, int), ScanArgs& p, const ScanShape& sh, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(sh.grid);
-  cfg.blockDim = dim3(sh.P * 32);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = sh.csize;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = sh.csize > 1 ? 1 : 0;
-  SQ_CUDA(cudaLaunchKernelEx(&cfg, kern, p, (int)sh.csize));
-  SQ_LAUNCHED();
-  return DELREC_OK;
-}
-
-template <class T, int P, bool POS>
-static int scan_fwd_p(ScanArgs& p, const ScanShape& sh, cudaStream_t st) {
-  return scan_launch(p.qz ? k_scan_fwd<T, P, POS, true> : k_scan_fwd<T, P, POS, false>, p, sh, st);
-}
-template <class T, int P, bool POS>
-static int scan_bwd_p(ScanArgs& p, const ScanShape& sh, cudaStream_t st) {
-  return scan_launch(p.qz ? k_scan_bwd<T, P, POS, true> : k_scan_bwd<T, P, POS, false>, p, sh, st);
-}
 
 // --------------------------------------------------------------------------------
 // block norm
@@ -182,85 +101,6 @@ static NormArgs norm_args(const delrec_block* s) {
 using namespace delrec;
 
 extern "C" {
-
-int delrec_gated_scan_forward(const delrec_scan* s, const void* z, const void* f, const float* h0,
-                              const void* lengths, const uint8_t* resets, void* h, float* hT, float* states,
-                              int8_t* qz, uint8_t* ez, int8_t* qf, uint8_t* ef, void* stream) {
-  int rc = check_scan(s);
-  if (rc) return rc;
-  if (!z || !f || !h) return DELREC_ERR_ARG;
-  const bool pack = qz || ez || qf || ef;
-  if (pack && (!(qz && ez && qf && ef) || s->G != s->N)) return DELREC_ERR_ARG;
-  ScanArgs p{};
-  ScanShape sh;
-  if ((rc = scan_shape(s, &p, &sh))) return rc;
-  p.z = z; p.f = f; p.h0 = h0; p.lengths = lengths; p.resets = resets; p.h = h; p.hT = hT; p.states = states;
-  p.qz = qz; p.ez = ez; p.qf = qf; p.ef = ef;
-  p.z_t = s->z_t; p.z_b = s->z_b; p.f_t = s->f_t; p.f_b = s->f_b; p.h_t = s->h_t; p.h_b = s->h_b;
-  const cudaStream_t st = (cudaStream_t)stream;
-  const bool pos = lengths || resets;
-  return by_dtype(s->dtype, [&](auto t) {
-    using T = decltype(t);
-    if (sh.P == 1) return pos ? scan_fwd_p<T, 1, true>(p, sh, st) : scan_fwd_p<T, 1, false>(p, sh, st);
-    return pos ? scan_fwd_p<T, kScanWarps, true>(p, sh, st) : scan_fwd_p<T, kScanWarps, false>(p, sh, st);
-  });
-}
-
-size_t delrec_gated_scan_backward_workspace(const delrec_scan* s) {
-  if (check_scan(s)) return 0;
-  const int D = s->N / s->G;
-  return D > 32 ? (size_t)s->T * s->B * s->G * ((D + 31) / 32) * sizeof(float) : 0;
-}
-
-int delrec_gated_scan_backward(const delrec_scan* s, const void* z, const void* f, const int8_t* qz,
-                               const uint8_t* ez, const int8_t* qf, const uint8_t* ef, const void* lengths,
-                               const uint8_t* resets, const float* states, const void* gh, const float* ghT,
-                               void* dz, void* df, float* dh0, void* ws, size_t wsb, void* stream) {
-  int rc = check_scan(s);
-  if (rc) return rc;
-  if (!states || (!qz != !ez) || (!qf != !ef) || (!qz && !z) || (!qf && !f) || (qf && !qz)) return DELREC_ERR_ARG;
-  ScanArgs p{};
-  ScanShape sh;
-  if ((rc = scan_shape(s, &p, &sh))) return rc;
-  const size_t need = df ? delrec_gated_scan_backward_workspace(s) : 0;
-  if (need && (!ws || ((uintptr_t)ws & 255) != 0 || wsb < need)) return DELREC_ERR_WORKSPACE;
-  p.z = z; p.f = f; p.lengths = lengths; p.resets = resets; p.states = const_cast<float*>(states);
-  p.qz = const_cast<int8_t*>(qz); p.ez = const_cast<uint8_t*>(ez);
-  p.qf = const_cast<int8_t*>(qf); p.ef = const_cast<uint8_t*>(ef);
-  p.gh = gh; p.ghT = ghT; p.dz = dz; p.df = df; p.dh0 = dh0; p.part = (float*)ws;
-  p.z_t = s->z_t; p.z_b = s->z_b; p.f_t = s->f_t; p.f_b = s->f_b; p.gh_t = s->gh_t; p.gh_b = s->gh_b;
-  p.dz_t = s->dz_t; p.dz_b = s->dz_b; p.df_t = s->df_t; p.df_b = s->df_b;
-  const cudaStream_t st = (cudaStream_t)stream;
-  const bool pos = lengths || resets;
-  return by_dtype(s->dtype, [&](auto t) {
-    using T = decltype(t);
-    int r;
-    if (sh.P == 1) r = pos ? scan_bwd_p<T, 1, true>(p, sh, st) : scan_bwd_p<T, 1, false>(p, sh, st);
-    else r = pos ? scan_bwd_p<T, kScanWarps, true>(p, sh, st) : scan_bwd_p<T, kScanWarps, false>(p, sh, st);
-    if (r) return r;
-    if (df && p.tph) {
-      k_scan_df_sum<T><<<seq_grid((size_t)p.T * p.B * p.G, 256, 8), 256, 0, st>>>(p);
-      SQ_LAUNCHED();
-    }
-    return (int)DELREC_OK;
-  });
-}
-
-int delrec_gated_step(const delrec_scan* s, const void* z, const void* f, const float* state,
-                      const uint8_t* active, void* h, float* next, void* stream) {
-  const int rc = check_scan(s);
-  if (rc) return rc;
-  if (s->T != 1 || !z || !f || !h || !next) return DELREC_ERR_ARG;
-  const cudaStream_t st = (cudaStream_t)stream;
-  return by_dtype(s->dtype, [&](auto t) {
-    using T = decltype(t);
-    k_gated_step<T><<<seq_grid((size_t)s->B * s->N, 128, 16), 128, 0, st>>>(
-        s->B, s->N, s->N / s->G, s->decay_input, (const T*)z, s->z_b, (const T*)f, s->f_b, state, active, (T*)h,
-        next);
-    SQ_LAUNCHED();
-    return (int)DELREC_OK;
-  });
-}
 
 int delrec_block_norm_forward(const delrec_block* s, const void* x, const void* y, const void* u, const float* w,
                               const float* scale, const float* next_w, const void* lengths, void* out, void* n,

@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .checkpoint8 import Packed8, empty8, pack8
+from .checkpoint8 import Packed8, empty8, pack8, unpack8
 
 SEGMENT = 16     # distance of the states kept for the backward pass
 
@@ -92,6 +92,8 @@ class GatedScan(torch.autograd.Function):
         if ctx.keep8:
             qz, ez, qf, ef, states, lengths, resets = ctx.saved_tensors
             pz, pf = Packed8(qz, ez, ctx.dtype), Packed8(qf, ef, ctx.dtype)
+            if ctx.scan.G != ctx.scan.N:    # the 8-bit kernel is for a gate per channel
+                z, f, pz, pf = unpack8(pz), unpack8(pf), None, None
             like_z, like_f = qz, qf
         else:
             z, f, states, lengths, resets = ctx.saved_tensors
@@ -111,7 +113,7 @@ class GatedScan(torch.autograd.Function):
         if T and B and N:
             # a copy of the descriptor: two backward passes of one graph may run at once
             s = _lib.Scan.from_buffer_copy(ctx.scan)
-            for name, t in (("gh", gh), ("dz", dz), ("df", df)):
+            for name, t in (("z", z), ("f", f), ("gh", gh), ("dz", dz), ("df", df)):
                 if t is not None:
                     setattr(s, name + "_t", t.stride(0))
                     setattr(s, name + "_b", t.stride(1))

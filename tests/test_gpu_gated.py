@@ -175,7 +175,11 @@ def test_saturated_gates(value):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_layouts(T, dtype):
     """Batch-major storage, channel slices, odd offsets, a gate expanded over time and rows, a
-    strided channel dimension: the same bits as contiguous tensors."""
+    strided channel dimension.  Alignment chooses how many channels a lane takes, and with it
+    the order in which steps are put together: both orders are within 16 u per step of the
+    exact value, carried on by gates below sigmoid(4.5) = 0.989, so within 2 * 16 u * 90 =
+    2^-12.5 of each other times the largest magnitude (about 4 here: 2^-10.5), and 16-bit
+    results within one step more."""
     from delrec.gated import gated_scan
     N, B = 32, 3
     g = torch.Generator().manual_seed(T)
@@ -188,14 +192,17 @@ def test_layouts(T, dtype):
         h, hT = gated_scan(z, f)
         return (h, hT, *torch.autograd.grad((h, hT), (z, f), (gh, torch.ones_like(hT))))
 
+    def near(a, b):
+        torch.testing.assert_close(a, b, rtol=2.0 ** -7 if a.dtype == BF16 else 0, atol=2.0 ** -10.5)
+
     base = go(z.contiguous(), f.contiguous(), gh.contiguous())
     channel_last = f.transpose(1, 2).contiguous().transpose(1, 2)
     for got in (go(z, f, gh), go(z.contiguous(), f, gh), go(z, channel_last, gh)):
         for a, b in zip(got, base):
-            assert torch.equal(a, b)
+            near(a, b)
     one = f[3:4, 1:2].expand(T, B, N)
     for a, b in zip(go(z, one, gh), go(z, one.contiguous(), gh)):
-        assert torch.equal(a, b)
+        near(a, b)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

@@ -99,10 +99,13 @@ def test_c_entry_points_reject_bad_arguments():
                                               p, None, ws, n, None)
 
     assert bwd(_scan(), states=None) == 1 and bwd(_scan(), z=None) == 1 and bwd(_scan(), qz=p) == 1
-    assert bwd(_scan(), qf=p, ef=p) == 1
+    assert bwd(_scan(), qf=p, ef=p) == 1 and bwd(_scan(G=4), qz=p, ez=p, qf=p, ef=p) == 1
+    strided = _scan()
+    strided.z_t = 1 << 31
+    assert fwd(strided) == 4 and bwd(strided) == 4
     wide = _scan(N=128, G=2)
     need = lib.delrec_gated_scan_backward_workspace(ctypes.byref(wide))
-    assert need == 4 * 2 * 2 * 2 * 4
+    assert need == 4 * 2 * 4 * 2 * 4
     assert bwd(wide, ws=None) == 3 and bwd(wide, n=need - 1) == 3 and bwd(wide, ws=ctypes.c_void_p(4097)) == 3
     assert lib.delrec_gated_scan_backward_workspace(ctypes.byref(_scan())) == 0
     assert lib.delrec_gated_scan_backward_workspace(None) == 0
