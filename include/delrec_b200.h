@@ -304,18 +304,19 @@ typedef struct delrec_scan {
 /* h_t = sigmoid(f_t) h_{t-1} + c_t z_t from h0 (B,N) (NULL: 0); resets (T,B) bytes or NULL:
  * nonzero drops h_{t-1} at that step.  Writes h, hT (B,N) (the state after the last
  * position; NULL to skip) and, for the backward, states (ceil(T/16), B, N): the state before
- * every 16th step (NULL to skip).  qz, ez, qf, ef (all or none, G = N): also writes z and f
- * in 8 bits (delrec_pack8's form). */
+ * every 16th step (NULL to skip).  qz, ez, qf, ef, odd (all or none, G = N): also writes z
+ * and f in 8 bits (delrec_pack8's form), and odd (ceil(T/16), B, ceil(N/32)): nonzero where a
+ * code of those 16 steps and 32 channels may stand for an infinity or NaN. */
 int delrec_gated_scan_forward(const delrec_scan* scan, const void* z, const void* f, const float* h0,
                               const void* lengths, const uint8_t* resets, void* h, float* hT, float* states,
-                              int8_t* qz, uint8_t* ez, int8_t* qf, uint8_t* ef, void* stream);
+                              int8_t* qz, uint8_t* ez, int8_t* qf, uint8_t* ef, uint8_t* odd, void* stream);
 /* Gradients from gh (NULL: 0) and ghT (NULL: 0): dz, df, dh0, any NULL to skip.  With qz,
- * ez, qf, ef (all or none, G = N), z and f are what those stand for.  h_{t-1} is recomputed
+ * ez, qf, ef, odd (all or none, G = N), z and f are what those stand for.  h_{t-1} is recomputed
  * from states. */
 size_t delrec_gated_scan_backward_workspace(const delrec_scan* scan);
 int delrec_gated_scan_backward(const delrec_scan* scan, const void* z, const void* f, const int8_t* qz,
-                               const uint8_t* ez, const int8_t* qf, const uint8_t* ef, const void* lengths,
-                               const uint8_t* resets, const float* states, const void* gh, const float* ghT,
+                               const uint8_t* ez, const int8_t* qf, const uint8_t* ef, const uint8_t* odd,
+                               const void* lengths, const uint8_t* resets, const float* states, const void* gh, const float* ghT,
                                void* dz, void* df, float* dh0, void* workspace, size_t workspace_bytes,
                                void* stream);
 /* One step (T is 1): h (B,N) and next (B,N) from z, f and state (B,N) (NULL: 0); next may be

@@ -7,7 +7,7 @@
 //   gate,  dh0 = a_0 r_0 G_0.
 //
 // Every step is an affine map h -> A h + H of its channel, and maps of consecutive steps
-// compose, so time is cut into segments: a warp holds one segment (S steps of 32 V channels,
+// compose, so time is cut into segments: a warp holds one segment (16 steps of 32 V channels,
 // V per lane) in registers, the P warps of a block hold P consecutive segments, and the
 // blocks of a cluster consecutive runs of those.  Each warp reduces its segment to (A, H),
 // the block (then the cluster, over distributed shared memory) folds the maps before it in
@@ -17,29 +17,34 @@
 // Bound by HBM (3 elements per channel-step forward, 5 backward) if the issue slots allow:
 // per element there are about 60 (fp32) or 30 (16-bit) of them in the time its bytes
 // take, and a straightforward kernel with bounds tests and 64-bit strides spends 80 forward
-// and 118 backward.  So segments that lie inside a sequence run without tests, strides are 32-bit,
-// 16-bit data goes two channels to a lane with a short exp, and the backward's map of the
-// reverse recurrence is built in the forward walk (H += g Pi a).  Backward does not read h:
-// the forward keeps the fp32 state before every 16th step (1/16 of an fp32 tensor) and each
-// segment recomputes its states from there, which also spares the rounding of a 16-bit h.
+// and 118 backward.  So 16-bit data goes two channels to a lane with a short exp, strides are
+// 32-bit, segments inside a sequence are stored without tests, and the backward's map of
+// the reverse recurrence is built in the forward walk (H += g Pi a).  Rows of 16-byte multiples are
+// staged: each warp copies its next segment into shared memory (cp.async) while it works on
+// the present one, so 16 warps per SM keep the memory busy at 128 registers a thread.
+// Backward does not read h: the forward keeps the fp32 state before every 16th step (1/16
+// of an fp32 tensor) and each segment recomputes its states from there, which also spares
+// the rounding of a 16-bit h.
 #pragma once
 
 #include <cooperative_groups.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "checkpoint8.cuh"
 #include "seq_common.cuh"
 
 namespace delrec {
 
-static constexpr int kSeg = 16;         // distance of the kept states; steps of a backward segment
+static constexpr int kSeg = 16;         // steps of a segment, the distance of the kept states
 static constexpr int kScanCluster = 16; // most blocks per cluster (above 8: not every GPU has room)
 
 struct ScanArgs {
   int T, B, N, G, D;
   int decay_input, wide;               // wide: lengths are int64
   int tiles, cpt;                      // channel tiles per row; channels of a tile
-  int split;                           // D > 32: tiles cut across gates, df goes through part
-  int ahead;                           // rows are whole aligned sectors: fetch the next wave to L2
+  int split;                           // D >= 32: tiles cut across gates, df goes through part
   const void *z, *f;
   int z_t, f_t, h_t;                   // element strides of time
   long long z_b, f_b, h_b;             // and of the batch
@@ -51,6 +56,7 @@ struct ScanArgs {
   float* states;                       // (ceil(T/16), B, N) or NULL
   int8_t *qz, *qf;                     // 8-bit z and f (T,B,N) with their exponents
   uint8_t *ez, *ef;
+  uint8_t* odd;                        // (ceil(T/16), B, groups): infinities or NaN among a segment's codes
   // backward
   const void* gh;
   int gh_t, dz_t, df_t;
@@ -62,8 +68,8 @@ struct ScanArgs {
 };
 
 // A lane's place in a tile: its first channel and its gate.  A tile is cpt consecutive
-// channels: 32 V (D = 1, or D > 32, where it may reach into a second gate), or the whole
-// gates that fit 32 lanes (1 < D <= 32).
+// channels: 32 V (D = 1, or D >= 32, where it may reach into a second gate), or the whole
+// gates that fit 32 lanes (1 < D < 32).
 struct Place {
   int c, g;
   bool on;
@@ -108,28 +114,32 @@ __device__ __forceinline__ void scan_exchange(ScanExchange<P, V>& sm, int buf, i
     // the block's map, every warp's in turn, into each block of the cluster; the warps
     // share the destinations
     cg::cluster_group cl = cg::this_cluster();
+    if (warp < csize) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      float2 t = P > 1 ? sm.own[buf][0][k][lane] : m[k];
+      for (int k = 0; k < V; ++k) {
+        float2 t = P > 1 ? sm.own[buf][0][k][lane] : m[k];
 #pragma unroll
-      for (int j = 1; j < P; ++j) {
-        const float2 n = sm.own[buf][j][k][lane];
-        const bool cut = POS && (__float_as_uint(n.x) == 0x80000000u || __float_as_uint(t.x) == 0x80000000u);
-        t = make_float2(cut ? -0.f : n.x * t.x, scan_apply<POS>(n, t.y));
+        for (int j = 1; j < P; ++j) {
+          const float2 n = sm.own[buf][j][k][lane];
+          const bool cut = POS && (__float_as_uint(n.x) == 0x80000000u || __float_as_uint(t.x) == 0x80000000u);
+          t = make_float2(cut ? -0.f : n.x * t.x, scan_apply<POS>(n, t.y));
+        }
+        for (int j = warp; j < csize; j += P) cl.map_shared_rank(&sm, j)->all[buf][rank][k][lane] = t;
       }
-      for (int j = warp; j < csize; j += P) cl.map_shared_rank(&sm, j)->all[buf][rank][k][lane] = t;
     }
     cl.sync();
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      float x = v[k], y = v[k];
+#pragma unroll 4
       for (int j = 0; j < csize; ++j) {
-        if (j == rank) x = y;
-        y = scan_apply<POS>(sm.all[buf][j][k][lane], y);
+        if (j == rank) in[k] = v[k];
+        v[k] = scan_apply<POS>(sm.all[buf][j][k][lane], v[k]);
       }
-      for (int j = 0; j < warp; ++j) x = scan_apply<POS>(sm.own[buf][j][k][lane], x);
-      in[k] = x;
-      v[k] = y;
+#pragma unroll
+      for (int j = 0; j < P - 1; ++j) {
+        const float x = scan_apply<POS>(sm.own[buf][j][k][lane], in[k]);
+        if (j < warp) in[k] = x;
+      }
     }
     return;
   }
@@ -159,31 +169,68 @@ __device__ __forceinline__ const E* at_step(const E* base, int stride, int i) {
 }
 
 // bit i: a reset at step tb + i (below n)
-template <int S>
 __device__ __forceinline__ unsigned scan_resets(const ScanArgs& p, int b, int tb, int n, int lane) {
   if (!p.resets) return 0u;
-  const bool r = lane < S && tb + lane < n && p.resets[(size_t)(tb + lane) * p.B + b];
+  const bool r = lane < kSeg && tb + lane < n && p.resets[(size_t)(tb + lane) * p.B + b];
   return __ballot_sync(0xffffffffu, r);
 }
 
-// The S x V elements of a segment, 0 past n (bounds) or where the lane is off.
-template <class T, int V, int S>
-__device__ __forceinline__ void scan_load(const T* base, int stride, int tb, int n, bool on, VecOf<T, V> (&r)[S]) {
-  if (on && tb + S <= n) {
+// ---------------------------------------------------------------------------------
+// inputs of a segment
+// ---------------------------------------------------------------------------------
+// How a kernel gets its inputs.  DIRECT: plain loads, any layout (V = 1).  STAGED: rows copied
+// through shared memory ahead of time; a gate per channel, rows and strides of 16-byte
+// multiples.  WIDE: D >= 32, plain loads; a tile reaches into two gates at most, so lanes 0-15
+// and 16-31 hold the 16 steps of one each and hand them round.
+enum : int { SCAN_DIRECT = 0, SCAN_STAGED = 1, SCAN_WIDE = 2 };
+
+template <int BYTES>
+struct alignas(BYTES == 16 ? 16 : BYTES) RawBytes {
+  char b[BYTES];
+};
+
+// 16 rows of ROWB bytes into shared memory, 16 bytes per copy; rows at or past n and
+// columns past the row's end (left bytes) become 0 without being read.
+template <int ROWB>
+__device__ __forceinline__ void stage_rows(unsigned dst, const char* row0, long long stride_bytes, int n, int left,
+                                           int lane) {
+  constexpr int CH = ROWB / 16;
 #pragma unroll
-    for (int i = 0; i < S; ++i) r[i] = *(const VecOf<T, V>*)at_step(base, stride, i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-      if (on && tb + i < n) {
-        r[i] = *(const VecOf<T, V>*)at_step(base, stride, i);
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) r[i].v[k] = from_f<T>(0.f);
-      }
+  for (int j = 0; j < kSeg * CH; j += 32) {
+    const int i = (j + lane) / CH, c = (j + lane) % CH * 16;
+    if (kSeg * CH >= 32 || lane < kSeg * CH) {
+      const bool ok = i < n && c < left;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * ROWB + c),
+                   "l"(ok ? row0 + i * stride_bytes + c : row0), "r"(ok ? 16 : 0));
     }
   }
 }
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void stage_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// plain loads of a segment's V = 1 channel, 0 at or past n or where the lane is off
+template <class E>
+__device__ __forceinline__ void direct_rows(const E* base, int stride, int n, bool on, E (&r)[kSeg]) {
+  if (on && n >= kSeg) {
+#pragma unroll
+    for (int i = 0; i < kSeg; ++i) r[i] = *at_step(base, stride, i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSeg; ++i) {
+      memset(&r[i], 0, sizeof(E));
+      if (on && i < n) r[i] = *at_step(base, stride, i);
+    }
+  }
+}
+
+// A position in a kernel's work: item (row and channel tile), wave of segments.
+struct Cursor {
+  int item, wv;
+};
+
 
 // The biased exponent of a value's 8-bit scale before its offset of 6: the float's own, one
 // more where its mantissa is past 126 / 64.  Monotone in |v|, so the group's largest key is
@@ -203,7 +250,7 @@ __device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) { return _
 template <int V>
 struct PackOut {
   int8_t *qz, *qf;
-  uint8_t *ez, *ef;
+  uint8_t *ez, *ef, *odd;
   int stride, estride;   // of a time step
 };
 // V codes of one step and channel pair
@@ -271,145 +318,14 @@ __device__ __forceinline__ void scan_pack(const VecOf<T, V> (&zr)[S], const VecO
     o.ef[(long long)hl * o.estride] = (uint8_t)q_key_exponent(mine >> 16);
   }
   const bool head = group_on && hl == 0;
+  if (head) *o.odd = (top & 0xffffu) >= 255u || (top >> 16) >= 255u;
   if (__any_sync(0xffffffffu, (top & 0xffffu) >= 255u))
     scan_pack_slow<T, V, S>(zr, o.qz, o.ez, o.stride, o.estride, n, on, head);
   if (__any_sync(0xffffffffu, (top >> 16) >= 255u))
     scan_pack_slow<T, V, S>(fr, o.qf, o.ef, o.stride, o.estride, n, on, head);
 }
 
-// Asks L2 for a segment's rows ahead of their loads: S rows of BYTES, a lane per 32-byte sector.
-template <int S, int BYTES, class T>
-__device__ __forceinline__ void scan_prefetch(const T* row0, int stride, int n, int lane) {
-  constexpr int PER = BYTES / 32;
-#pragma unroll
-  for (int j = 0; j < S * PER; j += 32) {
-    const int i = (j + lane) / PER, s = (j + lane) % PER;
-    if (i < n) {
-      const char* a = (const char*)(row0 + (long long)i * stride) + s * 32;
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(a));
-    }
-  }
-}
-
-// PACK (D = 1): also writes z and f in 8 bits; a tile is V groups of 32 channels.
-template <class T, int V, int S, int P, bool POS, bool PACK>
-__global__ void __launch_bounds__(P * 32, (PACK ? 16 : 24) / P) k_scan_fwd(ScanArgs p, int csize) {
-  __shared__ ScanExchange<P, V> sm;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = csize > 1 ? (int)(blockIdx.x % csize) : 0;
-  const int seg = rank * P + warp, wave = P * S * csize;
-  const int items = p.B * p.tiles, step = gridDim.x / csize;
-  int buf = 0;
-  for (int item = blockIdx.x / csize; item < items; item += step) {
-    const int b = item / p.tiles, tile = item - b * p.tiles;
-    const Place pl = scan_place<V>(p, tile, lane);
-    const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
-    const T* z = (const T*)p.z + b * p.z_b + pl.c + (long long)seg * S * p.z_t;
-    const T* f = (const T*)p.f + b * p.f_b + pl.g + (long long)seg * S * p.f_t;
-    T* h = (T*)p.h + b * p.h_b + pl.c + (long long)seg * S * p.h_t;
-    float v[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = (pl.on && p.h0) ? p.h0[(size_t)b * p.N + pl.c + k] : 0.f;
-    for (int t0 = 0; t0 < p.T; t0 += wave, buf ^= 1) {
-      const int tb = t0 + seg * S;
-      VecOf<T, V> zr[S], fr[S];
-      scan_load<T, V, S>(z, p.z_t, tb, len, pl.on, zr);
-      scan_load<T, V, S>(f, p.f_t, tb, len, pl.on, fr);
-      const unsigned cut = POS ? scan_resets<S>(p, b, tb, len, lane) : 0u;
-      if (p.ahead) {
-        // the next wave of this item, or the first of the next one
-        const bool more = t0 + wave < p.T;
-        const int ni = more ? item : item + step;
-        if (ni < items) {
-          const int nb = ni / p.tiles, nt = ni - nb * p.tiles, tn = (more ? t0 + wave : 0) + seg * S;
-          scan_prefetch<S, 32 * V * (int)sizeof(T)>((const T*)p.z + nb * p.z_b + nt * p.cpt + (long long)tn * p.z_t,
-                                                    p.z_t, p.T - tn, lane);
-          scan_prefetch<S, 32 * V * (int)sizeof(T)>((const T*)p.f + nb * p.f_b + nt * p.cpt + (long long)tn * p.f_t,
-                                                    p.f_t, p.T - tn, lane);
-        }
-      }
-      float a[S][V], x[S][V];
-      float2 m[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < S; ++i)
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float zf = to_f(zr[i].v[k]);
-          float om;
-          sigmoid_pair<Accurate<T>::value>(to_f(fr[i].v[k]), a[i][k], om);
-          x[i][k] = p.decay_input ? om * zf : zf;
-        }
-      if (PACK && tb < p.T) {
-        const size_t row = (size_t)tb * p.B + b;
-        const int groups = (p.N + kQGroup - 1) / kQGroup, grp = tile * V + lane * V / 32;
-        PackOut<V> o;
-        o.qz = p.qz + row * p.N + pl.c; o.qf = p.qf + row * p.N + pl.c;
-        o.ez = p.ez + row * groups + grp; o.ef = p.ef + row * groups + grp;
-        o.stride = p.B * p.N; o.estride = p.B * groups;
-        scan_pack<T, V, S>(zr, fr, o, p.T - tb, pl.on, grp < groups, lane);
-      }
-      if (tb + S > len) {
-#pragma unroll
-        for (int i = 0; i < S; ++i)
-#pragma unroll
-          for (int k = 0; k < V; ++k)
-            if (tb + i >= len) { a[i][k] = 1.f; x[i][k] = 0.f; }
-      }
-#pragma unroll
-      for (int i = 0; i < S; ++i)
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          if (POS && ((cut >> i) & 1)) m[k] = make_float2(0.f, x[i][k]);
-          else m[k] = make_float2(m[k].x * a[i][k], fmaf(a[i][k], m[k].y, x[i][k]));
-        }
-      if (POS && cut) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) m[k].x = -0.f;
-      }
-      float s[V];
-      scan_exchange<P, V, POS>(sm, buf, warp, lane, rank, csize, m, v, s);
-      if (p.states && pl.on && tb < p.T && tb % kSeg == 0) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) p.states[((size_t)(tb / kSeg) * p.B + b) * p.N + pl.c + k] = s[k];
-      }
-      if (pl.on && tb + S <= len) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          VecOf<T, V> o;
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            s[k] = (POS && ((cut >> i) & 1)) ? x[i][k] : fmaf(a[i][k], s[k], x[i][k]);
-            o.v[k] = from_f<T>(s[k]);
-          }
-          *(VecOf<T, V>*)at_step(h, p.h_t, i) = o;
-        }
-      } else if (pl.on) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          VecOf<T, V> o;
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            s[k] = (POS && ((cut >> i) & 1)) ? x[i][k] : fmaf(a[i][k], s[k], x[i][k]);
-            o.v[k] = from_f<T>(tb + i < len ? s[k] : 0.f);
-          }
-          if (tb + i < p.T) *(VecOf<T, V>*)at_step(h, p.h_t, i) = o;
-        }
-      }
-      z += (long long)wave * p.z_t;
-      f += (long long)wave * p.f_t;
-      h += (long long)wave * p.h_t;
-    }
-    if (p.hT && pl.on && rank == 0 && warp == 0) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) p.hT[(size_t)b * p.N + pl.c + k] = v[k];
-    }
-  }
-  if (csize > 1) cooperative_groups::this_cluster().sync();   // no block leaves while its peers may still write to it
-}
-
-// Sum of v over the lanes of a gate of D <= 32 lanes (d: the lane's place in it), in the
+// Sum of v over the lanes of a gate of D < 32 lanes (d: the lane's place in it), in the
 // gate's lane 0.  A fixed tree.
 __device__ __forceinline__ float gate_sum(float v, int d, int D) {
   for (int o = 16; o > 0; o >>= 1) {
@@ -440,6 +356,12 @@ __device__ __forceinline__ float warp_sum16(const float (&x)[16], int lane) {
 
 // A gate as one register: the smaller of a and 1 - a, signed as f.  The larger is 1 - |w|,
 // to one rounding.
+template <bool ACCURATE>
+__device__ __forceinline__ float gate_fold(float f) {
+  float big, small;
+  sigmoid_parts<ACCURATE>(f, big, small);
+  return f >= 0.f ? small : -small;
+}
 __device__ __forceinline__ void gate_unfold(float w, float& a, float& om) {
   const float s = fabsf(w), l = 1.f - s;
   const bool pos = !(__float_as_uint(w) >> 31);
@@ -447,110 +369,281 @@ __device__ __forceinline__ void gate_unfold(float w, float& a, float& om) {
   om = pos ? s : l;
 }
 
-// An 8-bit segment: codes of S x V channels, the scales of its steps spread over the lanes.
-template <int V, int S>
-struct Scan8 {
-  VecOf<int8_t, V> q[S];
-  float scale;                         // lane j: of step j (V = 1), of step j / 2, group j & 1 (V = 2)
+
+// ---------------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------------
+// PACK (D = 1): also writes z and f in 8 bits; a tile is V groups of 32 channels.
+template <class T, int V, int P, bool POS, bool PACK, int MODE>
+struct ScanFwd {
+  static constexpr int S = kSeg, ROWB = 32 * V * (int)sizeof(T);
+  static constexpr int STAGE = MODE == SCAN_STAGED ? 2 * S * ROWB : 0;   // bytes of a warp's segment
+  static constexpr int SMEM = 2 * P * STAGE;
+  // 16-bit pairs and packing take 128 registers, single channels 80
+  static constexpr int WARPS = V == 2 || PACK ? 16 : 24;
 };
-template <int V, int S>
-__device__ __forceinline__ void scan_load8(const ScanArgs& p, const int8_t* q, const uint8_t* e, int b, int tb, int n,
-                                           int tile, const Place& pl, int lane, Scan8<V, S>& r) {
-  const int groups = (p.N + kQGroup - 1) / kQGroup;
-  const int step = lane / V, grp = tile * V + lane % V;
-  r.scale = 1.f;
-  if (step < S && tb + step < n && grp < groups)
-    r.scale = q_scale(e[((size_t)(tb + step) * p.B + b) * groups + grp]);
-  const int8_t* base = q + ((size_t)tb * p.B + b) * p.N + pl.c;
-  const int stride = p.B * p.N;
-  if (pl.on && tb + S <= n) {
+template <class T, int V, int P, bool POS, bool PACK, int MODE>
+__global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WARPS / P) k_scan_fwd(ScanArgs p, int csize) {
+  using K = ScanFwd<T, V, P, POS, PACK, MODE>;
+  constexpr int S = kSeg, ROWB = K::ROWB;
+  __shared__ ScanExchange<P, V> sm;
+  extern __shared__ __align__(16) char stage[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = csize > 1 ? (int)(blockIdx.x % csize) : 0;
+  const int seg = rank * P + warp, wave = P * S * csize, waves = (p.T + wave - 1) / wave;
+  const int items = p.B * p.tiles, step = gridDim.x / csize;
+  char* mine = stage + warp * 2 * K::STAGE;
+  // copies the segment of a cursor into half h of this warp's stage
+  auto fetch = [&](Cursor c, int h) {
+    if (MODE == SCAN_STAGED && c.item < items) {
+      const int b = c.item / p.tiles, c0 = (c.item - b * p.tiles) * 32 * V, tb = c.wv * wave + seg * S;
+      const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
+      const int n = len - tb, left = (p.N - c0) * (int)sizeof(T);
+      const unsigned dst = (unsigned)__cvta_generic_to_shared(mine + h * K::STAGE);
+      stage_rows<ROWB>(dst, (const char*)((const T*)p.z + b * p.z_b + c0 + (long long)tb * p.z_t),
+                       (long long)p.z_t * (int)sizeof(T), n, left, lane);
+      stage_rows<ROWB>(dst + S * ROWB, (const char*)((const T*)p.f + b * p.f_b + c0 + (long long)tb * p.f_t),
+                       (long long)p.f_t * (int)sizeof(T), n, left, lane);
+    }
+    if (MODE == SCAN_STAGED) stage_commit();
+  };
+  Cursor cur{(int)blockIdx.x / csize, 0};
+  fetch(cur, 0);
+  float v[V];
+  for (int buf = 0; cur.item < items; buf ^= 1) {
+    Cursor nxt{cur.item, cur.wv + 1};
+    if (nxt.wv == waves) nxt = Cursor{cur.item + step, 0};
+    __syncwarp();   // all lanes are past their reads of the half that is written now
+    fetch(nxt, buf ^ 1);
+    const int b = cur.item / p.tiles, tile = cur.item - b * p.tiles;
+    const Place pl = scan_place<V>(p, tile, lane);
+    const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
+    const int tb = cur.wv * wave + seg * S, n = len - tb;
+    if (cur.wv == 0) {
 #pragma unroll
-    for (int i = 0; i < S; ++i) r.q[i] = *(const VecOf<int8_t, V>*)at_step(base, stride, i);
-  } else {
+      for (int k = 0; k < V; ++k) v[k] = (pl.on && p.h0) ? p.h0[(size_t)b * p.N + pl.c + k] : 0.f;
+    }
+    const unsigned cut = POS ? scan_resets(p, b, tb, len, lane) : 0u;
+    VecOf<T, V> zr[S], fr[S];
+    float wide = 0.f;
+    int edge = 32;
+    if constexpr (MODE == SCAN_STAGED) {
+      stage_wait<1>();
+      __syncwarp();
+      const char* r = mine + buf * K::STAGE + lane * V * (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        zr[i] = *(const VecOf<T, V>*)(r + i * ROWB);
+        fr[i] = *(const VecOf<T, V>*)(r + (S + i) * ROWB);
+      }
+    } else {
+      static_assert(V == 1, "plain loads take one channel to a lane");
+      T r[S];
+      direct_rows<T>((const T*)p.z + b * p.z_b + pl.c + (long long)tb * p.z_t, p.z_t, n, pl.on, r);
+#pragma unroll
+      for (int i = 0; i < S; ++i) zr[i].v[0] = r[i];
+      if constexpr (MODE == SCAN_DIRECT) {
+        direct_rows<T>((const T*)p.f + b * p.f_b + pl.g + (long long)tb * p.f_t, p.f_t, n, pl.on, r);
+#pragma unroll
+        for (int i = 0; i < S; ++i) fr[i].v[0] = r[i];
+      } else {
+        const int g0 = tile * 32 / p.D, g = g0 + (lane >> 4), i = lane & 15;
+        edge = (g0 + 1) * p.D - tile * 32;
+        const bool ok = g < p.G && i < n;
+        wide = gate_fold<Accurate<T>::value>(
+            ok ? to_f(((const T*)p.f)[b * p.f_b + g + (long long)(tb + i) * p.f_t]) : 0.f);
+      }
+    }
+    if (PACK && tb < p.T) {
+      const size_t row = (size_t)tb * p.B + b;
+      const int groups = (p.N + kQGroup - 1) / kQGroup, grp = tile * V + lane * V / 32;
+      PackOut<V> o;
+      o.qz = p.qz + row * p.N + pl.c; o.qf = p.qf + row * p.N + pl.c;
+      o.ez = p.ez + row * groups + grp; o.ef = p.ef + row * groups + grp;
+      o.stride = p.B * p.N; o.estride = p.B * groups;
+      o.odd = p.odd + ((size_t)(tb / kSeg) * p.B + b) * groups + grp;
+      scan_pack<T, V, S>(zr, fr, o, p.T - tb, pl.on, grp < groups, lane);
+    }
+    float a[S][V], x[S][V];
+    float2 m[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
 #pragma unroll
     for (int i = 0; i < S; ++i) {
+      float w = 0.f;
+      if (MODE == SCAN_WIDE) w = __shfl_sync(0xffffffffu, wide, i + (lane >= edge ? 16 : 0));
 #pragma unroll
-      for (int k = 0; k < V; ++k) r.q[i].v[k] = 0;
-      if (pl.on && tb + i < n) r.q[i] = *(const VecOf<int8_t, V>*)at_step(base, stride, i);
+      for (int k = 0; k < V; ++k) {
+        const float zf = to_f(zr[i].v[k]);
+        float om;
+        if (MODE == SCAN_WIDE) gate_unfold(w, a[i][k], om);
+        else sigmoid_pair<Accurate<T>::value>(to_f(fr[i].v[k]), a[i][k], om);
+        x[i][k] = p.decay_input ? om * zf : zf;
+      }
     }
+    if (n < S) {
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (i >= n) { a[i][k] = 1.f; x[i][k] = 0.f; }
+    }
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if (POS && ((cut >> i) & 1)) m[k] = make_float2(0.f, x[i][k]);
+        else m[k] = make_float2(m[k].x * a[i][k], fmaf(a[i][k], m[k].y, x[i][k]));
+      }
+    if (POS && cut) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) m[k].x = -0.f;
+    }
+    float s[V];
+    scan_exchange<P, V, POS>(sm, buf, warp, lane, rank, csize, m, v, s);
+    if (pl.on && tb < p.T) {
+      if (p.states) {
+        VecOf<float, V> o;
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.v[k] = s[k];
+        *(VecOf<float, V>*)(p.states + ((size_t)(tb / kSeg) * p.B + b) * p.N + pl.c) = o;
+      }
+      T* h = (T*)p.h + b * p.h_b + pl.c + (long long)tb * p.h_t;
+      const int nT = p.T - tb;
+      if (n >= S) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          VecOf<T, V> o;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            s[k] = (POS && ((cut >> i) & 1)) ? x[i][k] : fmaf(a[i][k], s[k], x[i][k]);
+            o.v[k] = from_f<T>(s[k]);
+          }
+          *(VecOf<T, V>*)at_step(h, p.h_t, i) = o;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          VecOf<T, V> o;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            s[k] = (POS && ((cut >> i) & 1)) ? x[i][k] : fmaf(a[i][k], s[k], x[i][k]);
+            o.v[k] = from_f<T>(i < n ? s[k] : 0.f);
+          }
+          if (i < nT) *(VecOf<T, V>*)at_step(h, p.h_t, i) = o;
+        }
+      }
+    }
+    if (nxt.wv == 0 && p.hT && pl.on && rank == 0 && warp == 0) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) p.hT[(size_t)b * p.N + pl.c + k] = v[k];
+    }
+    cur = nxt;
   }
+  if (MODE == SCAN_STAGED) stage_wait<0>();
+  if (csize > 1) cooperative_groups::this_cluster().sync();   // no block leaves while its peers may still write to it
 }
+
+// ---------------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------------
 // A code as a float without its scale: the byte (offset by 128) as the mantissa of 2^23.
-__device__ __forceinline__ float code_value(int8_t q) {
-  return __uint_as_float(0x4b000000u | (uint8_t)(q ^ (int8_t)0x80)) - 8388736.f;
+__device__ __forceinline__ float code_value(unsigned offset_code) {
+  return __uint_as_float(0x4b000000u | offset_code) - 8388736.f;
+}
+
+// What a backward segment reads: z and f as values or codes, g = gh, the scales of the steps
+// spread over the lanes (lane j: step j, or step j / 2 of group j & 1 for V = 2), this lane's
+// share of the gates (WIDE).
+template <class T, int V, bool B8>
+struct ScanIn {
+  RawBytes<(B8 ? 1 : (int)sizeof(T)) * V> z[kSeg], f[kSeg];
+  VecOf<T, V> g[kSeg];
+  float sz, sf, wide;
+  int edge;
+};
+template <class T, int V>
+__device__ __forceinline__ float raw_value(const RawBytes<(int)sizeof(T) * V>& r, int k) {
+  return to_f(((const VecOf<T, V>*)&r)->v[k]);
 }
 
 // The walk of one backward segment in time order: gates w, df factors e, and the segment's map
 // of the reverse recurrence, in forward order: G enters at the end times Pi a, and g_i times
-// the gates up to i.  SLOW: 8-bit codes may stand for infinities and NaN.
-template <class T, int V, bool POS, bool B8, bool SLOW>
-__device__ __forceinline__ float scan_walk(const ScanArgs& p, const VecOf<T, V> (&zr)[kSeg], const VecOf<T, V> (&fr)[kSeg],
-                                           const VecOf<T, V> (&g)[kSeg], const Scan8<V, kSeg>& z8,
-                                           const Scan8<V, kSeg>& f8, unsigned cut, int n, int lane, float (&s)[V],
-                                           float (&w)[kSeg][V], float (&e)[kSeg][V], float2 (&m)[V]) {
-  float top = 0.f;   // the largest code
+// the gates up to i.  PLAIN: all 16 steps are inside the sequence, no code stands for an infinity
+// or NaN.
+template <class T, int V, bool POS, bool B8, int MODE, bool PLAIN>
+__device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, B8>& r, unsigned cut, int n, int lane,
+                                          float (&s)[V], float (&w)[kSeg][V], float (&e)[kSeg][V], float2 (&m)[V]) {
 #pragma unroll
   for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
 #pragma unroll
   for (int i = 0; i < kSeg; ++i) {
-    float sz = 0.f, sf = 0.f;
+    float sz = 0.f, sf = 0.f, ww = 0.f;
     if (B8) {
       const int src = V == 1 ? i : 2 * i + (lane >> 4);
-      sz = __shfl_sync(0xffffffffu, z8.scale, src);
-      sf = __shfl_sync(0xffffffffu, f8.scale, src);
+      sz = __shfl_sync(0xffffffffu, r.sz, src);
+      sf = __shfl_sync(0xffffffffu, r.sf, src);
     }
+    if (MODE == SCAN_WIDE) ww = __shfl_sync(0xffffffffu, r.wide, i + (lane >= r.edge ? 16 : 0));
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      float zf, ff;
-      if (!B8) {
-        zf = to_f(zr[i].v[k]);
-        ff = to_f(fr[i].v[k]);
-      } else if (SLOW) {
-        zf = q_decode(z8.q[i].v[k], sz);
-        ff = q_decode(f8.q[i].v[k], sf);
+      float zf, ff = 0.f;
+      if constexpr (!B8) {
+        zf = raw_value<T, V>(r.z[i], k);
+        if (MODE != SCAN_WIDE) ff = raw_value<T, V>(r.f[i], k);
+      } else if constexpr (!PLAIN) {
+        zf = q_decode((int8_t)r.z[i].b[k], sz);
+        ff = q_decode((int8_t)r.f[i].b[k], sf);
       } else {
-        zf = code_value(z8.q[i].v[k]);
-        ff = code_value(f8.q[i].v[k]);
-        top = fmaxf(top, fmaxf(fabsf(zf), fabsf(ff)));
+        zf = code_value((uint8_t)r.z[i].b[k] ^ 0x80u);
+        ff = code_value((uint8_t)r.f[i].b[k] ^ 0x80u);
         zf *= sz;
         ff *= sf;
       }
-      float big, small;
-      sigmoid_parts<Accurate<T>::value>(ff, big, small);
-      const bool pos = ff >= 0.f;
-      const float a = pos ? big : small, om = pos ? small : big;
-      w[i][k] = pos ? small : -small;
+      float a, om, both;   // both = a (1 - a)
+      if (MODE == SCAN_WIDE) {
+        gate_unfold(ww, a, om);
+        both = a * om;
+        w[i][k] = ww;
+      } else {
+        float big, small;
+        sigmoid_parts<Accurate<T>::value>(ff, big, small);
+        const bool pos = ff >= 0.f;
+        a = pos ? big : small;
+        om = pos ? small : big;
+        both = big * small;
+        w[i][k] = pos ? small : -small;
+      }
       if (POS && ((cut >> i) & 1)) s[k] = 0.f;
-      const float d = p.decay_input ? s[k] - zf : s[k];
-      e[i][k] = big * small * d;
+      e[i][k] = both * (p.decay_input ? s[k] - zf : s[k]);
       s[k] = fmaf(a, s[k], p.decay_input ? om * zf : zf);
       if (POS && (cut & ((2u << i) - 1))) {
         m[k].x = 0.f;
-      } else if (i < n) {
+      } else if (PLAIN || i < n) {
         m[k].x *= a;
-        m[k].y = fmaf(m[k].x, to_f(g[i].v[k]), m[k].y);
+        m[k].y = fmaf(m[k].x, to_f(r.g[i].v[k]), m[k].y);
       }
     }
   }
-  return top;
 }
 
 // The walk back: q is the gradient that enters the segment's last step.  WHOLE: all its
 // steps are inside the sequence.  e[i] becomes df.
-template <class T, int V, bool POS, bool WHOLE>
-__device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const VecOf<T, V> (&g)[kSeg], const float (&w)[kSeg][V],
+template <class T, int V, bool POS, bool WHOLE, class G>
+__device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const G& g, const float (&w)[kSeg][V],
                                                float (&e)[kSeg][V], float (&q)[V], unsigned cut, int n, int nT, T* dz,
                                                T* df) {
 #pragma unroll
   for (int i = kSeg - 1; i >= 0; --i) {
+    const VecOf<T, V> gi = g(i);
     VecOf<T, V> oz, of;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float a, om;
       gate_unfold(w[i][k], a, om);
-      const float G = q[k] + to_f(g[i].v[k]);
-      float dzv = p.decay_input ? om * G : G, dfv = e[i][k] * G;
-      float nq = (POS && ((cut >> i) & 1)) ? 0.f : a * G;
+      const float G_ = q[k] + to_f(gi.v[k]);
+      float dzv = p.decay_input ? om * G_ : G_, dfv = e[i][k] * G_;
+      float nq = (POS && ((cut >> i) & 1)) ? 0.f : a * G_;
       if (!WHOLE && i >= n) { dzv = 0.f; dfv = 0.f; nq = q[k]; }
       q[k] = nq;
       e[i][k] = dfv;
@@ -565,132 +658,197 @@ __device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const VecOf<T,
 }
 
 // B8 (D = 1): z and f come from their 8-bit form.
-template <class T, int V, int P, bool POS, bool B8>
+template <class T, int V, int P, bool B8, int MODE>
+struct ScanBwd {
+  static constexpr int S = kSeg, E = B8 ? 1 : (int)sizeof(T);
+  static constexpr int ROWB = 32 * V * E, ROWG = 32 * V * (int)sizeof(T);   // bytes of a row of z or f, of gh
+  static constexpr int STAGE = MODE == SCAN_STAGED ? S * (2 * ROWB + ROWG) : 0;
+  static constexpr int SMEM = 2 * P * STAGE;
+};
+template <class T, int V, int P, bool POS, bool B8, int MODE>
 __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csize) {
-  constexpr int S = kSeg;
+  using K = ScanBwd<T, V, P, B8, MODE>;
+  using E = std::conditional_t<B8, int8_t, T>;
+  constexpr int S = kSeg, ROWB = K::ROWB, ROWG = K::ROWG;
   __shared__ ScanExchange<P, V> sm;
+  extern __shared__ __align__(16) char stage[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = csize > 1 ? (int)(blockIdx.x % csize) : 0;
   const int wave = P * S * csize, waves = (p.T + wave - 1) / wave;
   // block rank 0, warp 0 hold the wave's last segment: the recurrence runs backward
   const int seg = (csize - 1 - rank) * P + (P - 1 - warp);
   const int items = p.B * p.tiles, step = gridDim.x / csize;
-  int buf = 0;
-  for (int item = blockIdx.x / csize; item < items; item += step) {
-    const int b = item / p.tiles, tile = item - b * p.tiles;
+  const int groups = (p.N + kQGroup - 1) / kQGroup;
+  char* mine = stage + warp * 2 * K::STAGE;
+  // z and f as tensors of E
+  const E* zp = B8 ? (const E*)p.qz : (const E*)p.z;
+  const E* fp = B8 ? (const E*)p.qf : (const E*)p.f;
+  const int z_t = B8 ? p.B * p.N : p.z_t, f_t = B8 ? p.B * p.N : p.f_t;
+  const long long z_b = B8 ? p.N : p.z_b, f_b = B8 ? p.N : p.f_b;
+  float s_ahead[V], sz_ahead = 0.f, sf_ahead = 0.f;
+  int odd_ahead = 0;
+  auto scales = [&](int b, int tile, int tb, int n, float& sz, float& sf, int& odd) {
+    const int i = lane / V, grp = tile * V + lane % V;
+    const bool ok = i < S && i < n && grp < groups;
+    const size_t o = ((size_t)(tb + i) * p.B + b) * groups + grp;
+    sz = ok ? q_scale(p.ez[o]) : 1.f;
+    sf = ok ? q_scale(p.ef[o]) : 1.f;
+    const int g0 = tile * V + (lane & (V - 1));
+    odd = tb < p.T && g0 < groups ? p.odd[((size_t)(tb / kSeg) * p.B + b) * groups + g0] : 0;
+  };
+  auto state = [&](int b, const Place& pl, int tb, float (&s)[V]) {
+    VecOf<float, V> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = 0.f;
+    if (pl.on && tb < p.T) o = *(const VecOf<float, V>*)(p.states + ((size_t)(tb / kSeg) * p.B + b) * p.N + pl.c);
+#pragma unroll
+    for (int k = 0; k < V; ++k) s[k] = o.v[k];
+  };
+  // copies the segment of a cursor into half h of this warp's stage, its state and scales
+  // into registers
+  auto fetch = [&](Cursor c, int h) {
+    if (MODE == SCAN_STAGED && c.item < items) {
+      const int b = c.item / p.tiles, tile = c.item - b * p.tiles, c0 = tile * 32 * V, tb = c.wv * wave + seg * S;
+      const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
+      const int n = len - tb, left = p.N - c0;
+      const unsigned dst = (unsigned)__cvta_generic_to_shared(mine + h * K::STAGE);
+      stage_rows<ROWB>(dst, (const char*)(zp + b * z_b + c0 + (long long)tb * z_t), (long long)z_t * K::E, n,
+                       left * K::E, lane);
+      stage_rows<ROWB>(dst + S * ROWB, (const char*)(fp + b * f_b + c0 + (long long)tb * f_t),
+                       (long long)f_t * K::E, n, left * K::E, lane);
+      stage_rows<ROWG>(dst + 2 * S * ROWB, (const char*)(p.gh ? (const T*)p.gh + b * p.gh_b + c0 + (long long)tb * p.gh_t
+                                                              : (const T*)p.states),
+                       (long long)p.gh_t * (int)sizeof(T), p.gh ? n : 0, left * (int)sizeof(T), lane);
+      state(b, scan_place<V>(p, tile, lane), tb, s_ahead);
+      if (B8) scales(b, tile, tb, n, sz_ahead, sf_ahead, odd_ahead);
+    }
+    if (MODE == SCAN_STAGED) stage_commit();
+  };
+  Cursor cur{(int)blockIdx.x / csize, waves - 1};
+  fetch(cur, 0);
+  float v[V];
+  for (int buf = 0; cur.item < items; buf ^= 1) {
+    Cursor nxt{cur.item, cur.wv - 1};
+    if (nxt.wv < 0) nxt = Cursor{cur.item + step, waves - 1};
+    const int b = cur.item / p.tiles, tile = cur.item - b * p.tiles;
     const Place pl = scan_place<V>(p, tile, lane);
     const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
-    const long long first = (long long)(waves - 1) * wave + (long long)seg * S;
-    const T* z = (const T*)p.z + b * p.z_b + pl.c + first * p.z_t;
-    const T* f = (const T*)p.f + b * p.f_b + pl.g + first * p.f_t;
-    const T* gh = (const T*)p.gh + b * p.gh_b + pl.c + first * p.gh_t;
-    T* dz = (T*)p.dz + b * p.dz_b + pl.c + first * p.dz_t;
-    T* df = (T*)p.df + b * p.df_b + pl.g + first * p.df_t;
-    float v[V];
+    const int tb = cur.wv * wave + seg * S, n = len - tb, nT = p.T - tb;
+    ScanIn<T, V, B8> r;
+    r.sz = sz_ahead; r.sf = sf_ahead; r.wide = 0.f; r.edge = 32;
+    int odd = odd_ahead;
+    float s[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = (pl.on && p.ghT) ? p.ghT[(size_t)b * p.N + pl.c + k] : 0.f;
-    for (int wv = waves - 1; wv >= 0; --wv, buf ^= 1) {
-      const int tb = wv * wave + seg * S;
-      VecOf<T, V> zr[S], fr[S], g[S];
-      Scan8<V, S> z8, f8;
-      if (B8) {
-        scan_load8<V, S>(p, p.qz, p.ez, b, tb, len, tile, pl, lane, z8);
-        scan_load8<V, S>(p, p.qf, p.ef, b, tb, len, tile, pl, lane, f8);
-      } else {
-        scan_load<T, V, S>(z, p.z_t, tb, len, pl.on, zr);
-        scan_load<T, V, S>(f, p.f_t, tb, len, pl.on, fr);
-      }
-      scan_load<T, V, S>(gh, p.gh_t, tb, len, pl.on && p.gh, g);
-      float s[V];
+    for (int k = 0; k < V; ++k) s[k] = s_ahead[k];
+    __syncwarp();   // all lanes are past their reads of the half that is written now
+    fetch(nxt, buf ^ 1);
+    if (cur.wv == waves - 1) {
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        s[k] = (pl.on && tb < p.T) ? p.states[((size_t)(tb / kSeg) * p.B + b) * p.N + pl.c + k] : 0.f;
-      const unsigned cut = POS ? scan_resets<S>(p, b, tb, len, lane) : 0u;
-      if (p.ahead) {
-        // the next wave of this item, or the first of the next one
-        const int ni = wv > 0 ? item : item + step;
-        if (ni < items) {
-          const int nb = ni / p.tiles, nt = ni - nb * p.tiles, tn = (wv > 0 ? wv - 1 : waves - 1) * wave + seg * S;
-          constexpr int R = 32 * V * (int)sizeof(T);
-          if (B8) {
-            const long long o = ((long long)tn * p.B + nb) * p.N + nt * p.cpt;
-            scan_prefetch<S, 32 * V>(p.qz + o, p.B * p.N, p.T - tn, lane);
-            scan_prefetch<S, 32 * V>(p.qf + o, p.B * p.N, p.T - tn, lane);
-          } else {
-            scan_prefetch<S, R>((const T*)p.z + nb * p.z_b + nt * p.cpt + (long long)tn * p.z_t, p.z_t, p.T - tn, lane);
-            scan_prefetch<S, R>((const T*)p.f + nb * p.f_b + nt * p.cpt + (long long)tn * p.f_t, p.f_t, p.T - tn, lane);
-          }
-          if (p.gh)
-            scan_prefetch<S, R>((const T*)p.gh + nb * p.gh_b + nt * p.cpt + (long long)tn * p.gh_t, p.gh_t, p.T - tn,
-                                lane);
-        }
-      }
-      float w[S][V], e[S][V];
-      float2 m[V];
-      const int n = len - tb, nT = p.T - tb;
-      const float top = n >= S ? scan_walk<T, V, POS, B8, false>(p, zr, fr, g, z8, f8, cut, S, lane, s, w, e, m)
-                               : scan_walk<T, V, POS, B8, false>(p, zr, fr, g, z8, f8, cut, n, lane, s, w, e, m);
-      if (B8 && __any_sync(0xffffffffu, top > 126.f)) {
-        // rare: infinities or NaN among the codes; all is read again, so that nothing is kept for it
-        scan_load8<V, S>(p, p.qz, p.ez, b, tb, len, tile, pl, lane, z8);
-        scan_load8<V, S>(p, p.qf, p.ef, b, tb, len, tile, pl, lane, f8);
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          s[k] = (pl.on && tb < p.T) ? p.states[((size_t)(tb / kSeg) * p.B + b) * p.N + pl.c + k] : 0.f;
-        scan_walk<T, V, POS, B8, true>(p, zr, fr, g, z8, f8, cut, n, lane, s, w, e, m);
-      }
-      if (POS && cut) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) m[k].x = -0.f;
-      }
-      float q[V];
-      scan_exchange<P, V, POS>(sm, buf, warp, lane, rank, csize, m, v, q);
-      T* dzp = pl.on ? (T*)p.dz : nullptr;
-      T* dfp = pl.on && p.D == 1 ? (T*)p.df : nullptr;
-      if (dzp) dzp = dz;
-      if (dfp) dfp = df;
-      if (n >= S) scan_walk_back<T, V, POS, true>(p, g, w, e, q, cut, n, nT, dzp, dfp);
-      else scan_walk_back<T, V, POS, false>(p, g, w, e, q, cut, n, nT, dzp, dfp);
-      if (V == 1 && p.D > 1 && p.df) {
-        if (p.split) {
-          // the tile's channels of its first gate, and of the one it reaches into
-          const int g0 = tile * 32 / p.D, edge = (g0 + 1) * p.D - tile * 32;
-          float x[S];
-#pragma unroll
-          for (int i = 0; i < S; ++i) x[i] = pl.on && lane < edge ? e[i][0] : 0.f;
-          const int t = tb + (lane >> 1);
-          const float s0 = warp_sum16(x, lane);
-          float s1 = 0.f;
-          if (edge < 32) {
-#pragma unroll
-            for (int i = 0; i < S; ++i) x[i] = pl.on && lane >= edge ? e[i][0] : 0.f;
-            s1 = warp_sum16(x, lane);
-          }
-          if (t < p.T) p.part[(((size_t)t * p.B + b) * p.tiles + tile) * 2 + (lane & 1)] = lane & 1 ? s1 : s0;
-        } else {
-          const int d = pl.c - pl.g * p.D;
-#pragma unroll
-          for (int i = 0; i < S; ++i) {
-            const float x = gate_sum(pl.on ? e[i][0] : 0.f, d, p.D);
-            if (pl.on && d == 0 && tb + i < p.T) *at_step(df, p.df_t, i) = from_f<T>(x);
-          }
-        }
-      }
-      z -= (long long)wave * p.z_t;
-      f -= (long long)wave * p.f_t;
-      gh -= (long long)wave * p.gh_t;
-      dz -= (long long)wave * p.dz_t;
-      df -= (long long)wave * p.df_t;
+      for (int k = 0; k < V; ++k) v[k] = (pl.on && p.ghT) ? p.ghT[(size_t)b * p.N + pl.c + k] : 0.f;
     }
-    if (p.dh0 && pl.on && rank == 0 && warp == 0) {
+    const unsigned cut = POS ? scan_resets(p, b, tb, len, lane) : 0u;
+    const char* rows = mine + buf * K::STAGE;
+    auto read = [&]() {
+      if constexpr (MODE == SCAN_STAGED) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          r.z[i] = *(const RawBytes<K::E * V>*)(rows + i * ROWB + lane * K::E * V);
+          r.f[i] = *(const RawBytes<K::E * V>*)(rows + (S + i) * ROWB + lane * K::E * V);
+          r.g[i] = *(const VecOf<T, V>*)(rows + 2 * S * ROWB + i * ROWG + lane * V * (int)sizeof(T));
+        }
+      } else {
+        static_assert(V == 1, "plain loads take one channel to a lane");
+        E x[S];
+        direct_rows<E>(zp + b * z_b + pl.c + (long long)tb * z_t, z_t, n, pl.on, x);
+#pragma unroll
+        for (int i = 0; i < S; ++i) memcpy(&r.z[i], &x[i], sizeof(E));
+        if constexpr (MODE == SCAN_DIRECT) {
+          direct_rows<E>(fp + b * f_b + pl.g + (long long)tb * f_t, f_t, n, pl.on, x);
+#pragma unroll
+          for (int i = 0; i < S; ++i) memcpy(&r.f[i], &x[i], sizeof(E));
+        }
+        T y[S];
+        direct_rows<T>((const T*)p.gh + b * p.gh_b + pl.c + (long long)tb * p.gh_t, p.gh_t, n, pl.on && p.gh, y);
+#pragma unroll
+        for (int i = 0; i < S; ++i) r.g[i].v[0] = y[i];
+      }
+    };
+    if (MODE == SCAN_STAGED) {
+      stage_wait<1>();
+      __syncwarp();
+    }
+    read();
+    if (MODE != SCAN_STAGED) {
+      state(b, pl, tb, s);
+      if (B8) scales(b, tile, tb, n, r.sz, r.sf, odd);
+    }
+    odd = B8 ? __any_sync(0xffffffffu, odd) : 0;
+    if constexpr (MODE == SCAN_WIDE) {
+      const int g0 = tile * 32 / p.D, g = g0 + (lane >> 4), i = lane & 15;
+      r.edge = (g0 + 1) * p.D - tile * 32;
+      const bool ok = g < p.G && i < n;
+      r.wide = gate_fold<Accurate<T>::value>(
+          ok ? to_f(((const T*)p.f)[b * p.f_b + g + (long long)(tb + i) * p.f_t]) : 0.f);
+    }
+    float w[S][V], e[S][V];
+    float2 m[V];
+    if (n >= S && !odd) scan_walk<T, V, POS, B8, MODE, true>(p, r, cut, n, lane, s, w, e, m);
+    else scan_walk<T, V, POS, B8, MODE, false>(p, r, cut, n, lane, s, w, e, m);
+    if (POS && cut) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) m[k].x = -0.f;
+    }
+    float q[V];
+    scan_exchange<P, V, POS>(sm, buf, warp, lane, rank, csize, m, v, q);
+    T* dz = pl.on && p.dz ? (T*)p.dz + b * p.dz_b + pl.c + (long long)tb * p.dz_t : nullptr;
+    T* df = pl.on && p.df && p.D == 1 ? (T*)p.df + b * p.df_b + pl.c + (long long)tb * p.df_t : nullptr;
+    // staged rows are read again rather than kept
+    auto g = [&](int i) -> VecOf<T, V> {
+      if constexpr (MODE == SCAN_STAGED)
+        return *(const VecOf<T, V>*)(rows + 2 * S * ROWB + i * ROWG + lane * V * (int)sizeof(T));
+      else
+        return r.g[i];
+    };
+    if (n >= S) scan_walk_back<T, V, POS, true>(p, g, w, e, q, cut, n, nT, dz, df);
+    else scan_walk_back<T, V, POS, false>(p, g, w, e, q, cut, n, nT, dz, df);
+    if constexpr (MODE == SCAN_WIDE) {
+      if (p.df) {
+        // the tile's channels of its first gate, and of the one it reaches into
+        float x[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) x[i] = pl.on && lane < r.edge ? e[i][0] : 0.f;
+        const int t = tb + (lane >> 1);
+        const float s0 = warp_sum16(x, lane);
+        float s1 = 0.f;
+        if (r.edge < 32) {
+#pragma unroll
+          for (int i = 0; i < S; ++i) x[i] = pl.on && lane >= r.edge ? e[i][0] : 0.f;
+          s1 = warp_sum16(x, lane);
+        }
+        if (t < p.T) p.part[(((size_t)t * p.B + b) * p.tiles + tile) * 2 + (lane & 1)] = lane & 1 ? s1 : s0;
+      }
+    } else if constexpr (MODE == SCAN_DIRECT && !B8) {
+      if (p.D > 1 && p.df) {
+        T* o = (T*)p.df + b * p.df_b + pl.g + (long long)tb * p.df_t;
+        const int d = pl.c - pl.g * p.D;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const float x = gate_sum(pl.on ? e[i][0] : 0.f, d, p.D);
+          if (pl.on && d == 0 && i < nT) *at_step(o, p.df_t, i) = from_f<T>(x);
+        }
+      }
+    }
+    if (nxt.wv == waves - 1 && p.dh0 && pl.on && rank == 0 && warp == 0) {
 #pragma unroll
       for (int k = 0; k < V; ++k) p.dh0[(size_t)b * p.N + pl.c + k] = v[k];
     }
+    cur = nxt;
   }
+  if (MODE == SCAN_STAGED) stage_wait<0>();
   if (csize > 1) cooperative_groups::this_cluster().sync();
 }
 
-// df[t,b,g] = the sums of the tiles that gate g spans (D > 32), in order
+// df[t,b,g] = the sums of the tiles that gate g spans (D >= 32), in order
 template <class T>
 __global__ void k_scan_df_sum(ScanArgs p) {
   const size_t n = (size_t)p.T * p.B * p.G;

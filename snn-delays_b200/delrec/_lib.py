@@ -108,9 +108,9 @@ _SIGS = {
     "delrec_readout_sum_backward": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
     "delrec_exchange_floor_workspace": (_S, [_P]),
     "delrec_exchange_floor": (_I, [_P, _P, _S, _P]),
-    "delrec_gated_scan_forward": (_I, [_P] * 14),
+    "delrec_gated_scan_forward": (_I, [_P] * 15),
     "delrec_gated_scan_backward_workspace": (_S, [_P]),
-    "delrec_gated_scan_backward": (_I, [_P] * 16 + [_S, _P]),
+    "delrec_gated_scan_backward": (_I, [_P] * 17 + [_S, _P]),
     "delrec_gated_step": (_I, [_P] * 8),
     "delrec_block_norm_forward": (_I, [_P] * 13),
     "delrec_block_norm_backward_workspace": (_S, [_P]),

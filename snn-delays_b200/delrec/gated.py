@@ -59,16 +59,17 @@ class GatedScan(torch.autograd.Function):
                       *z.stride()[:2], *f.stride()[:2], *h.stride()[:2])
         states = torch.empty(-(-T // SEGMENT), B, N, device=dev) if train else None
         keep8 = bool(checkpoint8) and train
-        pz = pf = None
+        pz = pf = odd = None
         if keep8 and G == N:
             pz, pf = empty8(z.shape, z.dtype, dev), empty8(f.shape, f.dtype, dev)
+            odd = torch.empty(*states.shape[:2], pz.e.shape[-1], dtype=torch.uint8, device=dev)
         if T and B and N:
             with _lib.on_device(z):
                 _lib.check(_lib.lib().delrec_gated_scan_forward(
                     ctypes.byref(s), z.data_ptr(), f.data_ptr(), _lib.addr(h0), _lib.addr(lengths),
                     _lib.addr(resets), h.data_ptr(), hT.data_ptr(), _lib.addr(states),
                     _lib.addr(pz and pz.q), _lib.addr(pz and pz.e), _lib.addr(pf and pf.q),
-                    _lib.addr(pf and pf.e), _lib.stream_ptr(dev)), "delrec_gated_scan_forward")
+                    _lib.addr(pf and pf.e), _lib.addr(odd), _lib.stream_ptr(dev)), "delrec_gated_scan_forward")
         elif h0 is not None:
             hT.copy_(h0.detach())
         else:
@@ -78,7 +79,7 @@ class GatedScan(torch.autograd.Function):
         if keep8:
             if pz is None:   # a shared gate is small against its channels: packed apart
                 pz, pf = pack8(z), pack8(f)
-            ctx.save_for_backward(pz.q, pz.e, pf.q, pf.e, states, lengths, resets)
+            ctx.save_for_backward(pz.q, pz.e, pf.q, pf.e, odd, states, lengths, resets)
         else:
             ctx.save_for_backward(z, f, states, lengths, resets)
         ctx.scan, ctx.keep8, ctx.dtype = s, keep8, z.dtype
@@ -88,9 +89,9 @@ class GatedScan(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gh, ghT):
-        z = f = pz = pf = None
+        z = f = pz = pf = odd = None
         if ctx.keep8:
-            qz, ez, qf, ef, states, lengths, resets = ctx.saved_tensors
+            qz, ez, qf, ef, odd, states, lengths, resets = ctx.saved_tensors
             pz, pf = Packed8(qz, ez, ctx.dtype), Packed8(qf, ef, ctx.dtype)
             if ctx.scan.G != ctx.scan.N:    # the 8-bit kernel is for a gate per channel
                 z, f, pz, pf = unpack8(pz), unpack8(pf), None, None
@@ -123,7 +124,7 @@ class GatedScan(torch.autograd.Function):
             with _lib.on_device(like_z):
                 _lib.check(lib.delrec_gated_scan_backward(
                     ctypes.byref(s), _lib.addr(z), _lib.addr(f), _lib.addr(pz and pz.q), _lib.addr(pz and pz.e),
-                    _lib.addr(pf and pf.q), _lib.addr(pf and pf.e), _lib.addr(lengths), _lib.addr(resets),
+                    _lib.addr(pf and pf.q), _lib.addr(pf and pf.e), _lib.addr(odd), _lib.addr(lengths), _lib.addr(resets),
                     states.data_ptr(), _lib.addr(gh), _lib.addr(ghT), _lib.addr(dz), _lib.addr(df),
                     _lib.addr(dh0), _lib.addr(ws), nbytes, _lib.stream_ptr(dev)), "delrec_gated_scan_backward")
         elif dh0 is not None:

@@ -82,24 +82,24 @@ def test_c_entry_points_reject_bad_arguments():
     lib = _lib.lib()
     p = _fake()
 
-    def fwd(s, z=p, f=p, h=p, q=(None,) * 4):
+    def fwd(s, z=p, f=p, h=p, q=(None,) * 5):
         return lib.delrec_gated_scan_forward(s and ctypes.byref(s), z, f, None, None, None, h, None, None, *q, None)
 
     assert fwd(None) == 1
     for bad in (dict(T=0), dict(B=0), dict(N=0), dict(G=0), dict(G=3), dict(dtype=3), dict(dtype=-1), dict(T=-4)):
         assert fwd(_scan(**bad)) == 1
     assert fwd(_scan(), z=None) == 1 and fwd(_scan(), f=None) == 1 and fwd(_scan(), h=None) == 1
-    assert fwd(_scan(), q=(p, None, p, p)) == 1                 # half of a packed pair
-    assert fwd(_scan(G=4), q=(p, p, p, p)) == 1                 # packing here is for a gate per channel
+    assert fwd(_scan(), q=(p, None, p, p, p)) == 1                 # half of a packed pair
+    assert fwd(_scan(G=4), q=(p, p, p, p, p)) == 1                 # packing here is for a gate per channel
     assert fwd(_scan(T=(1 << 30) + 1)) == 4
     assert fwd(_scan(B=1 << 27, N=1024, G=1024)) == 4           # more rows than a grid holds
 
-    def bwd(s, z=p, f=p, qz=None, ez=None, qf=None, ef=None, states=p, ws=p, n=1 << 20):
-        return lib.delrec_gated_scan_backward(ctypes.byref(s), z, f, qz, ez, qf, ef, None, None, states, p, None, p,
-                                              p, None, ws, n, None)
+    def bwd(s, z=p, f=p, qz=None, ez=None, qf=None, ef=None, odd=None, states=p, ws=p, n=1 << 20):
+        return lib.delrec_gated_scan_backward(ctypes.byref(s), z, f, qz, ez, qf, ef, odd, None, None, states, p, None,
+                                              p, p, None, ws, n, None)
 
     assert bwd(_scan(), states=None) == 1 and bwd(_scan(), z=None) == 1 and bwd(_scan(), qz=p) == 1
-    assert bwd(_scan(), qf=p, ef=p) == 1 and bwd(_scan(G=4), qz=p, ez=p, qf=p, ef=p) == 1
+    assert bwd(_scan(), qf=p, ef=p) == 1 and bwd(_scan(G=4), qz=p, ez=p, qf=p, ef=p, odd=p) == 1
     strided = _scan()
     strided.z_t = 1 << 31
     assert fwd(strided) == 4 and bwd(strided) == 4
