@@ -55,35 +55,111 @@ __device__ __forceinline__ __half q_store<__half>(float v, int q) {
   return __float2half_rn(q >= 127 || q <= -127 ? v : fminf(fmaxf(v, -65504.f), 65504.f));
 }
 
-// x (rows, N) contiguous -> q (rows, N), e (rows, ceil(N / 32)): a warp per group, a lane
-// per channel.
-template <class T>
-__global__ void __launch_bounds__(256) k_pack8(long long groups, int gpr, int N, const T* __restrict__ x,
-                                               int8_t* __restrict__ q, uint8_t* __restrict__ e) {
+// x (rows, N) contiguous <-> q (rows, N), e (rows, ceil(N / 32)).  A thread takes V consecutive
+// channels of a row (16 bytes of x where rows allow it), so 32 / V lanes hold a group; a
+// block covers whole rows of threads side by side (span = lanes of a row, rounded up to whole
+// groups), or walks along rows wider than a block, and steps down the rows without divisions, U
+// rows in flight.  HBM bounds both: x once, q and e once.
+struct Q8Args {
+  long long rows;
+  int N, gpr, span, rpb;   // groups and lanes of a row, rows side by side in a block
+  const void* x;
+  void* out;
+  int8_t* q;
+  uint8_t* e;
+};
+template <int V>
+__device__ __forceinline__ unsigned group_mask(int lane) {
+  constexpr int L = 32 / V;
+  return V == 1 ? 0xffffffffu : ((1u << L) - 1u) << (lane & ~(L - 1));
+}
+
+template <class T, int V>
+__global__ void __launch_bounds__(512) k_pack8(Q8Args p) {
+  constexpr int L = 32 / V, U = V == 1 ? 2 : 4;
   const int lane = threadIdx.x & 31;
-  const long long stride = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long g = blockIdx.x * (long long)(blockDim.x >> 5) + (threadIdx.x >> 5); g < groups; g += stride) {
-    const long long row = g / gpr;
-    const int c = (int)(g - row * gpr) * kQGroup + lane;
-    const bool on = c < N;
-    const float v = on ? to_f(x[row * N + c]) : 0.f;
-    const unsigned ex = q_exponent(__reduce_max_sync(0xffffffffu, q_magnitude(v)));
-    if (on) q[row * N + c] = (int8_t)q_encode(v, q_inverse_scale(ex));
-    if (lane == 0) e[g] = (uint8_t)ex;
+  const unsigned mask = group_mask<V>(lane);
+  const int sub = threadIdx.x / p.span;
+  const long long step = (long long)gridDim.x * p.rpb;
+  for (int l = threadIdx.x - sub * p.span; l < p.span; l += blockDim.x) {
+    const int c = l * V;
+    const bool on = c < p.N;
+    for (long long r0 = blockIdx.x * (long long)p.rpb + sub; r0 < p.rows; r0 += U * step) {
+      VecOf<T, V> raw[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const long long r = r0 + j * step;
+#pragma unroll
+        for (int k = 0; k < V; ++k) raw[j].v[k] = from_f<T>(0.f);
+        if (on && r < p.rows) raw[j] = *(const VecOf<T, V>*)((const T*)p.x + r * p.N + c);
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const long long r = r0 + j * step;
+        if (r >= p.rows) break;     // the same for the lanes of a group
+        unsigned top = 0;
+#pragma unroll
+        for (int k = 0; k < V; ++k) top = max(top, __float_as_uint(to_f(raw[j].v[k])) & 0x7fffffffu);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+        unsigned ex, code[V];
+        if (top < __float_as_uint(kQLargest)) {
+          // the sum's low byte is rint(x / s): the quotient is exact, the addition rounds
+          ex = q_exponent(top);
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            code[k] = __float_as_uint(fmaf(to_f(raw[j].v[k]), q_inverse_scale(ex), 12582912.f));
+        } else {
+          top = 0;
+#pragma unroll
+          for (int k = 0; k < V; ++k) top = max(top, q_magnitude(to_f(raw[j].v[k])));
+#pragma unroll
+          for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+          ex = q_exponent(top);
+#pragma unroll
+          for (int k = 0; k < V; ++k) code[k] = (unsigned)q_encode(to_f(raw[j].v[k]), q_inverse_scale(ex));
+        }
+        if (on) {
+          VecOf<int8_t, V> o;
+#pragma unroll
+          for (int k = 0; k < V; ++k) o.v[k] = (int8_t)code[k];
+          *(VecOf<int8_t, V>*)(p.q + r * p.N + c) = o;
+          if (c % kQGroup == 0) p.e[r * p.gpr + c / kQGroup] = (uint8_t)ex;
+        }
+      }
+    }
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) k_unpack8(long long groups, int gpr, int N, const int8_t* __restrict__ q,
-                                                 const uint8_t* __restrict__ e, T* __restrict__ x) {
-  const int lane = threadIdx.x & 31;
-  const long long stride = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long g = blockIdx.x * (long long)(blockDim.x >> 5) + (threadIdx.x >> 5); g < groups; g += stride) {
-    const long long row = g / gpr;
-    const int c = (int)(g - row * gpr) * kQGroup + lane;
-    if (c < N) {
-      const int v = q[row * N + c];
-      x[row * N + c] = q_store<T>(q_decode(v, q_scale(e[g])), v);
+template <class T, int V>
+__global__ void __launch_bounds__(512) k_unpack8(Q8Args p) {
+  constexpr int U = V == 1 ? 2 : 4;
+  const int sub = threadIdx.x / p.span;
+  const long long step = (long long)gridDim.x * p.rpb;
+  for (int l = threadIdx.x - sub * p.span; l < p.span; l += blockDim.x) {
+    const int c = l * V;
+    if (c >= p.N) continue;
+    for (long long r0 = blockIdx.x * (long long)p.rpb + sub; r0 < p.rows; r0 += U * step) {
+      VecOf<int8_t, V> raw[U];
+      uint8_t e[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const long long r = r0 + j * step;
+        if (r < p.rows) {
+          raw[j] = *(const VecOf<int8_t, V>*)(p.q + r * p.N + c);
+          e[j] = p.e[r * p.gpr + c / kQGroup];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const long long r = r0 + j * step;
+        if (r >= p.rows) break;
+        const float s = q_scale(e[j]);
+        VecOf<T, V> o;
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.v[k] = q_store<T>(q_decode(raw[j].v[k], s), raw[j].v[k]);
+        *(VecOf<T, V>*)((T*)p.out + r * p.N + c) = o;
+      }
     }
   }
 }

@@ -77,6 +77,21 @@ struct Accurate {
   static constexpr bool value = sizeof(T) == 4;
 };
 
+// A gate as one register: the smaller of a and 1 - a, signed as f.  The larger is 1 - |w|,
+// to one rounding.
+template <bool ACCURATE>
+__device__ __forceinline__ float gate_fold(float f) {
+  float big, small;
+  sigmoid_parts<ACCURATE>(f, big, small);
+  return f >= 0.f ? small : -small;
+}
+__device__ __forceinline__ void gate_unfold(float w, float& a, float& om) {
+  const float s = fabsf(w), l = 1.f - s;
+  const bool pos = !(__float_as_uint(w) >> 31);
+  a = pos ? l : s;
+  om = pos ? s : l;
+}
+
 // V consecutive elements as one aligned access
 template <class T, int V>
 struct alignas(sizeof(T) * V) VecOf {

@@ -18,7 +18,10 @@ static int check_block(const delrec_block* s) {
   if (s->dtype < DELREC_F32 || s->dtype > DELREC_F16 || s->gate < GATE_NONE || s->gate > GATE_SILU)
     return DELREC_ERR_ARG;
   if (!(s->eps > 0.f)) return DELREC_ERR_ARG;
-  if (s->N > kNormMax) return DELREC_ERR_UNSUPPORTED;
+  if (s->N > kNormMax || (long long)s->T * s->B > 0x7fffffffLL - kSeqSMs * 16) return DELREC_ERR_UNSUPPORTED;
+  for (long long st : {s->x_t, s->x_b, s->y_t, s->y_b, s->u_t, s->u_b, s->o_t, s->o_b, s->n_t, s->n_b, s->gx_t,
+                       s->gx_b, s->gn_t, s->gn_b, s->dx_t, s->dx_b, s->dy_t, s->dy_b, s->du_t, s->du_b})
+    if (st < -0x7fffffffLL || st > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   return DELREC_OK;
 }
 
@@ -40,60 +43,97 @@ struct NormAlign {
 };
 
 struct NormShape {
-  int V, IT, threads, grid;
+  int V, IT, threads;
+  int grid;   // blocks launched, set by the launch
 };
-static NormShape norm_shape(int N, long long rows, int V, int most_threads) {
-  NormShape s;
+static NormShape norm_shape(int N, int V, int most_threads) {
+  NormShape s{};
   s.V = V;
   const int vecs = (N + V - 1) / V;
   s.IT = 1;
   while ((vecs + s.IT - 1) / s.IT > most_threads) s.IT *= 2;   // N <= 16384: at most 32 elements a thread
   s.threads = ((vecs + s.IT - 1) / s.IT + 31) / 32 * 32;
-  const int per_sm = std::max(1, std::min(16, 1024 / s.threads));
-  s.grid = (int)std::min<long long>(rows, (long long)kSeqSMs * per_sm);
   return s;
 }
-
-using NormKernel = void (*)(NormArgs);
-template <class T, int V, bool BWD, bool GATE, int IT = 1>
-static NormKernel norm_kernel(int it) {
-  if constexpr (V * IT <= 32) {
-    if (it == IT) return BWD ? k_norm_bwd<T, V, IT, GATE> : k_norm_fwd<T, V, IT, GATE>;
-    return norm_kernel<T, V, BWD, GATE, 2 * IT>(it);
-  }
-  return nullptr;
-}
-template <class T, int V, bool BWD>
-static int norm_launch(NormArgs a, int gate, const NormShape& s, cudaStream_t st) {
-  NormKernel k = gate == GATE_NONE ? norm_kernel<T, V, BWD, false>(s.IT) : norm_kernel<T, V, BWD, true>(s.IT);
-  if (!k) return DELREC_ERR_UNSUPPORTED;
-  a.kind = gate;
-  k<<<s.grid, s.threads, 0, st>>>(a);
-  SQ_LAUNCHED();
-  return DELREC_OK;
-}
-// the widest access the tensors allow, 16 bytes at most
-template <class T, bool BWD>
-static int norm_run(const NormArgs& a, int gate, const NormShape& s, cudaStream_t st) {
-  constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
-  if (s.V == V16) return norm_launch<T, V16, BWD>(a, gate, s, st);
-  if (s.V == V8) return norm_launch<T, V8, BWD>(a, gate, s, st);
-  return norm_launch<T, 1, BWD>(a, gate, s, st);
-}
-static int norm_width(const NormAlign& al) { return al.ok[1] ? 16 / al.esz : (al.ok[0] ? 8 / al.esz : 1); }
 static int norm_most_blocks(const delrec_block* s) {
   return (int)std::min<long long>((long long)s->T * s->B, (long long)kSeqSMs * 16);
 }
 static size_t norm_bwd_ws(const delrec_block* s) { return (size_t)norm_most_blocks(s) * 2 * s->N * sizeof(float); }
 
+// as many blocks as fit at once: each walks its rows
+template <class K>
+static int norm_start(K kern, int row_bytes, const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
+  const int smem = 2 * row_bytes * s.threads;
+  if (smem > 40 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  int per_sm = 0;
+  SQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem));
+  s.grid = std::min(most, std::max(1, std::min(per_sm, 16)) * kSeqSMs);
+  kern<<<s.grid, s.threads, smem, st>>>(a);
+  SQ_LAUNCHED();
+  return DELREC_OK;
+}
+template <class T, int V, bool BWD, bool GATE, int IT = 1>
+static int norm_by_it(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
+  if constexpr (V * IT <= 32) {
+    if (s.IT != IT) return norm_by_it<T, V, BWD, GATE, 2 * IT>(a, s, most, st);
+    if constexpr (BWD)
+      return norm_start(k_norm_bwd<T, V, IT, GATE>, NormStage<T, V, IT, GATE ? 5 : 4>::ROW, a, s, most, st);
+    else
+      return norm_start(k_norm_fwd<T, V, IT, GATE>, NormStage<T, V, IT, GATE ? 3 : 2>::ROW, a, s, most, st);
+  }
+  return DELREC_ERR_UNSUPPORTED;
+}
+template <class T, int V, bool BWD>
+static int norm_by_gate(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
+  return a.kind == GATE_NONE ? norm_by_it<T, V, BWD, false>(a, s, most, st) : norm_by_it<T, V, BWD, true>(a, s, most, st);
+}
+// the widest access the tensors allow, 16 bytes at most
+template <class T, bool BWD>
+static int norm_run(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
+  constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
+  if (s.V == V16) return norm_by_gate<T, V16, BWD>(a, s, most, st);
+  if (s.V == V8) return norm_by_gate<T, V8, BWD>(a, s, most, st);
+  return norm_by_gate<T, 1, BWD>(a, s, most, st);
+}
+static int norm_width(const NormAlign& al) { return al.ok[1] ? 16 / al.esz : (al.ok[0] ? 8 / al.esz : 1); }
+
 static NormArgs norm_args(const delrec_block* s) {
   NormArgs a{};
   a.T = s->T; a.B = s->B; a.N = s->N; a.wide = s->lengths_wide; a.eps = s->eps;
-  a.x_t = s->x_t; a.x_b = s->x_b; a.y_t = s->y_t; a.y_b = s->y_b; a.u_t = s->u_t; a.u_b = s->u_b;
-  a.o_t = s->o_t; a.o_b = s->o_b; a.n_t = s->n_t; a.n_b = s->n_b;
-  a.gx_t = s->gx_t; a.gx_b = s->gx_b; a.gn_t = s->gn_t; a.gn_b = s->gn_b;
-  a.dx_t = s->dx_t; a.dx_b = s->dx_b; a.dy_t = s->dy_t; a.dy_b = s->dy_b; a.du_t = s->du_t; a.du_b = s->du_b;
+  a.x_t = (int)s->x_t; a.x_b = (int)s->x_b; a.y_t = (int)s->y_t; a.y_b = (int)s->y_b; a.u_t = (int)s->u_t; a.u_b = (int)s->u_b;
+  a.o_t = (int)s->o_t; a.o_b = (int)s->o_b; a.n_t = (int)s->n_t; a.n_b = (int)s->n_b;
+  a.gx_t = (int)s->gx_t; a.gx_b = (int)s->gx_b; a.gn_t = (int)s->gn_t; a.gn_b = (int)s->gn_b;
+  a.dx_t = (int)s->dx_t; a.dx_b = (int)s->dx_b; a.dy_t = (int)s->dy_t; a.dy_b = (int)s->dy_b; a.du_t = (int)s->du_t; a.du_b = (int)s->du_b;
   return a;
+}
+
+// --------------------------------------------------------------------------------
+// 8-bit checkpoints
+// --------------------------------------------------------------------------------
+template <class T, int V, bool PACK>
+static int q8_launch(Q8Args a, cudaStream_t st) {
+  constexpr int L = 32 / V, most = 512;
+  a.gpr = (a.N + kQGroup - 1) / kQGroup;
+  a.span = a.gpr * L;
+  a.rpb = std::max(1, most / a.span);
+  const int threads = std::min(most, a.span * a.rpb);
+  const long long blocks = (a.rows + a.rpb - 1) / a.rpb;
+  const int grid = (int)std::min<long long>(blocks, (long long)kSeqSMs * 4);
+  if (PACK) k_pack8<T, V><<<grid, threads, 0, st>>>(a);
+  else k_unpack8<T, V><<<grid, threads, 0, st>>>(a);
+  SQ_LAUNCHED();
+  return DELREC_OK;
+}
+// 16 bytes of x a thread where every row is so aligned, 8 of a 16-bit type, else one value
+template <class T, bool PACK>
+static int q8_run(const Q8Args& a, const void* x, cudaStream_t st) {
+  constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
+  const auto fits = [&](int V) {
+    return a.N % V == 0 && (uintptr_t)x % (V * sizeof(T)) == 0 && (uintptr_t)a.q % V == 0;
+  };
+  if (fits(V16)) return q8_launch<T, V16, PACK>(a, st);
+  if (fits(V8)) return q8_launch<T, V8, PACK>(a, st);
+  return q8_launch<T, 1, PACK>(a, st);
 }
 
 }  // namespace delrec
@@ -120,9 +160,10 @@ int delrec_block_norm_forward(const delrec_block* s, const void* x, const void* 
     al.add(out, s->o_t, s->o_b);
     if (gate != GATE_NONE) al.add(u, s->u_t, s->u_b);
   }
-  const NormShape sh = norm_shape(s->N, (long long)s->T * s->B, norm_width(al), kNormThreads);
+  NormShape sh = norm_shape(s->N, norm_width(al), kNormThreads);
+  a.kind = gate;
   return by_dtype(s->dtype, [&](auto t) {
-    return norm_run<decltype(t), false>(a, gate, sh, (cudaStream_t)stream);
+    return norm_run<decltype(t), false>(a, sh, norm_most_blocks(s), (cudaStream_t)stream);
   });
 }
 
@@ -155,11 +196,12 @@ int delrec_block_norm_backward(const delrec_block* s, const void* x, const void*
       al.add(du, s->du_t, s->du_b);
     }
   }
-  const NormShape sh = norm_shape(s->N, (long long)s->T * s->B, norm_width(al), kNormThreads);
+  NormShape sh = norm_shape(s->N, norm_width(al), kNormThreads);
+  a.kind = gate;
   const cudaStream_t st = (cudaStream_t)stream;
-  const int r = by_dtype(s->dtype, [&](auto t) { return norm_run<decltype(t), true>(a, gate, sh, st); });
+  const int r = by_dtype(s->dtype, [&](auto t) { return norm_run<decltype(t), true>(a, sh, norm_most_blocks(s), st); });
   if (r || !sums) return r;
-  k_norm_dw<<<(s->N + 31) / 32, 256, 0, st>>>(s->N, sh.grid, (const float*)ws, w, scale, dw, dscale, dnext_w);
+  k_norm_dw<<<dim3((s->N + 31) / 32, dnext_w ? 2 : 1), 1024, 0, st>>>(s->N, sh.grid, (const float*)ws, w, scale, dw, dscale, dnext_w);
   SQ_LAUNCHED();
   return DELREC_OK;
 }
@@ -167,27 +209,17 @@ int delrec_block_norm_backward(const delrec_block* s, const void* x, const void*
 int delrec_pack8(long long rows, int N, int dtype, const void* x, int8_t* q, uint8_t* e, void* stream) {
   if (rows < 0 || N < 1 || rows > (1LL << 62) / N || !x || !q || !e) return DELREC_ERR_ARG;
   if (rows == 0) return DELREC_OK;
-  const int gpr = (N + kQGroup - 1) / kQGroup;
-  const long long groups = rows * gpr;
-  return by_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    k_pack8<T><<<seq_grid((size_t)groups, 8, 16), 256, 0, (cudaStream_t)stream>>>(groups, gpr, N, (const T*)x, q, e);
-    SQ_LAUNCHED();
-    return (int)DELREC_OK;
-  });
+  Q8Args a{};
+  a.rows = rows; a.N = N; a.x = x; a.q = q; a.e = e;
+  return by_dtype(dtype, [&](auto t) { return q8_run<decltype(t), true>(a, x, (cudaStream_t)stream); });
 }
 
 int delrec_unpack8(long long rows, int N, int dtype, const int8_t* q, const uint8_t* e, void* x, void* stream) {
   if (rows < 0 || N < 1 || rows > (1LL << 62) / N || !x || !q || !e) return DELREC_ERR_ARG;
   if (rows == 0) return DELREC_OK;
-  const int gpr = (N + kQGroup - 1) / kQGroup;
-  const long long groups = rows * gpr;
-  return by_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    k_unpack8<T><<<seq_grid((size_t)groups, 8, 16), 256, 0, (cudaStream_t)stream>>>(groups, gpr, N, q, e, (T*)x);
-    SQ_LAUNCHED();
-    return (int)DELREC_OK;
-  });
+  Q8Args a{};
+  a.rows = rows; a.N = N; a.out = x; a.q = const_cast<int8_t*>(q); a.e = const_cast<uint8_t*>(e);
+  return by_dtype(dtype, [&](auto t) { return q8_run<decltype(t), false>(a, x, (cudaStream_t)stream); });
 }
 
 }  // extern "C"
