@@ -174,15 +174,15 @@ def stream_ptr(device=None):
 SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def require_sequence(*tensors):
-    """The dtype code of the first tensor; raises unless all are CUDA tensors of a type the
-    sequence operators take."""
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError("delrec_b200 runs on CUDA tensors only (there is no CPU path)")
-        if t.dtype not in SEQ_DTYPES:
-            raise RuntimeError(f"delrec_b200 expects float32, bfloat16 or float16 tensors, got {t.dtype}")
-    return SEQ_DTYPES[tensors[0].dtype]
+def require_sequence(t):
+    """The dtype code of t; raises unless it is a CUDA tensor of a type the sequence operators
+    take."""
+    if not t.is_cuda:
+        raise RuntimeError("delrec_b200 runs on CUDA tensors only (there is no CPU path)")
+    code = SEQ_DTYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"delrec_b200 expects float32, bfloat16 or float16 tensors, got {t.dtype}")
+    return code
 
 
 def require_lengths(lengths, B, device):
@@ -198,29 +198,29 @@ def rows(t):
 
 def empty_rows(like, dtype=None):
     """An output shaped like ``like`` with contiguous channels: its layout where that is dense."""
-    r = torch.empty_like(like, dtype=dtype)
-    return r if r.stride(-1) == 1 or r.shape[-1] <= 1 else torch.empty(like.shape, dtype=dtype or like.dtype,
-                                                                       device=like.device)
+    r = torch.empty_like(like) if dtype is None else torch.empty_like(like, dtype=dtype)
+    return r if r.stride(-1) == 1 or r.shape[-1] <= 1 else torch.empty(r.shape, dtype=r.dtype, device=r.device)
 
 
 def addr(t):
     return None if t is None else t.data_ptr()
 
 
-class on_device:
-    """Makes a tensor's device current where it is not, for the launches inside."""
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, t):
-        index = t.device.index
-        self.guard = None if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def launch(what, device, *args):
+    """Calls the C entry point ``what`` with args and the current stream of ``device``, which
+    is made the current device where it is not."""
+    index = device.index
+    fn = getattr(_lib or lib(), what)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
 def scratch(nbytes, device):

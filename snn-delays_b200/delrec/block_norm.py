@@ -23,11 +23,31 @@ from . import _lib
 GATES = {"none": 0, "sigmoid": 1, "silu": 2}
 
 
-def _strides(b, **tensors):
-    for name, t in tensors.items():
-        if t is not None:
-            setattr(b, name + "_t", t.stride(0))
-            setattr(b, name + "_b", t.stride(1))
+def _strides(*tensors):
+    r = []
+    for t in tensors:
+        r += t.stride()[:2] if t is not None else (0, 0)
+    return r
+
+
+def _wide(lengths):
+    return 1 if lengths is not None and lengths.dtype == torch.int64 else 0
+
+
+def _forward(x, y, u, w, scale, nw, lengths, kind, eps, has_next, train):
+    """(x', n, 1/rms of y, 1/rms of x'), None where there is none: one launch."""
+    T, B, N = x.shape
+    dev = x.device
+    out = _lib.empty_rows(x) if y is not None else None
+    n = _lib.empty_rows(x) if has_next else None
+    ry = torch.empty(T, B, device=dev) if train and y is not None else None
+    rx = torch.empty(T, B, device=dev) if train and has_next else None
+    if T and B and N:
+        b = _lib.Block(T, B, N, _lib.SEQ_DTYPES[x.dtype], kind, _wide(lengths), eps, 0, *_strides(x, y, u, out, n))
+        A = _lib.addr
+        _lib.launch("delrec_block_norm_forward", dev, ctypes.byref(b), x.data_ptr(), A(y), A(u), A(w), A(scale), A(nw),
+                    A(lengths), A(out), A(n), A(ry), A(rx))
+    return out, n, ry, rx
 
 
 class BlockNormFn(torch.autograd.Function):
@@ -37,87 +57,86 @@ class BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, u, w, scale, nw, lengths, kind, eps, has_next):
         ctx.set_materialize_grads(False)
-        x, y, u = (None if t is None else _lib.rows(t.detach()) for t in (x, y, u))
-        w, scale, nw = (None if t is None else t.detach().contiguous() for t in (w, scale, nw))
-        T, B, N = x.shape
-        dev = x.device
-        out = _lib.empty_rows(x) if y is not None else None
-        n = _lib.empty_rows(x) if has_next else None
-        train = any(ctx.needs_input_grad[:6])
-        ry = torch.empty(T, B, device=dev) if train and y is not None else None
-        rx = torch.empty(T, B, device=dev) if train and has_next else None
-        b = _lib.Block(T, B, N, _lib.SEQ_DTYPES[x.dtype], kind,
-                       int(lengths is not None and lengths.dtype == torch.int64), eps, 0)
-        _strides(b, x=x, y=y, u=u, o=out, n=n)
-        if T and B and N:
-            A = _lib.addr
-            with _lib.on_device(x):
-                _lib.check(_lib.lib().delrec_block_norm_forward(
-                    ctypes.byref(b), A(x), A(y), A(u), A(w), A(scale), A(nw), A(lengths), A(out), A(n), A(ry),
-                    A(rx), _lib.stream_ptr(dev)), "delrec_block_norm_forward")
-        if train:
-            ctx.save_for_backward(x if has_next else None, y, u, w, scale, nw, lengths, ry, rx)
-            ctx.block, ctx.shape, ctx.dtype, ctx.has_next = b, (T, B, N), x.dtype, has_next
-        outs = tuple(t for t in (out, n) if t is not None)
-        return outs if len(outs) > 1 else outs[0]
+        out, n, ry, rx = _forward(x, y, u, w, scale, nw, lengths, kind, eps, has_next, True)
+        ctx.save_for_backward(x if has_next else None, y, u, w, scale, nw, lengths, ry, rx)
+        ctx.meta = x.shape, x.dtype, kind, eps, has_next
+        if out is None:
+            return n
+        return (out, n) if has_next else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         x, y, u, w, scale, nw, lengths, ry, rx = ctx.saved_tensors
-        T, B, N = ctx.shape
+        (T, B, N), dtype, kind, eps, has_next = ctx.meta
         gx = grads[0] if y is not None else None
-        gn = grads[-1] if ctx.has_next else None
+        gn = grads[-1] if has_next else None
         if gx is None and gn is None:
             return (None,) * 10
-        gx, gn = (None if g is None else _lib.rows(g) for g in (gx, gn))
-        dev = (gx if gx is not None else gn).device
+        if gx is not None:
+            gx = _lib.rows(gx)
+        if gn is not None:
+            gn = _lib.rows(gn)
         need = ctx.needs_input_grad
         like = x if x is not None else y
-        new = lambda want: _lib.empty_rows(like) if want else None   # noqa: E731
-        vec = lambda want: torch.empty(N, device=dev) if want else None   # noqa: E731
-        dx, dy, du = new(need[0]), new(need[1]), new(need[2])
-        dw, ds, dn = vec(need[3]), vec(need[4]), vec(need[5])
-        if not (T and B and N):
+        dev = like.device
+        dx = _lib.empty_rows(like) if need[0] else None
+        dy = _lib.empty_rows(like) if need[1] else None
+        du = _lib.empty_rows(like) if need[2] else None
+        dw = torch.empty(N, device=dev) if need[3] else None
+        ds = torch.empty(N, device=dev) if need[4] else None
+        dn = torch.empty(N, device=dev) if need[5] else None
+        if T and B and N:
+            b = _lib.Block(T, B, N, _lib.SEQ_DTYPES[dtype], kind, _wide(lengths), eps, 0,
+                           *_strides(x, y, u, None, None, gx, gn, dx, dy, du))
+            ws, nbytes = None, 0
+            if dw is not None or ds is not None or dn is not None:
+                nbytes = _lib.lib().delrec_block_norm_backward_workspace(ctypes.byref(b))
+                ws = _lib.scratch(nbytes, dev)
+            A = _lib.addr
+            _lib.launch("delrec_block_norm_backward", dev, ctypes.byref(b), A(x), A(y), A(u), A(w), A(scale), A(nw),
+                        A(lengths), A(ry), A(rx), A(gx), A(gn), A(dx), A(dy), A(du), A(dw), A(ds), A(dn), A(ws), nbytes)
+        else:
             for t in (dw, ds, dn):
                 if t is not None:
                     t.zero_()
-            return dx, dy, du, dw, ds, dn, None, None, None, None
-        b = _lib.Block.from_buffer_copy(ctx.block)
-        _strides(b, gx=gx, gn=gn, dx=dx, dy=dy, du=du)
-        lib, A = _lib.lib(), _lib.addr
-        sums = any(t is not None for t in (dw, ds, dn))
-        nbytes = lib.delrec_block_norm_backward_workspace(ctypes.byref(b)) if sums else 0
-        ws = _lib.scratch(nbytes, dev)
-        with _lib.on_device(like):
-            _lib.check(lib.delrec_block_norm_backward(
-                ctypes.byref(b), A(x), A(y), A(u), A(w), A(scale), A(nw), A(lengths), A(ry), A(rx), A(gx), A(gn),
-                A(dx), A(dy), A(du), A(dw), A(ds), A(dn), A(ws), nbytes, _lib.stream_ptr(dev)),
-                "delrec_block_norm_backward")
         return dx, dy, du, dw, ds, dn, None, None, None, None
 
 
+def _run(x, y, u, w, scale, nw, lengths, kind, eps, has_next):
+    """(x', n) through autograd where a gradient is wanted, else plainly."""
+    args = [None if t is None else _lib.rows(t) for t in (x, y, u)]
+    args += [None if t is None else t.contiguous() for t in (w, scale, nw)]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        r = BlockNormFn.apply(*args, lengths, kind, eps, has_next)
+        if y is None:
+            return None, r
+        return r if has_next else (r, None)
+    return _forward(*args, lengths, kind, eps, has_next, False)[:2]
+
+
 def _check(x, others, weights, lengths, eps):
-    _lib.require_sequence(x, *(t for t in others if t is not None))
-    if x.dim() != 3:
-        raise RuntimeError(f"delrec_b200: x must be (T, B, N), got {tuple(x.shape)}")
+    _lib.require_sequence(x)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if len(shape) != 3:
+        raise RuntimeError(f"delrec_b200: x must be (T, B, N), got {tuple(shape)}")
     for t in others:
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device):
             raise RuntimeError("delrec_b200: x, y and gate must share shape, dtype and device")
     for w in weights:
-        if w is not None and (w.shape != (x.shape[-1],) or w.dtype != torch.float32 or w.device != x.device):
-            raise RuntimeError(f"delrec_b200: weights must be ({x.shape[-1]},) float32 on {x.device}")
+        if w is not None and (w.shape != shape[2:] or w.dtype != torch.float32 or w.device != device):
+            raise RuntimeError(f"delrec_b200: weights must be ({shape[2]},) float32 on {device}")
     if not eps > 0:
         raise RuntimeError("delrec_b200: eps must be positive")
     if lengths is not None:
-        _lib.require_lengths(lengths, x.shape[1], x.device)
+        _lib.require_lengths(lengths, shape[1], device)
 
 
 def block_norm(x, weight=None, *, eps=1e-5, lengths=None):
     """x (T,B,N) -> x / rms(x) * weight.  ``lengths`` (B,): positions t >= lengths[b] are not
     read, their outputs and gradients are 0.  Strides of T and B are free."""
     _check(x, (), (weight,), lengths, eps)
-    return BlockNormFn.apply(x, None, None, None, None, weight, lengths, 0, eps, True)
+    return _run(x, None, None, None, None, weight, lengths, 0, eps, True)[1]
 
 
 def block_join(x, y, weight=None, *, gate=None, gate_act="sigmoid", scale=None, next_weight=None,
@@ -138,5 +157,4 @@ def block_join(x, y, weight=None, *, gate=None, gate_act="sigmoid", scale=None, 
     if next_weight is not None and not has_next:
         raise RuntimeError("delrec_b200: next_weight without a next norm")
     kind = GATES[gate_act] if gate is not None else 0
-    r = BlockNormFn.apply(x, y, gate if kind else None, weight, scale, next_weight, lengths, kind, eps, has_next)
-    return r if has_next else (r, None)
+    return _run(x, y, gate if kind else None, weight, scale, next_weight, lengths, kind, eps, has_next)

@@ -41,32 +41,34 @@ def pack8(x) -> Packed8:
     code = _lib.require_sequence(x)
     if x.dim() == 0:
         raise RuntimeError("delrec_b200: pack8 expects at least one dimension")
-    x = x.detach().contiguous()
-    p = empty8(x.shape, x.dtype, x.device)
-    if x.numel():
-        with _lib.on_device(x):
-            _lib.check(_lib.lib().delrec_pack8(x.numel() // x.shape[-1], x.shape[-1], code, x.data_ptr(),
-                                               p.q.data_ptr(), p.e.data_ptr(), _lib.stream_ptr(x.device)),
-                       "delrec_pack8")
+    x = x.contiguous()
+    shape, device = x.shape, x.device
+    p = empty8(shape, x.dtype, device)
+    n = x.numel()
+    if n:
+        _lib.launch("delrec_pack8", device, n // shape[-1], shape[-1], code, x.data_ptr(), p.q.data_ptr(),
+                    p.e.data_ptr())
     return p
 
 
 def unpack8(packed: Packed8, dtype=None):
-    """The tensor that ``packed`` stands for, in its own dtype or the given one."""
-    q, e = packed.q, packed.e
-    dtype = packed.dtype if dtype is None else dtype
-    if dtype not in _lib.SEQ_DTYPES:
-        raise RuntimeError(f"delrec_b200 expects float32, bfloat16 or float16, got {dtype}")
-    if not (q.is_cuda and e.device == q.device):
+    """The tensor that ``packed`` stands for, in its own dtype or the given one (float16
+    saturates at its largest value)."""
+    q, e, own = packed
+    code = _lib.SEQ_DTYPES.get(dtype or own)
+    if code is None:
+        raise RuntimeError(f"delrec_b200 expects float32, bfloat16 or float16, got {dtype or own}")
+    device = q.device
+    if not q.is_cuda or e.device != device:
         raise RuntimeError("delrec_b200 runs on CUDA tensors only (there is no CPU path)")
-    if (q.dtype, e.dtype) != (torch.int8, torch.uint8) or q.dim() == 0 \
-            or e.shape != (*q.shape[:-1], -(-q.shape[-1] // GROUP)):
+    shape = q.shape
+    if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() == 0 \
+            or e.shape != (*shape[:-1], -(-shape[-1] // GROUP)):
         raise RuntimeError("delrec_b200: not a Packed8 (int8 (..., N) with uint8 (..., ceil(N / 32)))")
     q, e = q.contiguous(), e.contiguous()
-    x = torch.empty(q.shape, dtype=dtype, device=q.device)
-    if x.numel():
-        with _lib.on_device(q):
-            _lib.check(_lib.lib().delrec_unpack8(q.numel() // q.shape[-1], q.shape[-1], _lib.SEQ_DTYPES[dtype],
-                                                 q.data_ptr(), e.data_ptr(), x.data_ptr(),
-                                                 _lib.stream_ptr(q.device)), "delrec_unpack8")
+    x = torch.empty(shape, dtype=dtype or own, device=device)
+    n = x.numel()
+    if n:
+        _lib.launch("delrec_unpack8", device, n // shape[-1], shape[-1], code, q.data_ptr(), e.data_ptr(),
+                    x.data_ptr())
     return x

@@ -24,109 +24,104 @@ SEGMENT = 16     # distance of the states kept for the backward pass
 
 
 def _check(z, f, dims, layout):
-    code = _lib.require_sequence(z, f)
-    if z.dim() != dims or f.dim() != dims or z.shape[:-1] != f.shape[:-1]:
-        raise RuntimeError(f"delrec_b200: z and f must be {layout}, got {tuple(z.shape)} and {tuple(f.shape)}")
+    code = _lib.require_sequence(z)
+    zs, fs = z.shape, f.shape
+    if len(zs) != dims or len(fs) != dims or zs[:-1] != fs[:-1]:
+        raise RuntimeError(f"delrec_b200: z and f must be {layout}, got {tuple(zs)} and {tuple(fs)}")
     if f.dtype != z.dtype or f.device != z.device:
         raise RuntimeError("delrec_b200: z and f must share dtype and device")
-    N, G = z.shape[-1], f.shape[-1]
-    if G == 0 or N % G:
-        if N or G:
-            raise RuntimeError(f"delrec_b200: the {G} gates of f must divide the {N} channels of z")
+    N, G = zs[-1], fs[-1]
+    if N != G and (G == 0 or N % G):
+        raise RuntimeError(f"delrec_b200: the {G} gates of f must divide the {N} channels of z")
     return code
 
 
-def _state(s, B, N, z, name):
-    if s is not None:
-        _lib.require_cuda(s)
-        if s.shape != (B, N) or s.device != z.device:
-            raise RuntimeError(f"delrec_b200: {name} must be ({B}, {N}) float32 on {z.device}")
+def _state(s, B, N, device, name):
+    _lib.require_cuda(s)
+    if s.shape != (B, N) or s.device != device:
+        raise RuntimeError(f"delrec_b200: {name} must be ({B}, {N}) float32 on {device}")
+
+
+def _forward(z, f, h0, lengths, resets, decay_input, train, keep8):
+    """(h, hT, states, 8-bit z and f with their marks or None): one launch."""
+    T, B, N = z.shape
+    G = f.shape[-1]
+    dev = z.device
+    h = _lib.empty_rows(z)
+    hT = torch.empty(B, N, device=dev)
+    states = torch.empty(-(-T // SEGMENT), B, N, device=dev) if train else None
+    bits = (None,) * 5
+    if keep8 and G == N:
+        pz, pf = empty8(z.shape, z.dtype, dev), empty8(f.shape, f.dtype, dev)
+        odd = torch.empty(states.shape[0], B, pz.e.shape[-1], dtype=torch.uint8, device=dev)
+        bits = (pz.q, pz.e, pf.q, pf.e, odd)
+    if T and B and N:
+        zt, zb, _ = z.stride()
+        ft, fb, _ = f.stride()
+        ht, hb, _ = h.stride()
+        s = _lib.Scan(T, B, N, G, _lib.SEQ_DTYPES[z.dtype], 1 if decay_input else 0,
+                      1 if lengths is not None and lengths.dtype == torch.int64 else 0, 0, zt, zb, ft, fb, ht, hb)
+        A = _lib.addr
+        _lib.launch("delrec_gated_scan_forward", dev, ctypes.byref(s), z.data_ptr(), f.data_ptr(), A(h0), A(lengths),
+                    A(resets), h.data_ptr(), hT.data_ptr(), A(states), A(bits[0]), A(bits[1]), A(bits[2]),
+                    A(bits[3]), A(bits[4]))
+    elif h0 is not None:
+        hT.copy_(h0)
+    else:
+        hT.zero_()
+    return h, hT, states, bits
 
 
 class GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, f, h0, lengths, resets, decay_input, checkpoint8):
-        T, B, N = z.shape
-        G = f.shape[-1]
         ctx.set_materialize_grads(False)
-        z, f = _lib.rows(z.detach()), _lib.rows(f.detach())
-        dev = z.device
-        h = _lib.empty_rows(z)
-        hT = torch.empty(B, N, device=dev)
-        train = any(ctx.needs_input_grad[:3])
-        s = _lib.Scan(T, B, N, G, _lib.SEQ_DTYPES[z.dtype], int(decay_input),
-                      int(lengths is not None and lengths.dtype == torch.int64), 0,
-                      *z.stride()[:2], *f.stride()[:2], *h.stride()[:2])
-        states = torch.empty(-(-T // SEGMENT), B, N, device=dev) if train else None
-        keep8 = bool(checkpoint8) and train
-        pz = pf = odd = None
-        if keep8 and G == N:
-            pz, pf = empty8(z.shape, z.dtype, dev), empty8(f.shape, f.dtype, dev)
-            odd = torch.empty(*states.shape[:2], pz.e.shape[-1], dtype=torch.uint8, device=dev)
-        if T and B and N:
-            with _lib.on_device(z):
-                _lib.check(_lib.lib().delrec_gated_scan_forward(
-                    ctypes.byref(s), z.data_ptr(), f.data_ptr(), _lib.addr(h0), _lib.addr(lengths),
-                    _lib.addr(resets), h.data_ptr(), hT.data_ptr(), _lib.addr(states),
-                    _lib.addr(pz and pz.q), _lib.addr(pz and pz.e), _lib.addr(pf and pf.q),
-                    _lib.addr(pf and pf.e), _lib.addr(odd), _lib.stream_ptr(dev)), "delrec_gated_scan_forward")
-        elif h0 is not None:
-            hT.copy_(h0.detach())
+        z, f = _lib.rows(z), _lib.rows(f)
+        h, hT, states, bits = _forward(z, f, h0, lengths, resets, decay_input, True, checkpoint8)
+        ctx.meta = z.shape, f.shape[-1], z.dtype, bool(decay_input), bool(checkpoint8), h0 is not None
+        if checkpoint8:
+            if bits[0] is None:   # a shared gate is small against its channels: packed apart
+                (qz, ez, _), (qf, ef, _) = pack8(z), pack8(f)
+                bits = (qz, ez, qf, ef, None)
+            ctx.save_for_backward(None, None, states, lengths, resets, *bits)
         else:
-            hT.zero_()
-        if not train:
-            return h, hT
-        if keep8:
-            if pz is None:   # a shared gate is small against its channels: packed apart
-                pz, pf = pack8(z), pack8(f)
-            ctx.save_for_backward(pz.q, pz.e, pf.q, pf.e, odd, states, lengths, resets)
-        else:
-            ctx.save_for_backward(z, f, states, lengths, resets)
-        ctx.scan, ctx.keep8, ctx.dtype = s, keep8, z.dtype
-        ctx.has_h0 = h0 is not None
+            ctx.save_for_backward(z, f, states, lengths, resets, *bits)
         return h, hT
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gh, ghT):
-        z = f = pz = pf = odd = None
-        if ctx.keep8:
-            qz, ez, qf, ef, odd, states, lengths, resets = ctx.saved_tensors
-            pz, pf = Packed8(qz, ez, ctx.dtype), Packed8(qf, ef, ctx.dtype)
-            if ctx.scan.G != ctx.scan.N:    # the 8-bit kernel is for a gate per channel
-                z, f, pz, pf = unpack8(pz), unpack8(pf), None, None
-            like_z, like_f = qz, qf
-        else:
-            z, f, states, lengths, resets = ctx.saved_tensors
-            like_z, like_f = z, f
         if gh is None and ghT is None:
             return (None,) * 7
-        dev = like_z.device
-        T, B, N = like_z.shape
-        if gh is not None:
-            gh = _lib.rows(gh)
-        if ghT is not None:
-            ghT = ghT.contiguous()
+        z, f, states, lengths, resets, qz, ez, qf, ef, odd = ctx.saved_tensors
+        (T, B, N), G, dtype, decay_input, keep8, has_h0 = ctx.meta
+        if keep8 and odd is None:       # the 8-bit kernel is for a gate per channel
+            z, f = unpack8(Packed8(qz, ez, dtype)), unpack8(Packed8(qf, ef, dtype))
+            qz = ez = qf = ef = None
         need_z, need_f, need_h = ctx.needs_input_grad[:3]
-        dz = _lib.empty_rows(like_z, ctx.dtype) if need_z else None
-        df = _lib.empty_rows(like_f, ctx.dtype) if need_f else None
-        dh0 = torch.empty(B, N, device=dev) if need_h and ctx.has_h0 else None
+        like_z, like_f = (qz, qf) if z is None else (z, f)
+        dev = states.device
+        dz = _lib.empty_rows(like_z, dtype) if need_z else None
+        df = _lib.empty_rows(like_f, dtype) if need_f else None
+        dh0 = torch.empty(B, N, device=dev) if need_h and has_h0 else None
         if T and B and N:
-            # a copy of the descriptor: two backward passes of one graph may run at once
-            s = _lib.Scan.from_buffer_copy(ctx.scan)
-            for name, t in (("z", z), ("f", f), ("gh", gh), ("dz", dz), ("df", df)):
-                if t is not None:
-                    setattr(s, name + "_t", t.stride(0))
-                    setattr(s, name + "_b", t.stride(1))
-            lib = _lib.lib()
-            nbytes = lib.delrec_gated_scan_backward_workspace(ctypes.byref(s)) if need_f else 0
-            ws = _lib.scratch(nbytes, dev)
-            with _lib.on_device(like_z):
-                _lib.check(lib.delrec_gated_scan_backward(
-                    ctypes.byref(s), _lib.addr(z), _lib.addr(f), _lib.addr(pz and pz.q), _lib.addr(pz and pz.e),
-                    _lib.addr(pf and pf.q), _lib.addr(pf and pf.e), _lib.addr(odd), _lib.addr(lengths), _lib.addr(resets),
-                    states.data_ptr(), _lib.addr(gh), _lib.addr(ghT), _lib.addr(dz), _lib.addr(df),
-                    _lib.addr(dh0), _lib.addr(ws), nbytes, _lib.stream_ptr(dev)), "delrec_gated_scan_backward")
+            if gh is not None:
+                gh = _lib.rows(gh)
+            if ghT is not None:
+                ghT = ghT.contiguous()
+            st = []
+            for t in (z, f, None, gh, dz, df):
+                st += t.stride()[:2] if t is not None else (0, 0)
+            s = _lib.Scan(T, B, N, G, _lib.SEQ_DTYPES[dtype], 1 if decay_input else 0,
+                          1 if lengths is not None and lengths.dtype == torch.int64 else 0, 0, *st)
+            ws, nbytes = None, 0
+            if need_f and G != N:
+                nbytes = _lib.lib().delrec_gated_scan_backward_workspace(ctypes.byref(s))
+                ws = _lib.scratch(nbytes, dev)
+            A = _lib.addr
+            _lib.launch("delrec_gated_scan_backward", dev, ctypes.byref(s), A(z), A(f), A(qz), A(ez), A(qf), A(ef),
+                        A(odd), A(lengths), A(resets), states.data_ptr(), A(gh), A(ghT), A(dz), A(df), A(dh0), A(ws),
+                        nbytes)
         elif dh0 is not None:
             dh0 = ghT.clone() if ghT is not None else dh0.zero_()
         return dz, df, dh0, None, None, None, None
@@ -149,14 +144,17 @@ def gated_scan(z, f, h0=None, *, lengths=None, resets=None, decay_input=True, ch
     restored z and f, with the states between two kept ones recomputed from them."""
     _check(z, f, 3, "(T, B, N) and (T, B, G)")
     T, B, N = z.shape
-    _state(h0, B, N, z, "h0")
+    if h0 is not None:
+        _state(h0, B, N, z.device, "h0")
     if lengths is not None:
         _lib.require_lengths(lengths, B, z.device)
     if resets is not None:
         if resets.shape != (T, B) or resets.dtype != torch.bool or resets.device != z.device:
             raise RuntimeError(f"delrec_b200: resets must be bool ({T}, {B}) on {z.device}")
         resets = resets.contiguous()
-    return GatedScan.apply(z, f, h0, lengths, resets, decay_input, checkpoint8)
+    if torch.is_grad_enabled() and (z.requires_grad or f.requires_grad or (h0 is not None and h0.requires_grad)):
+        return GatedScan.apply(z, f, h0, lengths, resets, decay_input, checkpoint8)
+    return _forward(_lib.rows(z), _lib.rows(f), h0, lengths, resets, decay_input, False, False)[:2]
 
 
 def gated_step(z, f, state=None, *, active=None, decay_input=True, out=None):
@@ -167,19 +165,21 @@ def gated_step(z, f, state=None, *, active=None, decay_input=True, out=None):
     No gradient passes; train with ``gated_scan``."""
     code = _check(z, f, 2, "(B, N) and (B, G)")
     B, N = z.shape
-    _state(state, B, N, z, "state")
-    _state(out, B, N, z, "out")
+    dev = z.device
+    if state is not None:
+        _state(state, B, N, dev, "state")
+    if out is not None:
+        _state(out, B, N, dev, "out")
     if active is not None:
-        if active.shape != (B,) or active.dtype != torch.bool or active.device != z.device:
-            raise RuntimeError(f"delrec_b200: active must be bool ({B},) on {z.device}")
+        if active.shape != (B,) or active.dtype != torch.bool or active.device != dev:
+            raise RuntimeError(f"delrec_b200: active must be bool ({B},) on {dev}")
         active = active.contiguous()
-    z, f = _lib.rows(z.detach()), _lib.rows(f.detach())
-    h = torch.empty(B, N, device=z.device, dtype=z.dtype)
-    nxt = torch.empty(B, N, device=z.device) if out is None else out
+    z, f = _lib.rows(z), _lib.rows(f)
+    h = torch.empty(B, N, device=dev, dtype=z.dtype)
+    nxt = torch.empty(B, N, device=dev) if out is None else out
     if B and N:
-        s = _lib.Scan(1, B, N, f.shape[1], code, int(decay_input), 0, 0, 0, z.stride(0), 0, f.stride(0))
-        with _lib.on_device(z):
-            _lib.check(_lib.lib().delrec_gated_step(
-                ctypes.byref(s), z.data_ptr(), f.data_ptr(), _lib.addr(state), _lib.addr(active), h.data_ptr(),
-                nxt.data_ptr(), _lib.stream_ptr(z.device)), "delrec_gated_step")
+        s = _lib.Scan(1, B, N, f.shape[1], code, 1 if decay_input else 0, 0, 0, 0, z.stride(0), 0, f.stride(0))
+        A = _lib.addr
+        _lib.launch("delrec_gated_step", dev, ctypes.byref(s), z.data_ptr(), f.data_ptr(), A(state), A(active),
+                    h.data_ptr(), nxt.data_ptr())
     return h, nxt
