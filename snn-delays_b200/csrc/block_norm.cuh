@@ -78,32 +78,35 @@ __device__ __forceinline__ const T* row_of(const void* p, const NormRow& r, int 
 
 // The inputs of a row, NT tensors of IT vectors per thread.  Vectors of 4 bytes and more are
 // copied into shared memory (cp.async) while the row before is worked on; every thread
-// copies what it will read itself, so no barrier is needed.  One slot per tensor, vector and
-// thread, two rows.
+// copies what it will read itself, so no barrier is needed.  A vector of all threads lies side
+// by side: copies that scatter a thread's vectors over shared memory cost a third more time.
 template <class T, int V, int IT, int NT>
 struct NormStage {
   static constexpr int VB = V * (int)sizeof(T);
   static constexpr bool STAGED = VB >= 4 && IT <= 2;
   static constexpr int ROW = STAGED ? NT * IT * VB : 0;   // bytes per thread and row
-  unsigned base;
-  char* mem;
-  __device__ __forceinline__ NormStage(char* m) : mem(m) {
-    base = STAGED ? (unsigned)__cvta_generic_to_shared(m) : 0;
+  unsigned base[2];
+  const char* mem[2];
+  int plane;   // bytes of one vector of all threads
+  __device__ __forceinline__ NormStage(char* m) {
+    plane = blockDim.x * VB;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mem[h] = m + h * (int)blockDim.x * ROW + threadIdx.x * VB;
+      base[h] = STAGED ? (unsigned)__cvta_generic_to_shared(mem[h]) : 0;
+    }
   }
-  __device__ __forceinline__ int slot(int half, int ten, int k) const {
-    return ((half * NT + ten) * IT + k) * (int)blockDim.x * VB + (int)threadIdx.x * VB;
-  }
-  __device__ __forceinline__ void copy(int half, int ten, const T* row, int N) const {
+  // col: this thread's first channel in the row
+  __device__ __forceinline__ void copy(unsigned at, int ten, const T* col, int left, int nthV) const {
     if constexpr (STAGED) {
 #pragma unroll
       for (int k = 0; k < IT; ++k) {
-        const int c = (k * (int)blockDim.x + (int)threadIdx.x) * V;
-        if (c < N) {
+        if (k * nthV < left) {
           if constexpr (VB == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + slot(half, ten, k)), "l"(row + c));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + (ten * IT + k) * plane), "l"(col + k * nthV));
           else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(base + slot(half, ten, k)), "l"(row + c),
-                         "n"(VB));
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at + (ten * IT + k) * plane),
+                         "l"(col + k * nthV), "n"(VB));
         }
       }
     }
@@ -116,11 +119,10 @@ struct NormStage {
     if (STAGED) asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
   }
   // vector k of tensor ten as floats; zeros past the row's end
-  __device__ __forceinline__ void read(int half, int ten, int k, const T* row, int N, float* o) const {
-    const int c = (k * (int)blockDim.x + (int)threadIdx.x) * V;
-    if (c < N) {
-      if constexpr (STAGED) unpack_vec<T, V>(*(const VecOf<T, V>*)(mem + slot(half, ten, k)), o);
-      else unpack_vec<T, V>(*(const VecOf<T, V>*)(row + c), o);
+  __device__ __forceinline__ void read(const char* at, int ten, int k, const T* col, int left, int nthV, float* o) const {
+    if (k * nthV < left) {
+      if constexpr (STAGED) unpack_vec<T, V>(*(const VecOf<T, V>*)(at + (ten * IT + k) * plane), o);
+      else unpack_vec<T, V>(*(const VecOf<T, V>*)(col + k * nthV), o);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = 0.f;
@@ -133,38 +135,28 @@ struct NormStage {
 __device__ __forceinline__ float block_sum(float v, float (*red)[32], int& slot) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int nw = blockDim.x >> 5;
+  const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
   if (nw == 1) return v;
-  if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = v;
+  if (lane == 0) red[slot][threadIdx.x >> 5] = v;
   __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < nw; ++i) s += red[slot][i];
+  v = (lane & 15) < nw ? red[slot][lane & 15] : 0.f;   // both halves of the warp
   slot ^= 1;
-  return s;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);   // at most 16 warps
+  return v;
 }
 
-// A gate's function and derivative from the folded sigmoid (its smaller side, signed as u).
-struct GateVal {
-  float a, da;
-};
-__device__ __forceinline__ GateVal gate_eval(float fold, float u, int kind) {
-  float sg, so;
-  gate_unfold(fold, sg, so);
-  GateVal g;
-  g.a = kind == GATE_SIGMOID ? sg : u * sg;
-  g.da = kind == GATE_SIGMOID ? sg * so : sg * fmaf(u, so, 1.f);
-  return g;
-}
-
-// E = V * IT elements per thread: vector k starts at channel (k * threads + thread) * V
-template <class T, int V, int IT, bool GATE>
+// E = V * IT elements per thread: vector k starts at channel (k * threads + thread) * V.
+// KIND: GATE_*.
+template <class T, int V, int IT, int KIND>
 __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
   __shared__ float red[2][32];
   extern __shared__ __align__(16) char norm_stage[];
   constexpr int E = V * IT;
+  constexpr bool GATE = KIND != GATE_NONE;
   using Stage = NormStage<T, V, IT, GATE ? 3 : 2>;
   const Stage st(norm_stage);
-  const int nth = blockDim.x, tid = threadIdx.x, rows = p.T * p.B;
+  const int nthV = blockDim.x * V, c0 = threadIdx.x * V, left = p.N - c0, rows = p.T * p.B;
   const float inv_n = 1.f / (float)p.N;
   const int gs = gridDim.x, gt = gs / p.B, gb = gs - gt * p.B;
   int slot = 0;
@@ -173,54 +165,59 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
   for (int k = 0; k < IT; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (k * nth + tid) * V + j;
+      const int c = c0 + k * nthV + j;
       const bool on = c < p.N;
       ws[k * V + j] = on ? (p.w ? p.w[c] : 1.f) * (p.scale ? p.scale[c] : 1.f) : 0.f;
       nw[k * V + j] = on ? (p.nw ? p.nw[c] : 1.f) : 0.f;
     }
-  auto xr = [&](const NormRow& r) { return row_of<T>(p.x, r, p.x_t, p.x_b); };
-  auto yr = [&](const NormRow& r) { return row_of<T>(p.y, r, p.y_t, p.y_b); };
-  auto ur = [&](const NormRow& r) { return row_of<T>(p.u, r, p.u_t, p.u_b); };
+  auto xr = [&](const NormRow& r) { return row_of<T>(p.x, r, p.x_t, p.x_b) + c0; };
+  auto yr = [&](const NormRow& r) { return row_of<T>(p.y, r, p.y_t, p.y_b) + c0; };
+  auto ur = [&](const NormRow& r) { return row_of<T>(p.u, r, p.u_t, p.u_b) + c0; };
   auto live_row = [&](const NormRow& r) { return !p.lengths || r.t < row_length(p.lengths, p.wide, r.b, p.T); };
-  auto fetch = [&](const NormRow& r, int half, bool live) {
+  auto fetch = [&](const NormRow& r, unsigned at, bool live) {
     if (live) {
-      st.copy(half, 0, xr(r), p.N);
-      if (p.y) st.copy(half, 1, yr(r), p.N);
-      if (GATE && p.y) st.copy(half, 2, ur(r), p.N);
+      st.copy(at, 0, xr(r), left, nthV);
+      if (p.y) {
+        st.copy(at, 1, yr(r), left, nthV);
+        if (GATE) st.copy(at, 2, ur(r), left, nthV);
+      }
     }
     st.commit();
   };
   NormRow cur;
   cur.init(blockIdx.x, p.B);
   bool live = live_row(cur);
-  fetch(cur, 0, live);
+  fetch(cur, st.base[0], live);
   for (int half = 0; cur.r < rows; half ^= 1) {
     NormRow nxt = cur;
     nxt.next(gs, gt, gb, p.B);
     const bool next_live = nxt.r < rows && live_row(nxt);
-    fetch(nxt, half ^ 1, next_live);
+    fetch(nxt, half ? st.base[0] : st.base[1], next_live);
+    const char* at = half ? st.mem[1] : st.mem[0];
     st.template wait<1>();
     float x[E], y[E], u[E];
     if (live) {
 #pragma unroll
       for (int k = 0; k < IT; ++k) {
-        st.read(half, 0, k, xr(cur), p.N, x + k * V);
-        if (p.y) st.read(half, 1, k, yr(cur), p.N, y + k * V);
-        if (GATE && p.y) st.read(half, 2, k, ur(cur), p.N, u + k * V);
+        st.read(at, 0, k, xr(cur), left, nthV, x + k * V);
+        if (p.y) {
+          st.read(at, 1, k, yr(cur), left, nthV, y + k * V);
+          if (GATE) st.read(at, 2, k, ur(cur), left, nthV, u + k * V);
+        }
       }
       if (p.y) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) s = fmaf(y[i], y[i], s);
         const float ry = rsqrtf(block_sum(s, red, slot) * inv_n + p.eps);
-        if (p.ry && tid == 0) p.ry[cur.r] = ry;
+        if (p.ry && threadIdx.x == 0) p.ry[cur.r] = ry;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           float g = ws[i];
           if (GATE) {
             float sg, so;
             sigmoid_pair<Accurate<T>::value>(u[i], sg, so);
-            g *= p.kind == GATE_SIGMOID ? sg : u[i] * sg;
+            g *= KIND == GATE_SIGMOID ? sg : u[i] * sg;
           }
           x[i] = fmaf(y[i] * ry, g, x[i]);
         }
@@ -230,12 +227,10 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
       for (int i = 0; i < E; ++i) x[i] = 0.f;
     }
     if (p.y) {
-      T* o = row_of<T>(p.out, cur, p.o_t, p.o_b);
+      T* o = row_of<T>(p.out, cur, p.o_t, p.o_b) + c0;
 #pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        const int c = (k * nth + tid) * V;
-        if (c < p.N) store_vec<T, V>(o + c, x + k * V);
-      }
+      for (int k = 0; k < IT; ++k)
+        if (k * nthV < left) store_vec<T, V>(o + k * nthV, x + k * V);
     }
     if (p.n) {
       float rx = 0.f;
@@ -244,19 +239,17 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
 #pragma unroll
         for (int i = 0; i < E; ++i) s = fmaf(x[i], x[i], s);
         rx = rsqrtf(block_sum(s, red, slot) * inv_n + p.eps);
-        if (p.rx && tid == 0) p.rx[cur.r] = rx;
+        if (p.rx && threadIdx.x == 0) p.rx[cur.r] = rx;
       }
-      T* o = row_of<T>(p.n, cur, p.n_t, p.n_b);
+      T* o = row_of<T>(p.n, cur, p.n_t, p.n_b) + c0;
 #pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        const int c = (k * nth + tid) * V;
-        if (c < p.N) {
+      for (int k = 0; k < IT; ++k)
+        if (k * nthV < left) {
           float v[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) v[j] = x[k * V + j] * rx * nw[k * V + j];
-          store_vec<T, V>(o + c, v);
+          store_vec<T, V>(o + k * nthV, v);
         }
-      }
     }
     cur = nxt;
     live = next_live;
@@ -264,14 +257,15 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
   st.template wait<0>();
 }
 
-template <class T, int V, int IT, bool GATE>
+template <class T, int V, int IT, int KIND>
 __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
   __shared__ float red[2][32];
   extern __shared__ __align__(16) char norm_stage[];
   constexpr int E = V * IT;
+  constexpr bool GATE = KIND != GATE_NONE;
   using Stage = NormStage<T, V, IT, GATE ? 5 : 4>;
   const Stage st(norm_stage);
-  const int nth = blockDim.x, tid = threadIdx.x, rows = p.T * p.B;
+  const int nthV = blockDim.x * V, c0 = threadIdx.x * V, left = p.N - c0, rows = p.T * p.B;
   const float inv_n = 1.f / (float)p.N;
   const int gs = gridDim.x, gt = gs / p.B, gb = gs - gt * p.B;
   int slot = 0;
@@ -280,30 +274,30 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
   for (int k = 0; k < IT; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (k * nth + tid) * V + j;
+      const int c = c0 + k * nthV + j;
       const bool on = c < p.N;
       ws[k * V + j] = on ? (p.w ? p.w[c] : 1.f) * (p.scale ? p.scale[c] : 1.f) : 0.f;
       nw[k * V + j] = on ? (p.nw ? p.nw[c] : 1.f) : 0.f;
       q[k * V + j] = qn[k * V + j] = 0.f;
     }
-  auto xr = [&](const NormRow& r) { return row_of<T>(p.x, r, p.x_t, p.x_b); };
-  auto yr = [&](const NormRow& r) { return row_of<T>(p.y, r, p.y_t, p.y_b); };
-  auto ur = [&](const NormRow& r) { return row_of<T>(p.u, r, p.u_t, p.u_b); };
-  auto gxr = [&](const NormRow& r) { return row_of<T>(p.gx, r, p.gx_t, p.gx_b); };
-  auto gnr = [&](const NormRow& r) { return row_of<T>(p.gn, r, p.gn_t, p.gn_b); };
+  auto xr = [&](const NormRow& r) { return row_of<T>(p.x, r, p.x_t, p.x_b) + c0; };
+  auto yr = [&](const NormRow& r) { return row_of<T>(p.y, r, p.y_t, p.y_b) + c0; };
+  auto ur = [&](const NormRow& r) { return row_of<T>(p.u, r, p.u_t, p.u_b) + c0; };
+  auto gxr = [&](const NormRow& r) { return row_of<T>(p.gx, r, p.gx_t, p.gx_b) + c0; };
+  auto gnr = [&](const NormRow& r) { return row_of<T>(p.gn, r, p.gn_t, p.gn_b) + c0; };
   auto live_row = [&](const NormRow& r) { return !p.lengths || r.t < row_length(p.lengths, p.wide, r.b, p.T); };
   float ry_ahead = 0.f, rx_ahead = 0.f;
-  auto fetch = [&](const NormRow& r, int half, bool live) {
+  auto fetch = [&](const NormRow& r, unsigned at, bool live) {
     if (live) {
-      if (p.gx) st.copy(half, 0, gxr(r), p.N);
+      if (p.gx) st.copy(at, 0, gxr(r), left, nthV);
       if (p.gn) {
-        st.copy(half, 1, gnr(r), p.N);
-        st.copy(half, 2, xr(r), p.N);
+        st.copy(at, 1, gnr(r), left, nthV);
+        st.copy(at, 2, xr(r), left, nthV);
         rx_ahead = p.rx[r.r];
       }
       if (p.y) {
-        st.copy(half, 3, yr(r), p.N);
-        if (GATE) st.copy(half, 4, ur(r), p.N);
+        st.copy(at, 3, yr(r), left, nthV);
+        if (GATE) st.copy(at, 4, ur(r), left, nthV);
         ry_ahead = p.ry[r.r];
       }
     }
@@ -312,69 +306,75 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
   NormRow cur;
   cur.init(blockIdx.x, p.B);
   bool live = live_row(cur);
-  fetch(cur, 0, live);
+  fetch(cur, st.base[0], live);
   for (int half = 0; cur.r < rows; half ^= 1) {
     const float ry = ry_ahead, rx = rx_ahead;
     NormRow nxt = cur;
     nxt.next(gs, gt, gb, p.B);
     const bool next_live = nxt.r < rows && live_row(nxt);
-    fetch(nxt, half ^ 1, next_live);
-    T* dx = p.dx ? row_of<T>(p.dx, cur, p.dx_t, p.dx_b) : nullptr;
-    T* dy = p.dy ? row_of<T>(p.dy, cur, p.dy_t, p.dy_b) : nullptr;
-    T* du = GATE && p.du ? row_of<T>(p.du, cur, p.du_t, p.du_b) : nullptr;
+    fetch(nxt, half ? st.base[0] : st.base[1], next_live);
+    const char* at = half ? st.mem[1] : st.mem[0];
+    T* dx = p.dx ? row_of<T>(p.dx, cur, p.dx_t, p.dx_b) + c0 : nullptr;
+    T* dy = p.dy ? row_of<T>(p.dy, cur, p.dy_t, p.dy_b) + c0 : nullptr;
+    T* du = GATE && p.du ? row_of<T>(p.du, cur, p.du_t, p.du_b) + c0 : nullptr;
     if (!live) {
+      float o[V];
 #pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        const int c = (k * nth + tid) * V;
-        float o[V];
+      for (int j = 0; j < V; ++j) o[j] = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = 0.f;
-        if (c < p.N) {
-          if (dx) store_vec<T, V>(dx + c, o);
-          if (dy) store_vec<T, V>(dy + c, o);
-          if (du) store_vec<T, V>(du + c, o);
+      for (int k = 0; k < IT; ++k)
+        if (k * nthV < left) {
+          if (dx) store_vec<T, V>(dx + k * nthV, o);
+          if (dy) store_vec<T, V>(dy + k * nthV, o);
+          if (du) store_vec<T, V>(du + k * nthV, o);
         }
-      }
       cur = nxt;
       live = next_live;
       continue;
     }
     st.template wait<1>();
-    float y[E], fold[E], g[E];
+    float y[E], a[E], da[E], g[E];   // yh; act; act'; the gradient
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] = 0.f;
     if (p.y) {
 #pragma unroll
-      for (int k = 0; k < IT; ++k) st.read(half, 3, k, yr(cur), p.N, y + k * V);
+      for (int k = 0; k < IT; ++k) st.read(at, 3, k, yr(cur), left, nthV, y + k * V);
 #pragma unroll
-      for (int i = 0; i < E; ++i) y[i] *= ry;   // yh
-      if (GATE) {
+      for (int i = 0; i < E; ++i) y[i] *= ry;
+    }
 #pragma unroll
-        for (int k = 0; k < IT; ++k) st.read(half, 4, k, ur(cur), p.N, fold + k * V);
+    for (int k = 0; k < IT; ++k) {
+      if (GATE) st.read(at, 4, k, ur(cur), left, nthV, da + k * V);
 #pragma unroll
-        for (int i = 0; i < E; ++i) fold[i] = gate_fold<Accurate<T>::value>(fold[i]);
+      for (int j = 0; j < V; ++j) {
+        const int i = k * V + j;
+        a[i] = 1.f;
+        if (GATE) {
+          const float u = da[i];
+          float sg, so;
+          sigmoid_pair<Accurate<T>::value>(u, sg, so);
+          a[i] = KIND == GATE_SIGMOID ? sg : u * sg;
+          da[i] = KIND == GATE_SIGMOID ? sg * so : sg * fmaf(u, so, 1.f);
+        }
       }
     }
-    // u is read again where it is needed beside its gate (silu)
-    auto u_of = [&](int k, float* o) { st.read(half, 4, k, ur(cur), p.N, o); };
 #pragma unroll
     for (int i = 0; i < E; ++i) g[i] = 0.f;
     if (p.gx) {
 #pragma unroll
-      for (int k = 0; k < IT; ++k) st.read(half, 0, k, gxr(cur), p.N, g + k * V);
+      for (int k = 0; k < IT; ++k) st.read(at, 0, k, gxr(cur), left, nthV, g + k * V);
     }
     if (p.gn) {
       float xh[E], v[E];
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < IT; ++k) {
-        float u[V];
-        st.read(half, 2, k, xr(cur), p.N, xh + k * V);
-        st.read(half, 1, k, gnr(cur), p.N, v + k * V);
-        if (GATE && p.y) u_of(k, u);
+        st.read(at, 2, k, xr(cur), left, nthV, xh + k * V);
+        st.read(at, 1, k, gnr(cur), left, nthV, v + k * V);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const int i = k * V + j;
-          if (p.y) xh[i] = fmaf(y[i], GATE ? ws[i] * gate_eval(fold[i], u[j], p.kind).a : ws[i], xh[i]);
-          xh[i] *= rx;
+          xh[i] = fmaf(y[i], ws[i] * a[i], xh[i]) * rx;
           qn[i] = fmaf(v[i], xh[i], qn[i]);
           v[i] *= nw[i];
           s = fmaf(v[i], xh[i], s);
@@ -386,40 +386,32 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
     }
     if (dx) {
 #pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        const int c = (k * nth + tid) * V;
-        if (c < p.N) store_vec<T, V>(dx + c, g + k * V);
-      }
+      for (int k = 0; k < IT; ++k)
+        if (k * nthV < left) store_vec<T, V>(dx + k * nthV, g + k * V);
     }
     if (p.y) {
       float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        float u[V], o[V];
-        if (GATE) u_of(k, u);
+      for (int i = 0; i < E; ++i) {
+        const float gy = g[i] * y[i];
+        q[i] = fmaf(gy, a[i], q[i]);
+        if (GATE) da[i] *= gy * ws[i];        // du
+        g[i] *= ws[i] * a[i];                 // v
+        s = fmaf(g[i], y[i], s);
+      }
+      if (GATE && du) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int i = k * V + j;
-          GateVal gv{1.f, 0.f};
-          if (GATE) gv = gate_eval(fold[i], u[j], p.kind);
-          const float gy = g[i] * y[i];
-          q[i] = fmaf(gy, gv.a, q[i]);
-          o[j] = gy * ws[i] * gv.da;            // du
-          g[i] *= ws[i] * gv.a;                 // v
-          s = fmaf(g[i], y[i], s);
-        }
-        const int c = (k * nth + tid) * V;
-        if (GATE && du && c < p.N) store_vec<T, V>(du + c, o);
+        for (int k = 0; k < IT; ++k)
+          if (k * nthV < left) store_vec<T, V>(du + k * nthV, da + k * V);
       }
       s = block_sum(s, red, slot) * inv_n;
       if (dy) {
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-          const int c = (k * nth + tid) * V;
           float o[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) o[j] = ry * fmaf(-y[k * V + j], s, g[k * V + j]);
-          if (c < p.N) store_vec<T, V>(dy + c, o);
+          if (k * nthV < left) store_vec<T, V>(dy + k * nthV, o);
         }
       }
     }
@@ -433,7 +425,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
     for (int k = 0; k < IT; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int c = (k * nth + tid) * V + j;
+        const int c = c0 + k * nthV + j;
         if (c < p.N) {
           o[c] = q[k * V + j];
           o[p.N + c] = qn[k * V + j];

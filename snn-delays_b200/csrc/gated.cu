@@ -14,11 +14,6 @@ static int check_scan(const delrec_scan* s) {
   return DELREC_OK;
 }
 
-struct ScanShape {
-  int V, P, csize, mode;
-  unsigned grid;
-};
-
 // What the inputs' rows allow: sixteen-byte copies (STAGED).
 struct ScanAlign {
   bool sixteen;
@@ -42,7 +37,7 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool sta
     if (st < -0x7fffffffLL || st > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   if ((long long)s->B * s->N > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   const int segs = (p->T + kSeg - 1) / kSeg;
-  sh->P = segs >= 5 ? 8 : (segs >= 2 ? 4 : 1);
+  sh->P = segs >= 2 ? 8 : 1;
   p->split = p->D >= 32;
   sh->mode = p->split ? SCAN_WIDE : (staged && p->D == 1 ? SCAN_STAGED : SCAN_DIRECT);
   // two channels to a lane (16-bit), unless that leaves SMs without a block even when a
@@ -54,86 +49,21 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool sta
   p->cpt = p->D == 1 || p->split ? 32 * sh->V : 32 / p->D * p->D;
   p->tiles = (p->N + p->cpt - 1) / p->cpt;
   const long long items = (long long)p->B * p->tiles;
-  // few rows: the blocks of a cluster share one row's time
+  // The blocks of a cluster share a row's time where that fills the SMs better: about two
+  // blocks of 8 warps fit an SM, the rounds they take fall with the cluster's size c, and
+  // each doubling costs some 6 % in exchanges (T=1021, 408 items: c = 1 takes two rounds for
+  // 1.4 blocks' work).
+  const long long slots = 2 * kSeqSMs * (8 / sh->P);
   int c = 1;
-  while (c < kScanCluster && items * c < 2 * kSeqSMs && sh->P * c < segs) c *= 2;
+  double best = 0;
+  for (int k = 1, lg = 0; k <= kScanCluster && (k == 1 || sh->P * k / 2 < segs); k *= 2, ++lg) {
+    const double cost = (double)((items * k + slots - 1) / slots) / k * (1 + 0.06 * lg);
+    if (k == 1 || cost < best) { best = cost; c = k; }
+  }
   sh->csize = c;
   if (items * c > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   sh->grid = (unsigned)(items * c);
   return DELREC_OK;
-}
-
-static int scan_launch(void (*kern)(ScanArgs, int), int smem, ScanArgs& p, ScanShape sh, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(sh.grid);
-  cfg.blockDim = dim3(sh.P * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  if (smem > 0) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = sh.csize;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = sh.csize > 1 ? 1 : 0;
-  if (sh.csize == 1 && sh.mode == SCAN_STAGED) {
-    // as many blocks as fit at once, each walking its items and copying the next ahead
-    int per_sm = 0;
-    SQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, sh.P * 32, smem));
-    cfg.gridDim.x = (unsigned)std::min<long long>(sh.grid, (long long)std::max(per_sm, 1) * kSeqSMs);
-  }
-  if (sh.csize > 8) {
-    // 16 blocks where the GPU has room for them, else the portable 8
-    int fit = 0;
-    SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    if (cudaOccupancyMaxActiveClusters(&fit, kern, &cfg) != cudaSuccess || fit < 1) {
-      (void)cudaGetLastError();
-      sh.csize = 8;
-      cfg.gridDim.x = sh.grid / 2;
-      at[0].val.clusterDim.x = 8;
-    }
-  }
-  SQ_CUDA(cudaLaunchKernelEx(&cfg, kern, p, (int)sh.csize));
-  SQ_LAUNCHED();
-  return DELREC_OK;
-}
-
-template <class T, int V, int P, bool POS, bool PACK, int MODE>
-static int fwd_launch(ScanArgs& p, const ScanShape& sh, cudaStream_t st) {
-  return scan_launch(k_scan_fwd<T, V, P, POS, PACK, MODE>, ScanFwd<T, V, P, POS, PACK, MODE>::SMEM, p, sh, st);
-}
-template <class T, int V, int P, bool POS, bool B8, int MODE>
-static int bwd_launch(ScanArgs& p, const ScanShape& sh, cudaStream_t st) {
-  return scan_launch(k_scan_bwd<T, V, P, POS, B8, MODE>, ScanBwd<T, V, P, B8, MODE>::SMEM, p, sh, st);
-}
-template <class T, bool POS, int P, bool Q8>
-static int scan_by_mode(ScanArgs& p, const ScanShape& sh, bool bwd, cudaStream_t st) {
-  if (sh.mode == SCAN_STAGED) {
-    if constexpr (sizeof(T) == 2)
-      if (sh.V == 2)
-        return bwd ? bwd_launch<T, 2, P, POS, Q8, SCAN_STAGED>(p, sh, st)
-                   : fwd_launch<T, 2, P, POS, Q8, SCAN_STAGED>(p, sh, st);
-    return bwd ? bwd_launch<T, 1, P, POS, Q8, SCAN_STAGED>(p, sh, st)
-               : fwd_launch<T, 1, P, POS, Q8, SCAN_STAGED>(p, sh, st);
-  }
-  if constexpr (!Q8)
-    if (sh.mode == SCAN_WIDE)
-      return bwd ? bwd_launch<T, 1, P, POS, false, SCAN_WIDE>(p, sh, st)
-                 : fwd_launch<T, 1, P, POS, false, SCAN_WIDE>(p, sh, st);
-  return bwd ? bwd_launch<T, 1, P, POS, Q8, SCAN_DIRECT>(p, sh, st)
-             : fwd_launch<T, 1, P, POS, Q8, SCAN_DIRECT>(p, sh, st);
-}
-template <class T, bool POS, int P>
-static int scan_by_q8(ScanArgs& p, const ScanShape& sh, bool bwd, cudaStream_t st) {
-  return p.qz ? scan_by_mode<T, POS, P, true>(p, sh, bwd, st) : scan_by_mode<T, POS, P, false>(p, sh, bwd, st);
-}
-template <class T, bool POS>
-static int scan_run(ScanArgs& p, const ScanShape& sh, bool bwd, cudaStream_t st) {
-  switch (sh.P) {
-    case 1: return scan_by_q8<T, POS, 1>(p, sh, bwd, st);
-    case 4: return scan_by_q8<T, POS, 4>(p, sh, bwd, st);
-    default: return scan_by_q8<T, POS, 8>(p, sh, bwd, st);
-  }
 }
 
 }  // namespace delrec
@@ -162,10 +92,7 @@ int delrec_gated_scan_forward(const delrec_scan* s, const void* z, const void* f
   p.z_t = (int)s->z_t; p.z_b = s->z_b; p.f_t = (int)s->f_t; p.f_b = s->f_b; p.h_t = (int)s->h_t; p.h_b = s->h_b;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool pos = lengths || resets;
-  return by_dtype(s->dtype, [&](auto t) {
-    using T = decltype(t);
-    return pos ? scan_run<T, true>(p, sh, false, st) : scan_run<T, false>(p, sh, false, st);
-  });
+  return scan_run_forward(s->dtype, p, sh, pos, st);
 }
 
 size_t delrec_gated_scan_backward_workspace(const delrec_scan* s) {
@@ -208,11 +135,11 @@ int delrec_gated_scan_backward(const delrec_scan* s, const void* z, const void* 
   p.dz_t = (int)s->dz_t; p.dz_b = s->dz_b; p.df_t = (int)s->df_t; p.df_b = s->df_b;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool pos = lengths || resets;
+  rc = scan_run_backward(s->dtype, p, sh, pos, st);
+  if (rc || !df || !p.split) return rc;
   return by_dtype(s->dtype, [&](auto t) {
     using T = decltype(t);
-    const int r = pos ? scan_run<T, true>(p, sh, true, st) : scan_run<T, false>(p, sh, true, st);
-    if (r) return r;
-    if (df && p.split) {
+    {
       k_scan_df_sum<T><<<seq_grid((size_t)p.T * p.B * p.G, 256, 8), 256, 0, st>>>(p);
       SQ_LAUNCHED();
     }

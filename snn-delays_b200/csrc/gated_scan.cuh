@@ -232,19 +232,64 @@ struct Cursor {
 };
 
 
-// The biased exponent of a value's 8-bit scale before its offset of 6: the float's own, one
-// more where its mantissa is past 126 / 64.  Monotone in |v|, so the group's largest key is
-// the key of its largest value.  255: not finite, or at the scale whose codes are cut.
-__device__ __forceinline__ unsigned q_key(float v) {
-  return ((__float_as_uint(v) & 0x7fffffffu) + 0x3ffffu) >> 23;
+// A magnitude as an integer of the same order, 16 bits: a 16-bit float's own bits; of an fp32
+// value what its scale depends on, its exponent, one more where its mantissa is past 126 / 64.
+__device__ __forceinline__ unsigned q_key(unsigned magnitude_bits) { return (magnitude_bits + 0x3ffffu) >> 23; }
+template <class T, int V>
+__device__ __forceinline__ unsigned pack_key(const VecOf<T, V>& z, const VecOf<T, V>& f) {
+  if constexpr (sizeof(T) == 4) {
+    unsigned kz = 0, kf = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      kz = max(kz, __float_as_uint(to_f(z.v[k])) & 0x7fffffffu);
+      kf = max(kf, __float_as_uint(to_f(f.v[k])) & 0x7fffffffu);
+    }
+    return q_key(kz) | q_key(kf) << 16;
+  } else if constexpr (V == 2) {
+    const unsigned a = *(const unsigned*)&z & 0x7fff7fffu, c = *(const unsigned*)&f & 0x7fff7fffu;
+    unsigned r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(a, c, 0x5410)), "r"(__byte_perm(a, c, 0x7632)));
+    return r;
+  } else {
+    return (*(const unsigned short*)&z & 0x7fffu) | (*(const unsigned short*)&f & 0x7fffu) << 16;
+  }
+}
+// A key's scale key: the biased exponent + 6 (255: not finite, or the scale whose codes are cut).
+template <class T>
+__device__ __forceinline__ unsigned scale_key(unsigned key) {
+  if constexpr (sizeof(T) == 4) return key;
+  else if constexpr (std::is_same_v<T, __half>) return q_key(__float_as_uint(__half2float(__ushort_as_half((unsigned short)key))));
+  else return q_key(key << 16);
 }
 __device__ __forceinline__ unsigned q_key_exponent(unsigned key) { return key < 7u ? 1u : key - 6u; }
 // Low byte: rint(v / s).  v / s is exact and at most 126, the addition rounds it to even.
-__device__ __forceinline__ unsigned q_code(float v, unsigned ex) {
-  return __float_as_uint(fmaf(v, q_inverse_scale(ex), 12582912.f));
+__device__ __forceinline__ unsigned q_code(float v, float inv) { return __float_as_uint(fmaf(v, inv, 12582912.f)); }
+// both 16-bit halves' maxima
+__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) {
+  unsigned r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
-// |-| of two 16-bit keys at once
-__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) { return __vmaxu2(a, b); }
+// Maxima (of 16-bit halves) of 16 values over the W = 32 or 16 lanes of a group: a lane returns
+// that of value lane % 16.  Each exchange halves the values a lane is concerned with.
+template <int W>
+__device__ __forceinline__ unsigned group_max16(const unsigned (&x)[16], int lane) {
+  unsigned v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool up = lane & 8;
+    v[j] = max_u16x2(up ? x[j + 8] : x[j], __shfl_xor_sync(0xffffffffu, up ? x[j] : x[j + 8], 8));
+  }
+#pragma unroll
+  for (int w = 4; w > 0; w >>= 1) {
+    const bool up = lane & w;
+#pragma unroll
+    for (int j = 0; j < w; ++j)
+      v[j] = max_u16x2(up ? v[j + w] : v[j], __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + w], w));
+  }
+  if (W == 32) v[0] = max_u16x2(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
+  return v[0];
+}
 
 // Where a segment's 8-bit form goes.
 template <int V>
@@ -277,52 +322,47 @@ __device__ __noinline__ void scan_pack_slow(const VecOf<T, V>* r, int8_t* q, uin
     }
   }
 }
-// A segment's z and f in 8 bits; n: its steps below T.  A group is the 32 channels of 32 / V
-// lanes; the keys of z and f share a register on their way through the lanes.
-template <class T, int V, int S>
-__device__ __forceinline__ void scan_pack(const VecOf<T, V> (&zr)[S], const VecOf<T, V> (&fr)[S], const PackOut<V>& o,
-                                          int n, bool on, bool group_on, int lane) {
-  constexpr int W = 32 / V;
-  const int hl = lane & (W - 1);
-  unsigned mine = 0, top = 0;
+// A segment's z and f in 8 bits; n: its steps.  A group is the 32 channels of 32 / V lanes; the
+// keys of z and f share a register on their way through the lanes, and lane i of a group
+// makes the scales of step i.
+template <class T, int V>
+__device__ __forceinline__ void scan_pack(const VecOf<T, V> (&zr)[kSeg], const VecOf<T, V> (&fr)[kSeg],
+                                          const PackOut<V>& o, int n, bool on, bool group_on, int lane) {
+  constexpr int S = kSeg, W = 32 / V;
+  const int hl = lane & 15;
+  unsigned key[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) key[i] = pack_key<T, V>(zr[i], fr[i]);
+  const unsigned mine = group_max16<W>(key, lane);
+  const unsigned kz = scale_key<T>(mine & 0xffffu), kf = scale_key<T>(mine >> 16);
+  const unsigned ez = q_key_exponent(kz), ef = q_key_exponent(kf);
+  const float iz = q_inverse_scale(ez), jf = q_inverse_scale(ef);
+  const int src = lane & ~(W - 1);
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    float zv[V], fv[V];
-    unsigned kz = 0, kf = 0;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      zv[k] = to_f(zr[i].v[k]);
-      fv[k] = to_f(fr[i].v[k]);
-      kz = max(kz, __float_as_uint(zv[k]) & 0x7fffffffu);
-      kf = max(kf, __float_as_uint(fv[k]) & 0x7fffffffu);
-    }
-    unsigned key = q_key(__uint_as_float(kz)) | q_key(__uint_as_float(kf)) << 16;
-#pragma unroll
-    for (int s = W / 2; s > 0; s >>= 1) key = max_u16x2(key, __shfl_xor_sync(0xffffffffu, key, s));
-    top = max_u16x2(top, key);
-    if (hl == i) mine = key;
-    const unsigned ez = q_key_exponent(key & 0xffffu), ef = q_key_exponent(key >> 16);
+    const float sz = __shfl_sync(0xffffffffu, iz, src + i), sf = __shfl_sync(0xffffffffu, jf, src + i);
     unsigned cz[V], cf[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      cz[k] = q_code(zv[k], ez);
-      cf[k] = q_code(fv[k], ef);
+      cz[k] = q_code(to_f(zr[i].v[k]), sz);
+      cf[k] = q_code(to_f(fr[i].v[k]), sf);
     }
     if (on && i < n) {
       store_codes<V>(at_step(o.qz, o.stride, i), cz);
       store_codes<V>(at_step(o.qf, o.stride, i), cf);
     }
   }
-  if (group_on && hl < n && hl < S) {
-    o.ez[(long long)hl * o.estride] = (uint8_t)q_key_exponent(mine & 0xffffu);
-    o.ef[(long long)hl * o.estride] = (uint8_t)q_key_exponent(mine >> 16);
+  const bool teller = group_on && (lane & (W - 1)) < S && hl < n;
+  if (teller) {
+    o.ez[(long long)hl * o.estride] = (uint8_t)ez;
+    o.ef[(long long)hl * o.estride] = (uint8_t)ef;
   }
-  const bool head = group_on && hl == 0;
-  if (head) *o.odd = (top & 0xffffu) >= 255u || (top >> 16) >= 255u;
-  if (__any_sync(0xffffffffu, (top & 0xffffu) >= 255u))
-    scan_pack_slow<T, V, S>(zr, o.qz, o.ez, o.stride, o.estride, n, on, head);
-  if (__any_sync(0xffffffffu, (top >> 16) >= 255u))
-    scan_pack_slow<T, V, S>(fr, o.qf, o.ef, o.stride, o.estride, n, on, head);
+  const unsigned odd_z = __ballot_sync(0xffffffffu, kz >= 255u), odd_f = __ballot_sync(0xffffffffu, kf >= 255u);
+  const bool head = group_on && (lane & (W - 1)) == 0;
+  const unsigned group = V == 1 ? 0xffffffffu : 0xffffu << src;
+  if (head) *o.odd = ((odd_z | odd_f) & group) != 0;
+  if (odd_z) scan_pack_slow<T, V, S>(zr, o.qz, o.ez, o.stride, o.estride, n, on, head);
+  if (odd_f) scan_pack_slow<T, V, S>(fr, o.qf, o.ef, o.stride, o.estride, n, on, head);
 }
 
 // Sum of v over the lanes of a gate of D < 32 lanes (d: the lane's place in it), in the
@@ -366,7 +406,7 @@ struct ScanFwd {
   // 16-bit pairs and packing take 128 registers, single channels 80
   static constexpr int WARPS = V == 2 || PACK ? 16 : 24;
 };
-template <class T, int V, int P, bool POS, bool PACK, int MODE>
+template <class T, int V, int P, bool POS, bool PACK, bool DI, int MODE>
 __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WARPS / P) k_scan_fwd(ScanArgs p, int csize) {
   using K = ScanFwd<T, V, P, POS, PACK, MODE>;
   constexpr int S = kSeg, ROWB = K::ROWB;
@@ -408,80 +448,84 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
       for (int k = 0; k < V; ++k) v[k] = (pl.on && p.h0) ? p.h0[(size_t)b * p.N + pl.c + k] : 0.f;
     }
     const unsigned cut = POS ? scan_resets(p, b, tb, len, lane) : 0u;
-    VecOf<T, V> zr[S], fr[S];
-    float wide = 0.f;
-    int edge = 32;
-    if constexpr (MODE == SCAN_STAGED) {
+    if (MODE == SCAN_STAGED) {
       stage_wait<1>();
       __syncwarp();
-      const char* r = mine + buf * K::STAGE + lane * V * (int)sizeof(T);
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        zr[i] = *(const VecOf<T, V>*)(r + i * ROWB);
-        fr[i] = *(const VecOf<T, V>*)(r + (S + i) * ROWB);
-      }
-    } else {
-      static_assert(V == 1, "plain loads take one channel to a lane");
-      T r[S];
-      direct_rows<T>((const T*)p.z + b * p.z_b + pl.c + (long long)tb * p.z_t, p.z_t, n, pl.on, r);
-#pragma unroll
-      for (int i = 0; i < S; ++i) zr[i].v[0] = r[i];
-      if constexpr (MODE == SCAN_DIRECT) {
-        direct_rows<T>((const T*)p.f + b * p.f_b + pl.g + (long long)tb * p.f_t, p.f_t, n, pl.on, r);
-#pragma unroll
-        for (int i = 0; i < S; ++i) fr[i].v[0] = r[i];
-      } else {
-        const int g0 = tile * 32 / p.D, g = g0 + (lane >> 4), i = lane & 15;
-        edge = (g0 + 1) * p.D - tile * 32;
-        const bool ok = g < p.G && i < n;
-        wide = gate_fold<Accurate<T>::value>(
-            ok ? to_f(((const T*)p.f)[b * p.f_b + g + (long long)(tb + i) * p.f_t]) : 0.f);
-      }
-    }
-    if (PACK && tb < p.T) {
-      const size_t row = (size_t)tb * p.B + b;
-      const int groups = (p.N + kQGroup - 1) / kQGroup, grp = tile * V + lane * V / 32;
-      PackOut<V> o;
-      o.qz = p.qz + row * p.N + pl.c; o.qf = p.qf + row * p.N + pl.c;
-      o.ez = p.ez + row * groups + grp; o.ef = p.ef + row * groups + grp;
-      o.stride = p.B * p.N; o.estride = p.B * groups;
-      o.odd = p.odd + ((size_t)(tb / kSeg) * p.B + b) * groups + grp;
-      scan_pack<T, V, S>(zr, fr, o, p.T - tb, pl.on, grp < groups, lane);
     }
     float a[S][V], x[S][V];
     float2 m[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
+    if (n > 0) {   // else the identity: past the sequence's end
+      VecOf<T, V> zr[S], fr[S];
+      float wide = 0.f;
+      int edge = 32;
+      if constexpr (MODE == SCAN_STAGED) {
+        const char* r = mine + buf * K::STAGE + lane * V * (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      float w = 0.f;
-      if (MODE == SCAN_WIDE) w = __shfl_sync(0xffffffffu, wide, i + (lane >= edge ? 16 : 0));
+        for (int i = 0; i < S; ++i) {
+          zr[i] = *(const VecOf<T, V>*)(r + i * ROWB);
+          fr[i] = *(const VecOf<T, V>*)(r + (S + i) * ROWB);
+        }
+      } else {
+        static_assert(V == 1, "plain loads take one channel to a lane");
+        T r[S];
+        direct_rows<T>((const T*)p.z + b * p.z_b + pl.c + (long long)tb * p.z_t, p.z_t, n, pl.on, r);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float zf = to_f(zr[i].v[k]);
-        float om;
-        if (MODE == SCAN_WIDE) gate_unfold(w, a[i][k], om);
-        else sigmoid_pair<Accurate<T>::value>(to_f(fr[i].v[k]), a[i][k], om);
-        x[i][k] = p.decay_input ? om * zf : zf;
+        for (int i = 0; i < S; ++i) zr[i].v[0] = r[i];
+        if constexpr (MODE == SCAN_DIRECT) {
+          direct_rows<T>((const T*)p.f + b * p.f_b + pl.g + (long long)tb * p.f_t, p.f_t, n, pl.on, r);
+#pragma unroll
+          for (int i = 0; i < S; ++i) fr[i].v[0] = r[i];
+        } else {
+          const int g0 = tile * 32 / p.D, g = g0 + (lane >> 4), i = lane & 15;
+          edge = (g0 + 1) * p.D - tile * 32;
+          const bool ok = g < p.G && i < n;
+          wide = gate_fold<Accurate<T>::value>(
+              ok ? to_f(((const T*)p.f)[b * p.f_b + g + (long long)(tb + i) * p.f_t]) : 0.f);
+        }
       }
-    }
-    if (n < S) {
+      if (PACK) {
+        const size_t row = (size_t)tb * p.B + b;
+        const int groups = (p.N + kQGroup - 1) / kQGroup, grp = tile * V + lane * V / 32;
+        PackOut<V> o;
+        o.qz = p.qz + row * p.N + pl.c; o.qf = p.qf + row * p.N + pl.c;
+        o.ez = p.ez + row * groups + grp; o.ef = p.ef + row * groups + grp;
+        o.stride = p.B * p.N; o.estride = p.B * groups;
+        o.odd = p.odd + ((size_t)(tb / kSeg) * p.B + b) * groups + grp;
+        scan_pack<T, V>(zr, fr, o, n, pl.on, grp < groups, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        float w = 0.f;
+        if (MODE == SCAN_WIDE) w = __shfl_sync(0xffffffffu, wide, i + (lane >= edge ? 16 : 0));
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float zf = to_f(zr[i].v[k]);
+          float om;
+          if (MODE == SCAN_WIDE) gate_unfold(w, a[i][k], om);
+          else sigmoid_pair<Accurate<T>::value>(to_f(fr[i].v[k]), a[i][k], om);
+          x[i][k] = DI ? om * zf : zf;
+        }
+      }
+      if (n < S) {
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (i >= n) { a[i][k] = 1.f; x[i][k] = 0.f; }
+      }
 #pragma unroll
       for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (i >= n) { a[i][k] = 1.f; x[i][k] = 0.f; }
-    }
+        for (int k = 0; k < V; ++k) {
+          if (POS && ((cut >> i) & 1)) m[k] = make_float2(0.f, x[i][k]);
+          else m[k] = make_float2(m[k].x * a[i][k], fmaf(a[i][k], m[k].y, x[i][k]));
+        }
+      if (POS && cut) {
 #pragma unroll
-    for (int i = 0; i < S; ++i)
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (POS && ((cut >> i) & 1)) m[k] = make_float2(0.f, x[i][k]);
-        else m[k] = make_float2(m[k].x * a[i][k], fmaf(a[i][k], m[k].y, x[i][k]));
+        for (int k = 0; k < V; ++k) m[k].x = -0.f;
       }
-    if (POS && cut) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) m[k].x = -0.f;
     }
     float s[V];
     scan_exchange<P, V, POS>(sm, buf, warp, lane, rank, csize, m, v, s);
@@ -511,7 +555,7 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
           VecOf<T, V> o;
 #pragma unroll
           for (int k = 0; k < V; ++k) {
-            s[k] = (POS && ((cut >> i) & 1)) ? x[i][k] : fmaf(a[i][k], s[k], x[i][k]);
+            if (i < n) s[k] = (POS && ((cut >> i) & 1)) ? x[i][k] : fmaf(a[i][k], s[k], x[i][k]);
             o.v[k] = from_f<T>(i < n ? s[k] : 0.f);
           }
           if (i < nT) *(VecOf<T, V>*)at_step(h, p.h_t, i) = o;
@@ -531,20 +575,40 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
 // ---------------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------------
-// A code as a float without its scale: the byte (offset by 128) as the mantissa of 2^23.
-__device__ __forceinline__ float code_value(unsigned offset_code) {
-  return __uint_as_float(0x4b000000u | offset_code) - 8388736.f;
+// Code k of a pair as a float without its scale: the byte (offset by 128) as the mantissa of 2^23.
+template <int V>
+__device__ __forceinline__ float code_value(const RawBytes<V>& r, int k) {
+  const unsigned x = V == 2 ? *(const unsigned short*)&r ^ 0x8080u : (unsigned)(uint8_t)r.b[0] ^ 0x80u;
+  return __uint_as_float(__byte_perm(x, 0x4b000000u, k ? 0x7651 : 0x7650)) - 8388736.f;
 }
 
-// What a backward segment reads: z and f as values or codes, g = gh, the scales of the steps
-// spread over the lanes (lane j: step j, or step j / 2 of group j & 1 for V = 2), this lane's
-// share of the gates (WIDE).
-template <class T, int V, bool B8>
+// What a backward segment reads: z and f as values or codes, g = gh (staged rows are read from
+// shared memory where they are needed, so that they hold no registers), the scales of the
+// steps spread over the lanes (lane j: step j, or step j / 2 of group j & 1 for V = 2), this
+// lane's share of the gates (WIDE).
+template <class T, int V, bool B8, int MODE>
 struct ScanIn {
-  RawBytes<(B8 ? 1 : (int)sizeof(T)) * V> z[kSeg], f[kSeg];
-  VecOf<T, V> g[kSeg];
+  static constexpr int E = B8 ? 1 : (int)sizeof(T), ROWB = 32 * V * E, ROWG = 32 * V * (int)sizeof(T);
+  static constexpr bool STAGED = MODE == SCAN_STAGED;
+  using Raw = RawBytes<E * V>;
+  const char *zf_row, *g_row;   // this lane's place in the staged rows
+  Raw z_[STAGED ? 1 : kSeg], f_[STAGED || MODE == SCAN_WIDE ? 1 : kSeg];
+  VecOf<T, V> g_[STAGED ? 1 : kSeg];
   float sz, sf, wide;
   int edge;
+  __device__ __forceinline__ Raw z(int i) const {
+    if constexpr (STAGED) return *(const Raw*)(zf_row + i * ROWB);
+    else return z_[i];
+  }
+  __device__ __forceinline__ Raw f(int i) const {
+    if constexpr (STAGED) return *(const Raw*)(zf_row + (kSeg + i) * ROWB);
+    else if constexpr (MODE == SCAN_DIRECT) return f_[i];
+    else return f_[0];
+  }
+  __device__ __forceinline__ VecOf<T, V> g(int i) const {
+    if constexpr (STAGED) return *(const VecOf<T, V>*)(g_row + i * ROWG);
+    else return g_[i];
+  }
 };
 template <class T, int V>
 __device__ __forceinline__ float raw_value(const RawBytes<(int)sizeof(T) * V>& r, int k) {
@@ -555,8 +619,8 @@ __device__ __forceinline__ float raw_value(const RawBytes<(int)sizeof(T) * V>& r
 // of the reverse recurrence, in forward order: G enters at the end times Pi a, and g_i times
 // the gates up to i.  PLAIN: all 16 steps are inside the sequence, no code stands for an infinity
 // or NaN.
-template <class T, int V, bool POS, bool B8, int MODE, bool PLAIN>
-__device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, B8>& r, unsigned cut, int n, int lane,
+template <class T, int V, bool POS, bool B8, bool DI, int MODE, bool PLAIN>
+__device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, B8, MODE>& r, unsigned cut, int n, int lane,
                                           float (&s)[V], float (&w)[kSeg][V], float (&e)[kSeg][V], float2 (&m)[V]) {
 #pragma unroll
   for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
@@ -569,20 +633,20 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, 
       sf = __shfl_sync(0xffffffffu, r.sf, src);
     }
     if (MODE == SCAN_WIDE) ww = __shfl_sync(0xffffffffu, r.wide, i + (lane >= r.edge ? 16 : 0));
+    const auto zi = r.z(i), fi = r.f(i);
+    const VecOf<T, V> gi = r.g(i);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float zf, ff = 0.f;
       if constexpr (!B8) {
-        zf = raw_value<T, V>(r.z[i], k);
-        if (MODE != SCAN_WIDE) ff = raw_value<T, V>(r.f[i], k);
+        zf = raw_value<T, V>(zi, k);
+        if (MODE != SCAN_WIDE) ff = raw_value<T, V>(fi, k);
       } else if constexpr (!PLAIN) {
-        zf = q_decode((int8_t)r.z[i].b[k], sz);
-        ff = q_decode((int8_t)r.f[i].b[k], sf);
+        zf = q_decode((int8_t)zi.b[k], sz);
+        ff = q_decode((int8_t)fi.b[k], sf);
       } else {
-        zf = code_value((uint8_t)r.z[i].b[k] ^ 0x80u);
-        ff = code_value((uint8_t)r.f[i].b[k] ^ 0x80u);
-        zf *= sz;
-        ff *= sf;
+        zf = code_value<V>(zi, k) * sz;
+        ff = code_value<V>(fi, k) * sf;
       }
       float a, om, both;   // both = a (1 - a)
       if (MODE == SCAN_WIDE) {
@@ -596,16 +660,16 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, 
         a = pos ? big : small;
         om = pos ? small : big;
         both = big * small;
-        w[i][k] = pos ? small : -small;
+        w[i][k] = __uint_as_float(__float_as_uint(small) | (__float_as_uint(ff) & 0x80000000u));
       }
       if (POS && ((cut >> i) & 1)) s[k] = 0.f;
-      e[i][k] = both * (p.decay_input ? s[k] - zf : s[k]);
-      s[k] = fmaf(a, s[k], p.decay_input ? om * zf : zf);
+      e[i][k] = both * (DI ? s[k] - zf : s[k]);
+      s[k] = fmaf(a, s[k], DI ? om * zf : zf);
       if (POS && (cut & ((2u << i) - 1))) {
         m[k].x = 0.f;
       } else if (PLAIN || i < n) {
         m[k].x *= a;
-        m[k].y = fmaf(m[k].x, to_f(r.g[i].v[k]), m[k].y);
+        m[k].y = fmaf(m[k].x, to_f(gi.v[k]), m[k].y);
       }
     }
   }
@@ -613,20 +677,20 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, 
 
 // The walk back: q is the gradient that enters the segment's last step.  WHOLE: all its
 // steps are inside the sequence.  e[i] becomes df.
-template <class T, int V, bool POS, bool WHOLE, class G>
-__device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const G& g, const float (&w)[kSeg][V],
+template <class T, int V, bool POS, bool DI, bool WHOLE, class In>
+__device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const In& r, const float (&w)[kSeg][V],
                                                float (&e)[kSeg][V], float (&q)[V], unsigned cut, int n, int nT, T* dz,
                                                T* df) {
 #pragma unroll
   for (int i = kSeg - 1; i >= 0; --i) {
-    const VecOf<T, V> gi = g(i);
+    const VecOf<T, V> gi = r.g(i);
     VecOf<T, V> oz, of;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float a, om;
       gate_unfold(w[i][k], a, om);
       const float G_ = q[k] + to_f(gi.v[k]);
-      float dzv = p.decay_input ? om * G_ : G_, dfv = e[i][k] * G_;
+      float dzv = DI ? om * G_ : G_, dfv = e[i][k] * G_;
       float nq = (POS && ((cut >> i) & 1)) ? 0.f : a * G_;
       if (!WHOLE && i >= n) { dzv = 0.f; dfv = 0.f; nq = q[k]; }
       q[k] = nq;
@@ -649,7 +713,7 @@ struct ScanBwd {
   static constexpr int STAGE = MODE == SCAN_STAGED ? S * (2 * ROWB + ROWG) : 0;
   static constexpr int SMEM = 2 * P * STAGE;
 };
-template <class T, int V, int P, bool POS, bool B8, int MODE>
+template <class T, int V, int P, bool POS, bool B8, bool DI, int MODE>
 __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csize) {
   using K = ScanBwd<T, V, P, B8, MODE>;
   using E = std::conditional_t<B8, int8_t, T>;
@@ -718,7 +782,7 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
     const Place pl = scan_place<V>(p, tile, lane);
     const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
     const int tb = cur.wv * wave + seg * S, n = len - tb, nT = p.T - tb;
-    ScanIn<T, V, B8> r;
+    ScanIn<T, V, B8, MODE> r;
     r.sz = sz_ahead; r.sf = sf_ahead; r.wide = 0.f; r.edge = 32;
     int odd = odd_ahead;
     float s[V];
@@ -731,38 +795,26 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
       for (int k = 0; k < V; ++k) v[k] = (pl.on && p.ghT) ? p.ghT[(size_t)b * p.N + pl.c + k] : 0.f;
     }
     const unsigned cut = POS ? scan_resets(p, b, tb, len, lane) : 0u;
-    const char* rows = mine + buf * K::STAGE;
-    auto read = [&]() {
-      if constexpr (MODE == SCAN_STAGED) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          r.z[i] = *(const RawBytes<K::E * V>*)(rows + i * ROWB + lane * K::E * V);
-          r.f[i] = *(const RawBytes<K::E * V>*)(rows + (S + i) * ROWB + lane * K::E * V);
-          r.g[i] = *(const VecOf<T, V>*)(rows + 2 * S * ROWB + i * ROWG + lane * V * (int)sizeof(T));
-        }
-      } else {
-        static_assert(V == 1, "plain loads take one channel to a lane");
-        E x[S];
-        direct_rows<E>(zp + b * z_b + pl.c + (long long)tb * z_t, z_t, n, pl.on, x);
-#pragma unroll
-        for (int i = 0; i < S; ++i) memcpy(&r.z[i], &x[i], sizeof(E));
-        if constexpr (MODE == SCAN_DIRECT) {
-          direct_rows<E>(fp + b * f_b + pl.g + (long long)tb * f_t, f_t, n, pl.on, x);
-#pragma unroll
-          for (int i = 0; i < S; ++i) memcpy(&r.f[i], &x[i], sizeof(E));
-        }
-        T y[S];
-        direct_rows<T>((const T*)p.gh + b * p.gh_b + pl.c + (long long)tb * p.gh_t, p.gh_t, n, pl.on && p.gh, y);
-#pragma unroll
-        for (int i = 0; i < S; ++i) r.g[i].v[0] = y[i];
-      }
-    };
-    if (MODE == SCAN_STAGED) {
+    r.zf_row = mine + buf * K::STAGE + lane * K::E * V;
+    r.g_row = mine + buf * K::STAGE + 2 * S * ROWB + lane * V * (int)sizeof(T);
+    if constexpr (MODE == SCAN_STAGED) {
       stage_wait<1>();
       __syncwarp();
-    }
-    read();
-    if (MODE != SCAN_STAGED) {
+    } else {
+      static_assert(V == 1, "plain loads take one channel to a lane");
+      E x[S];
+      T y[S];
+      direct_rows<E>(zp + b * z_b + pl.c + (long long)tb * z_t, z_t, n, pl.on, x);
+#pragma unroll
+      for (int i = 0; i < S; ++i) memcpy(&r.z_[i], &x[i], sizeof(E));
+      if constexpr (MODE == SCAN_DIRECT) {
+        direct_rows<E>(fp + b * f_b + pl.g + (long long)tb * f_t, f_t, n, pl.on, x);
+#pragma unroll
+        for (int i = 0; i < S; ++i) memcpy(&r.f_[i], &x[i], sizeof(E));
+      }
+      direct_rows<T>((const T*)p.gh + b * p.gh_b + pl.c + (long long)tb * p.gh_t, p.gh_t, n, pl.on && p.gh, y);
+#pragma unroll
+      for (int i = 0; i < S; ++i) r.g_[i].v[0] = y[i];
       state(b, pl, tb, s);
       if (B8) scales(b, tile, tb, n, r.sz, r.sf, odd);
     }
@@ -776,8 +828,12 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
     }
     float w[S][V], e[S][V];
     float2 m[V];
-    if (n >= S && !odd) scan_walk<T, V, POS, B8, MODE, true>(p, r, cut, n, lane, s, w, e, m);
-    else scan_walk<T, V, POS, B8, MODE, false>(p, r, cut, n, lane, s, w, e, m);
+#pragma unroll
+    for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
+    if (n > 0) {   // else the identity: past the sequence's end
+      if (n >= S && !odd) scan_walk<T, V, POS, B8, DI, MODE, true>(p, r, cut, n, lane, s, w, e, m);
+      else scan_walk<T, V, POS, B8, DI, MODE, false>(p, r, cut, n, lane, s, w, e, m);
+    }
     if (POS && cut) {
 #pragma unroll
       for (int k = 0; k < V; ++k) m[k].x = -0.f;
@@ -786,27 +842,33 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
     scan_exchange<P, V, POS>(sm, buf, warp, lane, rank, csize, m, v, q);
     T* dz = pl.on && p.dz ? (T*)p.dz + b * p.dz_b + pl.c + (long long)tb * p.dz_t : nullptr;
     T* df = pl.on && p.df && p.D == 1 ? (T*)p.df + b * p.df_b + pl.c + (long long)tb * p.df_t : nullptr;
-    // staged rows are read again rather than kept
-    auto g = [&](int i) -> VecOf<T, V> {
-      if constexpr (MODE == SCAN_STAGED)
-        return *(const VecOf<T, V>*)(rows + 2 * S * ROWB + i * ROWG + lane * V * (int)sizeof(T));
-      else
-        return r.g[i];
-    };
-    if (n >= S) scan_walk_back<T, V, POS, true>(p, g, w, e, q, cut, n, nT, dz, df);
-    else scan_walk_back<T, V, POS, false>(p, g, w, e, q, cut, n, nT, dz, df);
+    if (n >= S) {
+      scan_walk_back<T, V, POS, DI, true>(p, r, w, e, q, cut, n, nT, dz, df);
+    } else if (n > 0) {
+      scan_walk_back<T, V, POS, DI, false>(p, r, w, e, q, cut, n, nT, dz, df);
+    } else {
+      VecOf<T, V> o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) o.v[k] = from_f<T>(0.f);
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (i < nT) {
+          if (dz) *(VecOf<T, V>*)at_step(dz, p.dz_t, i) = o;
+          if (df) *(VecOf<T, V>*)at_step(df, p.df_t, i) = o;
+        }
+    }
     if constexpr (MODE == SCAN_WIDE) {
       if (p.df) {
         // the tile's channels of its first gate, and of the one it reaches into
         float x[S];
 #pragma unroll
-        for (int i = 0; i < S; ++i) x[i] = pl.on && lane < r.edge ? e[i][0] : 0.f;
+        for (int i = 0; i < S; ++i) x[i] = pl.on && n > 0 && lane < r.edge ? e[i][0] : 0.f;
         const int t = tb + (lane >> 1);
         const float s0 = warp_sum16(x, lane);
         float s1 = 0.f;
         if (r.edge < 32) {
 #pragma unroll
-          for (int i = 0; i < S; ++i) x[i] = pl.on && lane >= r.edge ? e[i][0] : 0.f;
+          for (int i = 0; i < S; ++i) x[i] = pl.on && n > 0 && lane >= r.edge ? e[i][0] : 0.f;
           s1 = warp_sum16(x, lane);
         }
         if (t < p.T) p.part[(((size_t)t * p.B + b) * p.tiles + tile) * 2 + (lane & 1)] = lane & 1 ? s1 : s0;
@@ -817,7 +879,7 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
         const int d = pl.c - pl.g * p.D;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-          const float x = gate_sum(pl.on ? e[i][0] : 0.f, d, p.D);
+          const float x = gate_sum(pl.on && n > 0 ? e[i][0] : 0.f, d, p.D);
           if (pl.on && d == 0 && i < nT) *at_step(o, p.df_t, i) = from_f<T>(x);
         }
       }
@@ -870,5 +932,17 @@ __global__ void __launch_bounds__(128) k_gated_step(int B, int N, int D, int dec
     next[e] = s;
   }
 }
+
+
+// ---------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------
+struct ScanShape {
+  int V, P, csize, mode;
+  unsigned grid;
+};
+// the kernels of a direction, by element type (gated_fwd.cu, gated_bwd.cu)
+int scan_run_forward(int dtype, ScanArgs& p, const ScanShape& sh, bool pos, cudaStream_t st);
+int scan_run_backward(int dtype, ScanArgs& p, const ScanShape& sh, bool pos, cudaStream_t st);
 
 }  // namespace delrec

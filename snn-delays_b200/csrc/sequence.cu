@@ -72,20 +72,22 @@ static int norm_start(K kern, int row_bytes, const NormArgs& a, NormShape& s, in
   SQ_LAUNCHED();
   return DELREC_OK;
 }
-template <class T, int V, bool BWD, bool GATE, int IT = 1>
+template <class T, int V, bool BWD, int KIND, int IT = 1>
 static int norm_by_it(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
   if constexpr (V * IT <= 32) {
-    if (s.IT != IT) return norm_by_it<T, V, BWD, GATE, 2 * IT>(a, s, most, st);
+    if (s.IT != IT) return norm_by_it<T, V, BWD, KIND, 2 * IT>(a, s, most, st);
     if constexpr (BWD)
-      return norm_start(k_norm_bwd<T, V, IT, GATE>, NormStage<T, V, IT, GATE ? 5 : 4>::ROW, a, s, most, st);
+      return norm_start(k_norm_bwd<T, V, IT, KIND>, NormStage<T, V, IT, KIND ? 5 : 4>::ROW, a, s, most, st);
     else
-      return norm_start(k_norm_fwd<T, V, IT, GATE>, NormStage<T, V, IT, GATE ? 3 : 2>::ROW, a, s, most, st);
+      return norm_start(k_norm_fwd<T, V, IT, KIND>, NormStage<T, V, IT, KIND ? 3 : 2>::ROW, a, s, most, st);
   }
   return DELREC_ERR_UNSUPPORTED;
 }
 template <class T, int V, bool BWD>
 static int norm_by_gate(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
-  return a.kind == GATE_NONE ? norm_by_it<T, V, BWD, false>(a, s, most, st) : norm_by_it<T, V, BWD, true>(a, s, most, st);
+  if (a.kind == GATE_NONE) return norm_by_it<T, V, BWD, GATE_NONE>(a, s, most, st);
+  if (a.kind == GATE_SIGMOID) return norm_by_it<T, V, BWD, GATE_SIGMOID>(a, s, most, st);
+  return norm_by_it<T, V, BWD, GATE_SILU>(a, s, most, st);
 }
 // the widest access the tensors allow, 16 bytes at most
 template <class T, bool BWD>
