@@ -27,6 +27,7 @@ static constexpr int kNormThreads = 512;
 
 struct NormArgs {
   int T, B, N, wide, kind;              // kind: the gate's function, where there is one
+  int slots;                            // rows in shared memory: one at work, the others on their way
   float eps;
   const void* lengths;
   const void *x, *y, *u;
@@ -77,24 +78,22 @@ __device__ __forceinline__ const T* row_of(const void* p, const NormRow& r, int 
 }
 
 // The inputs of a row, NT tensors of IT vectors per thread.  Vectors of 4 bytes and more are
-// copied into shared memory (cp.async) while the row before is worked on; every thread
+// copied into shared memory (cp.async) while rows before are worked on; every thread
 // copies what it will read itself, so no barrier is needed.  A vector of all threads lies side
 // by side: copies that scatter a thread's vectors over shared memory cost a third more time.
 template <class T, int V, int IT, int NT>
 struct NormStage {
   static constexpr int VB = V * (int)sizeof(T);
-  static constexpr bool STAGED = VB >= 4 && IT <= 2;
+  static constexpr bool STAGED = VB >= 4 && VB * IT <= 32;   // two rows of 5 tensors and 512 threads fit 160 KB
   static constexpr int ROW = STAGED ? NT * IT * VB : 0;   // bytes per thread and row
-  unsigned base[2];
-  const char* mem[2];
-  int plane;   // bytes of one vector of all threads
+  unsigned base;
+  const char* mem;
+  int plane, size;   // bytes of one vector of all threads, of a slot
   __device__ __forceinline__ NormStage(char* m) {
     plane = blockDim.x * VB;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mem[h] = m + h * (int)blockDim.x * ROW + threadIdx.x * VB;
-      base[h] = STAGED ? (unsigned)__cvta_generic_to_shared(mem[h]) : 0;
-    }
+    size = blockDim.x * ROW;
+    mem = m + threadIdx.x * VB;
+    base = STAGED ? (unsigned)__cvta_generic_to_shared(mem) : 0;
   }
   // col: this thread's first channel in the row
   __device__ __forceinline__ void copy(unsigned at, int ten, const T* col, int left, int nthV) const {
@@ -114,9 +113,12 @@ struct NormStage {
   __device__ __forceinline__ void commit() const {
     if (STAGED) asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  template <int LEFT>
-  __device__ __forceinline__ void wait() const {
-    if (STAGED) asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+  // until the row at work is there: the slots - 1 rows copied after it may be on their way
+  __device__ __forceinline__ void wait(int slots) const {
+    if (!STAGED) return;
+    if (slots == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (slots == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   // vector k of tensor ten as floats; zeros past the row's end
   __device__ __forceinline__ void read(const char* at, int ten, int k, const T* col, int left, int nthV, float* o) const {
@@ -184,17 +186,24 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
     }
     st.commit();
   };
-  NormRow cur;
+  NormRow cur, ahead;
   cur.init(blockIdx.x, p.B);
-  bool live = live_row(cur);
-  fetch(cur, st.base[0], live);
-  for (int half = 0; cur.r < rows; half ^= 1) {
-    NormRow nxt = cur;
-    nxt.next(gs, gt, gb, p.B);
-    const bool next_live = nxt.r < rows && live_row(nxt);
-    fetch(nxt, half ? st.base[0] : st.base[1], next_live);
-    const char* at = half ? st.mem[1] : st.mem[0];
-    st.template wait<1>();
+  ahead = cur;
+  unsigned lives = 0;   // bit k: row k of those under way, from the one at work on
+  for (int k = 0; k < p.slots - 1; ++k) {
+    const bool l = ahead.r < rows && live_row(ahead);
+    lives |= (unsigned)l << k;
+    fetch(ahead, st.base + k * st.size, l);
+    ahead.next(gs, gt, gb, p.B);
+  }
+  for (int slot_now = 0; cur.r < rows; slot_now = slot_now == p.slots - 1 ? 0 : slot_now + 1) {
+    const bool live = lives & 1;
+    const bool l = ahead.r < rows && live_row(ahead);
+    fetch(ahead, st.base + (slot_now ? slot_now - 1 : p.slots - 1) * st.size, l);
+    lives = (lives >> 1) | (unsigned)l << (p.slots - 2);
+    ahead.next(gs, gt, gb, p.B);
+    const char* at = st.mem + slot_now * st.size;
+    st.wait(p.slots);
     float x[E], y[E], u[E];
     if (live) {
 #pragma unroll
@@ -251,10 +260,9 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
           store_vec<T, V>(o + k * nthV, v);
         }
     }
-    cur = nxt;
-    live = next_live;
+    cur.next(gs, gt, gb, p.B);
   }
-  st.template wait<0>();
+  st.wait(0);
 }
 
 template <class T, int V, int IT, int KIND>
@@ -286,34 +294,48 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
   auto gxr = [&](const NormRow& r) { return row_of<T>(p.gx, r, p.gx_t, p.gx_b) + c0; };
   auto gnr = [&](const NormRow& r) { return row_of<T>(p.gn, r, p.gn_t, p.gn_b) + c0; };
   auto live_row = [&](const NormRow& r) { return !p.lengths || r.t < row_length(p.lengths, p.wide, r.b, p.T); };
-  float ry_ahead = 0.f, rx_ahead = 0.f;
   auto fetch = [&](const NormRow& r, unsigned at, bool live) {
     if (live) {
       if (p.gx) st.copy(at, 0, gxr(r), left, nthV);
       if (p.gn) {
         st.copy(at, 1, gnr(r), left, nthV);
         st.copy(at, 2, xr(r), left, nthV);
-        rx_ahead = p.rx[r.r];
       }
       if (p.y) {
         st.copy(at, 3, yr(r), left, nthV);
         if (GATE) st.copy(at, 4, ur(r), left, nthV);
-        ry_ahead = p.ry[r.r];
       }
     }
     st.commit();
   };
-  NormRow cur;
+  NormRow cur, ahead;
   cur.init(blockIdx.x, p.B);
-  bool live = live_row(cur);
-  fetch(cur, st.base[0], live);
-  for (int half = 0; cur.r < rows; half ^= 1) {
+  ahead = cur;
+  unsigned lives = 0;   // bit k: row k of those under way, from the one at work on
+  for (int k = 0; k < p.slots - 1; ++k) {
+    const bool l = ahead.r < rows && live_row(ahead);
+    lives |= (unsigned)l << k;
+    fetch(ahead, st.base + k * st.size, l);
+    ahead.next(gs, gt, gb, p.B);
+  }
+  // the kept 1/rms of the row at work, read a row ahead
+  auto kept = [&](int r, float& y, float& x) {
+    if (r < rows) {
+      if (p.y) y = p.ry[r];
+      if (p.gn) x = p.rx[r];
+    }
+  };
+  float ry_ahead = 0.f, rx_ahead = 0.f;
+  kept(cur.r, ry_ahead, rx_ahead);
+  for (int slot_now = 0; cur.r < rows; slot_now = slot_now == p.slots - 1 ? 0 : slot_now + 1) {
+    const bool live = lives & 1;
     const float ry = ry_ahead, rx = rx_ahead;
-    NormRow nxt = cur;
-    nxt.next(gs, gt, gb, p.B);
-    const bool next_live = nxt.r < rows && live_row(nxt);
-    fetch(nxt, half ? st.base[0] : st.base[1], next_live);
-    const char* at = half ? st.mem[1] : st.mem[0];
+    kept(cur.r + gs, ry_ahead, rx_ahead);
+    const bool l = ahead.r < rows && live_row(ahead);
+    fetch(ahead, st.base + (slot_now ? slot_now - 1 : p.slots - 1) * st.size, l);
+    lives = (lives >> 1) | (unsigned)l << (p.slots - 2);
+    ahead.next(gs, gt, gb, p.B);
+    const char* at = st.mem + slot_now * st.size;
     T* dx = p.dx ? row_of<T>(p.dx, cur, p.dx_t, p.dx_b) + c0 : nullptr;
     T* dy = p.dy ? row_of<T>(p.dy, cur, p.dy_t, p.dy_b) + c0 : nullptr;
     T* du = GATE && p.du ? row_of<T>(p.du, cur, p.du_t, p.du_b) + c0 : nullptr;
@@ -328,11 +350,10 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
           if (dy) store_vec<T, V>(dy + k * nthV, o);
           if (du) store_vec<T, V>(du + k * nthV, o);
         }
-      cur = nxt;
-      live = next_live;
+      cur.next(gs, gt, gb, p.B);
       continue;
     }
-    st.template wait<1>();
+    st.wait(p.slots);
     float y[E], a[E], da[E], g[E];   // yh; act; act'; the gradient
 #pragma unroll
     for (int i = 0; i < E; ++i) y[i] = 0.f;
@@ -415,10 +436,9 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
         }
       }
     }
-    cur = nxt;
-    live = next_live;
+    cur.next(gs, gt, gb, p.B);
   }
-  st.template wait<0>();
+  st.wait(0);
   if (p.part) {
     float* o = p.part + (size_t)blockIdx.x * 2 * p.N;
 #pragma unroll

@@ -37,7 +37,7 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool sta
     if (st < -0x7fffffffLL || st > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   if ((long long)s->B * s->N > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   const int segs = (p->T + kSeg - 1) / kSeg;
-  sh->P = segs >= 2 ? 8 : 1;
+  sh->P = segs >= 2 ? kScanWarps : 1;
   p->split = p->D >= 32;
   sh->mode = p->split ? SCAN_WIDE : (staged && p->D == 1 ? SCAN_STAGED : SCAN_DIRECT);
   // two channels to a lane (16-bit), unless that leaves SMs without a block even when a
@@ -53,7 +53,7 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool sta
   // blocks of 8 warps fit an SM, the rounds they take fall with the cluster's size c, and
   // each doubling costs some 6 % in exchanges (T=1021, 408 items: c = 1 takes two rounds for
   // 1.4 blocks' work).
-  const long long slots = 2 * kSeqSMs * (8 / sh->P);
+  const long long slots = 2 * kSeqSMs * 8 / sh->P;
   int c = 1;
   double best = 0;
   for (int k = 1, lg = 0; k <= kScanCluster && (k == 1 || sh->P * k / 2 < segs); k *= 2, ++lg) {

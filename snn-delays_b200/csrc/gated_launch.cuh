@@ -59,7 +59,7 @@ template <class Kernel, class T, bool POS, bool DI>
 static int scan_by_size(ScanArgs& p, const ScanShape& sh, cudaStream_t st) {
   if (sh.P == 1)
     return p.qz ? scan_by_mode<Kernel, T, POS, DI, 1, true>(p, sh, st) : scan_by_mode<Kernel, T, POS, DI, 1, false>(p, sh, st);
-  return p.qz ? scan_by_mode<Kernel, T, POS, DI, 8, true>(p, sh, st) : scan_by_mode<Kernel, T, POS, DI, 8, false>(p, sh, st);
+  return p.qz ? scan_by_mode<Kernel, T, POS, DI, kScanWarps, true>(p, sh, st) : scan_by_mode<Kernel, T, POS, DI, kScanWarps, false>(p, sh, st);
 }
 template <class Kernel>
 static int scan_run(int dtype, ScanArgs& p, const ScanShape& sh, bool pos, cudaStream_t st) {

@@ -38,6 +38,7 @@
 namespace delrec {
 
 static constexpr int kSeg = 16;         // steps of a segment, the distance of the kept states
+static constexpr int kScanWarps = 8;    // segments (warps) of a block, unless there is one
 static constexpr int kScanCluster = 16; // most blocks per cluster (above 8: not every GPU has room)
 
 struct ScanArgs {
@@ -189,20 +190,29 @@ struct alignas(BYTES == 16 ? 16 : BYTES) RawBytes {
   char b[BYTES];
 };
 
-// 16 rows of ROWB bytes into shared memory, 16 bytes per copy; rows at or past n and
-// columns past the row's end (left bytes) become 0 without being read.
-template <int ROWB>
-__device__ __forceinline__ void stage_rows(unsigned dst, const char* row0, long long stride_bytes, int n, int left,
-                                           int lane) {
-  constexpr int CH = ROWB / 16;
+// 16 rows of ROWB bytes into shared memory, 16 bytes per copy, stride elements of E apart; rows
+// at or past n and columns past the row's end (left bytes) become 0 without being read.
+template <int ROWB, class E>
+__device__ __forceinline__ void stage_rows(unsigned dst, const E* row0, int stride, int n, int left, int lane) {
+  constexpr int CH = ROWB / 16, PER = 32 / CH;   // copies of a row, rows of one round
+  const int i0 = lane / CH, c = lane % CH * 16;
+  const char* src = (const char*)row0 + c;
+  dst += i0 * ROWB + c;
+  if (n >= kSeg && left >= ROWB) {
 #pragma unroll
-  for (int j = 0; j < kSeg * CH; j += 32) {
-    const int i = (j + lane) / CH, c = (j + lane) % CH * 16;
-    if (kSeg * CH >= 32 || lane < kSeg * CH) {
-      const bool ok = i < n && c < left;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * ROWB + c),
-                   "l"(ok ? row0 + i * stride_bytes + c : row0), "r"(ok ? 16 : 0));
-    }
+    for (int j = 0; j < kSeg; j += PER)
+      if (PER <= kSeg || i0 < kSeg)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + j * ROWB),
+                     "l"(src + (long long)stride * ((i0 + j) * (int)sizeof(E))));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kSeg; j += PER)
+      if (PER <= kSeg || i0 < kSeg) {
+        const bool ok = i0 + j < n && c < left;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * ROWB),
+                     "l"(ok ? src + (long long)stride * ((i0 + j) * (int)sizeof(E)) : (const char*)row0),
+                     "r"(ok ? 16 : 0));
+      }
   }
 }
 __device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -226,9 +236,15 @@ __device__ __forceinline__ void direct_rows(const E* base, int stride, int n, bo
   }
 }
 
-// A position in a kernel's work: item (row and channel tile), wave of segments.
+// A position in a kernel's work: item (row b and channel tile), wave of segments.
 struct Cursor {
-  int item, wv;
+  int item, b, tile, wv;
+  __device__ __forceinline__ void start(int it, int tiles, int first) {
+    item = it;
+    b = it / tiles;
+    tile = it - b * tiles;
+    wv = first;
+  }
 };
 
 
@@ -420,26 +436,25 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
   // copies the segment of a cursor into half h of this warp's stage
   auto fetch = [&](Cursor c, int h) {
     if (MODE == SCAN_STAGED && c.item < items) {
-      const int b = c.item / p.tiles, c0 = (c.item - b * p.tiles) * 32 * V, tb = c.wv * wave + seg * S;
+      const int b = c.b, c0 = c.tile * 32 * V, tb = c.wv * wave + seg * S;
       const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
       const int n = len - tb, left = (p.N - c0) * (int)sizeof(T);
       const unsigned dst = (unsigned)__cvta_generic_to_shared(mine + h * K::STAGE);
-      stage_rows<ROWB>(dst, (const char*)((const T*)p.z + b * p.z_b + c0 + (long long)tb * p.z_t),
-                       (long long)p.z_t * (int)sizeof(T), n, left, lane);
-      stage_rows<ROWB>(dst + S * ROWB, (const char*)((const T*)p.f + b * p.f_b + c0 + (long long)tb * p.f_t),
-                       (long long)p.f_t * (int)sizeof(T), n, left, lane);
+      stage_rows<ROWB>(dst, (const T*)p.z + b * p.z_b + c0 + (long long)tb * p.z_t, p.z_t, n, left, lane);
+      stage_rows<ROWB>(dst + S * ROWB, (const T*)p.f + b * p.f_b + c0 + (long long)tb * p.f_t, p.f_t, n, left, lane);
     }
     if (MODE == SCAN_STAGED) stage_commit();
   };
-  Cursor cur{(int)blockIdx.x / csize, 0};
+  Cursor cur;
+  cur.start((int)blockIdx.x / csize, p.tiles, 0);
   fetch(cur, 0);
   float v[V];
   for (int buf = 0; cur.item < items; buf ^= 1) {
-    Cursor nxt{cur.item, cur.wv + 1};
-    if (nxt.wv == waves) nxt = Cursor{cur.item + step, 0};
+    Cursor nxt = cur;
+    if (++nxt.wv == waves) nxt.start(cur.item + step, p.tiles, 0);
     __syncwarp();   // all lanes are past their reads of the half that is written now
     fetch(nxt, buf ^ 1);
-    const int b = cur.item / p.tiles, tile = cur.item - b * p.tiles;
+    const int b = cur.b, tile = cur.tile;
     const Place pl = scan_place<V>(p, tile, lane);
     const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
     const int tb = cur.wv * wave + seg * S, n = len - tb;
@@ -756,29 +771,27 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
   // into registers
   auto fetch = [&](Cursor c, int h) {
     if (MODE == SCAN_STAGED && c.item < items) {
-      const int b = c.item / p.tiles, tile = c.item - b * p.tiles, c0 = tile * 32 * V, tb = c.wv * wave + seg * S;
+      const int b = c.b, tile = c.tile, c0 = tile * 32 * V, tb = c.wv * wave + seg * S;
       const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
       const int n = len - tb, left = p.N - c0;
       const unsigned dst = (unsigned)__cvta_generic_to_shared(mine + h * K::STAGE);
-      stage_rows<ROWB>(dst, (const char*)(zp + b * z_b + c0 + (long long)tb * z_t), (long long)z_t * K::E, n,
-                       left * K::E, lane);
-      stage_rows<ROWB>(dst + S * ROWB, (const char*)(fp + b * f_b + c0 + (long long)tb * f_t),
-                       (long long)f_t * K::E, n, left * K::E, lane);
-      stage_rows<ROWG>(dst + 2 * S * ROWB, (const char*)(p.gh ? (const T*)p.gh + b * p.gh_b + c0 + (long long)tb * p.gh_t
-                                                              : (const T*)p.states),
-                       (long long)p.gh_t * (int)sizeof(T), p.gh ? n : 0, left * (int)sizeof(T), lane);
+      stage_rows<ROWB>(dst, zp + b * z_b + c0 + (long long)tb * z_t, z_t, n, left * K::E, lane);
+      stage_rows<ROWB>(dst + S * ROWB, fp + b * f_b + c0 + (long long)tb * f_t, f_t, n, left * K::E, lane);
+      const T* gh = p.gh ? (const T*)p.gh + b * p.gh_b + c0 + (long long)tb * p.gh_t : (const T*)p.states;
+      stage_rows<ROWG>(dst + 2 * S * ROWB, gh, p.gh_t, p.gh ? n : 0, left * (int)sizeof(T), lane);
       state(b, scan_place<V>(p, tile, lane), tb, s_ahead);
       if (B8) scales(b, tile, tb, n, sz_ahead, sf_ahead, odd_ahead);
     }
     if (MODE == SCAN_STAGED) stage_commit();
   };
-  Cursor cur{(int)blockIdx.x / csize, waves - 1};
+  Cursor cur;
+  cur.start((int)blockIdx.x / csize, p.tiles, waves - 1);
   fetch(cur, 0);
   float v[V];
   for (int buf = 0; cur.item < items; buf ^= 1) {
-    Cursor nxt{cur.item, cur.wv - 1};
-    if (nxt.wv < 0) nxt = Cursor{cur.item + step, waves - 1};
-    const int b = cur.item / p.tiles, tile = cur.item - b * p.tiles;
+    Cursor nxt = cur;
+    if (--nxt.wv < 0) nxt.start(cur.item + step, p.tiles, waves - 1);
+    const int b = cur.b, tile = cur.tile;
     const Place pl = scan_place<V>(p, tile, lane);
     const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
     const int tb = cur.wv * wave + seg * S, n = len - tb, nT = p.T - tb;

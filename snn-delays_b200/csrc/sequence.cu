@@ -18,7 +18,7 @@ static int check_block(const delrec_block* s) {
   if (s->dtype < DELREC_F32 || s->dtype > DELREC_F16 || s->gate < GATE_NONE || s->gate > GATE_SILU)
     return DELREC_ERR_ARG;
   if (!(s->eps > 0.f)) return DELREC_ERR_ARG;
-  if (s->N > kNormMax || (long long)s->T * s->B > 0x7fffffffLL - kSeqSMs * 16) return DELREC_ERR_UNSUPPORTED;
+  if (s->N > kNormMax || (long long)s->T * s->B > 0x7fffffffLL - 4 * kSeqSMs * 16) return DELREC_ERR_UNSUPPORTED;
   for (long long st : {s->x_t, s->x_b, s->y_t, s->y_b, s->u_t, s->u_b, s->o_t, s->o_b, s->n_t, s->n_b, s->gx_t,
                        s->gx_b, s->gn_t, s->gn_b, s->dx_t, s->dx_b, s->dy_t, s->dy_b, s->du_t, s->du_b})
     if (st < -0x7fffffffLL || st > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
@@ -46,12 +46,17 @@ struct NormShape {
   int V, IT, threads;
   int grid;   // blocks launched, set by the launch
 };
-static NormShape norm_shape(int N, int V, int most_threads) {
+static NormShape norm_shape(int N, int V, int esz, int most_threads) {
   NormShape s{};
   s.V = V;
   const int vecs = (N + V - 1) / V;
+  // 16 bytes of each tensor to a thread where that leaves a warp: what a row costs besides its
+  // channels (addresses, two sums) is some 130 operations a thread (fp16 N=700 in 8-byte
+  // vectors, one of them 61 us, two 47 us); more costs blocks per SM (fp32 N=512 forward, 16 bytes
+  // 111 us, 32 bytes 125 us).  N <= 16384: at most 32 channels.
   s.IT = 1;
-  while ((vecs + s.IT - 1) / s.IT > most_threads) s.IT *= 2;   // N <= 16384: at most 32 elements a thread
+  while (s.IT * V * esz < 16 && vecs > 32 * s.IT) s.IT *= 2;
+  while ((vecs + s.IT - 1) / s.IT > most_threads) s.IT *= 2;
   s.threads = ((vecs + s.IT - 1) / s.IT + 31) / 32 * 32;
   return s;
 }
@@ -60,13 +65,19 @@ static int norm_most_blocks(const delrec_block* s) {
 }
 static size_t norm_bwd_ws(const delrec_block* s) { return (size_t)norm_most_blocks(s) * 2 * s->N * sizeof(float); }
 
-// as many blocks as fit at once: each walks its rows
+// As many blocks as fit at once: each walks its rows, the next on its way.  Where two blocks
+// or fewer fit an SM they cannot cover each other's waits, and a third row in flight pays
+// (N=2048 bf16 backward 509 -> 372 us); where five fit it costs (N=512 fp32 backward 165 -> 183 us).
 template <class K>
-static int norm_start(K kern, int row_bytes, const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
-  const int smem = 2 * row_bytes * s.threads;
-  if (smem > 40 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  int per_sm = 0;
-  SQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem));
+static int norm_start(K kern, int row_bytes, NormArgs a, NormShape& s, int most, cudaStream_t st) {
+  int per_sm = 0, smem = 0;
+  for (a.slots = 2; a.slots <= 3; ++a.slots) {
+    smem = a.slots * row_bytes * s.threads;
+    if (smem > 40 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    SQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem));
+    if (per_sm > 2 || row_bytes == 0 || 3 * row_bytes * s.threads > 100 * 1024) break;
+  }
+  if (a.slots > 3) a.slots = 3;
   s.grid = std::min(most, std::max(1, std::min(per_sm, 16)) * kSeqSMs);
   kern<<<s.grid, s.threads, smem, st>>>(a);
   SQ_LAUNCHED();
@@ -162,7 +173,7 @@ int delrec_block_norm_forward(const delrec_block* s, const void* x, const void* 
     al.add(out, s->o_t, s->o_b);
     if (gate != GATE_NONE) al.add(u, s->u_t, s->u_b);
   }
-  NormShape sh = norm_shape(s->N, norm_width(al), kNormThreads);
+  NormShape sh = norm_shape(s->N, norm_width(al), al.esz, kNormThreads);
   a.kind = gate;
   return by_dtype(s->dtype, [&](auto t) {
     return norm_run<decltype(t), false>(a, sh, norm_most_blocks(s), (cudaStream_t)stream);
@@ -198,7 +209,7 @@ int delrec_block_norm_backward(const delrec_block* s, const void* x, const void*
       al.add(du, s->du_t, s->du_b);
     }
   }
-  NormShape sh = norm_shape(s->N, norm_width(al), kNormThreads);
+  NormShape sh = norm_shape(s->N, norm_width(al), al.esz, kNormThreads);
   a.kind = gate;
   const cudaStream_t st = (cudaStream_t)stream;
   const int r = by_dtype(s->dtype, [&](auto t) { return norm_run<decltype(t), true>(a, sh, norm_most_blocks(s), st); });
