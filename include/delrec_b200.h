@@ -359,9 +359,15 @@ int delrec_block_norm_backward(const delrec_block* block, const void* x, const v
  * -128 NaN.  Restored to fp16 it saturates at fp16's largest value. */
 int delrec_pack8(long long rows, int N, int dtype, const void* x, int8_t* q, uint8_t* e, void* stream);
 int delrec_unpack8(long long rows, int N, int dtype, const int8_t* q, const uint8_t* e, void* x, void* stream);
-/* delrec_linear_backward with x (M,K) in 8 bits: its values have 7 significant bits, so one
- * bf16 piece carries each exactly and dW takes three piece products.  Same workspace as
- * delrec_linear_backward with x_binary = 1. */
+/* delrec_linear_forward that also writes x (M,K) in 8 bits, q and e as delrec_pack8, from the
+ * same read (same workspace).  A real x's piece products are summed smallest first, which
+ * is a little more exact; for x_binary = 1 out has delrec_linear_forward's bits. */
+int delrec_linear_forward8(int M, int K, int N, const float* x, const float* W, const float* bias, int x_binary,
+                           float* out, int8_t* q, uint8_t* e, void* workspace, size_t workspace_bytes,
+                           void* stream);
+/* delrec_linear_backward with x in 8 bits: its values have 7 significant bits, so one bf16
+ * piece carries each exactly and dW takes three piece products. */
+size_t delrec_linear_backward8_workspace(int M, int K, int N);
 int delrec_linear_backward8(int M, int K, int N, const int8_t* q, const uint8_t* e, const float* W,
                             const float* gout, float* dx, float* dW, float* dbias, void* workspace,
                             size_t workspace_bytes, void* stream);

@@ -817,12 +817,17 @@ static LinPlan plan_linear(int K, int N, int x_binary) {
 }
 // The piece products with i + j <= 2 of two 3-piece operands (or the 3 products of a
 // 1-piece spike operand with the 3 pieces of the other), each operand's pieces stored once
-static void lin_products(GemmArgs* g, int a_pieces) {
+// last_first: the smallest products first.  The tensor core's accumulator cuts each sum off at
+// its own magnitude (half a unit of 2^-23 of it, on average, per 16 reduction steps, always
+// toward zero), which costs nothing while the sum is small: with the large product last its
+// steps alone count (K=700: 7.8e-6 -> 1.3e-6 of the result).
+static void lin_products(GemmArgs* g, int a_pieces, bool last_first = false) {
   static const int pa6[6] = {0, 1, 2, 0, 1, 0}, pb6[6] = {0, 0, 0, 1, 1, 2};
   g->nprod = a_pieces == 1 ? 3 : 6;
   for (int q = 0; q < g->nprod; ++q) {
-    g->pa[q] = a_pieces == 1 ? 0 : pa6[q];
-    g->pb[q] = a_pieces == 1 ? q : pb6[q];
+    const int at = last_first ? g->nprod - 1 - q : q;
+    g->pa[at] = a_pieces == 1 ? 0 : pa6[q];
+    g->pb[at] = a_pieces == 1 ? q : pb6[q];
   }
 }
 static int lin_ksplit(int M, int N, int K, int nprod) {
@@ -879,8 +884,27 @@ static size_t linear_bwd_ws(int M, int K, int N, int xb) {
                                  gemm1_part_bytes(3 * p.Np, p.Kp, M, kLinMaxSplit)));
   return c.off;
 }
+// The weight gradient from an 8-bit input: the rows in segments, each summed in an accumulator of
+// its own, the three pieces of gout in turn, the smallest first.  Segments of 1024 rows (64
+// steps at full size: 1e-6 of the result), longer ones past 64 segments, whose N x Kp partials
+// cost more than they give.
+static int lin8_rows(int M) { return M <= 1024 ? M : std::max(1024, ((M + 63) / 64 + 63) / 64 * 64); }
+static int lin8_ksplit(int M) { return (M + lin8_rows(M) - 1) / lin8_rows(M); }
+static size_t linear_bwd8_ws(int M, int K, int N) {
+  const LinPlan p = plan_linear(K, N, 1);
+  Carve c(nullptr, (size_t)-1);
+  c.take<__nv_bfloat16>((size_t)M * p.Kp);
+  c.take<__nv_bfloat16>((size_t)M * 3 * p.Np);
+  c.take<__nv_bfloat16>((size_t)3 * p.Np * p.Kp);
+  c.take<float>((size_t)N * p.Kp);
+  c.take<unsigned char>(std::max(gemm_partial_bytes(M, K, lin_ksplit(M, K, p.Np, 6), 1),
+                                 gemm_partial_bytes(N, p.Kp, lin8_ksplit(M), 1)));
+  return c.off;
+}
+// q8, e8: also writes x in 8 bits, from the same read, and sums real x's products smallest first
 static int run_linear_forward(int M, int K, int N, const float* x, const float* W, const float* bias, int xb,
-                              float* out, void* ws, size_t wsb, cudaStream_t st) {
+                              float* out, void* ws, size_t wsb, cudaStream_t st, int8_t* q8 = nullptr,
+                              uint8_t* e8 = nullptr) {
   if (M <= 0 || K <= 0 || N <= 0 || !x || !W || !out) return DELREC_ERR_ARG;
   if (((uintptr_t)ws & 255) != 0 || wsb < linear_fwd_ws(M, K, N, xb)) return DELREC_ERR_WORKSPACE;
   const LinPlan p = plan_linear(K, N, xb);
@@ -891,8 +915,13 @@ static int run_linear_forward(int M, int K, int N, const float* x, const float* 
   float* part = (float*)c.take<unsigned char>(gemm_partial_bytes(M, N, ks, 1));
   if (!c.ok) return DELREC_ERR_WORKSPACE;
   // rows [x0 (x1 x2)] and [W0 W1 W2], the ones / bias column at K
-  k_pack_rows<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, x, K, nullptr, 1, p.nbx,
-                                                                   kPatDistinct3, xb, X);
+  if (q8) {
+    const int gp = (p.Kp / 8 + 3) / 4 * 4;
+    k_pack_rows_keep<<<grid_for((size_t)M * gp, 256), 256, 0, st>>>(M, K, p.Kp, gp, x, p.nbx, xb, X, q8, e8);
+  } else {
+    k_pack_rows<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, x, K, nullptr, 1, p.nbx,
+                                                                     kPatDistinct3, xb, X);
+  }
   DR_LAUNCHED();
   k_pack_rows<<<grid_for((size_t)N * p.Kp / 8, 256), 256, 0, st>>>(N, K, p.Kp, W, K, bias, 0, 3, kPatDistinct3, 0,
                                                                    Wp);
@@ -907,7 +936,7 @@ static int run_linear_forward(int M, int K, int N, const float* x, const float* 
   Bw.n = 3; Bw.rows = N; Bw.cols = p.Kp; Bw.ld = 3LL * p.Kp;
   GemmArgs g{};
   g.M = M; g.N = N; g.K = p.Kp; g.nseg = 1;
-  lin_products(&g, p.nbx);
+  lin_products(&g, p.nbx, q8 && !xb);
   g.ksplit = ks;
   g.D = out; g.ldd = N; g.mode = GEMM_STORE;
   return gemm_run(A, Bw, g, 1, gemm_pick_bn(N), part, st, &g_launches);
@@ -919,16 +948,18 @@ static int run_linear_backward(int M, int K, int N, const float* x, const float*
                                const int8_t* q8 = nullptr, const uint8_t* e8 = nullptr) {
   if (M <= 0 || K <= 0 || N <= 0 || !gout || (dx && !W) || ((dW || dbias) && !x && !(q8 && e8)))
     return DELREC_ERR_ARG;
-  if (((uintptr_t)ws & 255) != 0 || wsb < linear_bwd_ws(M, K, N, xb)) return DELREC_ERR_WORKSPACE;
+  if (((uintptr_t)ws & 255) != 0 || wsb < (e8 ? linear_bwd8_ws(M, K, N) : linear_bwd_ws(M, K, N, xb)))
+    return DELREC_ERR_WORKSPACE;
   const LinPlan p = plan_linear(K, N, xb);
   Carve c(ws, wsb);
   __nv_bfloat16* X = c.take<__nv_bfloat16>((size_t)M * p.nbx * p.Kp);
   __nv_bfloat16* G = c.take<__nv_bfloat16>((size_t)M * 3 * p.Np);
   __nv_bfloat16* Wt = c.take<__nv_bfloat16>((size_t)3 * p.Np * p.Kp);
-  float* D = c.take<float>((size_t)3 * p.Np * p.Kp);
+  float* D = c.take<float>(e8 ? (size_t)N * p.Kp : (size_t)3 * p.Np * p.Kp);
   const int ksx = lin_ksplit(M, K, p.Np, 6);
-  float* part = (float*)c.take<unsigned char>(std::max(gemm_partial_bytes(M, K, ksx, 1),
-                                                       gemm1_part_bytes(3 * p.Np, p.Kp, M, kLinMaxSplit)));
+  float* part = (float*)c.take<unsigned char>(
+      std::max(gemm_partial_bytes(M, K, ksx, 1), e8 ? gemm_partial_bytes(N, p.Kp, lin8_ksplit(M), 1)
+                                                    : gemm1_part_bytes(3 * p.Np, p.Kp, M, kLinMaxSplit)));
   if (!c.ok) return DELREC_ERR_WORKSPACE;
   // G = [g0 g1 g2] per row (gb blocks): the three pieces of gout, each stored once
   const int gb = 3;
@@ -949,18 +980,34 @@ static int run_linear_backward(int M, int K, int N, const float* x, const float*
     Bw.n = 3; Bw.rows = p.Np; Bw.cols = K; Bw.ld = p.Kp; Bw.mn_major = 1;
     GemmArgs g{};
     g.M = M; g.N = K; g.K = p.Np; g.nseg = 1;
-    lin_products(&g, 3);
+    lin_products(&g, 3, e8 != nullptr);
     g.ksplit = ksx;
     g.D = dx; g.ldd = K; g.mode = GEMM_STORE;
     const int rc = gemm_run(A, Bw, g, 1, gemm_pick_bn(K), part, st, &g_launches);
     if (rc) return rc;
   }
   if (dW || dbias) {
-    if (q8)
+    if (q8) {
       k_pack_rows8<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, q8, e8, X);
-    else
-      k_pack_rows<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, x, K, nullptr, 1, p.nbx,
-                                                                       kPatDistinct3, xb, X);
+      DR_LAUNCHED();
+      // D[n][k'] = sum_m sum_i G_i[m][n] X[m][k']
+      GemmSide A{};
+      for (int i = 0; i < 3; ++i) A.p[i] = G + (size_t)i * p.Np;
+      A.n = 3; A.rows = M; A.cols = N; A.ld = (long long)gb * p.Np; A.mn_major = 1;
+      GemmArgs g{};
+      g.M = N; g.N = p.Kp; g.K = lin8_rows(M); g.nprod = 3;
+      g.nseg = g.ksplit = lin8_ksplit(M);
+      g.a_k_seg = g.b_k_seg = g.K;
+      for (int i = 0; i < 3; ++i) { g.pa[i] = 2 - i; g.pb[i] = 0; }
+      g.D = D; g.ldd = p.Kp; g.mode = GEMM_STORE;
+      const int rc = gemm_run(A, mnmajor_operand(X, M, p.Kp, p.Kp), g, 1, gemm_pick_bn(p.Kp), part, st, &g_launches);
+      if (rc) return rc;
+      k_linear_dw_split<<<grid_for((size_t)N * (K + 1), 256), 256, 0, st>>>(N, K, p.Kp, D, dW, dbias);
+      DR_LAUNCHED();
+      return DELREC_OK;
+    }
+    k_pack_rows<<<grid_for((size_t)M * p.Kp / 8, 256), 256, 0, st>>>(M, K, p.Kp, x, K, nullptr, 1, p.nbx,
+                                                                     kPatDistinct3, xb, X);
     DR_LAUNCHED();
     // D[c][k'] (+)= sum_m G'[m][c] X_a[m][k'] over the M rows, c < (3-a) Np
     for (int a = 0; a < p.nbx; ++a) {
@@ -1801,11 +1848,21 @@ int delrec_linear_backward(int M, int K, int N, const float* x, const float* W, 
                              (cudaStream_t)stream);
 }
 
+int delrec_linear_forward8(int M, int K, int N, const float* x, const float* W, const float* bias, int x_binary,
+                           float* out, int8_t* q, uint8_t* e, void* ws, size_t wsb, void* stream) {
+  if (!q || !e) return DELREC_ERR_ARG;
+  return run_linear_forward(M, K, N, x, W, bias, x_binary ? 1 : 0, out, ws, wsb, (cudaStream_t)stream, q, e);
+}
+size_t delrec_linear_backward8_workspace(int M, int K, int N) {
+  return (M > 0 && K > 0 && N > 0) ? linear_bwd8_ws(M, K, N) : 0;
+}
 int delrec_linear_backward8(int M, int K, int N, const int8_t* q, const uint8_t* e, const float* W,
                             const float* gout, float* dx, float* dW, float* dbias, void* ws, size_t wsb,
                             void* stream) {
+  static const uint8_t none = 0;   // marks the 8-bit path where x is not read
   if ((dW || dbias) && !(q && e)) return DELREC_ERR_ARG;
-  return run_linear_backward(M, K, N, nullptr, W, gout, 1, dx, dW, dbias, ws, wsb, (cudaStream_t)stream, q, e);
+  return run_linear_backward(M, K, N, nullptr, W, gout, 1, dx, dW, dbias, ws, wsb, (cudaStream_t)stream, q,
+                             e ? e : &none);
 }
 
 int delrec_hybrid_delay_grad(int N, int LM, const float* C, const float* W, const float* d, float sigma,

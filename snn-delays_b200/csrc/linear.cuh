@@ -253,22 +253,111 @@ __global__ void k_linear_dw_reduce(int N, int K, int Np, int Kp, const float* __
   }
 }
 
+// k_pack_rows of the projection's input (ones column at K) that also writes its 8-bit form
+// (checkpoint8.cuh) from the same read: four threads of 8 columns hold a group of 32, a row's
+// chunks are padded to whole groups (gp of them).
+__global__ void k_pack_rows_keep(int R, int K, int Wd, int gp, const float* __restrict__ src, int nb, int binary,
+                                 __nv_bfloat16* __restrict__ out, int8_t* __restrict__ q, uint8_t* __restrict__ e) {
+  const size_t row_out = (size_t)nb * Wd, total = (size_t)R * gp;
+  const int gpr = (K + kQGroup - 1) / kQGroup, lane = threadIdx.x & 31;
+  const unsigned mask = 0xfu << (lane & 28);
+  const bool vec = (K & 3) == 0 && ((uintptr_t)src & 15) == 0, qvec = (K & 3) == 0 && ((uintptr_t)q & 3) == 0;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
+    const size_t r = i / gp;
+    const int c0 = (int)(i - r * gp) * 8;
+    float v[8];
+    const float* sp = src + r * K + c0;
+    if (vec && c0 + 8 <= K) {
+      const float4 x0 = __ldcs((const float4*)sp), x1 = __ldcs((const float4*)sp + 1);
+      v[0] = x0.x; v[1] = x0.y; v[2] = x0.z; v[3] = x0.w;
+      v[4] = x1.x; v[5] = x1.y; v[6] = x1.z; v[7] = x1.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c0 + j < K ? sp[j] : 0.f;
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, q_magnitude(v[j]));
+    top = max(top, __shfl_xor_sync(mask, top, 1));
+    top = max(top, __shfl_xor_sync(mask, top, 2));
+    const unsigned ex = q_exponent(top);
+    const float inv = q_inverse_scale(ex);
+    unsigned lo = 0, hi = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lo |= (unsigned)(uint8_t)q_encode(v[j], inv) << (8 * j);
+      hi |= (unsigned)(uint8_t)q_encode(v[4 + j], inv) << (8 * j);
+    }
+    int8_t* qp = q + r * K + c0;
+    if (qvec && c0 + 8 <= K) {
+      ((unsigned*)qp)[0] = lo;
+      ((unsigned*)qp)[1] = hi;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + j < K) qp[j] = (int8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    }
+    if (c0 < K && c0 % kQGroup == 0) e[r * gpr + c0 / kQGroup] = (uint8_t)ex;
+    if (c0 >= Wd) continue;
+    Pieces3 p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (binary && c0 + j < K && !(v[j] == 0.f || v[j] == 1.f)) flag_status(ST_SHAPE);
+      p[j] = split3(c0 + j == K ? 1.f : v[j]);
+    }
+    uint4* o = (uint4*)(out + r * row_out + c0);
+#pragma unroll
+    for (int b = 0; b < 3; ++b)
+      if (b < nb) {
+        uint4 w;
+        w.x = pack_bf16x2(p[0].p[b], p[1].p[b]);
+        w.y = pack_bf16x2(p[2].p[b], p[3].p[b]);
+        w.z = pack_bf16x2(p[4].p[b], p[5].p[b]);
+        w.w = pack_bf16x2(p[6].p[b], p[7].p[b]);
+        o[(size_t)b * (Wd >> 3)] = w;
+      }
+  }
+}
+
+// dW[n*K + c] = D[n][c], dbias[n] = D[n][K]; D (N, Kp) row-major
+__global__ void k_linear_dw_split(int N, int K, int Kp, const float* __restrict__ D, float* __restrict__ dW,
+                                  float* __restrict__ dbias) {
+  const size_t total = (size_t)N * (K + 1);
+  for (size_t e = blockIdx.x * (size_t)blockDim.x + threadIdx.x; e < total; e += (size_t)gridDim.x * blockDim.x) {
+    const int n = (int)(e / (K + 1)), c = (int)(e % (K + 1));
+    const float v = D[(size_t)n * Kp + c];
+    if (c < K) {
+      if (dW) dW[(size_t)n * K + c] = v;
+    } else if (dbias) {
+      dbias[n] = v;
+    }
+  }
+}
+
 // The projections' bf16 operand rows from x (R, K) in 8 bits: out[r][c] = x (c < K), 1 (c ==
 // K: the bias column), 0 (K < c < Wd).  Exact: 7 significant bits.  Wd is a multiple of 8; a
 // thread writes 8 columns, all of one group.
 __global__ void k_pack_rows8(int R, int K, int Wd, const int8_t* __restrict__ q, const uint8_t* __restrict__ e,
                              __nv_bfloat16* __restrict__ out) {
   const int chunks = Wd >> 3, gpr = (K + kQGroup - 1) / kQGroup;
+  const bool vec = (K & 3) == 0 && ((uintptr_t)q & 3) == 0;
   const size_t total = (size_t)R * chunks;
   for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
     const size_t r = i / chunks;
     const int c0 = (int)(i - r * chunks) * 8;
     const float s = c0 < K ? q_scale(e[r * gpr + c0 / kQGroup]) : 1.f;
     __align__(16) __nv_bfloat16 v[8];
+    if (vec && c0 + 8 <= K) {
+      const unsigned* p = (const unsigned*)(q + r * K + c0);
+      const unsigned w[2] = {__ldcs(p), __ldcs(p + 1)};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = c0 + j;
-      v[j] = __float2bfloat16_rn(c < K ? q_decode(q[r * K + c], s) : (c == K ? 1.f : 0.f));
+      for (int j = 0; j < 8; ++j) v[j] = __float2bfloat16_rn(q_decode((int8_t)(w[j >> 2] >> (8 * (j & 3))), s));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = c0 + j;
+        v[j] = __float2bfloat16_rn(c < K ? q_decode(q[r * K + c], s) : (c == K ? 1.f : 0.f));
+      }
     }
     *(uint4*)(out + r * Wd + c0) = *(const uint4*)v;
   }

@@ -117,6 +117,8 @@ _SIGS = {
     "delrec_block_norm_backward": (_I, [_P] * 19 + [_S, _P]),
     "delrec_pack8": (_I, [ctypes.c_longlong, _I, _I, _P, _P, _P, _P]),
     "delrec_unpack8": (_I, [ctypes.c_longlong, _I, _I, _P, _P, _P, _P]),
+    "delrec_linear_forward8": (_I, [_I, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _S, _P]),
+    "delrec_linear_backward8_workspace": (_S, [_I, _I, _I]),
     "delrec_linear_backward8": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
 }
 

@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .checkpoint8 import pack8
+from .checkpoint8 import empty8
 
 
 def _is_binary(x):
@@ -45,16 +45,23 @@ class LinearFn(torch.autograd.Function):
         out = torch.empty(M, N, device=dev, dtype=torch.float32)
         w = weight.detach()
         b = bias.detach() if bias is not None else None
+        # only the parameter gradients read x
+        ctx.packed = bool(checkpoint8)
+        keep = None
+        if ctx.packed and (ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2])):
+            keep = empty8(x2.shape, x2.dtype, dev)
         if M > 0:
             lib = _lib.lib()
             ws = _lib.workspace(lib.delrec_linear_forward_workspace(M, K, N, int(binary)), dev)
             P = _lib.ptr
-            _lib.check(lib.delrec_linear_forward(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(ws),
-                                                 ws.numel(), _lib.stream_ptr(dev)), "delrec_linear_forward")
-        ctx.packed = bool(checkpoint8)
+            if keep is not None:
+                _lib.check(lib.delrec_linear_forward8(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(keep.q),
+                                                      P(keep.e), P(ws), ws.numel(), _lib.stream_ptr(dev)),
+                           "delrec_linear_forward8")
+            else:
+                _lib.check(lib.delrec_linear_forward(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(ws),
+                                                     ws.numel(), _lib.stream_ptr(dev)), "delrec_linear_forward")
         if ctx.packed:
-            # only the parameter gradients read x
-            keep = pack8(x2) if ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2]) else None
             ctx.save_for_backward(keep and keep.q, w, keep and keep.e)
         else:
             ctx.save_for_backward(x2, w, None)
@@ -83,14 +90,14 @@ class LinearFn(torch.autograd.Function):
             db = db.zero_() if db is not None else None
         elif need_dx or need_dw or need_db:
             lib = _lib.lib()
-            one_piece = ctx.binary or ctx.packed
-            ws = _lib.workspace(lib.delrec_linear_backward_workspace(M, K, N, int(one_piece)), dev)
             P = _lib.ptr
             if ctx.packed:
+                ws = _lib.workspace(lib.delrec_linear_backward8_workspace(M, K, N), dev)
                 _lib.check(lib.delrec_linear_backward8(M, K, N, P(x2), P(e), P(w), P(g), P(dx), P(dw), P(db),
                                                        P(ws), ws.numel(), _lib.stream_ptr(dev)),
                            "delrec_linear_backward8")
                 return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None
+            ws = _lib.workspace(lib.delrec_linear_backward_workspace(M, K, N, int(ctx.binary)), dev)
             _lib.check(lib.delrec_linear_backward(M, K, N, P(x2), P(w), P(g), int(ctx.binary), P(dx), P(dw),
                                                   P(db), P(ws), ws.numel(), _lib.stream_ptr(dev)),
                        "delrec_linear_backward")

@@ -80,14 +80,14 @@ def test_training_pass():
 
 
 def test_checkpoints_keep_the_forward_and_come_near_the_gradients():
-    """8-bit checkpoints: the same output; the gradients point the same way.  Each restored value
+    """8-bit checkpoints: the same output to fp32 accuracy; the gradients point the same way.  Each restored value
     is within 2^-7 of its group's largest, so a gradient summed over T B positions of random
     sign stays within a few percent of its norm."""
     model, x, g, lengths = _case()
     small = Stack(checkpoint8=True).cuda()
     small.load_state_dict(model.state_dict())
     a, b = model(x, lengths.cuda()), small(x, lengths.cuda())
-    assert torch.equal(a, b)
+    assert (a - b).abs().max() <= 1e-4 * a.abs().max()
     ga = torch.autograd.grad(a, list(model.parameters()), g)
     gb = torch.autograd.grad(b, list(small.parameters()), g)
     for u, v in zip(ga, gb):

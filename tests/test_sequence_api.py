@@ -140,6 +140,9 @@ def test_c_entry_points_reject_bad_arguments():
     assert lib.delrec_pack8(1 << 61, 4, 0, p, p, p, None) == 1
     assert lib.delrec_linear_backward8(4, 4, 4, None, None, p, p, p, p, None, p, 1 << 20, None) == 1
     assert lib.delrec_linear_backward8(4, 4, 4, p, p, p, p, p, p, None, p, 16, None) == 3
+    assert lib.delrec_linear_forward8(4, 4, 4, p, p, None, 0, p, None, p, p, 1 << 20, None) == 1
+    assert lib.delrec_linear_forward8(4, 4, 4, p, p, None, 0, p, p, p, p, 16, None) == 3
+    assert lib.delrec_linear_backward8_workspace(0, 4, 4) == 0
 
 
 def test_oracle_restores_within_half_a_step():
