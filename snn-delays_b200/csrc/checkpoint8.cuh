@@ -75,7 +75,7 @@ __device__ __forceinline__ unsigned group_mask(int lane) {
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(512) k_pack8(Q8Args p) {
+__global__ void __launch_bounds__(512, 2) k_pack8(Q8Args p) {
   constexpr int L = 32 / V, U = V == 1 ? 2 : 4;
   const int lane = threadIdx.x & 31;
   const unsigned mask = group_mask<V>(lane);
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(512) k_pack8(Q8Args p) {
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(512) k_unpack8(Q8Args p) {
+__global__ void __launch_bounds__(512, 2) k_unpack8(Q8Args p) {
   constexpr int U = V == 1 ? 2 : 4;
   const int sub = threadIdx.x / p.span;
   const long long step = (long long)gridDim.x * p.rpb;

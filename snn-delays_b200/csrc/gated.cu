@@ -30,7 +30,7 @@ struct ScanAlign {
   }
 };
 
-static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool staged) {
+static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool staged, bool q8) {
   p->T = s->T; p->B = s->B; p->N = s->N; p->G = s->G; p->D = s->N / s->G;
   p->decay_input = s->decay_input; p->wide = s->lengths_wide;
   for (long long st : {s->z_t, s->f_t, s->h_t, s->gh_t, s->dz_t, s->df_t})
@@ -61,6 +61,9 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool sta
     if (k == 1 || cost < best) { best = cost; c = k; }
   }
   sh->csize = c;
+  // a cluster's exchange costs as much as some 16 steps: segments of 32 where there are enough,
+  // and where two blocks' stages still fit an SM (16-bit)
+  sh->R = c > 1 && s->dtype != DELREC_F32 && sh->mode == SCAN_STAGED && sh->V == 1 && sh->P > 1 && !q8 && segs >= 2 * sh->P * c ? 2 : 1;
   if (items * c > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   sh->grid = (unsigned)(items * c);
   return DELREC_OK;
@@ -86,7 +89,7 @@ int delrec_gated_scan_forward(const delrec_scan* s, const void* z, const void* f
   al.input(z, s->z_t, s->z_b, s->N * al.esz, al.esz);
   al.input(f, s->f_t, s->f_b, s->N * al.esz, al.esz);
   al.output(h, s->h_t, s->h_b);
-  if ((rc = scan_shape(s, &p, &sh, al.sixteen))) return rc;
+  if ((rc = scan_shape(s, &p, &sh, al.sixteen, pack))) return rc;
   p.z = z; p.f = f; p.h0 = h0; p.lengths = lengths; p.resets = resets; p.h = h; p.hT = hT; p.states = states;
   p.qz = qz; p.ez = ez; p.qf = qf; p.ef = ef; p.odd = odd;
   p.z_t = (int)s->z_t; p.z_b = s->z_b; p.f_t = (int)s->f_t; p.f_b = s->f_b; p.h_t = (int)s->h_t; p.h_b = s->h_b;
@@ -123,7 +126,7 @@ int delrec_gated_scan_backward(const delrec_scan* s, const void* z, const void* 
   al.input(gh, s->gh_t, s->gh_b, s->N * al.esz, al.esz);
   al.output(dz, s->dz_t, s->dz_b);
   al.output(df, s->df_t, s->df_b);
-  if ((rc = scan_shape(s, &p, &sh, al.sixteen))) return rc;
+  if ((rc = scan_shape(s, &p, &sh, al.sixteen, pack))) return rc;
   const size_t need = df ? delrec_gated_scan_backward_workspace(s) : 0;
   if (need && (!ws || ((uintptr_t)ws & 255) != 0 || wsb < need)) return DELREC_ERR_WORKSPACE;
   p.z = z; p.f = f; p.lengths = lengths; p.resets = resets; p.states = const_cast<float*>(states);

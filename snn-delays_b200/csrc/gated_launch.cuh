@@ -43,17 +43,19 @@ static inline int scan_launch(void (*kern)(ScanArgs, int), int smem, ScanArgs& p
   return DELREC_OK;
 }
 
-// Kernel: the direction's launcher, Kernel::run<T, V, P, POS, Q8, DI, MODE>(p, sh, st)
+// Kernel: the direction's launcher, Kernel::run<T, V, P, R, POS, Q8, DI, MODE>(p, sh, st)
 template <class Kernel, class T, bool POS, bool DI, int P, bool Q8>
 static int scan_by_mode(ScanArgs& p, const ScanShape& sh, cudaStream_t st) {
   if (sh.mode == SCAN_STAGED) {
     if constexpr (sizeof(T) == 2)
-      if (sh.V == 2) return Kernel::template run<T, 2, P, POS, Q8, DI, SCAN_STAGED>(p, sh, st);
-    return Kernel::template run<T, 1, P, POS, Q8, DI, SCAN_STAGED>(p, sh, st);
+      if (sh.V == 2) return Kernel::template run<T, 2, P, 1, POS, Q8, DI, SCAN_STAGED>(p, sh, st);
+    if constexpr (!Q8 && P > 1 && sizeof(T) == 2)
+      if (sh.R == 2) return Kernel::template run<T, 1, P, 2, POS, false, DI, SCAN_STAGED>(p, sh, st);
+    return Kernel::template run<T, 1, P, 1, POS, Q8, DI, SCAN_STAGED>(p, sh, st);
   }
   if constexpr (!Q8)
-    if (sh.mode == SCAN_WIDE) return Kernel::template run<T, 1, P, POS, false, DI, SCAN_WIDE>(p, sh, st);
-  return Kernel::template run<T, 1, P, POS, Q8, DI, SCAN_DIRECT>(p, sh, st);
+    if (sh.mode == SCAN_WIDE) return Kernel::template run<T, 1, P, 1, POS, false, DI, SCAN_WIDE>(p, sh, st);
+  return Kernel::template run<T, 1, P, 1, POS, Q8, DI, SCAN_DIRECT>(p, sh, st);
 }
 template <class Kernel, class T, bool POS, bool DI>
 static int scan_by_size(ScanArgs& p, const ScanShape& sh, cudaStream_t st) {

@@ -170,9 +170,10 @@ __device__ __forceinline__ const E* at_step(const E* base, int stride, int i) {
 }
 
 // bit i: a reset at step tb + i (below n)
+template <int S>
 __device__ __forceinline__ unsigned scan_resets(const ScanArgs& p, int b, int tb, int n, int lane) {
   if (!p.resets) return 0u;
-  const bool r = lane < kSeg && tb + lane < n && p.resets[(size_t)(tb + lane) * p.B + b];
+  const bool r = lane < S && tb + lane < n && p.resets[(size_t)(tb + lane) * p.B + b];
   return __ballot_sync(0xffffffffu, r);
 }
 
@@ -190,24 +191,24 @@ struct alignas(BYTES == 16 ? 16 : BYTES) RawBytes {
   char b[BYTES];
 };
 
-// 16 rows of ROWB bytes into shared memory, 16 bytes per copy, stride elements of E apart; rows
+// S rows of ROWB bytes into shared memory, 16 bytes per copy, stride elements of E apart; rows
 // at or past n and columns past the row's end (left bytes) become 0 without being read.
-template <int ROWB, class E>
+template <int ROWB, int S, class E>
 __device__ __forceinline__ void stage_rows(unsigned dst, const E* row0, int stride, int n, int left, int lane) {
   constexpr int CH = ROWB / 16, PER = 32 / CH;   // copies of a row, rows of one round
   const int i0 = lane / CH, c = lane % CH * 16;
   const char* src = (const char*)row0 + c;
   dst += i0 * ROWB + c;
-  if (n >= kSeg && left >= ROWB) {
+  if (n >= S && left >= ROWB) {
 #pragma unroll
-    for (int j = 0; j < kSeg; j += PER)
-      if (PER <= kSeg || i0 < kSeg)
+    for (int j = 0; j < S; j += PER)
+      if (PER <= S || i0 < S)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + j * ROWB),
                      "l"(src + (long long)stride * ((i0 + j) * (int)sizeof(E))));
   } else {
 #pragma unroll
-    for (int j = 0; j < kSeg; j += PER)
-      if (PER <= kSeg || i0 < kSeg) {
+    for (int j = 0; j < S; j += PER)
+      if (PER <= S || i0 < S) {
         const bool ok = i0 + j < n && c < left;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * ROWB),
                      "l"(ok ? src + (long long)stride * ((i0 + j) * (int)sizeof(E)) : (const char*)row0),
@@ -414,18 +415,20 @@ __device__ __forceinline__ float warp_sum16(const float (&x)[16], int lane) {
 // forward
 // ---------------------------------------------------------------------------------
 // PACK (D = 1): also writes z and f in 8 bits; a tile is V groups of 32 channels.
-template <class T, int V, int P, bool POS, bool PACK, int MODE>
+// R: 16-step pieces of a segment; two (plain staged kernels) where a cluster's exchanges are many.
+template <class T, int V, int P, int R, bool POS, bool PACK, int MODE>
 struct ScanFwd {
-  static constexpr int S = kSeg, ROWB = 32 * V * (int)sizeof(T);
+  static constexpr int S = kSeg * R, ROWB = 32 * V * (int)sizeof(T);
   static constexpr int STAGE = MODE == SCAN_STAGED ? 2 * S * ROWB : 0;   // bytes of a warp's segment
   static constexpr int SMEM = 2 * P * STAGE;
   // 16-bit pairs and packing take 128 registers, single channels 80
-  static constexpr int WARPS = V == 2 || PACK ? 16 : 24;
+  static constexpr int WARPS = V == 2 || R == 2 || PACK ? 16 : 24;
 };
-template <class T, int V, int P, bool POS, bool PACK, bool DI, int MODE>
-__global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WARPS / P) k_scan_fwd(ScanArgs p, int csize) {
-  using K = ScanFwd<T, V, P, POS, PACK, MODE>;
-  constexpr int S = kSeg, ROWB = K::ROWB;
+template <class T, int V, int P, int R, bool POS, bool PACK, bool DI, int MODE>
+__global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, R, POS, PACK, MODE>::WARPS / P) k_scan_fwd(ScanArgs p, int csize) {
+  using K = ScanFwd<T, V, P, R, POS, PACK, MODE>;
+  constexpr int S = K::S, ROWB = K::ROWB;
+  static_assert(R == 1 || (MODE == SCAN_STAGED && !PACK), "longer segments are for plain staged inputs");
   __shared__ ScanExchange<P, V> sm;
   extern __shared__ __align__(16) char stage[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -440,8 +443,8 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
       const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
       const int n = len - tb, left = (p.N - c0) * (int)sizeof(T);
       const unsigned dst = (unsigned)__cvta_generic_to_shared(mine + h * K::STAGE);
-      stage_rows<ROWB>(dst, (const T*)p.z + b * p.z_b + c0 + (long long)tb * p.z_t, p.z_t, n, left, lane);
-      stage_rows<ROWB>(dst + S * ROWB, (const T*)p.f + b * p.f_b + c0 + (long long)tb * p.f_t, p.f_t, n, left, lane);
+      stage_rows<ROWB, S>(dst, (const T*)p.z + b * p.z_b + c0 + (long long)tb * p.z_t, p.z_t, n, left, lane);
+      stage_rows<ROWB, S>(dst + S * ROWB, (const T*)p.f + b * p.f_b + c0 + (long long)tb * p.f_t, p.f_t, n, left, lane);
     }
     if (MODE == SCAN_STAGED) stage_commit();
   };
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = (pl.on && p.h0) ? p.h0[(size_t)b * p.N + pl.c + k] : 0.f;
     }
-    const unsigned cut = POS ? scan_resets(p, b, tb, len, lane) : 0u;
+    const unsigned cut = POS ? scan_resets<S>(p, b, tb, len, lane) : 0u;
     if (MODE == SCAN_STAGED) {
       stage_wait<1>();
       __syncwarp();
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
           fr[i] = *(const VecOf<T, V>*)(r + (S + i) * ROWB);
         }
       } else {
-        static_assert(V == 1, "plain loads take one channel to a lane");
+        static_assert(V == 1 && R == 1, "plain loads take one channel and 16 steps to a lane");
         T r[S];
         direct_rows<T>((const T*)p.z + b * p.z_b + pl.c + (long long)tb * p.z_t, p.z_t, n, pl.on, r);
 #pragma unroll
@@ -500,7 +503,7 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
               ok ? to_f(((const T*)p.f)[b * p.f_b + g + (long long)(tb + i) * p.f_t]) : 0.f);
         }
       }
-      if (PACK) {
+      if constexpr (PACK) {
         const size_t row = (size_t)tb * p.B + b;
         const int groups = (p.N + kQGroup - 1) / kQGroup, grp = tile * V + lane * V / 32;
         PackOut<V> o;
@@ -545,17 +548,21 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
     float s[V];
     scan_exchange<P, V, POS>(sm, buf, warp, lane, rank, csize, m, v, s);
     if (pl.on && tb < p.T) {
-      if (p.states) {
-        VecOf<float, V> o;
+      // the state before step i, a multiple of 16
+      auto keep = [&](int i) {
+        if (p.states && tb + i < p.T) {
+          VecOf<float, V> o;
 #pragma unroll
-        for (int k = 0; k < V; ++k) o.v[k] = s[k];
-        *(VecOf<float, V>*)(p.states + ((size_t)(tb / kSeg) * p.B + b) * p.N + pl.c) = o;
-      }
+          for (int k = 0; k < V; ++k) o.v[k] = s[k];
+          *(VecOf<float, V>*)(p.states + ((size_t)((tb + i) / kSeg) * p.B + b) * p.N + pl.c) = o;
+        }
+      };
       T* h = (T*)p.h + b * p.h_b + pl.c + (long long)tb * p.h_t;
       const int nT = p.T - tb;
       if (n >= S) {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
+          if (i % kSeg == 0) keep(i);
           VecOf<T, V> o;
 #pragma unroll
           for (int k = 0; k < V; ++k) {
@@ -567,6 +574,7 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, POS, PACK, MODE>::WAR
       } else {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
+          if (i % kSeg == 0) keep(i);
           VecOf<T, V> o;
 #pragma unroll
           for (int k = 0; k < V; ++k) {
@@ -601,14 +609,14 @@ __device__ __forceinline__ float code_value(const RawBytes<V>& r, int k) {
 // shared memory where they are needed, so that they hold no registers), the scales of the
 // steps spread over the lanes (lane j: step j, or step j / 2 of group j & 1 for V = 2), this
 // lane's share of the gates (WIDE).
-template <class T, int V, bool B8, int MODE>
+template <class T, int V, int S, bool B8, int MODE>
 struct ScanIn {
   static constexpr int E = B8 ? 1 : (int)sizeof(T), ROWB = 32 * V * E, ROWG = 32 * V * (int)sizeof(T);
   static constexpr bool STAGED = MODE == SCAN_STAGED;
   using Raw = RawBytes<E * V>;
   const char *zf_row, *g_row;   // this lane's place in the staged rows
-  Raw z_[STAGED ? 1 : kSeg], f_[STAGED || MODE == SCAN_WIDE ? 1 : kSeg];
-  VecOf<T, V> g_[STAGED ? 1 : kSeg];
+  Raw z_[STAGED ? 1 : S], f_[STAGED || MODE == SCAN_WIDE ? 1 : S];
+  VecOf<T, V> g_[STAGED ? 1 : S];
   float sz, sf, wide;
   int edge;
   __device__ __forceinline__ Raw z(int i) const {
@@ -616,7 +624,7 @@ struct ScanIn {
     else return z_[i];
   }
   __device__ __forceinline__ Raw f(int i) const {
-    if constexpr (STAGED) return *(const Raw*)(zf_row + (kSeg + i) * ROWB);
+    if constexpr (STAGED) return *(const Raw*)(zf_row + (S + i) * ROWB);
     else if constexpr (MODE == SCAN_DIRECT) return f_[i];
     else return f_[0];
   }
@@ -632,15 +640,15 @@ __device__ __forceinline__ float raw_value(const RawBytes<(int)sizeof(T) * V>& r
 
 // The walk of one backward segment in time order: gates w, df factors e, and the segment's map
 // of the reverse recurrence, in forward order: G enters at the end times Pi a, and g_i times
-// the gates up to i.  PLAIN: all 16 steps are inside the sequence, no code stands for an infinity
+// the gates up to i.  PLAIN: all steps are inside the sequence, no code stands for an infinity
 // or NaN.
-template <class T, int V, bool POS, bool B8, bool DI, int MODE, bool PLAIN>
-__device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, B8, MODE>& r, unsigned cut, int n, int lane,
-                                          float (&s)[V], float (&w)[kSeg][V], float (&e)[kSeg][V], float2 (&m)[V]) {
+template <class T, int V, int S, bool POS, bool B8, bool DI, int MODE, bool PLAIN>
+__device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, S, B8, MODE>& r, unsigned cut, int n, int lane,
+                                          float (&s)[V], float (&w)[S][V], float (&e)[S][V], float2 (&m)[V]) {
 #pragma unroll
   for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < kSeg; ++i) {
+  for (int i = 0; i < S; ++i) {
     float sz = 0.f, sf = 0.f, ww = 0.f;
     if (B8) {
       const int src = V == 1 ? i : 2 * i + (lane >> 4);
@@ -692,12 +700,12 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, 
 
 // The walk back: q is the gradient that enters the segment's last step.  WHOLE: all its
 // steps are inside the sequence.  e[i] becomes df.
-template <class T, int V, bool POS, bool DI, bool WHOLE, class In>
-__device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const In& r, const float (&w)[kSeg][V],
-                                               float (&e)[kSeg][V], float (&q)[V], unsigned cut, int n, int nT, T* dz,
+template <class T, int V, int S, bool POS, bool DI, bool WHOLE, class In>
+__device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const In& r, const float (&w)[S][V],
+                                               float (&e)[S][V], float (&q)[V], unsigned cut, int n, int nT, T* dz,
                                                T* df) {
 #pragma unroll
-  for (int i = kSeg - 1; i >= 0; --i) {
+  for (int i = S - 1; i >= 0; --i) {
     const VecOf<T, V> gi = r.g(i);
     VecOf<T, V> oz, of;
 #pragma unroll
@@ -721,18 +729,19 @@ __device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const In& r, c
 }
 
 // B8 (D = 1): z and f come from their 8-bit form.
-template <class T, int V, int P, bool B8, int MODE>
+template <class T, int V, int P, int R, bool B8, int MODE>
 struct ScanBwd {
-  static constexpr int S = kSeg, E = B8 ? 1 : (int)sizeof(T);
+  static constexpr int S = kSeg * R, E = B8 ? 1 : (int)sizeof(T);
   static constexpr int ROWB = 32 * V * E, ROWG = 32 * V * (int)sizeof(T);   // bytes of a row of z or f, of gh
   static constexpr int STAGE = MODE == SCAN_STAGED ? S * (2 * ROWB + ROWG) : 0;
   static constexpr int SMEM = 2 * P * STAGE;
 };
-template <class T, int V, int P, bool POS, bool B8, bool DI, int MODE>
+template <class T, int V, int P, int R, bool POS, bool B8, bool DI, int MODE>
 __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csize) {
-  using K = ScanBwd<T, V, P, B8, MODE>;
+  using K = ScanBwd<T, V, P, R, B8, MODE>;
+  static_assert(R == 1 || (MODE == SCAN_STAGED && !B8), "longer segments are for plain staged inputs");
   using E = std::conditional_t<B8, int8_t, T>;
-  constexpr int S = kSeg, ROWB = K::ROWB, ROWG = K::ROWG;
+  constexpr int S = K::S, ROWB = K::ROWB, ROWG = K::ROWG;
   __shared__ ScanExchange<P, V> sm;
   extern __shared__ __align__(16) char stage[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -775,10 +784,10 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
       const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
       const int n = len - tb, left = p.N - c0;
       const unsigned dst = (unsigned)__cvta_generic_to_shared(mine + h * K::STAGE);
-      stage_rows<ROWB>(dst, zp + b * z_b + c0 + (long long)tb * z_t, z_t, n, left * K::E, lane);
-      stage_rows<ROWB>(dst + S * ROWB, fp + b * f_b + c0 + (long long)tb * f_t, f_t, n, left * K::E, lane);
+      stage_rows<ROWB, S>(dst, zp + b * z_b + c0 + (long long)tb * z_t, z_t, n, left * K::E, lane);
+      stage_rows<ROWB, S>(dst + S * ROWB, fp + b * f_b + c0 + (long long)tb * f_t, f_t, n, left * K::E, lane);
       const T* gh = p.gh ? (const T*)p.gh + b * p.gh_b + c0 + (long long)tb * p.gh_t : (const T*)p.states;
-      stage_rows<ROWG>(dst + 2 * S * ROWB, gh, p.gh_t, p.gh ? n : 0, left * (int)sizeof(T), lane);
+      stage_rows<ROWG, S>(dst + 2 * S * ROWB, gh, p.gh_t, p.gh ? n : 0, left * (int)sizeof(T), lane);
       state(b, scan_place<V>(p, tile, lane), tb, s_ahead);
       if (B8) scales(b, tile, tb, n, sz_ahead, sf_ahead, odd_ahead);
     }
@@ -795,7 +804,7 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
     const Place pl = scan_place<V>(p, tile, lane);
     const int len = POS ? row_length(p.lengths, p.wide, b, p.T) : p.T;
     const int tb = cur.wv * wave + seg * S, n = len - tb, nT = p.T - tb;
-    ScanIn<T, V, B8, MODE> r;
+    ScanIn<T, V, S, B8, MODE> r;
     r.sz = sz_ahead; r.sf = sf_ahead; r.wide = 0.f; r.edge = 32;
     int odd = odd_ahead;
     float s[V];
@@ -807,7 +816,7 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = (pl.on && p.ghT) ? p.ghT[(size_t)b * p.N + pl.c + k] : 0.f;
     }
-    const unsigned cut = POS ? scan_resets(p, b, tb, len, lane) : 0u;
+    const unsigned cut = POS ? scan_resets<S>(p, b, tb, len, lane) : 0u;
     r.zf_row = mine + buf * K::STAGE + lane * K::E * V;
     r.g_row = mine + buf * K::STAGE + 2 * S * ROWB + lane * V * (int)sizeof(T);
     if constexpr (MODE == SCAN_STAGED) {
@@ -844,8 +853,8 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
 #pragma unroll
     for (int k = 0; k < V; ++k) m[k] = make_float2(1.f, 0.f);
     if (n > 0) {   // else the identity: past the sequence's end
-      if (n >= S && !odd) scan_walk<T, V, POS, B8, DI, MODE, true>(p, r, cut, n, lane, s, w, e, m);
-      else scan_walk<T, V, POS, B8, DI, MODE, false>(p, r, cut, n, lane, s, w, e, m);
+      if (n >= S && !odd) scan_walk<T, V, S, POS, B8, DI, MODE, true>(p, r, cut, n, lane, s, w, e, m);
+      else scan_walk<T, V, S, POS, B8, DI, MODE, false>(p, r, cut, n, lane, s, w, e, m);
     }
     if (POS && cut) {
 #pragma unroll
@@ -856,9 +865,9 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
     T* dz = pl.on && p.dz ? (T*)p.dz + b * p.dz_b + pl.c + (long long)tb * p.dz_t : nullptr;
     T* df = pl.on && p.df && p.D == 1 ? (T*)p.df + b * p.df_b + pl.c + (long long)tb * p.df_t : nullptr;
     if (n >= S) {
-      scan_walk_back<T, V, POS, DI, true>(p, r, w, e, q, cut, n, nT, dz, df);
+      scan_walk_back<T, V, S, POS, DI, true>(p, r, w, e, q, cut, n, nT, dz, df);
     } else if (n > 0) {
-      scan_walk_back<T, V, POS, DI, false>(p, r, w, e, q, cut, n, nT, dz, df);
+      scan_walk_back<T, V, S, POS, DI, false>(p, r, w, e, q, cut, n, nT, dz, df);
     } else {
       VecOf<T, V> o;
 #pragma unroll
@@ -951,7 +960,7 @@ __global__ void __launch_bounds__(128) k_gated_step(int B, int N, int D, int dec
 // host
 // ---------------------------------------------------------------------------------
 struct ScanShape {
-  int V, P, csize, mode;
+  int V, P, R, csize, mode;
   unsigned grid;
 };
 // the kernels of a direction, by element type (gated_fwd.cu, gated_bwd.cu)

@@ -131,9 +131,11 @@ static int q8_launch(Q8Args a, cudaStream_t st) {
   a.rpb = std::max(1, most / a.span);
   const int threads = std::min(most, a.span * a.rpb);
   const long long blocks = (a.rows + a.rpb - 1) / a.rpb;
-  const int grid = (int)std::min<long long>(blocks, (long long)kSeqSMs * 4);
-  if (PACK) k_pack8<T, V><<<grid, threads, 0, st>>>(a);
-  else k_unpack8<T, V><<<grid, threads, 0, st>>>(a);
+  void (*kern)(Q8Args) = PACK ? k_pack8<T, V> : k_unpack8<T, V>;
+  int per_sm = 1;   // as many blocks as fit at once
+  if (blocks > kSeqSMs) SQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0));
+  const int grid = (int)std::min<long long>(blocks, (long long)kSeqSMs * std::max(per_sm, 1));
+  kern<<<grid, threads, 0, st>>>(a);
   SQ_LAUNCHED();
   return DELREC_OK;
 }

@@ -65,42 +65,49 @@ class BlockNormFn(torch.autograd.Function):
         return (out, n) if has_next else out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
-        x, y, u, w, scale, nw, lengths, ry, rx = ctx.saved_tensors
-        (T, B, N), dtype, kind, eps, has_next = ctx.meta
-        gx = grads[0] if y is not None else None
-        gn = grads[-1] if has_next else None
-        if gx is None and gn is None:
-            return (None,) * 10
-        if gx is not None:
-            gx = _lib.rows(gx)
-        if gn is not None:
-            gn = _lib.rows(gn)
-        need = ctx.needs_input_grad
-        like = x if x is not None else y
-        dev = like.device
-        dx = _lib.empty_rows(like) if need[0] else None
-        dy = _lib.empty_rows(like) if need[1] else None
-        du = _lib.empty_rows(like) if need[2] else None
-        dw = torch.empty(N, device=dev) if need[3] else None
-        ds = torch.empty(N, device=dev) if need[4] else None
-        dn = torch.empty(N, device=dev) if need[5] else None
-        if T and B and N:
-            b = _lib.Block(T, B, N, _lib.SEQ_DTYPES[dtype], kind, _wide(lengths), eps, 0,
-                           *_strides(x, y, u, None, None, gx, gn, dx, dy, du))
-            ws, nbytes = None, 0
-            if dw is not None or ds is not None or dn is not None:
-                nbytes = _lib.lib().delrec_block_norm_backward_workspace(ctypes.byref(b))
-                ws = _lib.scratch(nbytes, dev)
-            A = _lib.addr
-            _lib.launch("delrec_block_norm_backward", dev, ctypes.byref(b), A(x), A(y), A(u), A(w), A(scale), A(nw),
-                        A(lengths), A(ry), A(rx), A(gx), A(gn), A(dx), A(dy), A(du), A(dw), A(ds), A(dn), A(ws), nbytes)
-        else:
-            for t in (dw, ds, dn):
-                if t is not None:
-                    t.zero_()
-        return dx, dy, du, dw, ds, dn, None, None, None, None
+        # the decorator's bookkeeping is wanted only where a second derivative could be
+        return (_once if torch.is_grad_enabled() else _backward)(ctx, *grads)
+
+
+def _backward(ctx, *grads):
+    x, y, u, w, scale, nw, lengths, ry, rx = ctx.saved_tensors
+    (T, B, N), dtype, kind, eps, has_next = ctx.meta
+    gx = grads[0] if y is not None else None
+    gn = grads[-1] if has_next else None
+    if gx is None and gn is None:
+        return (None,) * 10
+    if gx is not None:
+        gx = _lib.rows(gx)
+    if gn is not None:
+        gn = _lib.rows(gn)
+    need = ctx.needs_input_grad
+    like = x if x is not None else y
+    dev = like.device
+    dx = _lib.empty_rows(like) if need[0] else None
+    dy = _lib.empty_rows(like) if need[1] else None
+    du = _lib.empty_rows(like) if need[2] else None
+    dw = torch.empty(N, device=dev) if need[3] else None
+    ds = torch.empty(N, device=dev) if need[4] else None
+    dn = torch.empty(N, device=dev) if need[5] else None
+    if T and B and N:
+        b = _lib.Block(T, B, N, _lib.SEQ_DTYPES[dtype], kind, _wide(lengths), eps, 0,
+                       *_strides(x, y, u, None, None, gx, gn, dx, dy, du))
+        ws, nbytes = None, 0
+        if dw is not None or ds is not None or dn is not None:
+            nbytes = _lib.lib().delrec_block_norm_backward_workspace(ctypes.byref(b))
+            ws = _lib.scratch(nbytes, dev)
+        A = _lib.addr
+        _lib.launch("delrec_block_norm_backward", dev, ctypes.byref(b), A(x), A(y), A(u), A(w), A(scale), A(nw),
+                    A(lengths), A(ry), A(rx), A(gx), A(gn), A(dx), A(dy), A(du), A(dw), A(ds), A(dn), A(ws), nbytes)
+    else:
+        for t in (dw, ds, dn):
+            if t is not None:
+                t.zero_()
+    return dx, dy, du, dw, ds, dn, None, None, None, None
+
+
+_once = once_differentiable(_backward)
 
 
 def _run(x, y, u, w, scale, nw, lengths, kind, eps, has_next):

@@ -89,42 +89,49 @@ class GatedScan(torch.autograd.Function):
         return h, hT
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, gh, ghT):
-        if gh is None and ghT is None:
-            return (None,) * 7
-        z, f, states, lengths, resets, qz, ez, qf, ef, odd = ctx.saved_tensors
-        (T, B, N), G, dtype, decay_input, keep8, has_h0 = ctx.meta
-        if keep8 and odd is None:       # the 8-bit kernel is for a gate per channel
-            z, f = unpack8(Packed8(qz, ez, dtype)), unpack8(Packed8(qf, ef, dtype))
-            qz = ez = qf = ef = None
-        need_z, need_f, need_h = ctx.needs_input_grad[:3]
-        like_z, like_f = (qz, qf) if z is None else (z, f)
-        dev = states.device
-        dz = _lib.empty_rows(like_z, dtype) if need_z else None
-        df = _lib.empty_rows(like_f, dtype) if need_f else None
-        dh0 = torch.empty(B, N, device=dev) if need_h and has_h0 else None
-        if T and B and N:
-            if gh is not None:
-                gh = _lib.rows(gh)
-            if ghT is not None:
-                ghT = ghT.contiguous()
-            st = []
-            for t in (z, f, None, gh, dz, df):
-                st += t.stride()[:2] if t is not None else (0, 0)
-            s = _lib.Scan(T, B, N, G, _lib.SEQ_DTYPES[dtype], 1 if decay_input else 0,
-                          1 if lengths is not None and lengths.dtype == torch.int64 else 0, 0, *st)
-            ws, nbytes = None, 0
-            if need_f and G != N:
-                nbytes = _lib.lib().delrec_gated_scan_backward_workspace(ctypes.byref(s))
-                ws = _lib.scratch(nbytes, dev)
-            A = _lib.addr
-            _lib.launch("delrec_gated_scan_backward", dev, ctypes.byref(s), A(z), A(f), A(qz), A(ez), A(qf), A(ef),
-                        A(odd), A(lengths), A(resets), states.data_ptr(), A(gh), A(ghT), A(dz), A(df), A(dh0), A(ws),
-                        nbytes)
-        elif dh0 is not None:
-            dh0 = ghT.clone() if ghT is not None else dh0.zero_()
-        return dz, df, dh0, None, None, None, None
+    def backward(ctx, *grads):
+        # the decorator's bookkeeping is wanted only where a second derivative could be
+        return (_once if torch.is_grad_enabled() else _backward)(ctx, *grads)
+
+
+def _backward(ctx, gh, ghT):
+    if gh is None and ghT is None:
+        return (None,) * 7
+    z, f, states, lengths, resets, qz, ez, qf, ef, odd = ctx.saved_tensors
+    (T, B, N), G, dtype, decay_input, keep8, has_h0 = ctx.meta
+    if keep8 and odd is None:       # the 8-bit kernel is for a gate per channel
+        z, f = unpack8(Packed8(qz, ez, dtype)), unpack8(Packed8(qf, ef, dtype))
+        qz = ez = qf = ef = None
+    need_z, need_f, need_h = ctx.needs_input_grad[:3]
+    like_z, like_f = (qz, qf) if z is None else (z, f)
+    dev = states.device
+    dz = _lib.empty_rows(like_z, dtype) if need_z else None
+    df = _lib.empty_rows(like_f, dtype) if need_f else None
+    dh0 = torch.empty(B, N, device=dev) if need_h and has_h0 else None
+    if T and B and N:
+        if gh is not None:
+            gh = _lib.rows(gh)
+        if ghT is not None:
+            ghT = ghT.contiguous()
+        st = []
+        for t in (z, f, None, gh, dz, df):
+            st += t.stride()[:2] if t is not None else (0, 0)
+        s = _lib.Scan(T, B, N, G, _lib.SEQ_DTYPES[dtype], 1 if decay_input else 0,
+                      1 if lengths is not None and lengths.dtype == torch.int64 else 0, 0, *st)
+        ws, nbytes = None, 0
+        if need_f and G != N:
+            nbytes = _lib.lib().delrec_gated_scan_backward_workspace(ctypes.byref(s))
+            ws = _lib.scratch(nbytes, dev)
+        A = _lib.addr
+        _lib.launch("delrec_gated_scan_backward", dev, ctypes.byref(s), A(z), A(f), A(qz), A(ez), A(qf), A(ef),
+                    A(odd), A(lengths), A(resets), states.data_ptr(), A(gh), A(ghT), A(dz), A(df), A(dh0), A(ws),
+                    nbytes)
+    elif dh0 is not None:
+        dh0 = ghT.clone() if ghT is not None else dh0.zero_()
+    return dz, df, dh0, None, None, None, None
+
+
+_once = once_differentiable(_backward)
 
 
 def gated_scan(z, f, h0=None, *, lengths=None, resets=None, decay_input=True, checkpoint8=False):
