@@ -148,6 +148,28 @@ __device__ __forceinline__ float block_sum(float v, float (*red)[32], int& slot)
   return v;
 }
 
+// Three sums at once.
+__device__ __forceinline__ void block_sum3(float (&v)[3], float (*red)[32], int& slot) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
+  if (nw == 1) return;
+  if (lane == 0) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) red[slot * 3 + k][threadIdx.x >> 5] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) v[k] = (lane & 15) < nw ? red[slot * 3 + k][lane & 15] : 0.f;
+  slot ^= 1;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+}
+
 // E = V * IT elements per thread: vector k starts at channel (k * threads + thread) * V.
 // KIND: GATE_*.
 template <class T, int V, int IT, int KIND>
@@ -265,9 +287,12 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
   st.wait(0);
 }
 
+// One barrier a row: with c = scale w act yh and g = gx + rx gn w_next, the sums that dx and
+// dy need are S1 = sum gn w_next xh, S2 = sum g c and S3 = sum xh c, since G = g - rx (S1 / N) xh
+// gives sum G c = S2 - rx (S1 / N) S3.  The difference loses no more than forming each G does.
 template <class T, int V, int IT, int KIND>
 __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
-  __shared__ float red[2][32];
+  __shared__ float red[6][32];
   extern __shared__ __align__(16) char norm_stage[];
   constexpr int E = V * IT;
   constexpr bool GATE = KIND != GATE_NONE;
@@ -354,22 +379,28 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
       continue;
     }
     st.wait(p.slots);
-    float y[E], a[E], da[E], g[E];   // yh; act; act'; the gradient
-#pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = 0.f;
-    if (p.y) {
-#pragma unroll
-      for (int k = 0; k < IT; ++k) st.read(at, 3, k, yr(cur), left, nthV, y + k * V);
-#pragma unroll
-      for (int i = 0; i < E; ++i) y[i] *= ry;
-    }
+    float y[E], a[E], da[E], g[E], xh[E];   // yh, act, act', the gradient, xh
+    float sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      if (GATE) st.read(at, 4, k, ur(cur), left, nthV, da + k * V);
+      float v[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int i = k * V + j;
+        y[i] = g[i] = xh[i] = v[j] = 0.f;
         a[i] = 1.f;
+      }
+      if (p.y) st.read(at, 3, k, yr(cur), left, nthV, y + k * V);
+      if (GATE) st.read(at, 4, k, ur(cur), left, nthV, da + k * V);
+      if (p.gx) st.read(at, 0, k, gxr(cur), left, nthV, g + k * V);
+      if (p.gn) {
+        st.read(at, 1, k, gnr(cur), left, nthV, v);
+        st.read(at, 2, k, xr(cur), left, nthV, xh + k * V);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int i = k * V + j;
+        y[i] *= ry;
         if (GATE) {
           const float u = da[i];
           float sg, so;
@@ -377,63 +408,34 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
           a[i] = KIND == GATE_SIGMOID ? sg : u * sg;
           da[i] = KIND == GATE_SIGMOID ? sg * so : sg * fmaf(u, so, 1.f);
         }
+        const float c = ws[i] * a[i] * y[i];
+        xh[i] = (xh[i] + c) * rx;               // rx = 0 without a next norm
+        qn[i] = fmaf(v[j], xh[i], qn[i]);
+        v[j] *= nw[i];
+        g[i] = fmaf(rx, v[j], g[i]);
+        sum[0] = fmaf(v[j], xh[i], sum[0]);
+        sum[1] = fmaf(g[i], c, sum[1]);
+        sum[2] = fmaf(xh[i], c, sum[2]);
       }
     }
+    block_sum3(sum, red, slot);
+    const float back = rx * (sum[0] * inv_n), s2 = (sum[1] - back * sum[2]) * inv_n;
 #pragma unroll
-    for (int i = 0; i < E; ++i) g[i] = 0.f;
-    if (p.gx) {
+    for (int k = 0; k < IT; ++k) {
+      float oy[V], ou[V];
 #pragma unroll
-      for (int k = 0; k < IT; ++k) st.read(at, 0, k, gxr(cur), left, nthV, g + k * V);
-    }
-    if (p.gn) {
-      float xh[E], v[E];
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        st.read(at, 2, k, xr(cur), left, nthV, xh + k * V);
-        st.read(at, 1, k, gnr(cur), left, nthV, v + k * V);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int i = k * V + j;
-          xh[i] = fmaf(y[i], ws[i] * a[i], xh[i]) * rx;
-          qn[i] = fmaf(v[i], xh[i], qn[i]);
-          v[i] *= nw[i];
-          s = fmaf(v[i], xh[i], s);
-        }
-      }
-      s = block_sum(s, red, slot) * inv_n;
-#pragma unroll
-      for (int i = 0; i < E; ++i) g[i] = fmaf(rx, fmaf(-xh[i], s, v[i]), g[i]);
-    }
-    if (dx) {
-#pragma unroll
-      for (int k = 0; k < IT; ++k)
-        if (k * nthV < left) store_vec<T, V>(dx + k * nthV, g + k * V);
-    }
-    if (p.y) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const float gy = g[i] * y[i];
+      for (int j = 0; j < V; ++j) {
+        const int i = k * V + j;
+        g[i] = fmaf(-back, xh[i], g[i]);
+        const float gw = g[i] * ws[i], gy = g[i] * y[i];
         q[i] = fmaf(gy, a[i], q[i]);
-        if (GATE) da[i] *= gy * ws[i];        // du
-        g[i] *= ws[i] * a[i];                 // v
-        s = fmaf(g[i], y[i], s);
+        ou[j] = GATE ? gw * y[i] * da[i] : 0.f;
+        oy[j] = ry * fmaf(-y[i], s2, gw * a[i]);
       }
-      if (GATE && du) {
-#pragma unroll
-        for (int k = 0; k < IT; ++k)
-          if (k * nthV < left) store_vec<T, V>(du + k * nthV, da + k * V);
-      }
-      s = block_sum(s, red, slot) * inv_n;
-      if (dy) {
-#pragma unroll
-        for (int k = 0; k < IT; ++k) {
-          float o[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) o[j] = ry * fmaf(-y[k * V + j], s, g[k * V + j]);
-          if (k * nthV < left) store_vec<T, V>(dy + k * nthV, o);
-        }
+      if (k * nthV < left) {
+        if (dx) store_vec<T, V>(dx + k * nthV, g + k * V);
+        if (dy) store_vec<T, V>(dy + k * nthV, oy);
+        if (GATE && du) store_vec<T, V>(du + k * nthV, ou);
       }
     }
     cur.next(gs, gt, gb, p.B);
