@@ -75,8 +75,8 @@ __device__ __forceinline__ unsigned group_mask(int lane) {
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(512, 2) k_pack8(Q8Args p) {
-  constexpr int L = 32 / V, U = V == 1 ? 2 : 4;
+__global__ void __launch_bounds__(512, 3) k_pack8(Q8Args p) {
+  constexpr int L = 32 / V, U = 2;
   const int lane = threadIdx.x & 31;
   const unsigned mask = group_mask<V>(lane);
   const int sub = threadIdx.x / p.span;
@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(512, 2) k_pack8(Q8Args p) {
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(512, 2) k_unpack8(Q8Args p) {
-  constexpr int U = V == 1 ? 2 : 4;
+__global__ void __launch_bounds__(512, 3) k_unpack8(Q8Args p) {
+  constexpr int U = 2;
   const int sub = threadIdx.x / p.span;
   const long long step = (long long)gridDim.x * p.rpb;
   for (int l = threadIdx.x - sub * p.span; l < p.span; l += blockDim.x) {

@@ -187,6 +187,13 @@ def require_sequence(t):
     return code
 
 
+def require_sizes(*sizes):
+    """The library's sizes are 32-bit."""
+    for n in sizes:
+        if n > 0x7fffffff:
+            raise RuntimeError(f"delrec_b200: a dimension of {n} is past the library's 32-bit sizes")
+
+
 def require_lengths(lengths, B, device):
     if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64) or lengths.device != device \
             or not lengths.is_contiguous():

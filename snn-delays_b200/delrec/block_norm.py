@@ -127,6 +127,7 @@ def _check(x, others, weights, lengths, eps):
     shape, dtype, device = x.shape, x.dtype, x.device
     if len(shape) != 3:
         raise RuntimeError(f"delrec_b200: x must be (T, B, N), got {tuple(shape)}")
+    _lib.require_sizes(*shape)
     for t in others:
         if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device):
             raise RuntimeError("delrec_b200: x, y and gate must share shape, dtype and device")

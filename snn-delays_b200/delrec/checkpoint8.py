@@ -41,6 +41,7 @@ def pack8(x) -> Packed8:
     code = _lib.require_sequence(x)
     if x.dim() == 0:
         raise RuntimeError("delrec_b200: pack8 expects at least one dimension")
+    _lib.require_sizes(x.shape[-1])
     x = x.contiguous()
     shape, device = x.shape, x.device
     p = empty8(shape, x.dtype, device)
@@ -65,6 +66,7 @@ def unpack8(packed: Packed8, dtype=None):
     if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() == 0 \
             or e.shape != (*shape[:-1], -(-shape[-1] // GROUP)):
         raise RuntimeError("delrec_b200: not a Packed8 (int8 (..., N) with uint8 (..., ceil(N / 32)))")
+    _lib.require_sizes(shape[-1])
     q, e = q.contiguous(), e.contiguous()
     x = torch.empty(shape, dtype=dtype or own, device=device)
     n = x.numel()

@@ -30,6 +30,7 @@ def _check(z, f, dims, layout):
         raise RuntimeError(f"delrec_b200: z and f must be {layout}, got {tuple(zs)} and {tuple(fs)}")
     if f.dtype != z.dtype or f.device != z.device:
         raise RuntimeError("delrec_b200: z and f must share dtype and device")
+    _lib.require_sizes(*zs)
     N, G = zs[-1], fs[-1]
     if N != G and (G == 0 or N % G):
         raise RuntimeError(f"delrec_b200: the {G} gates of f must divide the {N} channels of z")

@@ -52,13 +52,15 @@ class LinearFn(torch.autograd.Function):
             keep = empty8(x2.shape, x2.dtype, dev)
         if M > 0:
             lib = _lib.lib()
-            ws = _lib.workspace(lib.delrec_linear_forward_workspace(M, K, N, int(binary)), dev)
+            nbytes = lib.delrec_linear_forward_workspace(M, K, N, int(binary))
             P = _lib.ptr
             if keep is not None:
+                ws = _lib.scratch(nbytes, dev)
                 _lib.check(lib.delrec_linear_forward8(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(keep.q),
                                                       P(keep.e), P(ws), ws.numel(), _lib.stream_ptr(dev)),
                            "delrec_linear_forward8")
             else:
+                ws = _lib.workspace(nbytes, dev)
                 _lib.check(lib.delrec_linear_forward(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(ws),
                                                      ws.numel(), _lib.stream_ptr(dev)), "delrec_linear_forward")
         if ctx.packed:
@@ -92,7 +94,7 @@ class LinearFn(torch.autograd.Function):
             lib = _lib.lib()
             P = _lib.ptr
             if ctx.packed:
-                ws = _lib.workspace(lib.delrec_linear_backward8_workspace(M, K, N), dev)
+                ws = _lib.scratch(lib.delrec_linear_backward8_workspace(M, K, N), dev)
                 _lib.check(lib.delrec_linear_backward8(M, K, N, P(x2), P(e), P(w), P(g), P(dx), P(dw), P(db),
                                                        P(ws), ws.numel(), _lib.stream_ptr(dev)),
                            "delrec_linear_backward8")

@@ -150,3 +150,118 @@ def test_captured_training_pass():
     torch.cuda.synchronize()
     for a, b in zip(got, go()):
         assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements (4.3 GB each): the last rows are those of a call on them alone."""
+    from delrec.block_norm import block_norm
+    from delrec.checkpoint8 import pack8, unpack8
+    from delrec.gated import gated_scan
+    Tb, Bb, Nb = 70000, 60, 520
+    z = torch.empty(Tb, Bb, Nb, dtype=torch.bfloat16, device="cuda").normal_()
+    assert z.numel() > 2 ** 31
+    f = torch.full((1, 1, 1), 3.0, dtype=torch.bfloat16, device="cuda").expand(Tb, Bb, 1)
+    tol = dict(rtol=2.0 ** -7, atol=2.0 ** -10.5)      # a step of bf16, sums in another order
+    h, hT = gated_scan(z, f)
+    one, last = gated_scan(z[:, -1:].contiguous(), f[:, -1:])
+    torch.testing.assert_close(h[:, -1:], one, **tol)
+    torch.testing.assert_close(hT[-1:], last, rtol=0, atol=2.0 ** -10.5)
+    del h
+    n = block_norm(z)
+    torch.testing.assert_close(n[-3:], block_norm(z[-3:].clone()), rtol=2.0 ** -7, atol=2.0 ** -18)
+    del n
+    p = pack8(z)
+    assert torch.equal(unpack8(p._replace(q=p.q[-3:], e=p.e[-3:])), unpack8(pack8(z[-3:].clone())))
+    assert torch.equal(unpack8(p)[-3:], unpack8(pack8(z[-3:].clone())))
+
+
+def test_backward_past_32_bits():
+    from delrec.gated import gated_scan
+    Tb, Bb, Nb = 4200, 1024, 512
+    z = torch.empty(Tb, Bb, Nb, dtype=torch.bfloat16, device="cuda").normal_()
+    f = torch.full((1, 1, 1), 1.0, dtype=torch.bfloat16, device="cuda").expand(Tb, Bb, Nb)
+    g = torch.ones(1, 1, 1, dtype=torch.bfloat16, device="cuda").expand(Tb, Bb, Nb)
+    for keep in (False, True):
+        zz = z.detach().requires_grad_(True)
+        h, _ = gated_scan(zz, f, checkpoint8=keep)
+        (dz,) = torch.autograd.grad(h, zz, g)
+        zs = z[:, -1:].clone().requires_grad_(True)
+        hs, _ = gated_scan(zs, f[:, -1:], checkpoint8=keep)
+        (ds,) = torch.autograd.grad(hs, zs, g[:, -1:])
+        torch.testing.assert_close(h[:, -1:], hs, rtol=2.0 ** -7, atol=2.0 ** -10.5)
+        torch.testing.assert_close(dz[:, -1:], ds, rtol=2.0 ** -7, atol=2.0 ** -10.5)
+        del h, dz
+
+
+def test_second_derivatives_are_refused():
+    from delrec.block_norm import block_norm
+    from delrec.gated import gated_scan
+    x = torch.randn(5, 2, 8, device="cuda", requires_grad=True)
+    for fn in (lambda: gated_scan(x, x)[0], lambda: block_norm(x)):
+        out = fn()
+        go = torch.randn_like(out).requires_grad_(True)
+        (g,) = torch.autograd.grad(out, x, go, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_two_streams_at_once():
+    """Training passes of two models' operators on two streams, interleaved: each has the results it has
+    alone."""
+    model, x, g, lengths = _case()
+    lengths = lengths.cuda()
+    small = Stack(checkpoint8=True).cuda()
+    small.load_state_dict(model.state_dict())
+
+    def go(m):
+        out = m(x, lengths)
+        return (out.detach(), *torch.autograd.grad(out, list(m.parameters()), g))
+
+    want = [go(model), go(small)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, m in enumerate((model, small)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(go(m))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for a, b in zip(r, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_two_graphs_with_8_bit_projections_at_once():
+    """Captured training passes with 8-bit projections share no scratch: replayed on two streams at once."""
+    from delrec.linear import linear
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    sets = [[torch.randn(s, device="cuda", generator=gen) for s in ((900, 130), (70, 130), (900, 70))] for _ in range(2)]
+
+    def go(x, w, g):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        out = linear(x, w, binary_input=False, checkpoint8=True)
+        return (out.detach(), *torch.autograd.grad(out, (x, w), g))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        go(*sets[0])
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [], []
+    for args in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(go(*args))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for st, graph in zip(streams, graphs):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, args in zip(outs, sets):
+        for a, b in zip(got, go(*args)):
+            assert torch.equal(a, b)

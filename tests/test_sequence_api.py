@@ -70,6 +70,19 @@ def test_shape_checks():
             block_norm.block_join(*args, **kw)
 
 
+def test_sizes_past_32_bits_are_refused():
+    from delrec import block_norm, checkpoint8, gated
+    big = 1 << 31
+    for shape in ((big, 1, 4), (1, big, 4), (1, 1, big)):
+        t = _Fake(*shape)
+        with pytest.raises(RuntimeError, match="32-bit"):
+            gated.gated_scan(t, t)
+        with pytest.raises(RuntimeError, match="32-bit"):
+            block_norm.block_norm(t)
+    with pytest.raises(RuntimeError, match="32-bit"):
+        checkpoint8.pack8(_Fake(big))
+
+
 def _scan(**kw):
     from delrec import _lib
     d = dict(T=4, B=2, N=8, G=8, dtype=0)
