@@ -18,6 +18,8 @@
 // the unrounded x'.
 #pragma once
 
+#include <string.h>
+
 #include "seq_common.cuh"
 
 namespace delrec {
@@ -27,6 +29,7 @@ static constexpr int kNormThreads = 512;
 
 struct NormArgs {
   int T, B, N, wide, kind;              // kind: the gate's function, where there is one
+  int pitch;                            // of rows, where all tensors share it (FLAT)
   int slots;                            // rows in shared memory: one at work, the others on their way
   float eps;
   const void* lengths;
@@ -45,16 +48,8 @@ struct NormArgs {
 };
 
 template <class T, int V>
-__device__ __forceinline__ void unpack_vec(const VecOf<T, V>& r, float* o) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = to_f(r.v[i]);
-}
-template <class T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float* o) {
-  VecOf<T, V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = from_f<T>(o[i]);
-  *(VecOf<T, V>*)p = r;
+  *(VecOf<T, V>*)p = pack_vec<T, V>(o);
 }
 
 // A row's place: row = t * B + b, stepped by the grid without a division.
@@ -68,13 +63,17 @@ struct NormRow {
     if (b >= B) { b -= B; ++t; }
   }
 };
-template <class T>
-__device__ __forceinline__ T* row_of(void* p, const NormRow& r, int st, int sb) {
-  return (T*)p + ((long long)r.t * st + (long long)r.b * sb);
+// This thread's first channel c0 of a row.  FLAT: every tensor's rows lie pitch apart, less
+// than 2^31 elements in all, so one 32-bit offset serves them all.
+template <class T, bool FLAT>
+__device__ __forceinline__ T* row_of(const NormArgs& a, void* p, const NormRow& r, int st, int sb, int c0) {
+  if (FLAT) return (T*)p + (r.r * a.pitch + c0);
+  return (T*)p + ((long long)r.t * st + (long long)r.b * sb + c0);
 }
-template <class T>
-__device__ __forceinline__ const T* row_of(const void* p, const NormRow& r, int st, int sb) {
-  return (const T*)p + ((long long)r.t * st + (long long)r.b * sb);
+template <class T, bool FLAT>
+__device__ __forceinline__ const T* row_of(const NormArgs& a, const void* p, const NormRow& r, int st, int sb, int c0) {
+  if (FLAT) return (const T*)p + (r.r * a.pitch + c0);
+  return (const T*)p + ((long long)r.t * st + (long long)r.b * sb + c0);
 }
 
 // The inputs of a row, NT tensors of IT vectors per thread.  Vectors of 4 bytes and more are
@@ -94,6 +93,16 @@ struct NormStage {
     size = blockDim.x * ROW;
     mem = m + threadIdx.x * VB;
     base = STAGED ? (unsigned)__cvta_generic_to_shared(mem) : 0;
+  }
+  // zeros, once, in the slots of vectors past the row's end: reads need no test
+  __device__ __forceinline__ void clear(int slots, int left, int nthV) const {
+    if constexpr (STAGED) {
+#pragma unroll
+      for (int k = 0; k < IT; ++k)
+        if (k * nthV >= left)
+          for (int i = 0; i < slots * NT; ++i)
+            memset(const_cast<char*>(mem) + i / NT * size + (i % NT * IT + k) * plane, 0, VB);
+    }
   }
   // col: this thread's first channel in the row
   __device__ __forceinline__ void copy(unsigned at, int ten, const T* col, int left, int nthV) const {
@@ -122,9 +131,10 @@ struct NormStage {
   }
   // vector k of tensor ten as floats; zeros past the row's end
   __device__ __forceinline__ void read(const char* at, int ten, int k, const T* col, int left, int nthV, float* o) const {
-    if (k * nthV < left) {
-      if constexpr (STAGED) unpack_vec<T, V>(*(const VecOf<T, V>*)(at + (ten * IT + k) * plane), o);
-      else unpack_vec<T, V>(*(const VecOf<T, V>*)(col + k * nthV), o);
+    if constexpr (STAGED) {
+      unpack_vec<T, V>(*(const VecOf<T, V>*)(at + (ten * IT + k) * plane), o);
+    } else if (k * nthV < left) {
+      unpack_vec<T, V>(*(const VecOf<T, V>*)(col + k * nthV), o);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = 0.f;
@@ -172,7 +182,7 @@ __device__ __forceinline__ void block_sum3(float (&v)[3], float (*red)[32], int&
 
 // E = V * IT elements per thread: vector k starts at channel (k * threads + thread) * V.
 // KIND: GATE_*.
-template <class T, int V, int IT, int KIND>
+template <class T, int V, int IT, int KIND, bool FLAT>
 __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
   __shared__ float red[2][32];
   extern __shared__ __align__(16) char norm_stage[];
@@ -194,9 +204,9 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
       ws[k * V + j] = on ? (p.w ? p.w[c] : 1.f) * (p.scale ? p.scale[c] : 1.f) : 0.f;
       nw[k * V + j] = on ? (p.nw ? p.nw[c] : 1.f) : 0.f;
     }
-  auto xr = [&](const NormRow& r) { return row_of<T>(p.x, r, p.x_t, p.x_b) + c0; };
-  auto yr = [&](const NormRow& r) { return row_of<T>(p.y, r, p.y_t, p.y_b) + c0; };
-  auto ur = [&](const NormRow& r) { return row_of<T>(p.u, r, p.u_t, p.u_b) + c0; };
+  auto xr = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.x, r, p.x_t, p.x_b, c0); };
+  auto yr = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.y, r, p.y_t, p.y_b, c0); };
+  auto ur = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.u, r, p.u_t, p.u_b, c0); };
   auto live_row = [&](const NormRow& r) { return !p.lengths || r.t < row_length(p.lengths, p.wide, r.b, p.T); };
   auto fetch = [&](const NormRow& r, unsigned at, bool live) {
     if (live) {
@@ -208,6 +218,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
     }
     st.commit();
   };
+  st.clear(p.slots, left, nthV);
   NormRow cur, ahead;
   cur.init(blockIdx.x, p.B);
   ahead = cur;
@@ -258,7 +269,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
       for (int i = 0; i < E; ++i) x[i] = 0.f;
     }
     if (p.y) {
-      T* o = row_of<T>(p.out, cur, p.o_t, p.o_b) + c0;
+      T* o = row_of<T, FLAT>(p, p.out, cur, p.o_t, p.o_b, c0);
 #pragma unroll
       for (int k = 0; k < IT; ++k)
         if (k * nthV < left) store_vec<T, V>(o + k * nthV, x + k * V);
@@ -272,7 +283,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
         rx = rsqrtf(block_sum(s, red, slot) * inv_n + p.eps);
         if (p.rx && threadIdx.x == 0) p.rx[cur.r] = rx;
       }
-      T* o = row_of<T>(p.n, cur, p.n_t, p.n_b) + c0;
+      T* o = row_of<T, FLAT>(p, p.n, cur, p.n_t, p.n_b, c0);
 #pragma unroll
       for (int k = 0; k < IT; ++k)
         if (k * nthV < left) {
@@ -290,7 +301,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_fwd(NormArgs p) {
 // One barrier a row: with c = scale w act yh and g = gx + rx gn w_next, the sums that dx and
 // dy need are S1 = sum gn w_next xh, S2 = sum g c and S3 = sum xh c, since G = g - rx (S1 / N) xh
 // gives sum G c = S2 - rx (S1 / N) S3.  The difference loses no more than forming each G does.
-template <class T, int V, int IT, int KIND>
+template <class T, int V, int IT, int KIND, bool FLAT>
 __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
   __shared__ float red[6][32];
   extern __shared__ __align__(16) char norm_stage[];
@@ -313,11 +324,11 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
       nw[k * V + j] = on ? (p.nw ? p.nw[c] : 1.f) : 0.f;
       q[k * V + j] = qn[k * V + j] = 0.f;
     }
-  auto xr = [&](const NormRow& r) { return row_of<T>(p.x, r, p.x_t, p.x_b) + c0; };
-  auto yr = [&](const NormRow& r) { return row_of<T>(p.y, r, p.y_t, p.y_b) + c0; };
-  auto ur = [&](const NormRow& r) { return row_of<T>(p.u, r, p.u_t, p.u_b) + c0; };
-  auto gxr = [&](const NormRow& r) { return row_of<T>(p.gx, r, p.gx_t, p.gx_b) + c0; };
-  auto gnr = [&](const NormRow& r) { return row_of<T>(p.gn, r, p.gn_t, p.gn_b) + c0; };
+  auto xr = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.x, r, p.x_t, p.x_b, c0); };
+  auto yr = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.y, r, p.y_t, p.y_b, c0); };
+  auto ur = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.u, r, p.u_t, p.u_b, c0); };
+  auto gxr = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.gx, r, p.gx_t, p.gx_b, c0); };
+  auto gnr = [&](const NormRow& r) { return row_of<T, FLAT>(p, p.gn, r, p.gn_t, p.gn_b, c0); };
   auto live_row = [&](const NormRow& r) { return !p.lengths || r.t < row_length(p.lengths, p.wide, r.b, p.T); };
   auto fetch = [&](const NormRow& r, unsigned at, bool live) {
     if (live) {
@@ -333,6 +344,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
     }
     st.commit();
   };
+  st.clear(p.slots, left, nthV);
   NormRow cur, ahead;
   cur.init(blockIdx.x, p.B);
   ahead = cur;
@@ -361,9 +373,9 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
     lives = (lives >> 1) | (unsigned)l << (p.slots - 2);
     ahead.next(gs, gt, gb, p.B);
     const char* at = st.mem + slot_now * st.size;
-    T* dx = p.dx ? row_of<T>(p.dx, cur, p.dx_t, p.dx_b) + c0 : nullptr;
-    T* dy = p.dy ? row_of<T>(p.dy, cur, p.dy_t, p.dy_b) + c0 : nullptr;
-    T* du = GATE && p.du ? row_of<T>(p.du, cur, p.du_t, p.du_b) + c0 : nullptr;
+    T* dx = p.dx ? row_of<T, FLAT>(p, p.dx, cur, p.dx_t, p.dx_b, c0) : nullptr;
+    T* dy = p.dy ? row_of<T, FLAT>(p, p.dy, cur, p.dy_t, p.dy_b, c0) : nullptr;
+    T* du = GATE && p.du ? row_of<T, FLAT>(p, p.du, cur, p.du_t, p.du_b, c0) : nullptr;
     if (!live) {
       float o[V];
 #pragma unroll
@@ -458,7 +470,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_bwd(NormArgs p) {
 
 // dw = scale Q, dscale = w Q (blockIdx.y = 0) and dw_next (1) from the blocks' partials: 32
 // channels and 32 runs of blocks per thread block, summed in a fixed order.
-__global__ void __launch_bounds__(1024) k_norm_dw(int N, int blocks, const float* __restrict__ part,
+static __global__ void __launch_bounds__(1024) k_norm_dw(int N, int blocks, const float* __restrict__ part,
                                                   const float* __restrict__ w, const float* __restrict__ scale,
                                                   float* __restrict__ dw, float* __restrict__ dscale,
                                                   float* __restrict__ dnw) {
@@ -486,5 +498,16 @@ __global__ void __launch_bounds__(1024) k_norm_dw(int N, int blocks, const float
     }
   }
 }
+
+// ---------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------
+struct NormShape {
+  int V, IT, threads;
+  int grid;   // blocks launched, set by the launch
+};
+// the kernels of a direction, by element type (norm_fwd.cu, norm_bwd.cu)
+int norm_run_forward(int dtype, const NormArgs& a, NormShape& s, int most, cudaStream_t st);
+int norm_run_backward(int dtype, const NormArgs& a, NormShape& s, int most, cudaStream_t st);
 
 }  // namespace delrec

@@ -359,10 +359,13 @@ __device__ __forceinline__ void scan_pack(const VecOf<T, V> (&zr)[kSeg], const V
   for (int i = 0; i < S; ++i) {
     const float sz = __shfl_sync(0xffffffffu, iz, src + i), sf = __shfl_sync(0xffffffffu, jf, src + i);
     unsigned cz[V], cf[V];
+    float zf[V], ff[V];
+    unpack_vec<T, V>(zr[i], zf);
+    unpack_vec<T, V>(fr[i], ff);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      cz[k] = q_code(to_f(zr[i].v[k]), sz);
-      cf[k] = q_code(to_f(fr[i].v[k]), sf);
+      cz[k] = q_code(zf[k], sz);
+      cf[k] = q_code(ff[k], sf);
     }
     if (on && i < n) {
       store_codes<V>(at_step(o.qz, o.stride, i), cz);
@@ -517,13 +520,15 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, R, POS, PACK, MODE>::
       for (int i = 0; i < S; ++i) {
         float w = 0.f;
         if (MODE == SCAN_WIDE) w = __shfl_sync(0xffffffffu, wide, i + (lane >= edge ? 16 : 0));
+        float zf[V], ff[V];
+        unpack_vec<T, V>(zr[i], zf);
+        if (MODE != SCAN_WIDE) unpack_vec<T, V>(fr[i], ff);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float zf = to_f(zr[i].v[k]);
           float om;
           if (MODE == SCAN_WIDE) gate_unfold(w, a[i][k], om);
-          else sigmoid_pair<Accurate<T>::value>(to_f(fr[i].v[k]), a[i][k], om);
-          x[i][k] = DI ? om * zf : zf;
+          else sigmoid_pair<Accurate<T>::value>(ff[k], a[i][k], om);
+          x[i][k] = DI ? om * zf[k] : zf[k];
         }
       }
       if (n < S) {
@@ -563,13 +568,10 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, R, POS, PACK, MODE>::
 #pragma unroll
         for (int i = 0; i < S; ++i) {
           if (i % kSeg == 0) keep(i);
-          VecOf<T, V> o;
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
+          for (int k = 0; k < V; ++k)
             s[k] = (POS && ((cut >> i) & 1)) ? x[i][k] : fmaf(a[i][k], s[k], x[i][k]);
-            o.v[k] = from_f<T>(s[k]);
-          }
-          *(VecOf<T, V>*)at_step(h, p.h_t, i) = o;
+          *(VecOf<T, V>*)at_step(h, p.h_t, i) = pack_vec<T, V>(s);
         }
       } else {
 #pragma unroll
@@ -633,11 +635,6 @@ struct ScanIn {
     else return g_[i];
   }
 };
-template <class T, int V>
-__device__ __forceinline__ float raw_value(const RawBytes<(int)sizeof(T) * V>& r, int k) {
-  return to_f(((const VecOf<T, V>*)&r)->v[k]);
-}
-
 // The walk of one backward segment in time order: gates w, df factors e, and the segment's map
 // of the reverse recurrence, in forward order: G enters at the end times Pi a, and g_i times
 // the gates up to i.  PLAIN: all steps are inside the sequence, no code stands for an infinity
@@ -657,13 +654,18 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, 
     }
     if (MODE == SCAN_WIDE) ww = __shfl_sync(0xffffffffu, r.wide, i + (lane >= r.edge ? 16 : 0));
     const auto zi = r.z(i), fi = r.f(i);
-    const VecOf<T, V> gi = r.g(i);
+    float gf[V], zv[V], fv[V];
+    unpack_vec<T, V>(r.g(i), gf);
+    if constexpr (!B8) {
+      unpack_vec<T, V>(*(const VecOf<T, V>*)&zi, zv);
+      if (MODE != SCAN_WIDE) unpack_vec<T, V>(*(const VecOf<T, V>*)&fi, fv);
+    }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float zf, ff = 0.f;
       if constexpr (!B8) {
-        zf = raw_value<T, V>(zi, k);
-        if (MODE != SCAN_WIDE) ff = raw_value<T, V>(fi, k);
+        zf = zv[k];
+        if (MODE != SCAN_WIDE) ff = fv[k];
       } else if constexpr (!PLAIN) {
         zf = q_decode((int8_t)zi.b[k], sz);
         ff = q_decode((int8_t)fi.b[k], sf);
@@ -692,7 +694,7 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& p, const ScanIn<T, V, 
         m[k].x = 0.f;
       } else if (PLAIN || i < n) {
         m[k].x *= a;
-        m[k].y = fmaf(m[k].x, to_f(gi.v[k]), m[k].y);
+        m[k].y = fmaf(m[k].x, gf[k], m[k].y);
       }
     }
   }
@@ -706,24 +708,23 @@ __device__ __forceinline__ void scan_walk_back(const ScanArgs& p, const In& r, c
                                                T* df) {
 #pragma unroll
   for (int i = S - 1; i >= 0; --i) {
-    const VecOf<T, V> gi = r.g(i);
-    VecOf<T, V> oz, of;
+    float gf[V], oz[V], of[V];
+    unpack_vec<T, V>(r.g(i), gf);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float a, om;
       gate_unfold(w[i][k], a, om);
-      const float G_ = q[k] + to_f(gi.v[k]);
+      const float G_ = q[k] + gf[k];
       float dzv = DI ? om * G_ : G_, dfv = e[i][k] * G_;
       float nq = (POS && ((cut >> i) & 1)) ? 0.f : a * G_;
       if (!WHOLE && i >= n) { dzv = 0.f; dfv = 0.f; nq = q[k]; }
       q[k] = nq;
-      e[i][k] = dfv;
-      oz.v[k] = from_f<T>(dzv);
-      of.v[k] = from_f<T>(dfv);
+      e[i][k] = of[k] = dfv;
+      oz[k] = dzv;
     }
     if (WHOLE || i < nT) {
-      if (dz) *(VecOf<T, V>*)at_step(dz, p.dz_t, i) = oz;
-      if (df) *(VecOf<T, V>*)at_step(df, p.df_t, i) = of;
+      if (dz) *(VecOf<T, V>*)at_step(dz, p.dz_t, i) = pack_vec<T, V>(oz);
+      if (df) *(VecOf<T, V>*)at_step(df, p.df_t, i) = pack_vec<T, V>(of);
     }
   }
 }

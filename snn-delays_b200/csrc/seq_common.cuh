@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/delrec_b200.h"
 
@@ -97,6 +98,43 @@ template <class T, int V>
 struct alignas(sizeof(T) * V) VecOf {
   T v[V];
 };
+// V elements <-> floats; 16-bit ones in pairs (one operation an element to widen, half a one
+// to round)
+template <class T, int V>
+__device__ __forceinline__ void unpack_vec(const VecOf<T, V>& r, float* o) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const unsigned w = ((const unsigned*)&r)[i / 2];
+      if constexpr (std::is_same_v<T, __half>) {
+        const float2 f = __half22float2(*(const __half2*)&w);
+        o[i] = f.x;
+        o[i + 1] = f.y;
+      } else {
+        o[i] = __uint_as_float(w << 16);
+        o[i + 1] = __uint_as_float(w & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = to_f(r.v[i]);
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ VecOf<T, V> pack_vec(const float* o) {
+  VecOf<T, V> r;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (std::is_same_v<T, __half>) ((__half2*)&r)[i / 2] = __floats2half2_rn(o[i], o[i + 1]);
+      else ((__nv_bfloat162*)&r)[i / 2] = __floats2bfloat162_rn(o[i], o[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = from_f<T>(o[i]);
+  }
+  return r;
+}
 
 // lengths (B) int32 or int64; NULL: every row is T long
 __device__ __forceinline__ int row_length(const void* lengths, int wide, int b, int T) {

@@ -25,11 +25,13 @@ static int check_block(const delrec_block* s) {
   return DELREC_OK;
 }
 
-// may every row of these tensors be read and written V elements at a time?
+// May every row of these tensors be read and written V elements at a time?  Do their rows lie
+// one pitch apart?
 struct NormAlign {
-  int esz;
+  int esz, B;
   bool ok[2];   // 8 and 16 bytes
-  explicit NormAlign(int esz_, int N) : esz(esz_) {
+  long long pitch = -1;   // -1: none seen, 0: not shared
+  NormAlign(int esz_, int N, int B_) : esz(esz_), B(B_) {
     ok[0] = (size_t)N * esz % 8 == 0;
     ok[1] = (size_t)N * esz % 16 == 0;
   }
@@ -39,13 +41,12 @@ struct NormAlign {
                                  (unsigned long long)(sb * esz);
     if (m & 7) ok[0] = false;
     if (m & 15) ok[1] = false;
+    if (st != B * sb || (pitch >= 0 && sb != pitch)) pitch = 0;
+    else pitch = sb;
   }
+  int flat(long long rows) const { return pitch > 0 && rows * pitch < 0x7fffffffLL ? (int)pitch : 0; }
 };
 
-struct NormShape {
-  int V, IT, threads;
-  int grid;   // blocks launched, set by the launch
-};
 static NormShape norm_shape(int N, int V, int esz, int most_threads) {
   NormShape s{};
   s.V = V;
@@ -65,49 +66,6 @@ static int norm_most_blocks(const delrec_block* s) {
 }
 static size_t norm_bwd_ws(const delrec_block* s) { return (size_t)norm_most_blocks(s) * 2 * s->N * sizeof(float); }
 
-// As many blocks as fit at once: each walks its rows, the next on its way.  Where two blocks
-// or fewer fit an SM they cannot cover each other's waits, and a third row in flight pays
-// (N=2048 bf16 backward 509 -> 372 us); where five fit it costs (N=512 fp32 backward 165 -> 183 us).
-template <class K>
-static int norm_start(K kern, int row_bytes, NormArgs a, NormShape& s, int most, cudaStream_t st) {
-  int per_sm = 0, smem = 0;
-  for (a.slots = 2; a.slots <= 3; ++a.slots) {
-    smem = a.slots * row_bytes * s.threads;
-    if (smem > 40 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    SQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem));
-    if (per_sm > 2 || row_bytes == 0 || 3 * row_bytes * s.threads > 100 * 1024) break;
-  }
-  if (a.slots > 3) a.slots = 3;
-  s.grid = std::min(most, std::max(1, std::min(per_sm, 16)) * kSeqSMs);
-  kern<<<s.grid, s.threads, smem, st>>>(a);
-  SQ_LAUNCHED();
-  return DELREC_OK;
-}
-template <class T, int V, bool BWD, int KIND, int IT = 1>
-static int norm_by_it(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
-  if constexpr (V * IT <= 32) {
-    if (s.IT != IT) return norm_by_it<T, V, BWD, KIND, 2 * IT>(a, s, most, st);
-    if constexpr (BWD)
-      return norm_start(k_norm_bwd<T, V, IT, KIND>, NormStage<T, V, IT, KIND ? 5 : 4>::ROW, a, s, most, st);
-    else
-      return norm_start(k_norm_fwd<T, V, IT, KIND>, NormStage<T, V, IT, KIND ? 3 : 2>::ROW, a, s, most, st);
-  }
-  return DELREC_ERR_UNSUPPORTED;
-}
-template <class T, int V, bool BWD>
-static int norm_by_gate(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
-  if (a.kind == GATE_NONE) return norm_by_it<T, V, BWD, GATE_NONE>(a, s, most, st);
-  if (a.kind == GATE_SIGMOID) return norm_by_it<T, V, BWD, GATE_SIGMOID>(a, s, most, st);
-  return norm_by_it<T, V, BWD, GATE_SILU>(a, s, most, st);
-}
-// the widest access the tensors allow, 16 bytes at most
-template <class T, bool BWD>
-static int norm_run(const NormArgs& a, NormShape& s, int most, cudaStream_t st) {
-  constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
-  if (s.V == V16) return norm_by_gate<T, V16, BWD>(a, s, most, st);
-  if (s.V == V8) return norm_by_gate<T, V8, BWD>(a, s, most, st);
-  return norm_by_gate<T, 1, BWD>(a, s, most, st);
-}
 static int norm_width(const NormAlign& al) { return al.ok[1] ? 16 / al.esz : (al.ok[0] ? 8 / al.esz : 1); }
 
 static NormArgs norm_args(const delrec_block* s) {
@@ -167,7 +125,7 @@ int delrec_block_norm_forward(const delrec_block* s, const void* x, const void* 
   a.x = x; a.y = y; a.u = u; a.w = w; a.scale = scale; a.nw = next_w; a.lengths = lengths;
   a.out = out; a.n = n; a.ry = ry; a.rx = rx;
   const int gate = y ? s->gate : GATE_NONE;
-  NormAlign al(s->dtype == DELREC_F32 ? 4 : 2, s->N);
+  NormAlign al(s->dtype == DELREC_F32 ? 4 : 2, s->N, s->B);
   al.add(x, s->x_t, s->x_b);
   al.add(n, s->n_t, s->n_b);
   if (y) {
@@ -177,9 +135,8 @@ int delrec_block_norm_forward(const delrec_block* s, const void* x, const void* 
   }
   NormShape sh = norm_shape(s->N, norm_width(al), al.esz, kNormThreads);
   a.kind = gate;
-  return by_dtype(s->dtype, [&](auto t) {
-    return norm_run<decltype(t), false>(a, sh, norm_most_blocks(s), (cudaStream_t)stream);
-  });
+  a.pitch = al.flat((long long)s->T * s->B);
+  return norm_run_forward(s->dtype, a, sh, norm_most_blocks(s), (cudaStream_t)stream);
 }
 
 size_t delrec_block_norm_backward_workspace(const delrec_block* s) { return check_block(s) ? 0 : norm_bwd_ws(s); }
@@ -198,7 +155,7 @@ int delrec_block_norm_backward(const delrec_block* s, const void* x, const void*
   a.ry = const_cast<float*>(ry); a.rx = const_cast<float*>(rx);
   a.gx = gx; a.gn = gn; a.dx = dx; a.dy = dy; a.du = du; a.part = sums ? (float*)ws : nullptr;
   const int gate = y ? s->gate : GATE_NONE;
-  NormAlign al(s->dtype == DELREC_F32 ? 4 : 2, s->N);
+  NormAlign al(s->dtype == DELREC_F32 ? 4 : 2, s->N, s->B);
   if (gn) al.add(x, s->x_t, s->x_b);
   al.add(gx, s->gx_t, s->gx_b);
   al.add(gn, s->gn_t, s->gn_b);
@@ -213,8 +170,9 @@ int delrec_block_norm_backward(const delrec_block* s, const void* x, const void*
   }
   NormShape sh = norm_shape(s->N, norm_width(al), al.esz, kNormThreads);
   a.kind = gate;
+  a.pitch = al.flat((long long)s->T * s->B);
   const cudaStream_t st = (cudaStream_t)stream;
-  const int r = by_dtype(s->dtype, [&](auto t) { return norm_run<decltype(t), true>(a, sh, norm_most_blocks(s), st); });
+  const int r = norm_run_backward(s->dtype, a, sh, norm_most_blocks(s), st);
   if (r || !sums) return r;
   k_norm_dw<<<dim3((s->N + 31) / 32, dnext_w ? 2 : 1), 1024, 0, st>>>(s->N, sh.grid, (const float*)ws, w, scale, dw, dscale, dnext_w);
   SQ_LAUNCHED();
