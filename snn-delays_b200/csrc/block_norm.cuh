@@ -15,7 +15,9 @@
 // channel), so HBM bounds it.  Sums are fp32: within a row a shuffle tree and one exchange through
 // shared memory; over rows per thread, then one partial per block and channel, summed in
 // block order by a second kernel (no atomics: the same bits every time).  n is formed from
-// the unrounded x'.
+// the unrounded x'.  Measured, forward / backward: T=250 B=256 N=512 fp32 112 / 166 us (5.8 / 6.3
+// TB/s); T=784 B=64 N=2048 bf16 168 / 347 us (6.1 / 4.7 TB/s), the latter bound by issue slots at the
+// 16 warps that 128 registers leave an SM.
 #pragma once
 
 #include <string.h>

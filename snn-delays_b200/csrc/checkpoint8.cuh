@@ -59,7 +59,9 @@ __device__ __forceinline__ __half q_store<__half>(float v, int q) {
 // channels of a row (16 bytes of x where rows allow it), so 32 / V lanes hold a group; a
 // block covers whole rows of threads side by side (span = lanes of a row, rounded up to whole
 // groups), or walks along rows wider than a block, and steps down the rows without divisions, U
-// rows in flight.  HBM bounds both: x once, q and e once.
+// rows in flight.  HBM bounds both: x once, q and e once (64000 x 700 fp32: packed in 50 us,
+// restored in 53, of 35 at the copy rate; registers are held to 40 for 40 warps an SM, which
+// beats more rows in flight on fewer warps, 49 and 59 us).
 struct Q8Args {
   long long rows;
   int N, gpr, span, rpb;   // groups and lanes of a row, rows side by side in a block
