@@ -45,23 +45,13 @@ __device__ __forceinline__ float q_decode(int q, float s) {
   return (float)q * s;
 }
 
-// A restored value in type T; fp16 saturates at its largest value.
-template <class T>
-__device__ __forceinline__ T q_store(float v, int q) {
-  return from_f<T>(v);
-}
-template <>
-__device__ __forceinline__ __half q_store<__half>(float v, int q) {
-  return __float2half_rn(q >= 127 || q <= -127 ? v : fminf(fmaxf(v, -65504.f), 65504.f));
-}
-
 // x (rows, N) contiguous <-> q (rows, N), e (rows, ceil(N / 32)).  A thread takes V consecutive
 // channels of a row (16 bytes of x where rows allow it), so 32 / V lanes hold a group; a
 // block covers whole rows of threads side by side (span = lanes of a row, rounded up to whole
 // groups), or walks along rows wider than a block, and steps down the rows without divisions, U
-// rows in flight.  HBM bounds both: x once, q and e once (64000 x 700 fp32: packed in 50 us,
-// restored in 53, of 35 at the copy rate; registers are held to 40 for 40 warps an SM, which
-// beats more rows in flight on fewer warps, 49 and 59 us).
+// rows in flight.  HBM bounds both: x once, q and e once (64000 x 700 fp32: packed in 47 us,
+// restored in 39, of 35 at the copy rate; registers are held to 40 for 40 warps an SM: more rows in
+// flight on fewer warps took longer, and places multiplied out for every row 53).
 struct Q8Args {
   long long rows;
   int N, gpr, span, rpb;   // groups and lanes of a row, rows side by side in a block
@@ -77,7 +67,7 @@ __device__ __forceinline__ unsigned group_mask(int lane) {
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(512, 3) k_pack8(Q8Args p) {
+__global__ void __launch_bounds__(512, V == 8 ? 2 : 3) k_pack8(Q8Args p) {
   constexpr int L = 32 / V, U = 2;
   const int lane = threadIdx.x & 31;
   const unsigned mask = group_mask<V>(lane);
@@ -86,81 +76,120 @@ __global__ void __launch_bounds__(512, 3) k_pack8(Q8Args p) {
   for (int l = threadIdx.x - sub * p.span; l < p.span; l += blockDim.x) {
     const int c = l * V;
     const bool on = c < p.N;
-    for (long long r0 = blockIdx.x * (long long)p.rpb + sub; r0 < p.rows; r0 += U * step) {
+    long long r = blockIdx.x * (long long)p.rpb + sub;
+    // places of row r, and from a row to the next one taken
+    const T* x = (const T*)p.x + r * p.N + c;
+    int8_t* q = p.q + r * p.N + c;
+    uint8_t* e = p.e + r * p.gpr + c / kQGroup;
+    const long long dn = step * p.N, de = step * p.gpr;
+    for (; r < p.rows; r += U * step) {
       VecOf<T, V> raw[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const long long r = r0 + j * step;
 #pragma unroll
         for (int k = 0; k < V; ++k) raw[j].v[k] = from_f<T>(0.f);
-        if (on && r < p.rows) raw[j] = *(const VecOf<T, V>*)((const T*)p.x + r * p.N + c);
+        if (on && r + j * step < p.rows) raw[j] = *(const VecOf<T, V>*)x;
+        x += dn;
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const long long r = r0 + j * step;
-        if (r >= p.rows) break;     // the same for the lanes of a group
-        unsigned top = 0;
+        if (r + j * step < p.rows) {     // the same for the lanes of a group
+          float v[V];
+          unpack_vec<T, V>(raw[j], v);
+          unsigned top = 0;
 #pragma unroll
-        for (int k = 0; k < V; ++k) top = max(top, __float_as_uint(to_f(raw[j].v[k])) & 0x7fffffffu);
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-        unsigned ex, code[V];
-        if (top < __float_as_uint(kQLargest)) {
-          // the sum's low byte is rint(x / s): the quotient is exact, the addition rounds
-          ex = q_exponent(top);
-#pragma unroll
-          for (int k = 0; k < V; ++k)
-            code[k] = __float_as_uint(fmaf(to_f(raw[j].v[k]), q_inverse_scale(ex), 12582912.f));
-        } else {
-          top = 0;
-#pragma unroll
-          for (int k = 0; k < V; ++k) top = max(top, q_magnitude(to_f(raw[j].v[k])));
+          for (int k = 0; k < V; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
 #pragma unroll
           for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-          ex = q_exponent(top);
+          unsigned ex, code[V];
+          if (top < __float_as_uint(kQLargest)) {
+            // the sum's low byte is rint(x / s): the quotient is exact, the addition rounds
+            ex = q_exponent(top);
+            const float inv = q_inverse_scale(ex);
 #pragma unroll
-          for (int k = 0; k < V; ++k) code[k] = (unsigned)q_encode(to_f(raw[j].v[k]), q_inverse_scale(ex));
-        }
-        if (on) {
-          VecOf<int8_t, V> o;
+            for (int k = 0; k < V; ++k) code[k] = __float_as_uint(fmaf(v[k], inv, 12582912.f));
+          } else {
+            top = 0;
 #pragma unroll
-          for (int k = 0; k < V; ++k) o.v[k] = (int8_t)code[k];
-          *(VecOf<int8_t, V>*)(p.q + r * p.N + c) = o;
-          if (c % kQGroup == 0) p.e[r * p.gpr + c / kQGroup] = (uint8_t)ex;
+            for (int k = 0; k < V; ++k) top = max(top, q_magnitude(v[k]));
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+            ex = q_exponent(top);
+#pragma unroll
+            for (int k = 0; k < V; ++k) code[k] = (unsigned)q_encode(v[k], q_inverse_scale(ex));
+          }
+          if (on) {
+            VecOf<int8_t, V> o;
+            if constexpr (V % 4 == 0) {
+#pragma unroll
+              for (int k = 0; k < V; k += 4)
+                ((unsigned*)&o)[k / 4] = __byte_perm(__byte_perm(code[k], code[k + 1], 0x0040),
+                                                     __byte_perm(code[k + 2], code[k + 3], 0x0040), 0x5410);
+            } else {
+#pragma unroll
+              for (int k = 0; k < V; ++k) o.v[k] = (int8_t)code[k];
+            }
+            *(VecOf<int8_t, V>*)q = o;
+            if (c % kQGroup == 0) *e = (uint8_t)ex;
+          }
         }
+        q += dn;
+        e += de;
       }
     }
   }
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(512, 3) k_unpack8(Q8Args p) {
+__global__ void __launch_bounds__(512, V == 8 ? 2 : 3) k_unpack8(Q8Args p) {
   constexpr int U = 2;
   const int sub = threadIdx.x / p.span;
   const long long step = (long long)gridDim.x * p.rpb;
   for (int l = threadIdx.x - sub * p.span; l < p.span; l += blockDim.x) {
     const int c = l * V;
     if (c >= p.N) continue;
-    for (long long r0 = blockIdx.x * (long long)p.rpb + sub; r0 < p.rows; r0 += U * step) {
+    long long r = blockIdx.x * (long long)p.rpb + sub;
+    // places of row r, and from a row to the next one taken
+    const int8_t* q = p.q + r * p.N + c;
+    const uint8_t* e = p.e + r * p.gpr + c / kQGroup;
+    T* out = (T*)p.out + r * p.N + c;
+    const long long dn = step * p.N, de = step * p.gpr;
+    for (; r < p.rows; r += U * step) {
       VecOf<int8_t, V> raw[U];
-      uint8_t e[U];
+      uint8_t ex[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const long long r = r0 + j * step;
-        if (r < p.rows) {
-          raw[j] = *(const VecOf<int8_t, V>*)(p.q + r * p.N + c);
-          e[j] = p.e[r * p.gpr + c / kQGroup];
+        if (r + j * step < p.rows) {
+          raw[j] = *(const VecOf<int8_t, V>*)q;
+          ex[j] = *e;
         }
+        q += dn;
+        e += de;
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const long long r = r0 + j * step;
-        if (r >= p.rows) break;
-        const float s = q_scale(e[j]);
-        VecOf<T, V> o;
+        if (r + j * step < p.rows) {
+          const float s = q_scale(ex[j]);
+          float v[V];
+          bool odd = false;   // a code of an infinity or NaN
 #pragma unroll
-        for (int k = 0; k < V; ++k) o.v[k] = q_store<T>(q_decode(raw[j].v[k], s), raw[j].v[k]);
-        *(VecOf<T, V>*)((T*)p.out + r * p.N + c) = o;
+          for (int k = 0; k < V; ++k) {
+            v[k] = (float)raw[j].v[k];
+            odd |= fabsf(v[k]) > 126.f;
+            v[k] *= s;
+          }
+          if (odd) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = q_decode(raw[j].v[k], s);
+          }
+          if constexpr (std::is_same_v<T, __half>) {   // saturates, unless the code is an infinity's
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+              if (abs((int)raw[j].v[k]) < 127) v[k] = fminf(fmaxf(v[k], -65504.f), 65504.f);
+          }
+          *(VecOf<T, V>*)out = pack_vec<T, V>(v);
+        }
+        out += dn;
       }
     }
   }
