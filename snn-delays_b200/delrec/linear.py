@@ -6,9 +6,11 @@ runs ``delrec_linear_forward`` / ``delrec_linear_backward``: bf16 tensor-core GE
 exact three-piece bf16 splits of the fp32 operands, fp32 accumulation.  When the input
 is a spike train (every value 0 or 1) one piece carries it exactly and the GEMMs are
 half as long; ``binary_input`` says so (True: promised, checked on the device through the
-status word; None: tested on each call).  Such a
-call sums a real input's products in another order, so its output may differ from that of
-a call without a gradient by fp32 rounding (a spike input's does not).  CUDA tensors only.
+status word; None: tested on each call).  ``checkpoint8=True`` keeps the input for the
+weight gradient in 8 bits (``checkpoint8.pack8``): a quarter of the memory, exact for spike
+trains.  Such a call sums a real input's products in another order, so its output may
+differ from that of a call without a gradient by fp32 rounding (a spike input's does not).
+CUDA tensors only.
 """
 
 from __future__ import annotations
