@@ -162,6 +162,16 @@ __device__ __forceinline__ void scan_exchange(ScanExchange<P, V>& sm, int buf, i
   }
 }
 
+// A block's shared memory may be written by another block of its cluster only once it has started:
+// every block tells so on entry and waits for the others before the first exchange, behind the
+// copies of its first segment.
+__device__ __forceinline__ void cluster_started(int csize) {
+  if (csize > 1) cooperative_groups::this_cluster().barrier_arrive();
+}
+__device__ __forceinline__ void cluster_wait_started(int csize) {
+  if (csize > 1) cooperative_groups::this_cluster().barrier_wait();
+}
+
 // base + i * stride elements: one 32 x 32 -> 64 bit multiply-add (i is a constant)
 template <class E>
 __device__ __forceinline__ E* at_step(E* base, int stride, int i) {
@@ -437,6 +447,7 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, R, POS, PACK, MODE>::
   static_assert(R == 1 || (MODE == SCAN_STAGED && !PACK), "longer segments are for plain staged inputs");
   __shared__ ScanExchange<P, V> sm;
   extern __shared__ __align__(16) char stage[];
+  cluster_started(csize);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = csize > 1 ? (int)(blockIdx.x % csize) : 0;
   const int seg = rank * P + warp, wave = P * S * csize, waves = (p.T + wave - 1) / wave;
@@ -457,6 +468,7 @@ __global__ void __launch_bounds__(P * 32, ScanFwd<T, V, P, R, POS, PACK, MODE>::
   Cursor cur;
   cur.start((int)blockIdx.x / csize, p.tiles, 0);
   fetch(cur, 0);
+  cluster_wait_started(csize);
   float v[V];
   for (int buf = 0; cur.item < items; buf ^= 1) {
     Cursor nxt = cur;
@@ -748,6 +760,7 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
   constexpr int S = K::S, ROWB = K::ROWB, ROWG = K::ROWG;
   __shared__ ScanExchange<P, V> sm;
   extern __shared__ __align__(16) char stage[];
+  cluster_started(csize);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = csize > 1 ? (int)(blockIdx.x % csize) : 0;
   const int wave = P * S * csize, waves = (p.T + wave - 1) / wave;
@@ -800,6 +813,7 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
   Cursor cur;
   cur.start((int)blockIdx.x / csize, p.tiles, waves - 1);
   fetch(cur, 0);
+  cluster_wait_started(csize);
   float v[V];
   for (int buf = 0; cur.item < items; buf ^= 1) {
     Cursor nxt = cur;
