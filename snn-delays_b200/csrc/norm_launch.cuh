@@ -13,14 +13,19 @@ namespace delrec {
 // (N=2048 bf16 backward 509 -> 372 us); where five fit it costs (N=512 fp32 backward 165 -> 183 us).
 // most_threads: of an SM; the backward's eight streams of rows slow the memory down past 640
 // threads (N=512 fp32: five blocks of 128 take 159 us, eight 182 us).
+static constexpr int kNormThirdRow = 100 * 1024;   // most shared memory of a block with a third row
 template <class K>
 static int norm_start(K kern, int row_bytes, int most_threads, NormArgs a, NormShape& s, int most, cudaStream_t st) {
+  // The limit on a launch's shared memory belongs to the kernel, not to the launch: it is always set
+  // to the most that any width asks of this kernel, so that calls of other widths from other host
+  // threads cannot lower it in between.
+  const int full = row_bytes * kNormThreads, limit = std::max(2 * full, std::min(3 * full, kNormThirdRow));
   int per_sm = 0, smem = 0;
   for (a.slots = 2; a.slots <= 3; ++a.slots) {
     smem = a.slots * row_bytes * s.threads;
-    if (smem > 40 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (smem > 40 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, limit));
     SQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem));
-    if (per_sm > 2 || row_bytes == 0 || 3 * row_bytes * s.threads > 100 * 1024) break;
+    if (per_sm > 2 || row_bytes == 0 || 3 * row_bytes * s.threads > kNormThirdRow) break;
   }
   if (a.slots > 3) a.slots = 3;
   s.grid = std::min(most, std::max(1, std::min({per_sm, 16, most_threads / s.threads})) * kSeqSMs);
