@@ -12,6 +12,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdelrec_b200.so")
@@ -198,6 +199,16 @@ def require_lengths(lengths, B, device):
     if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64) or lengths.device != device \
             or not lengths.is_contiguous():
         raise RuntimeError(f"delrec_b200: lengths must be contiguous int32 or int64 ({B},) on {device}")
+
+
+def refuse_tangents(*tensors):
+    """Raises where a tensor carries a forward-mode tangent: the operators have no forward-mode
+    derivative, and a call outside autograd would drop the tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:       # no level is open, so there are none
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("delrec_b200: the sequence operators have no forward-mode derivative")
 
 
 def rows(t):

@@ -119,6 +119,7 @@ def _run(x, y, u, w, scale, nw, lengths, kind, eps, has_next):
         if y is None:
             return None, r
         return r if has_next else (r, None)
+    _lib.refuse_tangents(*args)
     return _forward(*args, lengths, kind, eps, has_next, False)[:2]
 
 

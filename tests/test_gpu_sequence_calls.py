@@ -39,3 +39,25 @@ def test_norms_from_two_host_threads():
     for t in threads:
         t.join()
     assert failed == [0, 0] and not wrong
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor needs no gradient of its own; its tangent is not dropped without a word."""
+    import torch.autograd.forward_ad as fw
+    from delrec.block_norm import block_join, block_norm
+    from delrec.gated import gated_scan, gated_step
+    z, f, h0, w = (torch.randn(s, device="cuda") for s in ((5, 2, 8), (5, 2, 8), (2, 8), (8,)))
+    with fw.dual_level():
+        dz, dh, dw = (fw.make_dual(t, torch.ones_like(t)) for t in (z, h0, w))
+        for call in (lambda: gated_scan(dz, f), lambda: gated_scan(z, dz), lambda: gated_scan(z, f, dh),
+                     lambda: gated_step(dz[0], f[0]), lambda: gated_step(z[0], dz[0]),
+                     lambda: gated_step(z[0], f[0], dh), lambda: block_norm(dz), lambda: block_norm(z, dw),
+                     lambda: block_join(z, dz), lambda: block_join(z, f, gate=dz), lambda: block_join(z, f, dw),
+                     lambda: block_join(z, f, scale=dw), lambda: block_join(z, f, next_weight=dw)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call()
+        want = gated_scan(z, f, h0)
+    # outside the level, and inside it without a tangent, the calls run
+    for a, b in zip(gated_scan(z, f, h0), want):
+        assert torch.equal(a, b)
