@@ -16,6 +16,7 @@ import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .checkpoint8 import Packed8, empty8, pack8, unpack8
@@ -169,9 +170,9 @@ def gated_scan(z, f, h0=None, *, lengths=None, resets=None, decay_input=True, ch
 def gated_step(z, f, state=None, *, active=None, decay_input=True, out=None):
     """One time step: z (B,N), f (B,G), state (B,N) float32 (None: 0) -> (h (B,N), next state).
 
-    ``out`` receives the next state and may be ``state`` itself (updated in place); None
-    allocates it.  ``active`` (B,) bool: a row with False keeps its state and gives h = 0.
-    No gradient passes; train with ``gated_scan``."""
+    ``out`` receives the next state and may be ``state`` itself (updated in place), but no
+    tensor that requires a gradient; None allocates it.  ``active`` (B,) bool: a row with
+    False keeps its state and gives h = 0.  No gradient passes; train with ``gated_scan``."""
     code = _check(z, f, 2, "(B, N) and (B, G)")
     B, N = z.shape
     dev = z.device
@@ -179,6 +180,8 @@ def gated_step(z, f, state=None, *, active=None, decay_input=True, out=None):
         _state(state, B, N, dev, "state")
     if out is not None:
         _state(out, B, N, dev, "out")
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise RuntimeError("delrec_b200: out must not require a gradient (no gradient passes)")
     if active is not None:
         if active.shape != (B,) or active.dtype != torch.bool or active.device != dev:
             raise RuntimeError(f"delrec_b200: active must be bool ({B},) on {dev}")
@@ -192,4 +195,6 @@ def gated_step(z, f, state=None, *, active=None, decay_input=True, out=None):
         A = _lib.addr
         _lib.launch("delrec_gated_step", dev, ctypes.byref(s), z.data_ptr(), f.data_ptr(), A(state), A(active),
                     h.data_ptr(), nxt.data_ptr())
+    if out is not None:
+        increment_version(out)       # who saved the old state for a gradient learns of it
     return h, nxt

@@ -61,3 +61,19 @@ def test_forward_mode_derivatives_are_refused():
     # outside the level, and inside it without a tangent, the calls run
     for a, b in zip(gated_scan(z, f, h0), want):
         assert torch.equal(a, b)
+
+
+def test_a_state_updated_in_place_is_seen_by_autograd():
+    from delrec.gated import gated_step
+    z, f, state = (torch.randn(2, 8, device="cuda") for _ in range(3))
+    w = torch.randn(2, 8, device="cuda", requires_grad=True)
+    saved = (state * w).sum()             # keeps state for w's gradient
+    gated_step(z, f, state, out=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    with pytest.raises(RuntimeError, match="out"):
+        gated_step(z, f, state, out=torch.zeros(2, 8, device="cuda", requires_grad=True))
+    with torch.inference_mode():          # a streaming state has no version there
+        s = torch.zeros(2, 8, device="cuda")
+        h, _ = gated_step(z, f, s, out=s)
+    assert torch.equal(h, s)
