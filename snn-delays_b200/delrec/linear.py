@@ -8,8 +8,9 @@ is a spike train (every value 0 or 1) one piece carries it exactly and the GEMMs
 half as long; ``binary_input`` says so (True: promised, checked on the device through the
 status word; None: tested on each call).  ``checkpoint8=True`` keeps the input for the
 weight gradient in 8 bits (``checkpoint8.pack8``): a quarter of the memory, exact for spike
-trains.  Such a call sums a real input's products in another order, so its output may
-differ from that of a call without a gradient by fp32 rounding (a spike input's does not).
+trains.  A call that keeps its input so sums a real input's products in another order, so its
+output may differ by fp32 rounding from that of a call that keeps nothing, under
+``torch.no_grad()`` for one (a spike input's does not).
 CUDA tensors only.
 """
 
@@ -49,7 +50,8 @@ class LinearFn(torch.autograd.Function):
         out = torch.empty(M, N, device=dev, dtype=torch.float32)
         w = weight.detach()
         b = bias.detach() if bias is not None else None
-        # only the parameter gradients read x
+        # only the parameter gradients read x; needs_input_grad tells of parameters without
+        # gradients enabled too, which is why ``linear`` asks for 8 bits only where they are
         ctx.packed = bool(checkpoint8)
         keep = None
         if ctx.packed and (ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2])):
@@ -161,7 +163,7 @@ def readout_time_sum(y, weight, bias=None):
 
 def linear(x, weight, bias=None, *, binary_input=None, checkpoint8=False):
     """x W^T + bias on the library's projection (see the module's description)."""
-    return LinearFn.apply(x, weight, bias, binary_input, checkpoint8)
+    return LinearFn.apply(x, weight, bias, binary_input, checkpoint8 and torch.is_grad_enabled())
 
 
 class Linear(torch.nn.Linear):
@@ -177,7 +179,7 @@ class Linear(torch.nn.Linear):
     def forward(self, x):
         if not x.is_cuda:
             raise RuntimeError("delrec_b200 runs on CUDA tensors only (there is no CPU path)")
-        return LinearFn.apply(x, self.weight, self.bias, self.binary_input, self.checkpoint8)
+        return linear(x, self.weight, self.bias, binary_input=self.binary_input, checkpoint8=self.checkpoint8)
 
     def extra_repr(self):
         r = super().extra_repr() + f", binary_input={self.binary_input}"

@@ -77,3 +77,18 @@ def test_a_state_updated_in_place_is_seen_by_autograd():
         s = torch.zeros(2, 8, device="cuda")
         h, _ = gated_step(z, f, s, out=s)
     assert torch.equal(h, s)
+
+
+@pytest.mark.parametrize("guard", [torch.no_grad, torch.inference_mode])
+def test_evaluation_keeps_nothing_in_8_bits(guard, monkeypatch):
+    """Without gradients a checkpoint8 layer is the plain one: nothing is packed, and the sums have the
+    plain order."""
+    from delrec import linear
+    plain = linear.Linear(700, 130, binary_input=False).cuda()
+    keep = linear.Linear(700, 130, binary_input=False, checkpoint8=True).cuda()
+    keep.load_state_dict(plain.state_dict())
+    x = torch.randn(300, 700, device="cuda")
+    monkeypatch.setattr(linear, "empty8", lambda *a: pytest.fail("packed in evaluation"))
+    with guard():
+        assert torch.equal(keep(x), plain(x))
+        assert torch.equal(linear.linear(x, keep.weight, keep.bias, binary_input=False, checkpoint8=True), plain(x))
