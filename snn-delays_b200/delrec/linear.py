@@ -30,8 +30,7 @@ def _is_binary(x):
     if x.data_ptr() % 16 != 0:
         x = x.clone()
     count = torch.empty(1, dtype=torch.int32, device=x.device)
-    _lib.check(_lib.lib().delrec_count_nonbinary(_lib.ptr(x), x.numel(), _lib.ptr(count),
-                                                 _lib.stream_ptr(x.device)), "delrec_count_nonbinary")
+    _lib.launch("delrec_count_nonbinary", x.device, _lib.ptr(x), x.numel(), _lib.ptr(count))
     return int(count.item()) == 0
 
 
@@ -62,13 +61,12 @@ class LinearFn(torch.autograd.Function):
             P = _lib.ptr
             if keep is not None:
                 ws = _lib.scratch(nbytes, dev)
-                _lib.check(lib.delrec_linear_forward8(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(keep.q),
-                                                      P(keep.e), P(ws), ws.numel(), _lib.stream_ptr(dev)),
-                           "delrec_linear_forward8")
+                _lib.launch("delrec_linear_forward8", dev, M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(keep.q),
+                            P(keep.e), P(ws), ws.numel())
             else:
                 ws = _lib.workspace(nbytes, dev)
-                _lib.check(lib.delrec_linear_forward(M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(ws),
-                                                     ws.numel(), _lib.stream_ptr(dev)), "delrec_linear_forward")
+                _lib.launch("delrec_linear_forward", dev, M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(ws),
+                            ws.numel())
         if ctx.packed:
             ctx.save_for_backward(keep and keep.q, w, keep and keep.e)
         else:
@@ -101,14 +99,12 @@ class LinearFn(torch.autograd.Function):
             P = _lib.ptr
             if ctx.packed:
                 ws = _lib.scratch(lib.delrec_linear_backward8_workspace(M, K, N), dev)
-                _lib.check(lib.delrec_linear_backward8(M, K, N, P(x2), P(e), P(w), P(g), P(dx), P(dw), P(db),
-                                                       P(ws), ws.numel(), _lib.stream_ptr(dev)),
-                           "delrec_linear_backward8")
+                _lib.launch("delrec_linear_backward8", dev, M, K, N, P(x2), P(e), P(w), P(g), P(dx), P(dw), P(db),
+                            P(ws), ws.numel())
                 return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None
             ws = _lib.workspace(lib.delrec_linear_backward_workspace(M, K, N, int(ctx.binary)), dev)
-            _lib.check(lib.delrec_linear_backward(M, K, N, P(x2), P(w), P(g), int(ctx.binary), P(dx), P(dw),
-                                                  P(db), P(ws), ws.numel(), _lib.stream_ptr(dev)),
-                       "delrec_linear_backward")
+            _lib.launch("delrec_linear_backward", dev, M, K, N, P(x2), P(w), P(g), int(ctx.binary), P(dx), P(dw),
+                        P(db), P(ws), ws.numel())
         return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None
 
 

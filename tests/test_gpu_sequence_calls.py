@@ -92,3 +92,32 @@ def test_evaluation_keeps_nothing_in_8_bits(guard, monkeypatch):
     with guard():
         assert torch.equal(keep(x), plain(x))
         assert torch.equal(linear.linear(x, keep.weight, keep.bias, binary_input=False, checkpoint8=True), plain(x))
+
+
+def test_linear8_makes_its_tensors_device_current(monkeypatch):
+    """The 8-bit projection launches with its tensors' device current, whichever was."""
+    from delrec.linear import linear
+    x = torch.randn(20, 40, device="cuda", requires_grad=True)
+    w = torch.randn(10, 40, device="cuda", requires_grad=True)
+
+    def go():
+        out = linear(x, w, checkpoint8=True)
+        return (out.detach(), *torch.autograd.grad(out, (x, w), torch.ones_like(out)))
+
+    want = go()
+    entered = []
+    guard = torch.cuda.device
+
+    class Recorded(guard):
+        def __init__(self, device):
+            super().__init__(device)
+            entered.append(device)
+
+    # another device seems to be current
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "device", Recorded)
+    got = go()
+    assert entered == [0, 0, 0]            # the test for spikes, forward, backward
+    monkeypatch.undo()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
