@@ -226,19 +226,17 @@ def addr(t):
     return None if t is None else t.data_ptr()
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def launch(what, device, *args):
     """Calls the C entry point ``what`` with args and the current stream of ``device``, which
     is made the current device where it is not."""
     index = device.index
     fn = getattr(_lib or lib(), what)
+    stream = torch._C._cuda_getCurrentRawStream     # a torch built without CUDA has none
     if index == torch._C._cuda_getDevice():
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(*args, stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(*args, stream(index))
     if rc:
         check(rc, what)
 
