@@ -306,7 +306,8 @@ typedef struct delrec_scan {
  * position; NULL to skip) and, for the backward, states (ceil(T/16), B, N): the state before
  * every 16th step (NULL to skip).  qz, ez, qf, ef, odd (all or none, G = N): also writes z
  * and f in 8 bits (delrec_pack8's form), and odd (ceil(T/16), B, ceil(N/32)): nonzero where a
- * code of those 16 steps and 32 channels may stand for an infinity or NaN. */
+ * code of those 16 steps and 32 channels may stand for an infinity or NaN.  T, and B times the
+ * tiles of at most 32 channels of a row, are at most 2^30, B N below 2^31. */
 int delrec_gated_scan_forward(const delrec_scan* scan, const void* z, const void* f, const float* h0,
                               const void* lengths, const uint8_t* resets, void* h, float* hT, float* states,
                               int8_t* qz, uint8_t* ez, int8_t* qf, uint8_t* ef, uint8_t* odd, void* stream);

@@ -49,6 +49,8 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool sta
   p->cpt = p->D == 1 || p->split ? 32 * sh->V : 32 / p->D * p->D;
   p->tiles = (p->N + p->cpt - 1) / p->cpt;
   const long long items = (long long)p->B * p->tiles;
+  // a block's next item, one grid (at most all items) further, has to fit 32 bits
+  if (items > 1LL << 30) return DELREC_ERR_UNSUPPORTED;
   // The blocks of a cluster share a row's time where that fills the SMs better: about two
   // blocks of 8 warps fit an SM, the rounds they take fall with the cluster's size c, and
   // each doubling costs some 6 % in exchanges (T=1021, 408 items: c = 1 takes two rounds for
