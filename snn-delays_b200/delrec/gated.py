@@ -128,8 +128,11 @@ def _backward(ctx, gh, ghT):
         _lib.launch("delrec_gated_scan_backward", dev, ctypes.byref(s), A(z), A(f), A(qz), A(ez), A(qf), A(ef),
                     A(odd), A(lengths), A(resets), states.data_ptr(), A(gh), A(ghT), A(dz), A(df), A(dh0), A(ws),
                     nbytes)
-    elif dh0 is not None:
-        dh0 = ghT.clone() if ghT is not None else dh0.zero_()
+    else:
+        if dh0 is not None:
+            dh0 = ghT.clone() if ghT is not None else dh0.zero_()
+        if df is not None:
+            df.zero_()               # gates without channels: their sums are empty
     return dz, df, dh0, None, None, None, None
 
 

@@ -121,3 +121,15 @@ def test_linear8_makes_its_tensors_device_current(monkeypatch):
     monkeypatch.undo()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_gates_without_channels_get_zero_gradients():
+    """N = 0 with gates: every gate's sum over its channels is empty."""
+    from delrec.gated import gated_scan
+    z = torch.randn(6, 3, 0, device="cuda", requires_grad=True)
+    f = torch.randn(6, 3, 4, device="cuda", requires_grad=True)
+    poison = torch.full((6, 3, 4), float("nan"), device="cuda")
+    h, hT = gated_scan(z, f)
+    del poison
+    dz, df = torch.autograd.grad((h, hT), (z, f), (torch.ones_like(h), torch.ones_like(hT)))
+    assert dz.shape == z.shape and torch.equal(df, torch.zeros_like(f))
