@@ -280,7 +280,9 @@ int delrec_count_nonbinary(const float* x, size_t n, unsigned int* count, void* 
  * (T,B,N) with element strides for T and B and contiguous channels; states, weights,
  * statistics and their gradients are fp32.  lengths (B), int32 or int64
  * (lengths_wide != 0), NULL for full rows: positions t >= lengths[b] are not read, their
- * outputs and gradients are written as 0.  Outputs do not overlap inputs unless stated. */
+ * outputs and gradients are written as 0.  Outputs do not overlap inputs unless stated.
+ * Pointers and strides are aligned to their element type; wider accesses are chosen where
+ * they allow them. */
 #define DELREC_F32 0
 #define DELREC_BF16 1
 #define DELREC_F16 2

@@ -14,9 +14,10 @@ static int check_scan(const delrec_scan* s) {
   return DELREC_OK;
 }
 
-// What the inputs' rows allow: sixteen-byte copies (STAGED).
+// What the tensors allow: sixteen-byte copies of the inputs' rows (STAGED), two channels at a time
+// of the states and the codes that a forward pass writes.
 struct ScanAlign {
-  bool sixteen;
+  bool sixteen, pairs = true;
   int esz;
   ScanAlign(const delrec_scan* s) : sixteen(s->G == s->N), esz(s->dtype == DELREC_F32 ? 4 : 2) {}
   void input(const void* ptr, long long st, long long sb, int row_bytes, int size) {
@@ -28,9 +29,12 @@ struct ScanAlign {
   void output(const void* ptr, long long st, long long sb) {
     if (ptr && esz == 2 && (((uintptr_t)ptr & 3) || (st & 1) || (sb & 1))) sixteen = false;
   }
+  void pair(const void* ptr, int size) {
+    if ((uintptr_t)ptr & (2 * size - 1)) pairs = false;
+  }
 };
 
-static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool staged, bool q8) {
+static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, const ScanAlign& al, bool q8) {
   p->T = s->T; p->B = s->B; p->N = s->N; p->G = s->G; p->D = s->N / s->G;
   p->decay_input = s->decay_input; p->wide = s->lengths_wide;
   for (long long st : {s->z_t, s->f_t, s->h_t, s->gh_t, s->dz_t, s->df_t})
@@ -39,10 +43,10 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, bool sta
   const int segs = (p->T + kSeg - 1) / kSeg;
   sh->P = segs >= 2 ? kScanWarps : 1;
   p->split = p->D >= 32;
-  sh->mode = p->split ? SCAN_WIDE : (staged && p->D == 1 ? SCAN_STAGED : SCAN_DIRECT);
+  sh->mode = p->split ? SCAN_WIDE : (al.sixteen && p->D == 1 ? SCAN_STAGED : SCAN_DIRECT);
   // two channels to a lane (16-bit), unless that leaves SMs without a block even when a
   // cluster shares each row's time
-  sh->V = sh->mode == SCAN_STAGED && s->dtype != DELREC_F32 &&
+  sh->V = sh->mode == SCAN_STAGED && s->dtype != DELREC_F32 && al.pairs &&
                   (long long)p->B * ((p->N + 63) / 64) * std::min(kScanCluster, (segs + sh->P - 1) / sh->P) >= 2 * kSeqSMs
               ? 2
               : 1;
@@ -91,7 +95,10 @@ int delrec_gated_scan_forward(const delrec_scan* s, const void* z, const void* f
   al.input(z, s->z_t, s->z_b, s->N * al.esz, al.esz);
   al.input(f, s->f_t, s->f_b, s->N * al.esz, al.esz);
   al.output(h, s->h_t, s->h_b);
-  if ((rc = scan_shape(s, &p, &sh, al.sixteen, pack))) return rc;
+  al.pair(states, sizeof(float));
+  al.pair(qz, 1);
+  al.pair(qf, 1);
+  if ((rc = scan_shape(s, &p, &sh, al, pack))) return rc;
   p.z = z; p.f = f; p.h0 = h0; p.lengths = lengths; p.resets = resets; p.h = h; p.hT = hT; p.states = states;
   p.qz = qz; p.ez = ez; p.qf = qf; p.ef = ef; p.odd = odd;
   p.z_t = (int)s->z_t; p.z_b = s->z_b; p.f_t = (int)s->f_t; p.f_b = s->f_b; p.h_t = (int)s->h_t; p.h_b = s->h_b;
@@ -128,7 +135,8 @@ int delrec_gated_scan_backward(const delrec_scan* s, const void* z, const void* 
   al.input(gh, s->gh_t, s->gh_b, s->N * al.esz, al.esz);
   al.output(dz, s->dz_t, s->dz_b);
   al.output(df, s->df_t, s->df_b);
-  if ((rc = scan_shape(s, &p, &sh, al.sixteen, pack))) return rc;
+  al.pair(states, sizeof(float));
+  if ((rc = scan_shape(s, &p, &sh, al, pack))) return rc;
   const size_t need = df ? delrec_gated_scan_backward_workspace(s) : 0;
   if (need && (!ws || ((uintptr_t)ws & 255) != 0 || wsb < need)) return DELREC_ERR_WORKSPACE;
   p.z = z; p.f = f; p.lengths = lengths; p.resets = resets; p.states = const_cast<float*>(states);

@@ -803,7 +803,8 @@ __global__ void __launch_bounds__(P * 32, 16 / P) k_scan_bwd(ScanArgs p, int csi
       const unsigned dst = (unsigned)__cvta_generic_to_shared(mine + h * K::STAGE);
       stage_rows<ROWB, S>(dst, zp + b * z_b + c0 + (long long)tb * z_t, z_t, n, left * K::E, lane);
       stage_rows<ROWB, S>(dst + S * ROWB, fp + b * f_b + c0 + (long long)tb * f_t, f_t, n, left * K::E, lane);
-      const T* gh = p.gh ? (const T*)p.gh + b * p.gh_b + c0 + (long long)tb * p.gh_t : (const T*)p.states;
+      // without gh its rows become 0; the copies want an aligned address all the same
+      const T* gh = p.gh ? (const T*)p.gh + b * p.gh_b + c0 + (long long)tb * p.gh_t : (const T*)zp;
       stage_rows<ROWG, S>(dst + 2 * S * ROWB, gh, p.gh_t, p.gh ? n : 0, left * (int)sizeof(T), lane);
       state(b, scan_place<V>(p, tile, lane), tb, s_ahead);
       if (B8) scales(b, tile, tb, n, sz_ahead, sf_ahead, odd_ahead);

@@ -36,3 +36,51 @@ def test_cluster_blocks_past_the_sequence_end(T, N, dtype):
         grads = torch.autograd.grad((h, hT), (z, f, h0), (d["gh"], d["ghT"]))
         for got, want in zip((h, hT, *grads), (first[0], first[1], *first[2])):
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("with_gh", [True, False])
+def test_c_buffers_at_odd_addresses(keep8, with_gh):
+    """States 4 bytes and codes one byte past an aligned address: a C caller's buffers promise no more than
+    their element's alignment, whatever the sizes lead to (here two channels to a lane)."""
+    import ctypes
+    from delrec import _lib
+    T, B, N = 40, 5, 64 * 60 + 16
+    c = _inputs(T, B, N, 1, BF16)
+    d = _cuda(c)
+    lib, S, G = _lib.lib(), -(-T // 16), -(-N // 32)
+
+    def odd(*shape, dtype=torch.float32):
+        return torch.zeros(torch.Size(shape).numel() + 1, dtype=dtype, device="cuda")[1:].view(shape)
+
+    h = torch.empty(T, B, N, dtype=BF16, device="cuda")
+    hT, states = odd(B, N), odd(S, B, N)
+    q = [odd(T, B, N, dtype=torch.int8), odd(T, B, G, dtype=torch.uint8), odd(T, B, N, dtype=torch.int8),
+         odd(T, B, G, dtype=torch.uint8), odd(S, B, G, dtype=torch.uint8)] if keep8 else [None] * 5
+    assert states.data_ptr() % 8 == 4 and (not keep8 or q[0].data_ptr() % 2 == 1)
+    A, stream = _lib.addr, torch.cuda.current_stream().cuda_stream
+    s = _lib.Scan(T, B, N, N, 1, 1, 0, 0, *(B * N, N) * 6)
+    assert lib.delrec_gated_scan_forward(ctypes.byref(s), A(d["z"]), A(d["f"]), A(d["h0"]), None, None, A(h), A(hT),
+                                         A(states), *map(A, q), stream) == 0
+    dz, df, dh0 = torch.empty_like(h), torch.empty_like(h), odd(B, N)
+    zf = [None, None] if keep8 else [A(d["z"]), A(d["f"])]
+    assert lib.delrec_gated_scan_backward(ctypes.byref(s), *zf, *map(A, q), None, None, A(states),
+                                          A(d["gh"]) if with_gh else None, A(d["ghT"]), A(dz), A(df), A(dh0), None, 0,
+                                          stream) == 0
+    r = O.gated_scan(c["z"], c["f"], c["h0"])
+    within(h, r["h"], r["err"], "h")
+    within(hT, r["hT"], r["errT"], "hT")
+    z, f, pre = c["z"].double(), c["f"].double(), r["pre"]
+    perr = torch.zeros_like(pre)
+    perr[1:] = r["err"][:-1]
+    if keep8:
+        z, f = O.restore8(z), O.restore8(f)
+        pre, e = O.recompute(z, f, pre)
+        perr = e + perr[torch.arange(T) // 16 * 16]
+        for got, e8, ref in ((q[0], q[1], z), (q[2], q[3], f)):
+            scale = ((e8.long().cpu() + (1023 - 127)) << 52).view(torch.float64).repeat_interleave(32, -1)[..., :N]
+            assert torch.equal(got.double().cpu() * scale, ref)
+    b = O.gated_scan_backward(z, f, pre, perr, c["gh"] if with_gh else torch.zeros_like(c["gh"]), c["ghT"])
+    within(dz, b["dz"], b["ez"], "dz")
+    within(df, b["df"], b["ef"], "df")
+    within(dh0, b["dh0"], b["e0"], "dh0")
