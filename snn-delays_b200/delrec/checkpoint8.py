@@ -2,8 +2,9 @@
 
 ``pack8`` stores rows of channels as int8 with one power-of-two scale per group of 32
 consecutive channels (8.25 bits a value), ``unpack8`` restores them.  A value is kept to
-within half a step, 2^-7 to 2^-8 of its group's largest magnitude; 0 / 1 spike trains,
-infinities and NaN come back exactly.  ``linear.Linear(checkpoint8=True)`` and
+within half a step, 1/252 to 1/126 of its group's largest magnitude m where 2^-120 <= m <
+63.5 * 2^122; within 2^-127 where m is smaller, within 2^122 where it is larger.  0 / 1 spike
+trains, infinities and NaN come back exactly.  ``linear.Linear(checkpoint8=True)`` and
 ``gated.gated_scan(checkpoint8=True)`` keep what they save for the backward pass this way.
 CUDA tensors only.
 """

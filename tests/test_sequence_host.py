@@ -32,3 +32,25 @@ def test_more_rows_than_the_scan_counts_are_refused():
                                              None) == 4
         assert lib.delrec_gated_scan_backward(ctypes.byref(s), p, p, *(None,) * 5, None, None, p, p, None, p, p, None,
                                               None, 0, None) == 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_stated_accuracy_of_the_8_bit_form(dtype):
+    """Half a step, at most 1/126 of the group's largest magnitude from 2^-120 to 63.5 * 2^122; 2^-127 below; at
+    63.5 * 2^122 and above a step of 2^122."""
+    from oracle import sequence_oracle as O
+    g = torch.Generator().manual_seed(3)
+    for top in (2.0 ** -120, 2.0 ** -24, 1.0, 63.1 / 64, 126.0, 126.5, 6e4, 63.4 * 2.0 ** 122):
+        if top > torch.finfo(dtype).max or top < torch.finfo(dtype).tiny / 1024:
+            continue
+        x = (torch.rand(200, 32, generator=g, dtype=torch.float64) * 2 - 1) * top
+        x[:, 0] = top
+        x = x.to(dtype).double()
+        m = x.abs().amax(-1, keepdim=True)
+        assert ((O.restore8(x) - x).abs() <= m / 126).all(), top
+    worst = torch.tensor([63.001, 0.5], dtype=torch.float64)      # a step of 1: half a one is 1 / 126.002
+    assert (O.restore8(worst) - worst).abs().max() / worst.max() > 1 / 126.1
+    tiny = torch.tensor([2.0 ** -121, 2.0 ** -127 * 1.001, -2.0 ** -128], dtype=torch.float64)
+    assert (O.restore8(tiny) - tiny).abs().max() <= 2.0 ** -127
+    huge = torch.tensor([float(torch.finfo(torch.float32).max), -63.6 * 2.0 ** 122, 1e38], dtype=torch.float64)
+    assert (O.restore8(huge) - huge).abs().max() <= 2.0 ** 122
