@@ -84,3 +84,82 @@ def test_c_buffers_at_odd_addresses(keep8, with_gh):
     within(dz, b["dz"], b["ez"], "dz")
     within(df, b["df"], b["ef"], "df")
     within(dh0, b["dh0"], b["e0"], "dh0")
+
+
+# (T, B, N): rows of two channels to a lane; one block a row, two and four blocks a row
+TWO = [(20, 5, 64 * 60 + 8), (150, 5, 64 * 30 + 40), (264, 5, 64 * 20), (600, 4, 64 * 20 - 8)]
+
+
+@pytest.mark.parametrize("decay_input", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,B,N", TWO)
+def test_two_channels_to_a_lane(T, B, N, dtype, decay_input):
+    c = _inputs(T, B, N, 1, dtype, ragged=True, resets=True)
+    c["lengths"][:4] = torch.tensor([T, 0, 17, T - 1])
+    _check(c, decay_input)
+    c["lengths"] = c["resets"] = None
+    _check(c, decay_input)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,B,N", [(20, 5, 64 * 60 + 16), (150, 5, 64 * 30 + 32), (264, 5, 64 * 20), (150, 5, 64 * 30 + 40)])
+def test_two_channels_to_a_lane_checkpoint8(T, B, N, dtype):
+    c = _inputs(T, B, N, 1, dtype, ragged=True, resets=True)
+    c["lengths"][:4] = torch.tensor([T, 0, 17, T - 1])
+    _check(c, checkpoint8=True)
+    _check(c, decay_input=False, checkpoint8=True)
+    c["lengths"] = c["resets"] = None
+    _check(c, checkpoint8=True)
+
+
+# segments of 32 steps: clusters of 16 blocks, and of two
+@pytest.mark.parametrize("decay_input", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,B,N", [(4200, 2, 40), (4111, 1, 32), (500, 4, 1120)])
+def test_segments_of_32_steps(T, B, N, dtype, decay_input):
+    c = _inputs(T, B, N, 1, dtype, mean=4.0)
+    _check(c, decay_input)
+    if B > 1:
+        c = _inputs(T, B, N, 1, dtype, ragged=True, resets=True, mean=4.0)
+        c["lengths"][:2] = torch.tensor([T - 13, 45])
+        _check(c, decay_input)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,B,N", [(45, 3, 40), (150, 3, 64), (150, 5, 64 * 30 + 32)])
+def test_checkpoint8_with_infinities_and_large_values(T, B, N, dtype):
+    """Codes that stand for infinities and NaN (the slow forms of packing and of the walk), and groups at
+    the largest scale, whose codes are cut.  The rest of z is as ever; a reset a few steps on keeps what
+    is not finite short.  The large values are positive and meet gradients below 2^-6, so that
+    a (1 - a) G (h - z) stays in range."""
+    c = _inputs(T, B, N, 1, dtype)
+    c["resets"] = torch.zeros(T, B, dtype=torch.bool)
+    for b, t, n, value in ((0, 3, 5, float("inf")), (1, 18, 33, float("-inf")), (2, 31, 0, float("nan")),
+                           (0, T - 9, 32, float("nan"))):
+        c["z"][t, b, n] = value
+        c["resets"][t + 4, b] = True
+    big = slice(32, 36)
+    c["z"][20:24, 0, big] = torch.tensor([3.39e38, 3.37e38, 2e38, 1e37]).to(dtype)
+    c["h0"][0, big] = c["h0"][0, big].abs()
+    c["resets"][24, 0] = True
+    c["gh"] *= 2.0 ** -9
+    c["ghT"] *= 2.0 ** -9
+    from delrec.gated import gated_scan
+    d = _cuda(c)
+    leaves = [d[k].requires_grad_(True) for k in ("z", "f", "h0")]
+    h, hT = gated_scan(*leaves, resets=d["resets"], checkpoint8=True)
+    grads = torch.autograd.grad((h, hT), leaves, (d["gh"], d["ghT"]))
+    r = O.gated_scan(c["z"], c["f"], c["h0"], resets=c["resets"])
+    within(h, r["h"], r["err"], "h")
+    within(hT, r["hT"], r["errT"], "hT")
+    z, f = O.restore8(c["z"].double()), O.restore8(c["f"].double())
+    pre, perr = O.recompute(z, f, r["pre"], resets=c["resets"])
+    # A kept state's bound rides along inside its segment, up to the first reset: behind one the state
+    # does not depend on it (and a bound of a state that is not finite is none).
+    seg = torch.arange(T) // 16 * 16
+    cut = torch.stack([c["resets"][int(s):t].any(0) for t, s in enumerate(seg)])        # a reset before step t
+    kept = torch.cat([torch.zeros_like(r["err"][:1]), r["err"][:-1]])[seg]
+    perr = perr + torch.where(cut[..., None], torch.zeros_like(kept), kept)
+    b = O.gated_scan_backward(z, f, pre, perr, c["gh"], c["ghT"], resets=c["resets"])
+    for got, k, e in zip(grads, ("dz", "df", "dh0"), ("ez", "ef", "e0")):
+        within(got, b[k], b[e], k)
