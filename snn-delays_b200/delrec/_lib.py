@@ -203,9 +203,8 @@ def require_lengths(lengths, B, device):
 
 def refuse_tangents(*tensors):
     """Raises where a tensor carries a forward-mode tangent: the operators have no forward-mode
-    derivative, and a call outside autograd would drop the tangent."""
-    if getattr(forward_ad, "_current_level", 0) < 0:       # no level is open, so there are none
-        return
+    derivative, and a call outside autograd would drop the tangent.  Called only where a
+    dual level is open (``forward_ad._current_level``), which small calls test at next to no cost."""
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError("delrec_b200: the sequence operators have no forward-mode derivative")

@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -119,7 +120,8 @@ def _run(x, y, u, w, scale, nw, lengths, kind, eps, has_next):
         if y is None:
             return None, r
         return r if has_next else (r, None)
-    _lib.refuse_tangents(*args)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _lib.refuse_tangents(*args)
     return _forward(*args, lengths, kind, eps, has_next, False)[:2]
 
 

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -166,7 +167,8 @@ def gated_scan(z, f, h0=None, *, lengths=None, resets=None, decay_input=True, ch
         resets = resets.contiguous()
     if torch.is_grad_enabled() and (z.requires_grad or f.requires_grad or (h0 is not None and h0.requires_grad)):
         return GatedScan.apply(z, f, h0, lengths, resets, decay_input, checkpoint8)
-    _lib.refuse_tangents(z, f, h0)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _lib.refuse_tangents(z, f, h0)
     return _forward(_lib.rows(z), _lib.rows(f), h0, lengths, resets, decay_input, False, False)[:2]
 
 
@@ -189,7 +191,8 @@ def gated_step(z, f, state=None, *, active=None, decay_input=True, out=None):
         if active.shape != (B,) or active.dtype != torch.bool or active.device != dev:
             raise RuntimeError(f"delrec_b200: active must be bool ({B},) on {dev}")
         active = active.contiguous()
-    _lib.refuse_tangents(z, f, state)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _lib.refuse_tangents(z, f, state)
     z, f = _lib.rows(z), _lib.rows(f)
     h = torch.empty(B, N, device=dev, dtype=z.dtype)
     nxt = torch.empty(B, N, device=dev) if out is None else out
