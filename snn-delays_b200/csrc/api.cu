@@ -820,7 +820,7 @@ static LinPlan plan_linear(int K, int N, int x_binary) {
 // last_first: the smallest products first.  The tensor core's accumulator cuts each sum off at
 // its own magnitude (half a unit of 2^-23 of it, on average, per 16 reduction steps, always
 // toward zero), which costs nothing while the sum is small: with the large product last its
-// steps alone count (K=700: 7.8e-6 -> 1.3e-6 of the result).
+// steps alone count (64000 x 700 -> 512, relative: output 7.5e-6 -> 6.6e-7, dx 5.7e-6 -> 4.7e-7).
 static void lin_products(GemmArgs* g, int a_pieces, bool last_first = false) {
   static const int pa6[6] = {0, 1, 2, 0, 1, 0}, pb6[6] = {0, 0, 0, 1, 1, 2};
   g->nprod = a_pieces == 1 ? 3 : 6;
@@ -886,8 +886,8 @@ static size_t linear_bwd_ws(int M, int K, int N, int xb) {
 }
 // The weight gradient from an 8-bit input: the rows in segments, each summed in an accumulator of
 // its own, the three pieces of gout in turn, the smallest first.  Segments of 1024 rows (64
-// steps at full size: 1e-6 of the result), longer ones past 64 segments, whose N x Kp partials
-// cost more than they give.
+// steps; 64000 x 700 -> 512: 2.6e-7 of the result), longer ones past 64 segments, whose N x Kp
+// partials cost more than they give.
 static int lin8_rows(int M) { return M <= 1024 ? M : std::max(1024, ((M + 63) / 64 + 63) / 64 * 64); }
 static int lin8_ksplit(int M) { return (M + lin8_rows(M) - 1) / lin8_rows(M); }
 static size_t linear_bwd8_ws(int M, int K, int N) {

@@ -50,7 +50,7 @@ __device__ __forceinline__ float q_decode(int q, float s) {
 // block covers whole rows of threads side by side (span = lanes of a row, rounded up to whole
 // groups), or walks along rows wider than a block, and steps down the rows without divisions, U
 // rows in flight.  HBM bounds both: x once, q and e once (64000 x 700 fp32: packed in 47 us,
-// restored in 39, of 35 at the copy rate; registers are held to 40 for 40 warps an SM: more rows in
+// restored in 39 to 43, of 35 at the copy rate; registers are held to 40 for 40 warps an SM: more rows in
 // flight on fewer warps took longer, and places multiplied out for every row 53).
 struct Q8Args {
   long long rows;

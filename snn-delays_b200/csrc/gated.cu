@@ -56,8 +56,8 @@ static int scan_shape(const delrec_scan* s, ScanArgs* p, ScanShape* sh, const Sc
   // a block's next item, one grid (at most all items) further, has to fit 32 bits
   if (items > 1LL << 30) return DELREC_ERR_UNSUPPORTED;
   // The blocks of a cluster share a row's time where that fills the SMs better: about two
-  // blocks of 8 warps fit an SM, the rounds they take fall with the cluster's size c, and
-  // each doubling costs some 6 % in exchanges (T=1021, 408 items: c = 1 takes two rounds for
+  // blocks of 8 warps fit an SM (of the plain 16-bit backward one), the rounds they take fall
+  // with the cluster's size c, and each doubling costs some 6 % in exchanges (T=1021, 408 items: c = 1 takes two rounds for
   // 1.4 blocks' work).
   const long long slots = 2 * kSeqSMs * 8 / sh->P;
   int c = 1;

@@ -21,13 +21,19 @@
 // 32-bit, segments inside a sequence are stored without tests, and the backward's map of
 // the reverse recurrence is built in the forward walk (H += g Pi a).  Rows of 16-byte multiples are
 // staged: each warp copies its next segment into shared memory (cp.async) while it works on
-// the present one, so 16 warps per SM keep the memory busy at 128 registers a thread.
+// the present one, so 16 warps per SM keep the memory busy at 128 registers a thread.  (The plain
+// 16-bit backward's 96 KB of stages and 24 of exchange let one block of 8 warps on an SM: it
+// is latency-bound.)  Other rows are read an element at a time, which costs half as much again.
 // Backward does not read h: the forward keeps the fp32 state before every 16th step (1/16
 // of an fp32 tensor) and each segment recomputes its states from there, which also spares
-// the rounding of a 16-bit h.  Measured: T=250 B=256 N=512 fp32 forward 69 us (5.6 TB/s, 39
-// operations an element), backward 108 us (5.8 TB/s, 65); T=784 B=256 N=512 bf16 with 8-bit
-// z and f forward 237 us (47), backward 246 us (56, of 44 that its bytes leave time for); one
-// sequence of 65536 steps, N=512 bf16, forward 106 us on 16-block clusters.
+// the rounding of a 16-bit h.  Measured: T=250 B=256 N=512 fp32 forward 72 us (5.6 TB/s, 39
+// operations an element), backward 113 us (5.9 TB/s, 65); the same in bf16 41 (5.0 TB/s) and 99 us
+// (3.4), fp16 41 and 84; T=784 B=256 N=512 bf16 with 8-bit z and f forward 232 us (47), backward
+// 244 us (56, of 44 that its bytes leave time for); one sequence of 65536 steps, N=512 bf16,
+// forward 106 us: 16 waves of segments one after another on 16-block clusters.
+//
+// An infinite state stays infinite or becomes NaN (a product of gates that underflows, times
+// infinity) up to the next reset; infinite gradients likewise.
 #pragma once
 
 #include <cooperative_groups.h>

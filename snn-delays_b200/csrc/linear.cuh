@@ -256,7 +256,7 @@ __global__ void k_linear_dw_reduce(int N, int K, int Np, int Kp, const float* __
 // k_pack_rows of the projection's input (ones column at K) that also writes its 8-bit form
 // (checkpoint8.cuh) from the same read: four threads of 8 columns hold a group of 32, a row's
 // chunks are padded to whole groups (gp of them).  Bound by HBM and by packing: 64000 x 700 in
-// 98 us, where the two passes it replaces take 70 + 50.
+// 96 us, where the two passes it replaces, k_pack_rows and k_pack8, take 104 + 47.
 __global__ void k_pack_rows_keep(int R, int K, int Wd, int gp, const float* __restrict__ src, int nb, int binary,
                                  __nv_bfloat16* __restrict__ out, int8_t* __restrict__ q, uint8_t* __restrict__ e) {
   const size_t row_out = (size_t)nb * Wd, total = (size_t)R * gp;

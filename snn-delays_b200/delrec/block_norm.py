@@ -7,7 +7,8 @@
 
 with rms(v) = sqrt(mean v^2 + eps) over the channels of a position.  Unlike
 ``neuron.BatchNorm1d`` a position's norm depends on no other one, so padded batches and
-streaming steps give the same numbers as whole sequences.  x, y and gate are (T,B,N)
+streaming steps give the same numbers as whole sequences.  The sum of a position's squares
+is float32 and has to stay below 3.4e38.  x, y and gate are (T,B,N)
 float32, bfloat16 or float16; the weights are (N,) float32.  CUDA tensors only.
 """
 

@@ -148,7 +148,8 @@ def gated_scan(z, f, h0=None, *, lengths=None, resets=None, decay_input=True, ch
     float32 state after the last.  ``lengths`` (B,) int32 / int64: sequence b has lengths[b]
     steps; later positions are not read, their h is 0, their gradients are 0, and hT is the
     state after the last step there is.  ``resets`` (T,B) bool: True drops the state before
-    that step (sequences packed one after another).  Strides of T and B are free (a
+    that step (sequences packed one after another).  A state that has become infinite stays
+    infinite or becomes NaN, up to the next reset.  Strides of T and B are free (a
     batch-major tensor passes as ``.transpose(0, 1)``); a strided channel dimension is copied.
 
     Gradients reach z, f and h0.  For the backward pass z and f are kept, and the state
