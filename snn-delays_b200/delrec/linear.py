@@ -36,7 +36,7 @@ def _is_binary(x):
 
 class LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, binary_input, checkpoint8=False):
+    def forward(ctx, x, weight, bias, binary_input, checkpoint8=False, grad=True):
         _lib.require_cuda(x, weight, bias)
         K = x.shape[-1]
         N = weight.shape[0]
@@ -50,21 +50,20 @@ class LinearFn(torch.autograd.Function):
         w = weight.detach()
         b = bias.detach() if bias is not None else None
         # only the parameter gradients read x; needs_input_grad tells of parameters without
-        # gradients enabled too, which is why ``linear`` asks for 8 bits only where they are
+        # gradients enabled too, so ``linear`` says whether they are
         ctx.packed = bool(checkpoint8)
         keep = None
-        if ctx.packed and (ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2])):
+        if ctx.packed and grad and (ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2])):
             keep = empty8(x2.shape, x2.dtype, dev)
         if M > 0:
             lib = _lib.lib()
             nbytes = lib.delrec_linear_forward_workspace(M, K, N, int(binary))
             P = _lib.ptr
+            ws = _lib.scratch(nbytes, dev) if ctx.packed else _lib.workspace(nbytes, dev)
             if keep is not None:
-                ws = _lib.scratch(nbytes, dev)
                 _lib.launch("delrec_linear_forward8", dev, M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(keep.q),
                             P(keep.e), P(ws), ws.numel())
             else:
-                ws = _lib.workspace(nbytes, dev)
                 _lib.launch("delrec_linear_forward", dev, M, K, N, P(x2), P(w), P(b), int(binary), P(out), P(ws),
                             ws.numel())
         if ctx.packed:
@@ -101,11 +100,11 @@ class LinearFn(torch.autograd.Function):
                 ws = _lib.scratch(lib.delrec_linear_backward8_workspace(M, K, N), dev)
                 _lib.launch("delrec_linear_backward8", dev, M, K, N, P(x2), P(e), P(w), P(g), P(dx), P(dw), P(db),
                             P(ws), ws.numel())
-                return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None
+                return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None, None
             ws = _lib.workspace(lib.delrec_linear_backward_workspace(M, K, N, int(ctx.binary)), dev)
             _lib.launch("delrec_linear_backward", dev, M, K, N, P(x2), P(w), P(g), int(ctx.binary), P(dx), P(dw),
                         P(db), P(ws), ws.numel())
-        return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None
+        return (dx.view(ctx.xshape) if dx is not None else None), dw, db, None, None, None
 
 
 class ReadoutTimeSum(torch.autograd.Function):
@@ -159,7 +158,7 @@ def readout_time_sum(y, weight, bias=None):
 
 def linear(x, weight, bias=None, *, binary_input=None, checkpoint8=False):
     """x W^T + bias on the library's projection (see the module's description)."""
-    return LinearFn.apply(x, weight, bias, binary_input, checkpoint8 and torch.is_grad_enabled())
+    return LinearFn.apply(x, weight, bias, binary_input, checkpoint8, torch.is_grad_enabled())
 
 
 class Linear(torch.nn.Linear):

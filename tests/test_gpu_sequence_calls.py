@@ -94,6 +94,40 @@ def test_evaluation_keeps_nothing_in_8_bits(guard, monkeypatch):
         assert torch.equal(linear.linear(x, keep.weight, keep.bias, binary_input=False, checkpoint8=True), plain(x))
 
 
+def test_evaluation_of_two_graphs_with_8_bit_projections(monkeypatch):
+    """Captured evaluation passes of checkpoint8 layers share no scratch: replayed on two streams at once."""
+    from delrec import _lib
+    from delrec.linear import linear
+    monkeypatch.setattr(_lib, "workspace", lambda *a: pytest.fail("scratch that outlives the call"))
+    sets = [[torch.randn(s, device="cuda") for s in ((900, 130), (70, 130))] for _ in range(2)]
+    for args in sets:
+        args[1].requires_grad_(True)
+
+    def go(x, w):
+        with torch.no_grad():
+            return linear(x, w, binary_input=False, checkpoint8=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [go(*args) for args in sets]
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for args in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(go(*args))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs, want):
+        assert torch.equal(a, b)
+
+
 def test_linear8_makes_its_tensors_device_current(monkeypatch):
     """The 8-bit projection launches with its tensors' device current, whichever was."""
     from delrec.linear import linear
