@@ -375,6 +375,109 @@ int delrec_linear_backward8(int M, int K, int N, const int8_t* q, const uint8_t*
                             const float* gout, float* dx, float* dW, float* dbias, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/* ---- short causal convolution ----------------------------------------------------------- */
+/* p_t = bias + sum_j w[:,j] x_{t-K+1+j}, y = act(p), one filter of K <= 8 taps per channel.  x, y,
+ * their gradients and the states are of one element type; w (N,K) and bias (N) float32.  Strides
+ * are in elements; channels are contiguous. */
+typedef struct delrec_conv {
+  int32_t T, B, N, K;
+  int32_t dtype;
+  int32_t act;           /* 0 none, 1 silu */
+  int32_t lengths_kind;  /* lengths (B): 0 int32, 1 int64, 2 one byte (a row has T steps or none) */
+  int32_t reserved;
+  int64_t x_t, x_b, y_t, y_b, gy_t, gy_b, dx_t, dx_b;
+} delrec_conv;
+
+/* state (K-1,B,N), NULL: zeros: the inputs before the first step, oldest first; next (K-1,B,N), NULL
+ * to skip: the last K-1 of each sequence.  With T = 1, next may be state.  bias NULL: 0.  lengths,
+ * resets NULL: whole sequences.  Rows past a length are not read, their y is 0. */
+int delrec_short_conv_forward(const delrec_conv* conv, const void* x, const float* w, const float* bias,
+                              const void* state, const void* lengths, const uint8_t* resets, void* y, void* next,
+                              void* stream);
+/* Gradients from gy (of y) and gs (of next), either NULL: 0.  Outputs NULL to skip; the workspace
+ * serves dw (N,K) and db (N). */
+size_t delrec_short_conv_backward_workspace(const delrec_conv* conv);
+int delrec_short_conv_backward(const delrec_conv* conv, const void* x, const float* w, const float* bias,
+                               const void* state, const void* lengths, const uint8_t* resets, const void* gy,
+                               const void* gs, void* dx, void* ds, float* dw, float* db, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* ---- selective state space scan ------------------------------------------------------------ */
+/* delta = softplus(dt + dt_bias) (softplus = 0: without softplus), h_t[n,s] = exp(delta A[n,s])
+ * h_{t-1}[n,s] + delta B_t[g,s] x_t[n], y_t[n] = (sum_s C_t[g,s] h_t[n,s] + D[n] x_t[n]) silu(gate_t[n]);
+ * group g serves N / G channels; S <= 128.  x, dt, gate, y (T,B,N) and Bm, Cm (T,B,G,S) of one element
+ * type; A (N,S), D, dt_bias (N), states (.., N,S) float32.  bm_*, cm_*: strides of T and B; (G,S) are
+ * contiguous. */
+typedef struct delrec_selective {
+  int32_t T, B, N, S, G;
+  int32_t dtype;
+  int32_t softplus;
+  int32_t lengths_wide;  /* lengths are int64 */
+  int64_t x_t, x_b, dt_t, dt_b, u_t, u_b, y_t, y_b;             /* x, dt, gate, y */
+  int64_t bm_t, bm_b, cm_t, cm_b;                               /* Bm, Cm */
+  int64_t gy_t, gy_b, dx_t, dx_b, ddt_t, ddt_b, du_t, du_b;     /* gradients of y, x, dt, gate */
+} delrec_selective;
+
+/* D, gate, dt_bias, h0 (B,N,S), lengths, resets (T,B): NULL for none.  hT (B,N,S) the state after the
+ * last step.  states (ceil(T/8),B,N,S), NULL without a backward pass: the state before every 8th.
+ * 16-byte aligned where S % 4 == 0: hT, states, dh0.  Rows past a length are not read, their y is 0. */
+size_t delrec_selective_forward_workspace(const delrec_selective* s);
+int delrec_selective_forward(const delrec_selective* s, const void* x, const void* dt, const float* A, const void* Bm,
+                             const void* Cm, const float* D, const void* gate, const float* dt_bias, const float* h0,
+                             const void* lengths, const uint8_t* resets, void* y, float* hT, float* states,
+                             void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients from gy (of y) and ghT (of hT), either NULL: 0.  Outputs NULL to skip; dB, dC (T,B,G,S)
+ * contiguous. */
+size_t delrec_selective_backward_workspace(const delrec_selective* s);
+int delrec_selective_backward(const delrec_selective* s, const void* x, const void* dt, const float* A, const void* Bm,
+                              const void* Cm, const float* D, const void* gate, const float* dt_bias,
+                              const void* lengths, const uint8_t* resets, const float* states, const void* gy,
+                              const float* ghT, void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD,
+                              void* dgate, float* ddt_bias, float* dh0, void* workspace, size_t workspace_bytes,
+                              void* stream);
+/* One time step (T = 1) of state (B,N,S) (NULL: 0) into next, which may be state.  active (B) bytes,
+ * NULL: all; a row that is not keeps its state and gives y = 0.  y (B,N) contiguous. */
+int delrec_selective_step(const delrec_selective* s, const void* x, const void* dt, const float* A, const void* Bm,
+                          const void* Cm, const float* D, const void* gate, const float* dt_bias, const float* state,
+                          const uint8_t* active, void* y, float* next, void* stream);
+
+/* ---- losses of a projection onto a vocabulary ------------------------------------------------ */
+/* Of z = x W^T + bias, which is never stored, over the T * B positions of x:
+ *   cross entropy   loss_m = logsumexp(z_m) - z_m[index_m]
+ *   distillation    loss_m = tau^2 sum_k p_k (log p_k - log q[index_mk]), p = softmax(logits_m / tau)
+ *                   over the K kept entries, q = softmax(z_m / tau) over the vocabulary
+ * x (T,B,D), W (V,D), bias (V) of one element type; W and bias contiguous.  A position does not count
+ * (loss and gradient 0) at or past lengths[b], where index is ignore_index, or where its list keeps
+ * nothing: an entry with a negative index or a logit of -inf is left out.  An index that is V or more
+ * (or negative and not ignore_index) makes the loss NaN and sets a bit of the status word.  D <= 8192,
+ * K <= 1024, T * B <= 2^24, V <= 2^30. */
+typedef struct delrec_vocab {
+  int32_t T, B, D, V, K;     /* K = 1 for the cross entropy */
+  int32_t dtype;
+  int32_t distill;
+  int32_t reduction;         /* 0 none: out (T,B); 1 mean over the positions that count; 2 sum: out (1) */
+  int32_t lengths_wide;      /* lengths are int64 */
+  int32_t index_wide;        /* index is int64 */
+  int32_t teacher_dtype;     /* of logits */
+  int32_t w_aligned;         /* W is 16-byte aligned */
+  float temperature;         /* tau > 0; 1 for the cross entropy */
+  int32_t reserved;
+  int64_t ignore_index;
+  int64_t x_t, x_b;
+} delrec_vocab;
+
+/* keep: what the backward pass takes over (256-byte aligned, as the workspaces). */
+size_t delrec_vocab_loss_keep(const delrec_vocab* s);
+size_t delrec_vocab_loss_forward_workspace(const delrec_vocab* s);
+int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* w, const void* bias, const void* index,
+                              const void* logits, const void* lengths, float* out, void* keep, size_t keep_bytes,
+                              void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients from g (of out).  dx (T,B,D), dw (V,D), db (V) contiguous, NULL to skip. */
+size_t delrec_vocab_loss_backward_workspace(const delrec_vocab* s);
+int delrec_vocab_loss_backward(const delrec_vocab* s, const void* x, const void* w, const void* bias, const float* g,
+                               const void* keep, size_t keep_bytes, void* dx, void* dw, void* db, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 /* ---- device status word ------------------------------------------------------------ */
 /* Kernels record internal inconsistencies (an out-of-range lag or index that was
  * skipped) in a device status word instead of trapping.  Reading it synchronizes. */

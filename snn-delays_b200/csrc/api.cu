@@ -1634,6 +1634,12 @@ static int run_backward(const delrec_layer* ly, int kind, const delrec_lif* lif,
   return DELREC_OK;
 }
 
+// the status word of the current device, for kernels of other translation units; NULL on failure
+int* status_word() {
+  void* p = nullptr;
+  return cudaGetSymbolAddress(&p, g_status) == cudaSuccess ? (int*)p : nullptr;
+}
+
 }  // namespace delrec
 
 using namespace delrec;

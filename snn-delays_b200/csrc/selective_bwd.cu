@@ -1,0 +1,8 @@
+// The selective scan's backward kernels.
+#include "selective_launch.cuh"
+
+namespace delrec {
+int sel_run_backward(int dtype, int L, int warps, const SelArgs& p, cudaStream_t st) {
+  return by_dtype(dtype, [&](auto t) { return sel_by_l<decltype(t), true>(L, warps, p, st); });
+}
+}  // namespace delrec

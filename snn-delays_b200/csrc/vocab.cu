@@ -1,0 +1,323 @@
+// extern "C" entry points of the vocabulary losses: argument checks, places in the workspace, the order
+// of launches.  No allocation happens here.
+#include <algorithm>
+
+#include "vocab_launch.cuh"
+#include "vocab_loss.cuh"
+
+namespace delrec {
+
+int* status_word();   // api.cu
+
+static int check_vocab(const delrec_vocab* s) {
+  if (!s || s->T < 1 || s->B < 1 || s->D < 1 || s->V < 1 || s->K < 1) return DELREC_ERR_ARG;
+  if (s->dtype < DELREC_F32 || s->dtype > DELREC_F16 || s->reduction < 0 || s->reduction > 2) return DELREC_ERR_ARG;
+  if (s->distill && (s->teacher_dtype < DELREC_F32 || s->teacher_dtype > DELREC_F16)) return DELREC_ERR_ARG;
+  if (!s->distill && s->K != 1) return DELREC_ERR_ARG;
+  if (!(s->temperature > 0.f) || !(s->temperature < 1e30f)) return DELREC_ERR_ARG;
+  if (s->D > kVocabMaxD || s->K > kVocabMaxK || s->V > (1 << 30) || (long long)s->T * s->B > (1 << 24))
+    return DELREC_ERR_UNSUPPORTED;
+  return DELREC_OK;
+}
+
+static size_t v256(size_t v) { return (v + 255) / 256 * 256; }
+struct VocabTake {
+  size_t total = 0;
+  size_t operator()(size_t bytes) {
+    const size_t at = total;
+    total += v256(bytes);
+    return at;
+  }
+};
+// what the backward pass takes over from the forward pass
+struct VocabKeep {
+  size_t rows, rowmap, pos, idx, p, y, lse, loss, total;
+  explicit VocabKeep(const delrec_vocab* s) {
+    const size_t M = (size_t)s->T * s->B, MK = M * s->K;
+    VocabTake take;
+    rows = take(4);
+    rowmap = take(M * 4);
+    pos = take(M * 4);
+    idx = take(MK * 4);
+    p = take(s->distill ? MK * 4 : 0);
+    y = take(MK * 4);
+    lse = take(M * 4);
+    loss = take(M * 4);
+    total = take.total;
+  }
+};
+
+static int vocab_bn(int n) { return n <= 128 ? 128 : 256; }
+// Parts of a reduction of kb 64-blocks over `tiles` output tiles: as many as fill the SMs' waves best, each
+// part at least 8 blocks; a further part has to save 5 % (its sums cross the memory once more).
+static int vocab_splits(long long tiles, long long kb) {
+  int best = 1;
+  double cost = (double)((tiles + kSeqSMs - 1) / kSeqSMs);
+  for (int k = 2; k <= 16 && k * 8 <= kb; ++k) {
+    const double c = (double)((tiles * k + kSeqSMs - 1) / kSeqSMs) / k;
+    if (c < cost * 0.95) { cost = c; best = k; }
+  }
+  return best;
+}
+
+struct VocabShape {
+  long long M, Mp, Dp, x_piece, w_piece, g_piece;
+  int pieces, esz, bnv, bnd, Vc, count;     // Vc columns in each of `count` pieces of the vocabulary
+  int dx_splits, dw_splits, db_runs;
+  bool w_direct;                            // W is an operand as it lies
+  size_t x, w, part, flags, h, each, G, coef, inv, dx, dw, db, total;
+};
+constexpr size_t kVocabBudget = 256u << 20;   // bytes of G at once
+static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
+  VocabShape h{};
+  h.M = (long long)s->T * s->B;
+  h.Mp = (h.M + 127) / 128 * 128;
+  h.Dp = (s->D + 7) / 8 * 8;
+  h.pieces = s->dtype == DELREC_F32 ? 3 : 1;
+  h.esz = s->dtype == DELREC_F32 ? 4 : 2;
+  h.x_piece = h.Mp * h.Dp;
+  h.w_piece = (long long)s->V * h.Dp;
+  h.bnv = vocab_bn(s->V);
+  h.bnd = vocab_bn(s->D);
+  VocabTake take;
+  h.x = take((size_t)h.x_piece * h.pieces * 2);
+  // whether W can be an operand as it lies is known at the call: room for its copy where it may be needed
+  h.w = take(h.pieces == 1 && s->D % 8 == 0 && s->w_aligned ? 0 : (size_t)h.w_piece * h.pieces * 2);
+  h.w_direct = h.pieces == 1 && s->D % 8 == 0 && s->w_aligned;
+  if (!backward) {
+    const long long tiles = (s->V + h.bnv - 1) / h.bnv * 2;
+    h.part = take((size_t)tiles * h.Mp * sizeof(float2));
+    h.flags = take(s->distill ? h.M : 0);
+    h.h = take((size_t)h.M * 4);
+  } else {
+    const long long fit = std::max<long long>(1024, (long long)(kVocabBudget / ((size_t)h.Mp * h.pieces * 2)));
+    h.count = (int)((s->V + fit - 1) / fit);
+    h.Vc = (int)(((s->V + h.count - 1) / h.count + 255) / 256 * 256);
+    h.count = (s->V + h.Vc - 1) / h.Vc;
+    h.g_piece = h.Mp * h.Vc;
+    const long long dtiles = (s->D + h.bnd - 1) / h.bnd;
+    h.dx_splits = vocab_splits((h.Mp / 128) * dtiles, std::min(h.Vc, s->V) / 64);
+    h.dw_splits = vocab_splits(((std::min(h.Vc, s->V) + 127) / 128) * dtiles, h.Mp / 64);
+    h.db_runs = (int)std::max<long long>(1, std::min<long long>(64, h.M / 64));
+    h.G = take((size_t)h.g_piece * h.pieces * 2);
+    h.coef = take((size_t)h.M * 4);
+    h.inv = take(4);
+    h.dx = take((size_t)h.dx_splits * h.Mp * h.Dp * 4);
+    h.dw = take(h.dw_splits > 1 ? (size_t)h.dw_splits * h.Vc * h.Dp * 4 : 0);
+    h.db = take((size_t)h.db_runs * h.Vc * 4);
+  }
+  h.total = take.total;
+  return h;
+}
+
+static VocabArgs vocab_args(const delrec_vocab* s, char* keep) {
+  const VocabKeep k(s);
+  VocabArgs a{};
+  a.T = s->T; a.B = s->B; a.D = s->D; a.V = s->V; a.K = s->K; a.M = s->T * s->B;
+  a.distill = s->distill; a.wide = s->lengths_wide; a.index_wide = s->index_wide; a.teacher = s->teacher_dtype;
+  a.ignore = s->ignore_index;
+  a.tau = s->temperature;
+  a.scale = 1.4426950408889634f / s->temperature;
+  a.x_t = s->x_t; a.x_b = s->x_b;
+  a.rows = (int*)(keep + k.rows);
+  a.rowmap = (int*)(keep + k.rowmap);
+  a.pos = (int*)(keep + k.pos);
+  a.idx = (int*)(keep + k.idx);
+  a.p = s->distill ? (float*)(keep + k.p) : nullptr;
+  a.y = (float*)(keep + k.y);
+  a.lse = (float*)(keep + k.lse);
+  a.loss = (float*)(keep + k.loss);
+  return a;
+}
+
+// the products of pieces, smallest first
+static void vg_products(VgArgs* g, int pieces) {
+  static const int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+  g->nprod = pieces == 3 ? 6 : 1;
+  for (int i = 0; i < g->nprod; ++i) {
+    g->pa[i] = pieces == 3 ? pa[i] : 0;
+    g->pb[i] = pieces == 3 ? pb[i] : 0;
+  }
+}
+
+template <class T>
+static int vocab_pack_t(const T* src, long long st, long long sb, int B, const int* rows, const int* rowmap, long long n,
+                        int D, int Dp, long long piece, void* out, cudaStream_t stream) {
+  constexpr int W = 16 / sizeof(T);
+  const bool vec = !(((uintptr_t)src) & 15) && st % W == 0 && sb % W == 0;
+  const int grid = seq_grid((size_t)(rows ? (n + 63) / 64 * 64 : n) * (Dp / 8), 256, 16);
+  if (vec) k_vocab_pack<T, true><<<grid, 256, 0, stream>>>(src, st, sb, B, rows, rowmap, n, D, Dp, piece, out);
+  else k_vocab_pack<T, false><<<grid, 256, 0, stream>>>(src, st, sb, B, rows, rowmap, n, D, Dp, piece, out);
+  SQ_LAUNCHED();
+  return DELREC_OK;
+}
+// x and (where it has to be) W as operands
+static int vocab_operands(const delrec_vocab* s, const VocabShape& h, const VocabArgs& a, const void* x, const void* w,
+                          char* ws, VgSide* X, VgSide* W, cudaStream_t st) {
+  *X = VgSide{ws + h.x, s->D, h.Mp, h.Dp, h.x_piece, h.pieces};
+  *W = VgSide{h.w_direct ? w : ws + h.w, s->D, s->V, h.Dp, h.w_piece, h.pieces};
+  return by_dtype(s->dtype, [&](auto t) {
+    using E = decltype(t);
+    int rc = vocab_pack_t<E>((const E*)x, s->x_t, s->x_b, s->B, a.rows, a.rowmap, h.M, s->D, (int)h.Dp, h.x_piece, ws + h.x, st);
+    if (rc == DELREC_OK && !h.w_direct)
+      rc = vocab_pack_t<E>((const E*)w, s->D, 0, 1, nullptr, nullptr, s->V, s->D, (int)h.Dp, h.w_piece, ws + h.w, st);
+    return rc;
+  });
+}
+
+}  // namespace delrec
+
+using namespace delrec;
+
+extern "C" {
+
+size_t delrec_vocab_loss_keep(const delrec_vocab* s) { return check_vocab(s) ? 0 : VocabKeep(s).total; }
+size_t delrec_vocab_loss_forward_workspace(const delrec_vocab* s) { return check_vocab(s) ? 0 : vocab_shape(s, false).total; }
+size_t delrec_vocab_loss_backward_workspace(const delrec_vocab* s) { return check_vocab(s) ? 0 : vocab_shape(s, true).total; }
+
+int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* w, const void* bias, const void* index,
+                              const void* logits, const void* lengths, float* out, void* keep, size_t keepb, void* ws,
+                              size_t wsb, void* stream) {
+  const int rc0 = check_vocab(s);
+  if (rc0) return rc0;
+  if (!x || !w || !index || !out || (s->distill && !logits)) return DELREC_ERR_ARG;
+  if (s->w_aligned && ((uintptr_t)w & 15)) return DELREC_ERR_ARG;
+  const VocabShape h = vocab_shape(s, false);
+  if (!keep || ((uintptr_t)keep & 255) || keepb < VocabKeep(s).total) return DELREC_ERR_WORKSPACE;
+  if (!ws || ((uintptr_t)ws & 255) || wsb < h.total) return DELREC_ERR_WORKSPACE;
+  char* base = (char*)ws;
+  VocabArgs a = vocab_args(s, (char*)keep);
+  a.x = x; a.w = w; a.bias = bias; a.index = index; a.logits = logits; a.lengths = lengths;
+  a.flags = (uint8_t*)(base + h.flags);
+  a.h = (float*)(base + h.h);
+  if (!(a.status = status_word())) return DELREC_ERR_CUDA;
+  const cudaStream_t st = (cudaStream_t)stream;
+  float* each = s->reduction == 0 ? out : nullptr;
+  if (s->distill) {
+    k_vocab_flags<<<(a.M + 7) / 8, 256, 0, st>>>(a);
+    SQ_LAUNCHED();
+  }
+  k_vocab_rows<<<(a.M + 1023) / 1024, 1024, 0, st>>>(a, each);
+  SQ_LAUNCHED();
+  VgSide X, W;
+  int rc = vocab_operands(s, h, a, x, w, base, &X, &W, st);
+  if (rc) return rc;
+  rc = by_dtype(s->dtype, [&](auto t) {
+    using E = decltype(t);
+    const size_t smem = ((size_t)(s->D + 3) / 4 * 4 + 2 * s->K) * 4;
+    const int nt = s->K == 1 ? 32 : 128;
+    if (!((uintptr_t)w & 15) && s->D % (16 / sizeof(E)) == 0) k_vocab_targets<E, true><<<a.M, nt, smem, st>>>(a);
+    else k_vocab_targets<E, false><<<a.M, nt, smem, st>>>(a);
+    SQ_LAUNCHED();
+    return (int)DELREC_OK;
+  });
+  if (rc) return rc;
+  VgArgs g{};
+  g.rows = a.rows;
+  g.M = -1; g.K = s->D; g.N = s->V; g.splits = 1; g.status = a.status; g.spin_ns = 2000000000ll;
+  vg_products(&g, h.pieces);
+  g.part = (float2*)(base + h.part); g.part_ld = h.Mp;
+  g.bias = bias; g.bias_code = s->dtype; g.scale = a.scale;
+  if ((rc = vg_logits(s->dtype == DELREC_F16, h.bnv, false, X, W, g, st))) return rc;
+  k_vocab_lse<<<(a.M + 31) / 32, 256, 0, st>>>(a, g.part, g.part_ld, (s->V + h.bnv - 1) / h.bnv * 2, each);
+  SQ_LAUNCHED();
+  if (!each) {
+    k_vocab_reduce<<<1, 1024, 0, st>>>(a, s->reduction == 1, out);
+    SQ_LAUNCHED();
+  }
+  return DELREC_OK;
+}
+
+int delrec_vocab_loss_backward(const delrec_vocab* s, const void* x, const void* w, const void* bias, const float* g_out,
+                               const void* keep, size_t keepb, void* dx, void* dw, void* db, void* ws, size_t wsb,
+                               void* stream) {
+  const int rc0 = check_vocab(s);
+  if (rc0) return rc0;
+  if (!x || !w || !g_out || (db && !bias)) return DELREC_ERR_ARG;
+  if (s->w_aligned && ((uintptr_t)w & 15)) return DELREC_ERR_ARG;
+  const VocabShape h = vocab_shape(s, true);
+  if (!keep || ((uintptr_t)keep & 255) || keepb < VocabKeep(s).total) return DELREC_ERR_WORKSPACE;
+  if (!ws || ((uintptr_t)ws & 255) || wsb < h.total) return DELREC_ERR_WORKSPACE;
+  char* base = (char*)ws;
+  VocabArgs a = vocab_args(s, (char*)const_cast<void*>(keep));
+  a.x = x; a.w = w; a.bias = bias;
+  if (!(a.status = status_word())) return DELREC_ERR_CUDA;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool f16 = s->dtype == DELREC_F16;
+  float *coef = (float*)(base + h.coef), *inv = (float*)(base + h.inv);
+  k_vocab_coef<<<1, 1024, 0, st>>>(a, s->reduction, g_out, coef, inv);
+  SQ_LAUNCHED();
+  VgSide X, W;
+  int rc = vocab_operands(s, h, a, x, w, base, &X, &W, st);
+  if (rc) return rc;
+  const VgSide G{base + h.G, h.Vc, h.Mp, h.Vc, h.g_piece, h.pieces};
+  const long long MK = (long long)a.M * a.K;
+  for (int c = 0; c < h.count; ++c) {
+    const int v0 = c * h.Vc, n = std::min(h.Vc, s->V - v0);
+    VgArgs g{};
+    g.rows = a.rows; g.status = a.status; g.spin_ns = 2000000000ll;
+    vg_products(&g, h.pieces);
+    {   // G = c softmax(z), then c (softmax(z) - p) at the targets
+      VgArgs q = g;
+      q.M = -1; q.K = s->D; q.N = n; q.splits = 1; q.b_mn = v0;
+      q.bias = bias; q.bias_code = s->dtype; q.scale = a.scale;
+      q.lse = a.lse; q.coef = coef; q.G = base + h.G; q.g_ld = h.Vc; q.g_piece = h.g_piece; q.pieces = h.pieces;
+      if ((rc = vg_logits(f16, h.bnv, true, X, W, q, st))) return rc;
+      const unsigned blocks = (unsigned)((MK + 255) / 256);
+      if (f16) k_vocab_patch<__half><<<blocks, 256, 0, st>>>(a, coef, v0, n, (__half*)(base + h.G), h.Vc, h.g_piece, h.pieces);
+      else k_vocab_patch<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, coef, v0, n, (__nv_bfloat16*)(base + h.G), h.Vc, h.g_piece, h.pieces);
+      SQ_LAUNCHED();
+    }
+    const int seg = h.pieces == 3 ? 16 : 0;
+    if (dw) {   // rows v0.. of G^T x
+      VgArgs q = g;
+      q.M = n; q.K = -1; q.N = s->D; q.splits = h.dw_splits; q.seg = seg; q.inv = inv;
+      if (h.dw_splits > 1) {
+        q.plane = (float*)(base + h.dw); q.plane_ld = h.Dp; q.plane_split = (long long)h.Vc * h.Dp;
+      } else {
+        q.out = dw; q.out_ld = s->D; q.out0 = v0;
+      }
+      if ((rc = vg_weights(s->dtype, h.bnd, G, X, q, st))) return rc;
+      if (h.dw_splits > 1) {
+        rc = by_dtype(s->dtype, [&](auto t) {
+          using E = decltype(t);
+          k_vocab_planes<E><<<seq_grid((size_t)n * ((s->D + 3) / 4), 256, 8), 256, 0, st>>>(
+              n, s->D, nullptr, q.plane, q.plane_ld, q.plane_split, q.splits, inv, (E*)dw + (long long)v0 * s->D);
+          SQ_LAUNCHED();
+          return (int)DELREC_OK;
+        });
+        if (rc) return rc;
+      }
+    }
+    if (dx) {   // += G W[v0..]
+      VgArgs q = g;
+      q.M = -1; q.K = n; q.N = s->D; q.splits = h.dx_splits; q.seg = seg; q.b_k = v0;
+      q.plane = (float*)(base + h.dx); q.plane_ld = h.Dp; q.plane_split = h.Mp * h.Dp; q.accumulate = c > 0;
+      if ((rc = vg_inputs(f16, h.bnd, G, W, q, st))) return rc;
+    }
+    if (db) {
+      float* part = (float*)(base + h.db);
+      const dim3 grid((n + 127) / 128, h.db_runs);
+      if (f16) k_vocab_db_part<__half><<<grid, 128, 0, st>>>(a.rows, (const __half*)(base + h.G), n, h.Vc, h.g_piece, h.pieces, part);
+      else k_vocab_db_part<__nv_bfloat16><<<grid, 128, 0, st>>>(a.rows, (const __nv_bfloat16*)(base + h.G), n, h.Vc, h.g_piece, h.pieces, part);
+      SQ_LAUNCHED();
+      rc = by_dtype(s->dtype, [&](auto t) {
+        using E = decltype(t);
+        k_vocab_db<E><<<(n + 255) / 256, 256, 0, st>>>(part, n, h.db_runs, inv, (E*)db + v0);
+        SQ_LAUNCHED();
+        return (int)DELREC_OK;
+      });
+      if (rc) return rc;
+    }
+  }
+  if (!dx) return DELREC_OK;
+  return by_dtype(s->dtype, [&](auto t) {
+    using E = decltype(t);
+    k_vocab_planes<E><<<seq_grid((size_t)h.M * ((s->D + 3) / 4), 256, 8), 256, 0, st>>>(
+        h.M, s->D, a.pos, (const float*)(base + h.dx), h.Dp, h.Mp * h.Dp, h.dx_splits, inv, (E*)dx);
+    SQ_LAUNCHED();
+    return (int)DELREC_OK;
+  });
+}
+
+}  // extern "C"

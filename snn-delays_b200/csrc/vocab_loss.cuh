@@ -1,0 +1,411 @@
+// The vocabulary losses' kernels around their matrix products (vocab_gemm.cuh).  Rows (positions) that
+// do not count are packed away first: the products run over the others only, and what stands in a
+// padded position is not read.
+//
+//   loss_m = tau^2 sum_k p_k (log p_k - log q_{i_k}),  q = softmax((x W^T + b) / tau)
+//   d loss_m / d z_v = tau (q_v - sum_{k: i_k = v} p_k)
+//
+// p = softmax(t / tau) over the K kept logits t of a teacher; the cross entropy is K = 1, p = 1,
+// tau = 1.  Logits are carried as y = z log2(e) / tau, sums in float32.
+#pragma once
+
+#include "seq_common.cuh"
+
+namespace delrec {
+
+constexpr int kVocabMaxD = 8192, kVocabMaxK = 1024;
+constexpr float kLn2v = 0.6931471805599453f;
+constexpr int kVocabIndexRange = 1 << 1;   // ST_INDEX_RANGE of the status word
+
+struct VocabArgs {
+  int T, B, D, V, K, M;            // M = T B positions
+  int distill, wide, index_wide, teacher;   // types of lengths, indices and the teacher's logits
+  long long ignore;
+  float tau, scale;                // scale = log2(e) / tau
+  long long x_t, x_b;
+  const void *x, *w, *bias, *index, *logits, *lengths;
+  uint8_t* flags;                  // (M) distillation: does the position count
+  int *rows, *rowmap, *pos;        // count; position of each packed row; packed row of each position or -1
+  int* idx;                        // (M, K) of packed rows; -1: left out or out of range
+  float *p, *y, *h, *lse, *loss;   // p and y (M, K); h, lse, loss (M): of packed rows
+  int* status;
+};
+
+__device__ __forceinline__ long long vocab_index(const VocabArgs& a, size_t i) {
+  return a.index_wide ? ((const long long*)a.index)[i] : (long long)((const int*)a.index)[i];
+}
+__device__ __forceinline__ float vocab_teacher(const VocabArgs& a, size_t i) {
+  switch (a.teacher) {
+    case DELREC_F32: return ((const float*)a.logits)[i];
+    case DELREC_BF16: return to_f(((const __nv_bfloat16*)a.logits)[i]);
+  }
+  return to_f(((const __half*)a.logits)[i]);
+}
+__device__ __forceinline__ bool vocab_live(const VocabArgs& a, int m) {
+  return !a.lengths || m / a.B < row_length(a.lengths, a.wide, m % a.B, a.T);
+}
+// a kept entry of the teacher's list
+__device__ __forceinline__ bool vocab_kept(long long i, float t) { return i >= 0 && t != -INFINITY; }
+
+// distillation: a position counts if its list keeps an entry.  One warp a position.
+static __global__ void __launch_bounds__(256) k_vocab_flags(const VocabArgs a) {
+  const int m = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (m >= a.M) return;
+  bool any = false;
+  if (vocab_live(a, m))
+    for (int k = lane; k < a.K; k += 32)
+      any |= vocab_kept(vocab_index(a, (size_t)m * a.K + k), vocab_teacher(a, (size_t)m * a.K + k));
+  any = __any_sync(0xffffffffu, any);
+  if (lane == 0) a.flags[m] = any;
+}
+__device__ __forceinline__ bool vocab_counts(const VocabArgs& a, int m) {
+  if (a.distill) return a.flags[m];
+  return vocab_live(a, m) && vocab_index(a, m) != a.ignore;
+}
+// Packs the rows that count, in order.  A block of 1024 counts those before its own by itself.
+// each (M) or NULL: the positions' losses, 0 where a position does not count.
+static __global__ void __launch_bounds__(1024) k_vocab_rows(const VocabArgs a, float* each) {
+  __shared__ int s_warp[32], s_before;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, first = blockIdx.x * 1024;
+  int before = 0;
+#pragma unroll 4
+  for (int m = tid; m < first; m += 1024) before += vocab_counts(a, m);
+  before = __reduce_add_sync(0xffffffffu, before);
+  if (lane == 0) s_warp[warp] = before;
+  __syncthreads();
+  if (warp == 0) {
+    const int v = __reduce_add_sync(0xffffffffu, s_warp[lane]);
+    if (lane == 0) s_before = v;
+  }
+  __syncthreads();
+  const int m = first + tid;
+  const bool on = m < a.M && vocab_counts(a, m);
+  const unsigned vote = __ballot_sync(0xffffffffu, on);
+  if (lane == 0) s_warp[warp] = __popc(vote);
+  __syncthreads();
+  int at = s_before, total = s_before;
+  for (int w = 0; w < 32; ++w) {
+    if (w < warp) at += s_warp[w];
+    total += s_warp[w];
+  }
+  at += __popc(vote & ((1u << lane) - 1u));
+  if (m < a.M) {
+    a.pos[m] = on ? at : -1;
+    if (on) a.rowmap[at] = m;
+    else if (each) each[m] = 0.f;
+  }
+  if (tid == 0 && first + 1024 >= a.M) *a.rows = total;
+}
+
+// Rows as tensor-core operands: out[piece][row][Dp], 16-bit types as they are, fp32 in three bf16 pieces
+// (v = p0 + p1 + p2 exactly).  rows NULL: n rows in place, else the packed rows of x and zero rows up to
+// the next 64.  A thread takes eight columns.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, long long st, long long sb, int B,
+                                                    const int* __restrict__ rows, const int* __restrict__ rowmap,
+                                                    long long n, int D, int Dp, long long piece, void* out) {
+  const int cols = Dp / 8;
+  const long long real = rows ? *rows : n, all = (rows ? (real + 63) / 64 * 64 : n) * cols;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+    const long long r = i / cols;
+    const int c = (int)(i % cols) * 8;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    if (r < real) {
+      const long long m = rows ? rowmap[r] : r;
+      const T* s = src + (rows ? m / B * st + m % B * sb : m * st) + c;
+      if (VEC && c + 8 <= D) {
+        constexpr int W = 16 / sizeof(T);
+#pragma unroll
+        for (int k = 0; k < 8; k += W) unpack_vec<T, W>(*(const VecOf<T, W>*)(s + k), v + k);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (c + k < D) v[k] = to_f(s[k]);
+      }
+    }
+    using E = std::conditional_t<std::is_same_v<T, __half>, __half, __nv_bfloat16>;
+    E* o = (E*)out + r * Dp + c;
+    constexpr int P = sizeof(T) == 4 ? 3 : 1;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const VecOf<E, 8> q = pack_vec<E, 8>(v);
+      *(VecOf<E, 8>*)(o + p * piece) = q;
+      if (p + 1 < P) {
+        float f[8];
+        unpack_vec<E, 8>(q, f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] -= f[k];
+      }
+    }
+  }
+}
+
+// The targets of packed row blockIdx.x: p, the sums of p over repeated indices, the targets' logits y
+// (dot products in float32) and h = sum p (log p - ln2 y).  One warp for K = 1, four else.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
+  extern __shared__ float smf[];
+  __shared__ float s_red[4];
+  const int r = blockIdx.x;
+  if (r >= *a.rows) return;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, W = nt / 32, K = a.K, D = a.D;
+  float* s_x = smf;                 // [D]
+  float* s_p = s_x + (D + 3) / 4 * 4;   // [K]
+  int* s_i = (int*)(s_p + K);       // [K]
+  const int m = a.rowmap[r];
+  const T* x = (const T*)a.x + m / a.B * a.x_t + m % a.B * a.x_b;
+  for (int d = tid; d < D; d += nt) s_x[d] = to_f(x[d]);
+  const auto all = [&](float v, bool max) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float u = __shfl_xor_sync(0xffffffffu, v, o);
+      v = max ? fmaxf(v, u) : v + u;
+    }
+    __syncthreads();
+    if (lane == 0) s_red[warp] = v;
+    __syncthreads();
+    v = s_red[0];
+    for (int w = 1; w < W; ++w) v = max ? fmaxf(v, s_red[w]) : v + s_red[w];
+    return v;
+  };
+  float top = -INFINITY;
+  for (int k = tid; k < K; k += nt) {
+    const size_t e = (size_t)m * K + k;
+    long long i = vocab_index(a, e);
+    float t = a.distill ? vocab_teacher(a, e) / a.tau : 0.f;
+    if (a.distill && !vocab_kept(i, t)) {
+      i = -1;
+      t = -INFINITY;
+    } else if (i < 0 || i >= a.V) {
+      atomicOr(a.status, kVocabIndexRange);
+      i = -2;
+    }
+    s_i[k] = (int)i;
+    s_p[k] = t;
+    top = fmaxf(top, t);
+  }
+  float h = 0.f;
+  if (a.distill) {
+    top = all(top, true);
+    float sum = 0.f;
+    for (int k = tid; k < K; k += nt) sum += s_i[k] == -1 ? 0.f : expf(s_p[k] - top);
+    sum = all(sum, false);
+    const float ls = logf(sum);
+    for (int k = tid; k < K; k += nt) {
+      const float lp = s_p[k] - top - ls, p = s_i[k] == -1 ? 0.f : expf(lp);
+      s_p[k] = p;
+      if (p != 0.f) h = fmaf(p, lp, h);
+    }
+  } else if (tid == 0) {
+    s_p[0] = 1.f;
+  }
+  __syncthreads();
+  if (a.p)
+    for (int k = tid; k < K; k += nt) {
+      float s = 0.f;
+      const int i = s_i[k];
+      for (int j = 0; j < K; ++j) s += s_i[j] == i ? s_p[j] : 0.f;
+      a.p[(size_t)r * K + k] = s;
+    }
+  // four targets at a time, their rows of W on the way together
+  const T* w = (const T*)a.w;
+  for (int k0 = warp * 4; k0 < K; k0 += W * 4) {
+    float dot[4] = {};
+    const T* row[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) row[j] = k0 + j < K && s_i[k0 + j] >= 0 ? w + (size_t)s_i[k0 + j] * D : nullptr;
+    if (VEC) {
+      constexpr int N = 16 / sizeof(T);
+      for (int d = lane * N; d < D; d += 32 * N) {
+        float xv[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) xv[i] = s_x[d + i];
+        VecOf<T, N> q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (row[j]) q[j] = *(const VecOf<T, N>*)(row[j] + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (row[j]) {
+            float f[N];
+            unpack_vec<T, N>(q[j], f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) dot[j] = fmaf(xv[i], f[i], dot[j]);
+          }
+      }
+    } else {
+      for (int d = lane; d < D; d += 32)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (row[j]) dot[j] = fmaf(s_x[d], to_f(row[j][d]), dot[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+      if (lane == 0 && k0 + j < K) {
+        const int i = s_i[k0 + j];
+        float y = (dot[j] + (a.bias && i >= 0 ? to_f(((const T*)a.bias)[i]) : 0.f)) * a.scale;
+        if (i == -2) y = __int_as_float(0x7fc00000);
+        a.y[(size_t)r * K + k0 + j] = y;
+        a.idx[(size_t)r * K + k0 + j] = max(i, -1);
+        if (i == -2 || (i >= 0 && s_p[k0 + j] != 0.f)) h = fmaf(-kLn2v * s_p[k0 + j], y, h);
+      }
+    }
+  }
+  h = all(h, false);
+  if (tid == 0) a.h[r] = h;
+}
+
+// A row's log-sum-exp from its tiles' maxima and sums, and its loss.  Block: 32 rows by 8 runs of tiles.
+static __global__ void __launch_bounds__(256) k_vocab_lse(const VocabArgs a, const float2* __restrict__ part,
+                                                          long long ld, int tiles, float* each) {
+  __shared__ float2 s[8][32];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int rows = *a.rows, r = blockIdx.x * 32 + lane;
+  if (blockIdx.x * 32 >= rows) return;
+  float top = -INFINITY, sum = 0.f;
+  if (r < rows)
+#pragma unroll 4
+    for (int t = run; t < tiles; t += 8) {
+      const float2 v = part[t * ld + r];
+      const float mx = fmaxf(top, v.x), at = mx == -INFINITY ? 0.f : mx;
+      sum = sum * exp2f(top - at) + v.y * exp2f(v.x - at);
+      top = mx;
+    }
+  s[run][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (run || r >= rows) return;
+  for (int k = 1; k < 8; ++k) {
+    const float2 v = s[k][lane];
+    const float mx = fmaxf(top, v.x), at = mx == -INFINITY ? 0.f : mx;
+    sum = sum * exp2f(top - at) + v.y * exp2f(v.x - at);
+    top = mx;
+  }
+  const float lse = top + log2f(sum);
+  a.lse[r] = lse;
+  const float loss = a.tau * a.tau * fmaf(kLn2v, lse, a.h[r]);
+  a.loss[r] = loss;
+  if (each) each[a.rowmap[r]] = loss;
+}
+// the sum or the mean of the rows' losses (0 of none), in a fixed order
+static __global__ void __launch_bounds__(1024) k_vocab_reduce(const VocabArgs a, int mean, float* out) {
+  __shared__ double s[32];
+  const int rows = *a.rows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double v = 0.0;
+#pragma unroll 4
+  for (int r = threadIdx.x; r < rows; r += 1024) v += a.loss[r];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0) s[warp] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    v = 0.0;
+    for (int w = 0; w < 32; ++w) v += s[w];
+    *out = (float)(mean && rows > 0 ? v / rows : v);
+  }
+}
+
+// c_r = g tau (/ count) of each packed row, brought to at most 2^14 by one power of two, whose inverse is
+// *inv: G = c (q - p) then fits fp16 with its small entries.  A row with a NaN loss has NaN gradients.
+static __global__ void __launch_bounds__(1024) k_vocab_coef(const VocabArgs a, int reduction, const float* __restrict__ g,
+                                                            float* coef, float* inv) {
+  __shared__ float s_top[32];
+  const int rows = *a.rows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float one = reduction == 0 ? 0.f : *g * a.tau / (reduction == 1 ? (float)max(rows, 1) : 1.f);
+  float top = 0.f;
+  for (int r = threadIdx.x; r < rows; r += 1024) {
+    const float c = fabsf(reduction == 0 ? g[a.rowmap[r]] * a.tau : one);
+    if (c < INFINITY) top = fmaxf(top, c);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+  for (int w = 0; w < 32; ++w) top = fmaxf(top, s_top[w]);
+  int e = 0;
+  frexpf(top, &e);                                        // top = f 2^e, f in [0.5, 1)
+  e = top > 0.f ? min(max(14 - e, -100), 120) : 0;
+  const float up = ldexpf(1.f, e);
+  for (int r = threadIdx.x; r < rows; r += 1024) {
+    const float c = reduction == 0 ? g[a.rowmap[r]] * a.tau : one, l = a.loss[r];
+    coef[r] = l != l ? l : c * up;
+  }
+  if (threadIdx.x == 0) *inv = ldexpf(1.f, -e);
+}
+
+// the targets' entries of a piece of G: c (q - p), each rounded once; repeated indices write the same
+template <class E>
+__global__ void __launch_bounds__(256) k_vocab_patch(const VocabArgs a, const float* __restrict__ coef, int v0, int n,
+                                                     E* G, long long ld, long long piece, int pieces) {
+  const long long e = blockIdx.x * 256LL + threadIdx.x;
+  const long long r = e / a.K;
+  if (r >= *a.rows) return;
+  const int i = a.idx[e] - v0;
+  if (i < 0 || i >= n) return;
+  float v = coef[r] * (exp2f(a.y[e] - a.lse[r]) - (a.p ? a.p[e] : 1.f));
+  for (int p = 0; p < pieces; ++p) {
+    const E q = from_f<E>(v);
+    G[p * piece + r * ld + i] = q;
+    v -= to_f(q);
+  }
+}
+
+// column sums of a piece of G over runs of rows: part[run][column]; then db
+template <class E>
+__global__ void __launch_bounds__(128) k_vocab_db_part(const int* __restrict__ rows, const E* __restrict__ G, int n,
+                                                       long long ld, long long piece, int pieces, float* part) {
+  const int c = blockIdx.x * 128 + threadIdx.x, run = blockIdx.y, runs = gridDim.y;
+  if (c >= n) return;
+  const long long R = *rows, r0 = R * run / runs, r1 = R * (run + 1) / runs;
+  float s = 0.f;
+#pragma unroll 8
+  for (long long r = r0; r < r1; ++r) {
+    float v = to_f(G[r * ld + c]);
+    for (int p = 1; p < pieces; ++p) v += to_f(G[p * piece + r * ld + c]);
+    s += v;
+  }
+  part[(long long)run * n + c] = s;
+}
+template <class T>
+__global__ void __launch_bounds__(256) k_vocab_db(const float* __restrict__ part, int n, int runs,
+                                                  const float* __restrict__ inv, T* db) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < runs; ++k) s += part[(long long)k * n + c];
+  db[c] = from_f<T>(s * *inv);
+}
+
+// out[row][D] = *inv * sum of planes[split][pos ? pos[row] : row], 0 where pos is -1
+template <class T>
+__global__ void __launch_bounds__(256) k_vocab_planes(long long n, int D, const int* __restrict__ pos,
+                                                      const float* __restrict__ plane, long long ld, long long split,
+                                                      int splits, const float* __restrict__ inv, T* out) {
+  const int cols = (D + 3) / 4;
+  const float up = *inv;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n * cols; i += gridDim.x * 256LL) {
+    const long long m = i / cols, r = pos ? pos[m] : m;
+    const int c = (int)(i % cols) * 4;
+    float v[4] = {};
+    if (r >= 0)
+      for (int s = 0; s < splits; ++s) {
+        const float4 q = *(const float4*)(plane + s * split + r * ld + c);
+        v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] *= up;
+    T* o = out + m * D + c;
+    if (D % 4 == 0) {
+      *(VecOf<T, 4>*)o = pack_vec<T, 4>(v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < D) o[k] = from_f<T>(v[k]);
+    }
+  }
+}
+
+}  // namespace delrec

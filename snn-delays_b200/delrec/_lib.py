@@ -61,6 +61,23 @@ class Block(ctypes.Structure):
                "gn_b", "dx_t", "dx_b", "dy_t", "dy_b", "du_t", "du_b")
 
 
+class Conv(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("T", "B", "N", "K", "dtype", "act", "lengths_kind", "reserved")] \
+        + _i64("x_t", "x_b", "y_t", "y_b", "gy_t", "gy_b", "dx_t", "dx_b")
+
+
+class Selective(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("T", "B", "N", "S", "G", "dtype", "softplus", "lengths_wide")] \
+        + _i64("x_t", "x_b", "dt_t", "dt_b", "u_t", "u_b", "y_t", "y_b", "bm_t", "bm_b", "cm_t", "cm_b", "gy_t",
+               "gy_b", "dx_t", "dx_b", "ddt_t", "ddt_b", "du_t", "du_b")
+
+
+class Vocab(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("T", "B", "D", "V", "K", "dtype", "distill", "reduction", "lengths_wide",
+                                              "index_wide", "teacher_dtype", "w_aligned")] \
+        + [("temperature", ctypes.c_float), ("reserved", ctypes.c_int32)] + _i64("ignore_index", "x_t", "x_b")
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
@@ -120,6 +137,19 @@ _SIGS = {
     "delrec_unpack8": (_I, [ctypes.c_longlong, _I, _I, _P, _P, _P, _P]),
     "delrec_linear_forward8": (_I, [_I, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _S, _P]),
     "delrec_linear_backward8_workspace": (_S, [_I, _I, _I]),
+    "delrec_short_conv_forward": (_I, [_P] * 10),
+    "delrec_short_conv_backward_workspace": (_S, [_P]),
+    "delrec_short_conv_backward": (_I, [_P] * 14 + [_S, _P]),
+    "delrec_selective_forward_workspace": (_S, [_P]),
+    "delrec_selective_forward": (_I, [_P] * 16 + [_S, _P]),
+    "delrec_selective_backward_workspace": (_S, [_P]),
+    "delrec_selective_backward": (_I, [_P] * 24 + [_S, _P]),
+    "delrec_selective_step": (_I, [_P] * 14),
+    "delrec_vocab_loss_keep": (_S, [_P]),
+    "delrec_vocab_loss_forward_workspace": (_S, [_P]),
+    "delrec_vocab_loss_forward": (_I, [_P] * 9 + [_S, _P, _S, _P]),
+    "delrec_vocab_loss_backward_workspace": (_S, [_P]),
+    "delrec_vocab_loss_backward": (_I, [_P] * 6 + [_S] + [_P] * 4 + [_S, _P]),
     "delrec_linear_backward8": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
 }
 
@@ -199,6 +229,22 @@ def require_lengths(lengths, B, device):
     if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64) or lengths.device != device \
             or not lengths.is_contiguous():
         raise RuntimeError(f"delrec_b200: lengths must be contiguous int32 or int64 ({B},) on {device}")
+
+
+def require_resets(resets, T, B, device):
+    if resets is None:
+        return None
+    if resets.shape != (T, B) or resets.dtype != torch.bool or resets.device != device:
+        raise RuntimeError(f"delrec_b200: resets must be bool ({T}, {B}) on {device}")
+    return resets.contiguous()
+
+
+def require_active(active, B, device):
+    if active is None:
+        return None
+    if active.shape != (B,) or active.dtype != torch.bool or active.device != device:
+        raise RuntimeError(f"delrec_b200: active must be bool ({B},) on {device}")
+    return active.contiguous()
 
 
 def refuse_tangents(*tensors):
