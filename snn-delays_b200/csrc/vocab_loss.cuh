@@ -216,30 +216,30 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
     const T* row[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) row[j] = k0 + j < K && s_i[k0 + j] >= 0 ? w + (size_t)s_i[k0 + j] * D : nullptr;
-    if (VEC) {
-      constexpr int N = 16 / sizeof(T);
-      for (int d = lane * N; d < D; d += 32 * N) {
-        float xv[N];
+    constexpr int N = 16 / sizeof(T);      // the same order of sums whatever the alignment
+    for (int d = lane * N; d < D; d += 32 * N) {
+      VecOf<T, N> q[4];
 #pragma unroll
-        for (int i = 0; i < N; ++i) xv[i] = s_x[d + i];
-        VecOf<T, N> q[4];
+      for (int j = 0; j < 4; ++j)
+        if (row[j]) {
+          if (VEC) {
+            q[j] = *(const VecOf<T, N>*)(row[j] + d);
+          } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (row[j]) q[j] = *(const VecOf<T, N>*)(row[j] + d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (row[j]) {
-            float f[N];
-            unpack_vec<T, N>(q[j], f);
-#pragma unroll
-            for (int i = 0; i < N; ++i) dot[j] = fmaf(xv[i], f[i], dot[j]);
+            for (int i = 0; i < N; ++i) q[j].v[i] = d + i < D ? row[j][d + i] : from_f<T>(0.f);
           }
-      }
-    } else {
-      for (int d = lane; d < D; d += 32)
+        }
+      float xv[N];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (row[j]) dot[j] = fmaf(s_x[d], to_f(row[j][d]), dot[j]);
+      for (int i = 0; i < N; ++i) xv[i] = d + i < D ? s_x[d + i] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (row[j]) {
+          float f[N];
+          unpack_vec<T, N>(q[j], f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) dot[j] = fmaf(xv[i], f[i], dot[j]);
+        }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
