@@ -24,30 +24,36 @@ static int sel_lanes(int S) {
 }
 
 struct SelShape {
-  int L, warps, CH, tiles, chunks, steps;
+  int L, tiles, chunks, steps;
 };
-// Blocks of up to `most` warps, none wider than a group.  Where rows and tiles leave SMs idle, time is
-// cut into chunks of at least 64 steps; a chunked pass does some 1.6 times the work, so there have to
-// be twice as many blocks to be had.
-static SelShape sel_shape(const delrec_selective* s, int most, int blocks) {
+// Time is cut into chunks of at least 64 steps where that fills the SMs better: `slots` blocks run at
+// once, so c chunks take ceil(blocks c / slots) / c of a sequence's time, and the maps that go before
+// them `more` as much again (T=1021 B=24 N=520 S=24: 480 blocks for 444 slots, two rounds uncut).  Past
+// four rounds uncut there is nothing to gain.
+static SelShape sel_shape(const delrec_selective* s, int slots, double more) {
   SelShape h{};
   h.L = sel_lanes(s->S);
-  const int cw = 32 / h.L * 4, Dg = s->N / s->G;
-  h.warps = std::min(most, (Dg + cw - 1) / cw);
-  h.CH = h.warps * cw;
-  h.tiles = (Dg + h.CH - 1) / h.CH;
+  const int CH = 256 / h.L, Dg = s->N / s->G;
+  h.tiles = (Dg + CH - 1) / CH;
   const long long base = (long long)h.tiles * s->G * s->B;
-  h.chunks = 1;
-  h.steps = (s->T + kSelSeg - 1) / kSelSeg * kSelSeg;
-  if (base * 2 <= blocks && s->T >= 2 * 64) {
-    const long long want = std::min<long long>(blocks / base, s->T / 64);
-    h.steps = (int)(((s->T + want - 1) / want + kSelSeg - 1) / kSelSeg * kSelSeg);
-    h.chunks = (s->T + h.steps - 1) / h.steps;
-  }
+  // of a padded batch's k chunks some (k + 1) / 2 hold steps, and the other blocks leave at once
+  const auto rounds = [&](long long k) {
+    const long long blocks = s->ragged ? base * (k + 1) / 2 : base * k;
+    return (double)((blocks + slots - 1) / slots);
+  };
+  int chunks = 1;
+  double best = rounds(1);
+  if (base < 4LL * slots)
+    for (int k = 2; k <= s->T / 64 && k <= 1024; ++k) {
+      const double cost = rounds(k) / k * (1 + more) * (1 + 0.001 * k);
+      if (cost < best) { best = cost; chunks = k; }
+    }
+  h.steps = ((s->T + chunks - 1) / chunks + kSelSeg - 1) / kSelSeg * kSelSeg;
+  h.chunks = (s->T + h.steps - 1) / h.steps;
   return h;
 }
-static SelShape sel_fwd_shape(const delrec_selective* s) { return sel_shape(s, 4, kSeqSMs * 4); }
-static SelShape sel_bwd_shape(const delrec_selective* s) { return sel_shape(s, 2, kSeqSMs * 4); }
+static SelShape sel_fwd_shape(const delrec_selective* s) { return sel_shape(s, kSeqSMs * 5, 0.6); }
+static SelShape sel_bwd_shape(const delrec_selective* s) { return sel_shape(s, kSeqSMs * 3, 0.35); }
 
 static size_t al256(size_t v) { return (v + 255) / 256 * 256; }
 struct SelPlan {   // places in the workspace
@@ -83,13 +89,18 @@ static SelPlan sel_bwd_plan(const delrec_selective* s) {
   return w;
 }
 
-// May all these tensors be read four elements at a time?
+// May all these tensors be read four, two elements at a time?
 struct SelAlign {
-  int esz;
-  bool ok;
-  SelAlign(const delrec_selective* s) : esz(s->dtype == DELREC_F32 ? 4 : 2), ok(s->N / s->G % 4 == 0) {}
+  int esz, vec;
+  SelAlign(const delrec_selective* s) : esz(s->dtype == DELREC_F32 ? 4 : 2), vec(s->N / s->G % 4 == 0 ? 4 : s->N / s->G % 2 == 0 ? 2 : 1) {}
+  bool fits(int V, const void* p, long long st, long long sb) const {
+    return !p || !(((uintptr_t)p % (V * esz)) || st % V || sb % V);
+  }
   void add(const void* p, long long st, long long sb) {
-    if (p && (((uintptr_t)p % (4 * esz)) || st % 4 || sb % 4)) ok = false;
+    while (vec > 1 && !fits(vec, p, st, sb)) vec /= 2;
+  }
+  bool states(const delrec_selective* s, const void* Bm, const void* Cm) const {
+    return s->S % 4 == 0 && fits(4, Bm, s->bm_t, s->bm_b) && fits(4, Cm, s->cm_t, s->cm_b);
   }
 };
 
@@ -97,7 +108,7 @@ static SelArgs sel_args(const delrec_selective* s, const SelShape& h, const SelP
   SelArgs p{};
   p.T = s->T; p.B = s->B; p.N = s->N; p.S = s->S; p.G = s->G; p.Dg = s->N / s->G;
   p.softplus = s->softplus; p.wide = s->lengths_wide;
-  p.chunks = h.chunks; p.steps = h.steps; p.tiles = h.tiles; p.CH = h.CH;
+  p.chunks = h.chunks; p.steps = h.steps; p.tiles = h.tiles;
   p.x_t = s->x_t; p.x_b = s->x_b; p.dt_t = s->dt_t; p.dt_b = s->dt_b; p.u_t = s->u_t; p.u_b = s->u_b;
   p.y_t = s->y_t; p.y_b = s->y_b; p.bm_t = s->bm_t; p.bm_b = s->bm_b; p.cm_t = s->cm_t; p.cm_b = s->cm_b;
   p.gy_t = s->gy_t; p.gy_b = s->gy_b; p.dx_t = s->dx_t; p.dx_b = s->dx_b; p.ddt_t = s->ddt_t; p.ddt_b = s->ddt_b;
@@ -137,8 +148,9 @@ int delrec_selective_forward(const delrec_selective* s, const void* x, const voi
   al.add(dt, s->dt_t, s->dt_b);
   al.add(gate, s->u_t, s->u_b);
   al.add(y, s->y_t, s->y_b);
-  p.vec = al.ok;
-  return sel_run_forward(s->dtype, h.L, h.warps, p, (cudaStream_t)stream);
+  p.vec = al.vec;
+  p.bcvec = al.states(s, Bm, Cm);
+  return sel_run_forward(s->dtype, h.L, p, (cudaStream_t)stream);
 }
 
 size_t delrec_selective_backward_workspace(const delrec_selective* s) {
@@ -175,9 +187,10 @@ int delrec_selective_backward(const delrec_selective* s, const void* x, const vo
   al.add(dx, s->dx_t, s->dx_b);
   al.add(ddt, s->ddt_t, s->ddt_b);
   al.add(dgate, s->du_t, s->du_b);
-  p.vec = al.ok;
+  p.vec = al.vec;
+  p.bcvec = al.states(s, Bm, Cm);
   const cudaStream_t st = (cudaStream_t)stream;
-  int r = sel_run_backward(s->dtype, h.L, h.warps, p, st);
+  int r = sel_run_backward(s->dtype, h.L, p, st);
   if (r) return r;
   const long long parts = (long long)h.chunks * s->B;
   const auto sum = [&](long long cols, const float* part, float* out) {

@@ -4,11 +4,10 @@
 //   h_t[s]  = exp(delta_t A[s]) h_{t-1}[s] + delta_t B_t[s] x_t
 //   y_t     = (sum_s C_t[s] h_t[s] + D x_t) silu(gate_t)
 //
-// A thread holds 4 channels x 4 states; L lanes (4 L >= S) share a channel's states, the other
-// 32 / L lane groups of a warp hold other channels.  So B_t and C_t are four values a thread, the
-// sums over states (y, dx, ddt) run over four values in the thread and then over L lanes, and those over
-// channels (dB, dC) over four values and then over 32 / L lanes: either way a
-// lane hands on half of what it holds at each exchange.  A block walks kSelSeg steps at a time, whose
+// A thread holds 2 channels x 4 states; L lanes (4 L >= S) share a channel's states, the other
+// 32 / L lane groups of a warp hold other channels.  The sums over states (y, dx, ddt) run over four
+// values in the thread and then over L lanes, those over channels (dB, dC) over two values and then
+// over 32 / L lanes: either way a lane hands on half of what it holds at each exchange.  A block walks kSelSeg steps at a time, whose
 // inputs it lays out in shared memory in float32; states stay in registers.
 //
 // The backward pass keeps the states before every kSelSeg-th step (written by the forward pass),
@@ -31,8 +30,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct SelArgs {
   int T, B, N, S, G, Dg;          // Dg = N / G channels to a group
-  int softplus, wide, vec;        // vec: rows of x, dt, gate, y and their gradients in fours
-  int chunks, steps, tiles, CH;   // chunks of `steps` rows; tiles of CH channels to a group
+  int softplus, wide, vec, bcvec; // vec: rows of x, dt, gate, y and their gradients in fours, twos or ones; bcvec: B and C in fours
+  int chunks, steps, tiles;       // chunks of `steps` rows; tiles of channels to a group
   const void *x, *dt, *Bm, *Cm, *gate;
   const float *A, *D, *bias, *h0;
   const void* lengths;
@@ -58,93 +57,175 @@ __device__ __forceinline__ float sel_exp2(float v) {
   return r;
 }
 
-// Sum of v[0..NV) over the lanes that differ in the bits FIRST, 2 FIRST, .. < LAST of the lane: at
-// each exchange a lane keeps half of the values.  Afterwards v[0 .. max(1, NV / lanes)) hold the
-// sums of the values from sel_owner on.
-template <int FIRST, int LAST, int NV>
-__device__ __forceinline__ void sel_sum(float* v, int lane) {
-  if constexpr (FIRST < LAST) {
-    if constexpr (NV > 1) {
-      constexpr int H = NV / 2;
-      const bool up = lane & FIRST;
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        const float keep = up ? v[i + H] : v[i], give = up ? v[i] : v[i + H];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, FIRST);
-      }
-      sel_sum<2 * FIRST, LAST, H>(v, lane);
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], FIRST);
-      sel_sum<2 * FIRST, LAST, 1>(v, lane);
-    }
-  }
+// Two floats in one register pair: sm_100 multiplies and adds them in one issue slot.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-template <int FIRST, int LAST, int NV>
-__device__ __forceinline__ int sel_owner(int lane) {
-  if constexpr (FIRST < LAST && NV > 1) return (lane & FIRST ? NV / 2 : 0) + sel_owner<2 * FIRST, LAST, NV / 2>(lane);
-  return 0;
+__device__ __forceinline__ void split(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
-// the first of the lanes that hold the same sums
-template <int FIRST, int LAST, int NV>
-__device__ __forceinline__ bool sel_first(int lane) {
-  if constexpr (FIRST < LAST) {
-    if constexpr (NV > 1) return sel_first<2 * FIRST, LAST, NV / 2>(lane);
-    else return !(lane & FIRST) && sel_first<2 * FIRST, LAST, 1>(lane);
-  }
-  return true;
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 exp22(f2 v) {
+  float a, b;
+  split(v, a, b);
+  return pair(sel_exp2(a), sel_exp2(b));
+}
+__device__ __forceinline__ float sel_rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-// delta and its derivative by dt
+// delta and its derivative by dt.  softplus(z) = max(z, 0) + log1p(t), t = exp(-|z|), with log1p(t) =
+// 2 artanh(s), s = t / (2 + t) <= 1/3, by its series up to s^15 (what is left out is below 2^-28 of it).
+template <bool GRAD>
 __device__ __forceinline__ float sel_delta(float z, int softplus, float& d) {
   if (!softplus) {
     d = 1.f;
     return z;
   }
-  const float t = expf(-fabsf(z)), r = 1.f / (1.f + t);
-  d = z >= 0.f ? r : t * r;
-  return fmaxf(z, 0.f) + log1pf(t);
+  const float t = sel_exp2(fabsf(z) * -kLog2e), s = t * sel_rcp(2.f + t), q = s * s;
+  if (GRAD) {
+    const float r = sel_rcp(1.f + t);
+    d = z >= 0.f ? r : t * r;
+  }
+  float p = fmaf(q, 1.f / 15, 1.f / 13);
+  p = fmaf(q, p, 1.f / 11);
+  p = fmaf(q, p, 1.f / 9);
+  p = fmaf(q, p, 1.f / 7);
+  p = fmaf(q, p, 1.f / 5);
+  p = fmaf(q, p, 1.f / 3);
+  const float s2 = s + s;
+  return fmaxf(z, 0.f) + fmaf(s2 * q, p, s2);
 }
 
-template <class T>
-__device__ __forceinline__ void sel_load4(const void* base, long long at, bool vec, int left, float* v) {
-  const T* p = (const T*)base + at;
-  if (vec && left >= 4) {
-    unpack_vec<T, 4>(*(const VecOf<T, 4>*)p, v);
+// W elements of the element type as they lie in memory, in whole registers: a load on its way is not
+// touched before it is needed
+template <class T, int W>
+struct RawOf {
+  uint32_t w[W * sizeof(T) / 4];
+};
+// how: 2 all W at once, 1 in pairs (an even number of them is there), 0 one by one
+template <class T, int W>
+__device__ __forceinline__ void sel_load(RawOf<T, W>& r, const T* p, int how, int left) {
+  if (how == 2) {
+    constexpr int B = W * sizeof(T);
+    if constexpr (B == 16) {
+      const uint4 v = *(const uint4*)p;
+      r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+    } else if constexpr (B == 8) {
+      const uint2 v = *(const uint2*)p;
+      r.w[0] = v.x; r.w[1] = v.y;
+    } else {
+      r.w[0] = *(const uint32_t*)p;
+    }
+  } else if (how == 1) {
+#pragma unroll
+    for (int i = 0; i < W; i += 2) {
+      if constexpr (sizeof(T) == 4) {
+        const uint2 v = i < left ? *(const uint2*)(p + i) : make_uint2(0u, 0u);
+        r.w[i] = v.x; r.w[i + 1] = v.y;
+      } else {
+        r.w[i / 2] = i < left ? *(const uint32_t*)(p + i) : 0u;
+      }
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < left ? to_f(p[i]) : 0.f;
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        r.w[i] = i < left ? ((const uint32_t*)p)[i] : 0u;
+      } else {
+        const uint32_t v = i < left ? ((const unsigned short*)p)[i] : 0u;
+        r.w[i / 2] = i & 1 ? r.w[i / 2] | v << 16 : v;
+      }
+    }
   }
 }
-template <class T>
-__device__ __forceinline__ void sel_store4(void* base, long long at, bool vec, int left, const float* v) {
-  T* p = (T*)base + at;
-  if (vec && left >= 4) {
-    *(VecOf<T, 4>*)p = pack_vec<T, 4>(v);
+template <class T, int W>
+__device__ __forceinline__ void sel_floats(const RawOf<T, W>& r, float* v) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(r.w[i]);
+    else if constexpr (std::is_same_v<T, __half>) v[i] = __half2float(__ushort_as_half((unsigned short)(r.w[i / 2] >> 16 * (i & 1))));
+    else v[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+  }
+}
+template <class T, int W>
+__device__ __forceinline__ void sel_store(T* p, int how, int left, const float* v) {
+  if (how == 2) {
+    *(VecOf<T, W>*)p = pack_vec<T, W>(v);
+  } else if (how == 1) {
+#pragma unroll
+    for (int i = 0; i < W; i += 2)
+      if (i < left) *(VecOf<T, 2>*)(p + i) = pack_vec<T, 2>(v + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < W; ++i)
       if (i < left) p[i] = from_f<T>(v[i]);
   }
 }
 __device__ __forceinline__ float4 f4(const float* v) { return make_float4(v[0], v[1], v[2], v[3]); }
+// v[i] <- v[i ^ x]
+__device__ __forceinline__ void swap4(float* v, int x) {
+  const float a = x & 2 ? v[2] : v[0], b = x & 2 ? v[3] : v[1], c = x & 2 ? v[0] : v[2], d = x & 2 ? v[1] : v[3];
+  v[0] = x & 1 ? b : a;
+  v[1] = x & 1 ? a : b;
+  v[2] = x & 1 ? d : c;
+  v[3] = x & 1 ? c : d;
+}
+
+constexpr int kSelThreads = 128, kSelWarps = kSelThreads / 32;
 
 // Where a thread stands: grid (chunk, b, group, tile), tile fastest.
-template <class T, int L>
+//
+// A thread holds a pair of channels (f2) and four states.  Its channel c is cl + (c ^ cx), its state s
+// is 4 sg + (s ^ sx), where cx and sx come from its lane: lanes that exchange halves of their sums then
+// keep the same registers and give the same ones away, and nothing has to be selected.  Swapped pairs
+// are laid out as a second copy in shared memory.
+//
+// A warp lays out (and writes back) its own channels, W to a lane; the block shares B and C.
+template <class T, int L, bool BWD>
 struct SelThread {
+  static constexpr int CG = 32 / L;            // pairs of channels in a warp
+  static constexpr int CW = 2 * CG;            // channels of a warp
+  static constexpr int CH = kSelWarps * CW;    // channels of a block
   static constexpr int SP = 4 * L;             // padded states
-  static constexpr int ROWS = L;               // rows that a block stages at once (threads / (CH / 4))
+  static constexpr int W = CW < 4 ? 2 : 4;     // channels that a lane lays out
+  static constexpr int Q = CW / W;             // lanes to a row
+  static constexpr int ROWS = 32 / Q;          // rows that a warp lays out at once
   static constexpr int NI = ROWS >= kSelSeg ? 1 : kSelSeg / ROWS;
+  static constexpr int CC = L >= 2 ? 2 : 1;    // copies of the channels' arrays
+  static constexpr int SC = BWD && CG >= 4 ? 2 : 1;   // copies of B and C
+  static constexpr int CO = kSelSeg * CW + (CW < 32 ? CW : 0);   // where the second copy starts: in other banks
+  static constexpr int AR = CC > 1 ? CO + kSelSeg * CW : kSelSeg * CW;   // a warp's array, in floats
+  static constexpr int BO = kSelSeg * SP + (SP < 32 ? SP : 0);
+  static constexpr int BC = SC > 1 ? BO + kSelSeg * SP : kSelSeg * SP;   // B or C, in floats
+  using Raw = RawOf<T, W>;
   const SelArgs& p;
-  int tid, lane, warp, sg, cl;                 // state group, first of the thread's channels in the tile
-  int tile, g, b, chunk, n0, nn;               // first channel of the tile, channels of the tile there are
+  int tid, lane, warp, sg, cl, cx, sx;
+  int tile, g, b, chunk, n0, nn;               // first channel of the warp, channels of the warp there are
   int t0, t1, len;                             // the chunk's rows; rows of the sequence
-  int col, row, left;                          // staging: columns 4 col .. of rows row, row + ROWS, ..
+  int col, row, left;                          // laying out: channels from col on of rows row, row + ROWS, ..
+  int how;                                     // see sel_load
   __device__ __forceinline__ SelThread(const SelArgs& p_) : p(p_) {
     tid = threadIdx.x;
     lane = tid & 31;
     warp = tid >> 5;
     sg = lane % L;
-    cl = (warp * (32 / L) + lane / L) * 4;
+    const int cg = lane / L;
+    cl = cg * 2;
+    cx = L >= 2 && sg & 1;
+    sx = BWD ? (CG >= 2 && cg & 1 ? 2 : 0) | (CG >= 4 && cg & 2 ? 1 : 0) : 0;
     long long i = blockIdx.x;
     tile = (int)(i % p.tiles);
     i /= p.tiles;
@@ -152,465 +233,720 @@ struct SelThread {
     i /= p.G;
     b = (int)(i % p.B);
     chunk = (int)(i / p.B);
-    n0 = g * p.Dg + tile * p.CH;
-    nn = min(p.CH, p.Dg - tile * p.CH);
+    const int c0 = tile * CH + warp * CW;
+    n0 = g * p.Dg + c0;
+    nn = max(0, min(CW, p.Dg - c0));
     t0 = chunk * p.steps;
     t1 = min(p.T, t0 + p.steps);
     len = row_length(p.lengths, p.wide, b, p.T);
-    const int cv = p.CH / 4;
-    col = tid % cv;
-    row = tid / cv;
-    left = max(0, min(4, nn - 4 * col));
+    col = lane % Q * W;
+    row = lane / Q;
+    left = max(0, min(W, nn - col));
+    how = p.vec == 4 && left == W ? 2 : p.vec >= 2;
   }
-  // element (channel c, state s) of the thread: is it there, and where in (.., N, S)
-  __device__ __forceinline__ bool there(int c, int s) const { return cl + c < nn && 4 * sg + s < p.S; }
-  __device__ __forceinline__ size_t at(int c, int s) const { return (size_t)(n0 + cl + c) * p.S + 4 * sg + s; }
-  __device__ __forceinline__ void load_state(const float* base, size_t lead, float (*h)[4]) const {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) h[c][s] = base && there(c, s) ? base[lead * p.N * p.S + at(c, s)] : 0.f;
+  // the thread's place in its row of the segment at t of a tensor (T,B,N)
+  template <class E>
+  __device__ __forceinline__ E* at(E* base, int t, long long st, long long sb) const {
+    return base + (t + row) * st + b * sb + n0 + col;
   }
-  __device__ __forceinline__ void store_state(float* base, size_t lead, const float (*h)[4]) const {
-    const bool four = p.S % 4 == 0;
+  // .. of B or C; the segment's rows are e / L of the thread's quads
+  __device__ __forceinline__ const T* bc_at(const void* base, int t, long long st, long long sb) const {
+    return (const T*)base + (t + tid / L) * st + b * sb + (long long)g * p.S + tid % L * 4;
+  }
+  // (.., N, S): register order.  One channel's four states are neighbours in memory; q points at
+  // those of the thread's pair in their order there, and moves on by whole (B,N,S).
+  __device__ __forceinline__ float* states_at(const float* base, size_t lead) const {
+    return const_cast<float*>(base) + (lead * p.N + n0 + cl) * p.S + 4 * sg;
+  }
+  __device__ __forceinline__ void read_states(const float* q, bool four, f2* h) const {
+    float v[2][4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) v[c][s] = 0.f;
       if (four) {
-        if (there(c, 0)) *(float4*)(base + lead * p.N * p.S + at(c, 0)) = f4(h[c]);
+        if (cl + c < nn && 4 * sg < p.S) *(float4*)v[c] = *(const float4*)(q + c * p.S);
       } else {
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-          if (there(c, s)) base[lead * p.N * p.S + at(c, s)] = h[c][s];
+          if (cl + c < nn && 4 * sg + s < p.S) v[c][s] = q[c * p.S + s];
+      }
+      if (BWD) swap4(v[c], sx);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) h[s] = pair(cx ? v[1][s] : v[0][s], cx ? v[0][s] : v[1][s]);
+  }
+  __device__ __forceinline__ void write_states(float* q, bool four, const f2* h) const {
+    float v[2][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float a, b;
+      split(h[s], a, b);
+      v[0][s] = cx ? b : a;
+      v[1][s] = cx ? a : b;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (BWD) swap4(v[c], sx);
+      if (four) {
+        if (cl + c < nn && 4 * sg < p.S) *(float4*)(q + c * p.S) = f4(v[c]);
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          if (cl + c < nn && 4 * sg + s < p.S) q[c * p.S + s] = v[c][s];
       }
     }
   }
-  __device__ __forceinline__ void load_decay(float (*A2)[4]) const {
+  __device__ __forceinline__ void load_state(const float* base, size_t lead, f2* h) const {
+    if (base) {
+      read_states(states_at(base, lead), p.S % 4 == 0 && !((uintptr_t)base & 15), h);
+    } else {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) A2[c][s] = there(c, s) ? p.A[at(c, s)] * kLog2e : 0.f;
-  }
-  // rows of B or C of a segment, 0 past the sequence's end and past S
-  __device__ __forceinline__ void stage_bc(const void* base, long long st, long long sb, int seg, float* dst) const {
-    for (int e = tid; e < kSelSeg * SP; e += blockDim.x) {
-      const int t = seg + e / SP, s = e % SP;
-      dst[e] = t < len && s < p.S ? to_f(((const T*)base)[t * st + b * sb + (long long)g * p.S + s]) : 0.f;
+      for (int s = 0; s < 4; ++s) h[s] = 0;
     }
   }
-  __device__ __forceinline__ void load_bias(float* v) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = p.bias && i < left ? p.bias[n0 + 4 * col + i] : 0.f;
+  __device__ __forceinline__ void store_state(float* base, size_t lead, const f2* h) const {
+    write_states(states_at(base, lead), p.S % 4 == 0, h);
   }
-  // a segment's dt: delta (0 past the end, which leaves a state as it is) and its derivative
-  __device__ __forceinline__ void delta4(const float* z, const float* bias, bool on, float* d, float* sig) const {
+  __device__ __forceinline__ void load_decay(f2* A2) const {
+    load_state(p.A, 0, A2);
+    const f2 k = pair(kLog2e, kLog2e);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      d[i] = sig[i] = 0.f;
-      if (on && i < left) d[i] = sel_delta(z[i] + bias[i], p.softplus, sig[i]);
+    for (int s = 0; s < 4; ++s) A2[s] = mul2(A2[s], k);
+  }
+  __device__ __forceinline__ void load_weights(const float* w, float* v) const {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = w && i < left ? w[n0 + col + i] : 0.f;
+  }
+  // rows of B or C of a segment, 0 past the sequence's end and past S; a second copy with neighbours
+  // swapped
+  static constexpr int BCN = (kSelSeg * L + kSelThreads - 1) / kSelThreads;
+  __device__ __forceinline__ void load_bc(const T* q, long long st, int seg, RawOf<T, 4>* v) const {
+    constexpr int step = kSelThreads / L;
+    const int n = p.S - tid % L * 4;
+#pragma unroll
+    for (int k = 0; k < BCN; ++k) {
+      const int r = tid / L + k * step;
+#pragma unroll
+      for (unsigned i = 0; i < sizeof(v[k].w) / 4; ++i) v[k].w[i] = 0;
+      if (n > 0 && r < kSelSeg && seg + r < len) sel_load<T, 4>(v[k], q + k * step * st, p.bcvec && n >= 4 ? 2 : 0, n);
     }
+  }
+  __device__ __forceinline__ void put_bc(const RawOf<T, 4>* v, float* dst) const {
+#pragma unroll
+    for (int k = 0; k < BCN; ++k) {
+      const int e = tid + k * kSelThreads;
+      if (e < kSelSeg * L) {
+        float f[4];
+        sel_floats<T, 4>(v[k], f);
+        *(float4*)(dst + 4 * e) = f4(f);
+        if (SC > 1) *(float4*)(dst + BO + 4 * e) = make_float4(f[1], f[0], f[3], f[2]);
+      }
+    }
+  }
+  __device__ __forceinline__ void get_bc(const float* src, int r, f2* v) const {
+    const float* q = src + (SC > 1 && sx & 1 ? BO : 0) + r * SP + 4 * sg;
+    float2 lo, hi;
+    if (SC > 1) {
+      lo = *(const float2*)(q + (sx & 2));
+      hi = *(const float2*)(q + ((sx & 2) ^ 2));
+    } else {
+      const float4 f = *(const float4*)q;
+      const bool up = BWD && sx & 2;
+      lo = up ? make_float2(f.z, f.w) : make_float2(f.x, f.y);
+      hi = up ? make_float2(f.x, f.y) : make_float2(f.z, f.w);
+    }
+    v[0] = pair(lo.x, lo.x); v[1] = pair(lo.y, lo.y); v[2] = pair(hi.x, hi.x); v[3] = pair(hi.y, hi.y);
+  }
+  // W channels of a row, and a copy with their pairs swapped
+  __device__ __forceinline__ void put(float* dst, int r, const float* v) const {
+    float* q = dst + r * CW + col;
+    if constexpr (W == 4) {
+      *(float4*)q = f4(v);
+      if (CC > 1) *(float4*)(q + CO) = make_float4(v[1], v[0], v[3], v[2]);
+    } else {
+      *(float2*)q = make_float2(v[0], v[1]);
+      if (CC > 1) *(float2*)(q + CO) = make_float2(v[1], v[0]);
+    }
+  }
+  __device__ __forceinline__ void get(const float* src, int r, float* v) const {
+    const float* q = src + r * CW + col;
+    if constexpr (W == 4) *(float4*)v = *(const float4*)q;
+    else *(float2*)v = *(const float2*)q;
+  }
+  __device__ __forceinline__ f2 get2(const float* src, int r) const {
+    return *(const f2*)(src + (CC > 1 && cx ? CO : 0) + r * CW + cl);
+  }
+  // A pair's sums over the L lanes of its channels: afterwards v[0 .. NV) hold those of channels cl + cx, ..
+  static constexpr int NV = L >= 2 ? 1 : 2;
+  __device__ __forceinline__ void sum_states(f2 o, float* v) const {
+    constexpr unsigned all = 0xffffffffu;
+    split(o, v[0], v[1]);
+    if (L >= 2) v[0] += __shfl_xor_sync(all, v[1], 1);
+#pragma unroll
+    for (int k = 2; k < L; k *= 2) v[0] += __shfl_xor_sync(all, v[0], k);
+  }
+  __device__ __forceinline__ bool owns() const { return L <= 2 || sg < 2; }
+  // writes the sums to their channels of row r
+  __device__ __forceinline__ void put_sums(float* dst, int r, const float* v) const {
+    float* q = dst + r * CW + cl + cx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) q[i] = v[i];
+  }
+  // resets of a segment: bit r
+  __device__ __forceinline__ uint32_t cuts(int seg, int end) const {
+    return p.resets ? __ballot_sync(0xffffffffu, lane < kSelSeg && seg + lane < end && p.resets[(size_t)(seg + lane) * p.B + b]) : 0u;
   }
 };
 
-__host__ __device__ constexpr int sel_fwd_smem(int L, int CH) { return (3 * kSelSeg * CH + 2 * kSelSeg * 4 * L) * 4; }
-
-// LOCAL: the chunk's map only (from a zero state), without C, the gate and y
 template <class T, int L, bool LOCAL>
-__global__ void __launch_bounds__(128) k_sel_fwd(const SelArgs p) {
-  using Th = SelThread<T, L>;
-  constexpr int SP = Th::SP, ROWS = Th::ROWS, NI = Th::NI;
+constexpr int sel_fwd_smem() {
+  using Th = SelThread<T, L, false>;
+  return kSelWarps * (2 * Th::AR + kSelSeg * Th::CW) * 4 + 4 * Th::BC * 4;
+}
+
+// LOCAL: the chunk's map only (from a zero state), without C, the gate and y.  A segment's inputs
+// are on their way while the one before is worked on; B and C have two places, so that the block
+// meets once a segment.
+template <class T, int L, bool LOCAL>
+__global__ void __launch_bounds__(kSelThreads, L >= 4 ? 5 : 3) k_sel_fwd(const SelArgs p) {
+  using Th = SelThread<T, L, false>;
+  constexpr int ROWS = Th::ROWS, NI = Th::NI, W = Th::W;
   extern __shared__ float4 sm4[];
-  __shared__ uint8_t s_cut[kSelSeg];
-  Th th(p);
-  const int CH = p.CH;
-  float* s_d = (float*)sm4;
-  float* s_x = s_d + kSelSeg * CH;
-  float* s_g = s_x + kSelSeg * CH;
-  float* s_B = s_g + kSelSeg * CH;
-  float* s_C = s_B + kSelSeg * SP;
-  const int end = min(th.t1, th.len), n = th.n0 + 4 * th.col;
-  const size_t BN = (size_t)p.chunks * p.B;
-  float A2[4][4], h[4][4], bias[4], Dv[4], sumd[4] = {};
+  const Th th(p);
+  float* s_bc = (float*)sm4;                                          // [2][B, C]
+  float* s_d = s_bc + 4 * Th::BC + th.warp * (2 * Th::AR + kSelSeg * Th::CW);
+  float* s_x = s_d + Th::AR;
+  float* s_o = s_x + Th::AR;
+  const int end = min(th.t1, th.len);
+  f2 A2[4], h[4], sumd = 0;
+  float bias[W], Dv[W];
   bool any_cut = false;
   th.load_decay(A2);
-  th.load_bias(bias);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) Dv[i] = p.D && th.cl + i < th.nn ? p.D[th.n0 + th.cl + i] : 0.f;
+  th.load_weights(p.bias, bias);
+  th.load_weights(p.D, Dv);
   if (LOCAL) th.load_state(nullptr, 0, h);
   else if (p.chunks > 1) th.load_state(p.loc, (size_t)th.chunk * p.B + th.b, h);
   else th.load_state(p.h0, th.b, h);
 
-  for (int seg = th.t0; seg < end; seg += kSelSeg) {
-    float x[NI][4], z[NI][4], u[NI][4];
+  // pointers that move on with the segments
+  const bool gate = !LOCAL && p.gate;
+  const T *px = th.at((const T*)p.x, th.t0, p.x_t, p.x_b), *pz = th.at((const T*)p.dt, th.t0, p.dt_t, p.dt_b),
+          *pu = gate ? th.at((const T*)p.gate, th.t0, p.u_t, p.u_b) : nullptr;
+  const T *pB = th.bc_at(p.Bm, th.t0, p.bm_t, p.bm_b), *pC = th.bc_at(p.Cm, th.t0, p.cm_t, p.cm_b);
+  T* py = th.at((T*)p.y, th.t0, p.y_t, p.y_b);
+  float* pst = !LOCAL && p.states ? th.states_at(p.states, (size_t)(th.t0 / kSelSeg) * p.B + th.b) : nullptr;
+  const bool four = p.S % 4 == 0;
+  typename Th::Raw rx[NI], rz[NI], ru[NI], cu[NI];
+  RawOf<T, 4> rB[Th::BCN], rC[Th::BCN];
+  uint32_t rcut = 0;
+  const auto fetch = [&](int seg) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = th.row + i * ROWS, t = seg + r;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[i][k] = z[i][k] = u[i][k] = 0.f;
       if (r < kSelSeg && t < end) {
-        sel_load4<T>(p.x, t * p.x_t + th.b * p.x_b + n, p.vec, th.left, x[i]);
-        sel_load4<T>(p.dt, t * p.dt_t + th.b * p.dt_b + n, p.vec, th.left, z[i]);
-        if (!LOCAL && p.gate) sel_load4<T>(p.gate, t * p.u_t + th.b * p.u_b + n, p.vec, th.left, u[i]);
+        sel_load<T, W>(rx[i], px + i * ROWS * p.x_t, th.how, th.left);
+        sel_load<T, W>(rz[i], pz + i * ROWS * p.dt_t, th.how, th.left);
+        if (gate) sel_load<T, W>(ru[i], pu + i * ROWS * p.u_t, th.how, th.left);
       }
     }
-    th.stage_bc(p.Bm, p.bm_t, p.bm_b, seg, s_B);
-    if (!LOCAL) th.stage_bc(p.Cm, p.cm_t, p.cm_b, seg, s_C);
-    if (th.tid < kSelSeg)
-      s_cut[th.tid] = p.resets && seg + th.tid < end ? p.resets[(size_t)(seg + th.tid) * p.B + th.b] : 0;
+    th.load_bc(pB, p.bm_t, seg, rB);
+    if (!LOCAL) th.load_bc(pC, p.cm_t, seg, rC);
+    rcut = th.cuts(seg, end);
+    px += kSelSeg * p.x_t;
+    pz += kSelSeg * p.dt_t;
+    if (gate) pu += kSelSeg * p.u_t;
+    pB += kSelSeg * p.bm_t;
+    pC += kSelSeg * p.cm_t;
+  };
+  if (th.t0 < end) fetch(th.t0);
+  int place = 0;
+  for (int seg = th.t0; seg < end; seg += kSelSeg, place ^= 1) {
+    const uint32_t cut = rcut;
+    float *s_B = s_bc + place * 2 * Th::BC, *s_C = s_B + Th::BC;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = th.row + i * ROWS;
-      if (r < kSelSeg) {
-        float d[4], sig[4];
-        th.delta4(z[i], bias, seg + r < end, d, sig);
-        *(float4*)(s_d + r * CH + 4 * th.col) = f4(d);
-        *(float4*)(s_x + r * CH + 4 * th.col) = f4(x[i]);
-        if (!LOCAL) {
+      if (r < kSelSeg) {   // past the end: delta 0 leaves a state as it is
+        float x[W] = {}, d[W] = {}, z[W], sig;
+        if (seg + r < end) {
+          sel_floats<T, W>(rx[i], x);
+          sel_floats<T, W>(rz[i], z);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float sg, so;
-            sigmoid_pair<Accurate<T>::value>(u[i][k], sg, so);
-            u[i][k] = p.gate ? u[i][k] * sg : 1.f;
-          }
-          *(float4*)(s_g + r * CH + 4 * th.col) = f4(u[i]);
+          for (int k = 0; k < W; ++k) d[k] = k < th.left ? sel_delta<false>(z[k] + bias[k], p.softplus, sig) : 0.f;
         }
+        th.put(s_d, r, d);
+        th.put(s_x, r, x);
       }
+      cu[i] = ru[i];
     }
+    th.put_bc(rB, s_B);
+    if (!LOCAL) th.put_bc(rC, s_C);
     __syncthreads();
-    if (!LOCAL && p.states) th.store_state(p.states, (size_t)(seg / kSelSeg) * p.B + th.b, h);
-#pragma unroll 2
-    for (int r = 0; r < kSelSeg; ++r) {
-      if (s_cut[r]) {
-        any_cut = true;
+    if (seg + kSelSeg < end) fetch(seg + kSelSeg);
+    if (pst) {
+      th.write_states(pst, four, h);
+      pst += (size_t)p.B * p.N * p.S;
+    }
+    any_cut |= cut != 0;
+    const auto step = [&](int r) {
+      f2 Bv[4], Cv[4];
+      const f2 d = th.get2(s_d, r), dx = mul2(d, th.get2(s_x, r));
+      th.get_bc(s_B, r, Bv);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int s = 0; s < 4; ++s) h[c][s] = 0.f;
-      }
-      const float4 d4 = *(const float4*)(s_d + r * CH + th.cl), x4 = *(const float4*)(s_x + r * CH + th.cl);
-      const float4 B4 = *(const float4*)(s_B + r * SP + 4 * th.sg);
-      const float d[4] = {d4.x, d4.y, d4.z, d4.w}, dx[4] = {d4.x * x4.x, d4.y * x4.y, d4.z * x4.z, d4.w * x4.w};
-      const float Bv[4] = {B4.x, B4.y, B4.z, B4.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) h[c][s] = fmaf(sel_exp2(d[c] * A2[c][s]), h[c][s], dx[c] * Bv[s]);
+      for (int s = 0; s < 4; ++s) h[s] = fma2(exp22(mul2(d, A2[s])), h[s], mul2(dx, Bv[s]));
       if (LOCAL) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) sumd[c] += d[c];
+        sumd = fma2(d, pair(1.f, 1.f), sumd);
       } else {
-        const float4 C4 = *(const float4*)(s_C + r * SP + 4 * th.sg);
-        const float Cv[4] = {C4.x, C4.y, C4.z, C4.w};
-        float o[4];
+        th.get_bc(s_C, r, Cv);
+        f2 o2 = mul2(Cv[0], h[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          o[c] = Cv[0] * h[c][0];
+        for (int s = 1; s < 4; ++s) o2 = fma2(Cv[s], h[s], o2);
+        float o[2];
+        th.sum_states(o2, o);
+        if (th.owns()) th.put_sums(s_o, r, o);
+      }
+    };
+    if (!cut) {            // steps without a branch between them
 #pragma unroll
-          for (int s = 1; s < 4; ++s) o[c] = fmaf(Cv[s], h[c][s], o[c]);
-          if (th.sg == 0) o[c] = fmaf(Dv[c], c == 0 ? x4.x : c == 1 ? x4.y : c == 2 ? x4.z : x4.w, o[c]);
+      for (int r = 0; r < kSelSeg; ++r) step(r);
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < kSelSeg; ++r) {
+        if (cut >> r & 1) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) h[s] = 0;
         }
-        sel_sum<1, L, 4>(o, th.lane);
-        if (sel_first<1, L, 4>(th.lane)) {
-          constexpr int NV = L >= 4 ? 1 : 4 / L;
-          float* q = s_g + r * CH + th.cl + sel_owner<1, L, 4>(th.lane);
-#pragma unroll
-          for (int i = 0; i < NV; ++i) q[i] *= o[i];
-        }
+        step(r);
       }
     }
-    __syncthreads();
+    __syncwarp();
     if (!LOCAL) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int r = th.row + i * ROWS, t = seg + r;
         if (r < kSelSeg && t < end) {
-          const float4 v = *(const float4*)(s_g + r * CH + 4 * th.col);
-          const float o[4] = {v.x, v.y, v.z, v.w};
-          sel_store4<T>(p.y, t * p.y_t + th.b * p.y_b + n, p.vec, th.left, o);
+          float o[W], x[W];
+          th.get(s_o, r, o);
+          th.get(s_x, r, x);
+#pragma unroll
+          for (int k = 0; k < W; ++k) o[k] = fmaf(Dv[k], x[k], o[k]);
+          if (gate) {
+            float u[W], sg, so;
+            sel_floats<T, W>(cu[i], u);
+#pragma unroll
+            for (int k = 0; k < W; ++k) {
+              sigmoid_pair<false>(u[k], sg, so);
+              o[k] *= u[k] * sg;
+            }
+          }
+          sel_store<T, W>(py + i * ROWS * p.y_t, th.how, th.left, o);
         }
       }
-      __syncthreads();
+      py += kSelSeg * p.y_t;
+      __syncwarp();
     }
   }
   if (LOCAL) {
     const size_t lead = (size_t)th.chunk * p.B + th.b;
     th.store_state(p.loc, lead, h);
-    if (th.sg == 0)
+    if (th.sg == 0) {   // cx = 0
+      float s[2];
+      split(sumd, s[0], s[1]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (th.cl + c < th.nn) p.sumd[lead * p.N + th.n0 + th.cl + c] = sumd[c];
+      for (int c = 0; c < 2; ++c)
+        if (th.cl + c < th.nn) p.sumd[lead * p.N + th.n0 + th.cl + c] = s[c];
+    }
     if (th.tid == 0 && th.tile == 0 && th.g == 0) p.cut[lead] = any_cut;
     return;
   }
-  const float zero[4] = {};
-  for (int t = max(th.t0, end) + th.row; t < th.t1; t += ROWS)
-    sel_store4<T>(p.y, t * p.y_t + th.b * p.y_b + n, p.vec, th.left, zero);
+  const float zero[W] = {};
+  for (int t = max(th.t0, end) + th.row; t < th.t1; t += ROWS) sel_store<T, W>(th.at((T*)p.y, t - th.row, p.y_t, p.y_b), th.how, th.left, zero);
   if (th.chunk == max(th.len - 1, 0) / p.steps) th.store_state(p.hT, th.b, h);
 }
 
 // The states (BACK: the gradients of the states) in front of (behind) each chunk, in place of its
 // own share: one thread per (b, n, s), in time order.  start: h0 or ghT.
 template <bool BACK>
-__global__ void __launch_bounds__(256) k_sel_join(const SelArgs p, const float* __restrict__ start) {
+__global__ void __launch_bounds__(64) k_sel_join(const SelArgs p, const float* __restrict__ start) {
   const size_t row = (size_t)p.N * p.S, all = row * p.B;
   const size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
   if (i >= all) return;
   const int b = (int)(i / row);
-  const size_t ns = i % row, n = ns / p.S;
+  const size_t ns = i - b * row, n = ns / p.S;
   const float A2 = p.A[ns] * kLog2e;
   float h = start ? start[i] : 0.f;
-  constexpr int U = 8;
+  constexpr int U = 16;                 // chunks whose maps are on their way together
   for (int c0 = 0; c0 < p.chunks; c0 += U) {
-    float loc[U], a[U];
+    float loc[U], d[U];
+    uint8_t cut[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int c = BACK ? p.chunks - 1 - (c0 + k) : c0 + k;
-      loc[k] = a[k] = 0.f;
-      if (c0 + k < p.chunks) {
-        const size_t lead = (size_t)c * p.B + b;
-        loc[k] = p.loc[lead * row + ns];
-        a[k] = p.cut[lead] ? -1.f : sel_exp2(A2 * p.sumd[lead * p.N + n]);
-      }
+      const int c = c0 + k < p.chunks ? (BACK ? p.chunks - 1 - (c0 + k) : c0 + k) : 0;
+      const size_t lead = (size_t)c * p.B + b;
+      loc[k] = p.loc[lead * row + ns];
+      d[k] = p.sumd[lead * p.N + n];
+      cut[k] = p.cut[lead];
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int c = BACK ? p.chunks - 1 - (c0 + k) : c0 + k;
       if (c0 + k < p.chunks) {
         p.loc[((size_t)c * p.B + b) * row + ns] = h;
-        h = a[k] < 0.f ? loc[k] : fmaf(a[k], h, loc[k]);
+        h = cut[k] ? loc[k] : fmaf(sel_exp2(A2 * d[k]), h, loc[k]);
       }
     }
   }
 }
 
-__host__ __device__ constexpr int sel_bwd_smem(int L, int CH, int warps, bool local) {
-  return ((local ? 2 : 5) * kSelSeg * CH + 2 * kSelSeg * 4 * L) * 4 +
-         (local ? 0 : (warps * kSelSeg * 2 * 4 * L) * 4 + kSelSeg * 4 * warps * 32 * 16);
+// places of the channels' sums of dB and dC: two, so that the block meets once a segment, unless they are large
+template <int L>
+constexpr int sel_reds() { return L >= 16 ? 1 : 2; }
+template <class T, int L, bool LOCAL>
+constexpr int sel_bwd_smem() {
+  using Th = SelThread<T, L, true>;
+  return kSelWarps * (LOCAL ? 2 : 3) * Th::AR * 4 + (LOCAL ? 2 : 4) * Th::BC * 4 +
+         (LOCAL ? 0 : sel_reds<L>() * kSelWarps * kSelSeg * 2 * Th::SP * 4 + (kSelSeg - 1) * 32 * kSelThreads);
 }
 
 // LOCAL: the chunk's share of the states' gradients only (from a zero gradient behind it)
 template <class T, int L, bool LOCAL>
-__global__ void __launch_bounds__(64) k_sel_bwd(const SelArgs p) {
-  using Th = SelThread<T, L>;
-  constexpr int SP = Th::SP, ROWS = Th::ROWS, NI = Th::NI, CG = 32 / L;
+__global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_bwd(const SelArgs p) {
+  using Th = SelThread<T, L, true>;
+  constexpr int SP = Th::SP, ROWS = Th::ROWS, NI = Th::NI, W = Th::W, CG = Th::CG, AR = Th::AR, BC = Th::BC;
+  constexpr int nt = kSelThreads, REDS = sel_reds<L>(), RED = kSelWarps * kSelSeg * 2 * SP;
   extern __shared__ float4 sm4[];
-  __shared__ uint8_t s_cut[kSelSeg];
-  Th th(p);
-  const int CH = p.CH, nt = blockDim.x, W = nt / 32;
-  float4* hist = sm4;                                            // [kSelSeg][4][nt]: the state before each step
-  float* s_d = (float*)(LOCAL ? sm4 : sm4 + kSelSeg * 4 * nt);
-  float* s_go = s_d + kSelSeg * CH;                              // gy silu(gate); LOCAL: the last array
-  float* s_C = s_go + kSelSeg * CH;
-  float* s_B = s_C + kSelSeg * SP;
-  float* s_x = s_B + kSelSeg * SP;
-  float* s_ds = s_x + kSelSeg * CH;                              // gy silu'(gate)
-  float* s_sg = s_ds + kSelSeg * CH;                             // d delta / d dt
-  float* s_red = s_sg + kSelSeg * CH;                            // [W][kSelSeg][2 SP]
-  const int end = min(th.t1, th.len), n = th.n0 + 4 * th.col;
+  const Th th(p);
+  ulonglong2* hist = (ulonglong2*)sm4;                           // [1 .. kSelSeg)[2][nt]: the state before each step
+  float* s_bc = (float*)(LOCAL ? hist : hist + (kSelSeg - 1) * 2 * nt);   // [2][C, B]
+  float* s_red = s_bc + (LOCAL ? 2 : 4) * BC;          // [REDS][warp][kSelSeg][2 SP]
+  float* s_d = (LOCAL ? s_red : s_red + REDS * RED) + th.warp * (LOCAL ? 2 : 3) * AR;   // later the sums for ddt
+  float* s_go = s_d + AR;                                        // gy silu(gate); later sum C h
+  float* s_x = s_go + AR;                                        // later sum G B; not in a LOCAL pass
+  const int end = min(th.t1, th.len);
   const size_t lead = (size_t)th.chunk * p.B + th.b;
-  float A2[4][4], G[4][4], dA[4][4] = {}, bias[4], sumd[4] = {};
-  constexpr int NV = L >= 4 ? 1 : 4 / L;
-  const int own = sel_owner<1, L, 4>(th.lane);
-  const bool first = sel_first<1, L, 4>(th.lane);
-  float Do[NV], dDo[NV] = {}, dbo[NV] = {};
+  f2 A2[4], G[4], dA[4], sumd = 0;
+  float bias[W], Dv[W], dD[W] = {}, db[W] = {};
   bool any_cut = false;
   th.load_decay(A2);
-  th.load_bias(bias);
+  th.load_weights(p.bias, bias);
+  th.load_weights(p.D, Dv);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) Do[i] = p.D && th.cl + own + i < th.nn ? p.D[th.n0 + th.cl + own + i] : 0.f;
+  for (int s = 0; s < 4; ++s) dA[s] = 0;
   if (LOCAL) th.load_state(nullptr, 0, G);
   else if (p.chunks > 1) th.load_state(p.loc, lead, G);
   else th.load_state(p.ghT, th.b, G);
 
+  const int segs = end > th.t0 ? (end - th.t0 + kSelSeg - 1) / kSelSeg : 0;
+  // pointers that move back with the segments
+  const int tl = th.t0 + max(segs - 1, 0) * kSelSeg;
+  const bool gate = p.gate, grad = p.gy;
+  const T *px = th.at((const T*)p.x, tl, p.x_t, p.x_b), *pz = th.at((const T*)p.dt, tl, p.dt_t, p.dt_b),
+          *pu = th.at((const T*)p.gate, tl, p.u_t, p.u_b), *pg = th.at((const T*)p.gy, tl, p.gy_t, p.gy_b);
+  const T *pB = th.bc_at(p.Bm, tl, p.bm_t, p.bm_b), *pC = th.bc_at(p.Cm, tl, p.cm_t, p.cm_b);
+  T *pdx = th.at((T*)p.dx, tl, p.dx_t, p.dx_b), *pdz = th.at((T*)p.ddt, tl, p.ddt_t, p.ddt_b),
+    *pdu = th.at((T*)p.dgate, tl, p.du_t, p.du_b);
+  const float* pst = LOCAL ? nullptr : th.states_at(p.states, (size_t)(tl / kSelSeg) * p.B + th.b);
+  const bool four = p.S % 4 == 0 && !((uintptr_t)p.states & 15);
   if (!LOCAL) {   // rows past the end: zero gradients
-    const float zero[4] = {};
+    const float zero[W] = {};
     for (int t = max(th.t0, end) + th.row; t < th.t1; t += ROWS) {
-      if (p.dx) sel_store4<T>(p.dx, t * p.dx_t + th.b * p.dx_b + n, p.vec, th.left, zero);
-      if (p.ddt) sel_store4<T>(p.ddt, t * p.ddt_t + th.b * p.ddt_b + n, p.vec, th.left, zero);
-      if (p.dgate) sel_store4<T>(p.dgate, t * p.du_t + th.b * p.du_b + n, p.vec, th.left, zero);
+      if (p.dx) sel_store<T, W>(th.at((T*)p.dx, t - th.row, p.dx_t, p.dx_b), th.how, th.left, zero);
+      if (p.ddt) sel_store<T, W>(th.at((T*)p.ddt, t - th.row, p.ddt_t, p.ddt_b), th.how, th.left, zero);
+      if (p.dgate) sel_store<T, W>(th.at((T*)p.dgate, t - th.row, p.du_t, p.du_b), th.how, th.left, zero);
     }
   }
   // dB and dC of all rows of the chunk are written, zeros past the end
-  const auto write_bc = [&](int seg, int rows) {
-    for (int e = th.tid; e < rows * 2 * SP; e += nt) {
-      const int r = e / (2 * SP), q = e % (2 * SP), s = q % SP, t = seg + r;
-      if (s < p.S) {
+  const long long bc_t = (long long)p.B * p.G * p.S, bc_0 = ((long long)th.tile * p.T * p.B + th.b) * p.G * p.S + (long long)th.g * p.S;
+  const auto write_bc = [&](int seg, const float* red) {
+#pragma unroll
+    for (int e0 = 0; e0 < kSelSeg * 2 * SP; e0 += nt) {
+      const int e = e0 + th.tid, r = e / (2 * SP), q = e % (2 * SP), s = q % SP, t = seg + r;
+      if (e < kSelSeg * 2 * SP && s < p.S && t < th.t1) {
         float v = 0.f;
         if (t < end)
-          for (int w = 0; w < W; ++w) v += s_red[(w * kSelSeg + r) * 2 * SP + q];
+#pragma unroll
+          for (int w = 0; w < kSelWarps; ++w) v += red[w * kSelSeg * 2 * SP + e];
         float* dst = q < SP ? p.dB : p.dC;
-        if (dst) dst[((((size_t)th.tile * p.T + t) * p.B + th.b) * p.G + th.g) * p.S + s] = v;
+        if (dst) dst[bc_0 + t * bc_t + s] = v;
       }
     }
   };
-  const int segs = end > th.t0 ? (end - th.t0 + kSelSeg - 1) / kSelSeg : 0;
-  if (!LOCAL && (p.dB || p.dC))
-    for (int seg = th.t0 + segs * kSelSeg; seg < th.t1; seg += kSelSeg) write_bc(seg, min(kSelSeg, th.t1 - seg));
+  const bool bc = !LOCAL && (p.dB || p.dC);
+  if (bc)
+    for (int seg = th.t0 + segs * kSelSeg; seg < th.t1; seg += kSelSeg) write_bc(seg, s_red);
 
-  for (int k = segs - 1; k >= 0; --k) {
-    const int seg = th.t0 + k * kSelSeg;
+  typename Th::Raw rx[NI], rz[NI], ru[NI], rg[NI];
+  RawOf<T, 4> rB[Th::BCN], rC[Th::BCN];
+  uint32_t rcut = 0;
+  f2 h[4];
+  const auto fetch = [&](int seg) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = th.row + i * ROWS, t = seg + r;
-      if (r < kSelSeg) {
-        float x[4] = {}, z[4] = {}, u[4] = {}, g[4] = {}, d[4], sig[4], gs[4];
-        const bool on = t < end;
-        if (on) {
-          if (!LOCAL) sel_load4<T>(p.x, t * p.x_t + th.b * p.x_b + n, p.vec, th.left, x);
-          sel_load4<T>(p.dt, t * p.dt_t + th.b * p.dt_b + n, p.vec, th.left, z);
-          if (p.gate) sel_load4<T>(p.gate, t * p.u_t + th.b * p.u_b + n, p.vec, th.left, u);
-          if (p.gy) sel_load4<T>(p.gy, t * p.gy_t + th.b * p.gy_b + n, p.vec, th.left, g);
-        }
-        th.delta4(z, bias, on, d, sig);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float sg, so;
-          sigmoid_pair<Accurate<T>::value>(u[q], sg, so);
-          gs[q] = g[q] * (sg * (1.f + u[q] * so));
-          g[q] *= p.gate ? u[q] * sg : 1.f;
-        }
-        const int o = r * CH + 4 * th.col;
-        *(float4*)(s_d + o) = f4(d);
-        *(float4*)(s_go + o) = f4(g);
-        if (!LOCAL) {
-          *(float4*)(s_x + o) = f4(x);
-          *(float4*)(s_ds + o) = f4(gs);
-          *(float4*)(s_sg + o) = f4(sig);
-        }
+      if (r < kSelSeg && t < end) {
+        if (!LOCAL) sel_load<T, W>(rx[i], px + i * ROWS * p.x_t, th.how, th.left);
+        sel_load<T, W>(rz[i], pz + i * ROWS * p.dt_t, th.how, th.left);
+        if (gate) sel_load<T, W>(ru[i], pu + i * ROWS * p.u_t, th.how, th.left);
+        if (grad) sel_load<T, W>(rg[i], pg + i * ROWS * p.gy_t, th.how, th.left);
       }
     }
-    th.stage_bc(p.Cm, p.cm_t, p.cm_b, seg, s_C);
-    if (!LOCAL) th.stage_bc(p.Bm, p.bm_t, p.bm_b, seg, s_B);
-    if (th.tid < kSelSeg)
-      s_cut[th.tid] = p.resets && seg + th.tid < end ? p.resets[(size_t)(seg + th.tid) * p.B + th.b] : 0;
-    float h[4][4];
-    if (!LOCAL) th.load_state(p.states, (size_t)(seg / kSelSeg) * p.B + th.b, h);
-    __syncthreads();
+    th.load_bc(pC, p.cm_t, seg, rC);
     if (!LOCAL) {
-#pragma unroll 2
-      for (int r = 0; r < kSelSeg; ++r) {
+      th.load_bc(pB, p.bm_t, seg, rB);
+      th.read_states(pst, four, h);
+      px -= kSelSeg * p.x_t;
+      pB -= kSelSeg * p.bm_t;
+      pst -= (size_t)p.B * p.N * p.S;
+    }
+    rcut = th.cuts(seg, end);
+    pz -= kSelSeg * p.dt_t;
+    pu -= kSelSeg * p.u_t;
+    pg -= kSelSeg * p.gy_t;
+    pC -= kSelSeg * p.cm_t;
+  };
+  if (segs > 0) fetch(th.t0 + (segs - 1) * kSelSeg);
+  int place = 0;
+  for (int k = segs - 1; k >= 0; --k, place ^= 1) {
+    const int seg = th.t0 + k * kSelSeg;
+    const uint32_t cut = rcut;
+    float *s_C = s_bc + place * (LOCAL ? 1 : 2) * BC, *s_B = s_C + BC;
+    float* red = s_red + (REDS > 1 ? place * RED : 0);
+    float x[NI][W], d[NI][W], sig[NI][W], go[NI][W], gs[NI][W];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) hist[(r * 4 + c) * nt + th.tid] = f4(h[c]);
-        if (s_cut[r]) {
+    for (int i = 0; i < NI; ++i) {
+      const int r = th.row + i * ROWS;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+      for (int q = 0; q < W; ++q) x[i][q] = d[i][q] = sig[i][q] = go[i][q] = gs[i][q] = 0.f;
+      if (r < kSelSeg) {
+        if (seg + r < end) {
+          float z[W], u[W];
+          if (!LOCAL) sel_floats<T, W>(rx[i], x[i]);
+          sel_floats<T, W>(rz[i], z);
+          if (grad) sel_floats<T, W>(rg[i], go[i]);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) h[c][s] = 0.f;
+          for (int q = 0; q < W; ++q) d[i][q] = q < th.left ? sel_delta<!LOCAL>(z[q] + bias[q], p.softplus, sig[i][q]) : 0.f;
+          if (gate) {
+            sel_floats<T, W>(ru[i], u);
+#pragma unroll
+            for (int q = 0; q < W; ++q) {
+              float sg, so;
+              sigmoid_pair<false>(u[q], sg, so);
+              gs[i][q] = go[i][q] * (sg * fmaf(u[q], so, 1.f));
+              go[i][q] *= u[q] * sg;
+            }
+          }
         }
-        const float4 d4 = *(const float4*)(s_d + r * CH + th.cl), x4 = *(const float4*)(s_x + r * CH + th.cl);
-        const float4 B4 = *(const float4*)(s_B + r * SP + 4 * th.sg);
-        const float d[4] = {d4.x, d4.y, d4.z, d4.w}, dx[4] = {d4.x * x4.x, d4.y * x4.y, d4.z * x4.z, d4.w * x4.w};
-        const float Bv[4] = {B4.x, B4.y, B4.z, B4.w};
+        th.put(s_d, r, d[i]);
+        th.put(s_go, r, go[i]);
+        if (!LOCAL) th.put(s_x, r, x[i]);
+      }
+    }
+    th.put_bc(rC, s_C);
+    if (!LOCAL) th.put_bc(rB, s_B);
+    __syncthreads();
+    if (bc && k + 1 < segs) {
+      write_bc(seg + kSelSeg, s_red + (REDS > 1 ? (place ^ 1) * RED : 0));
+      if (REDS == 1) __syncthreads();
+    }
+    f2 first[4] = {};
+    if (!LOCAL) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+      for (int s = 0; s < 4; ++s) first[s] = h[s];
+      const auto step = [&](int r) {
+        f2 Bv[4];
+        const f2 dd = th.get2(s_d, r), dx = mul2(dd, th.get2(s_x, r));
+        th.get_bc(s_B, r, Bv);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) h[c][s] = fmaf(sel_exp2(d[c] * A2[c][s]), h[c][s], dx[c] * Bv[s]);
+        for (int s = 0; s < 4; ++s) h[s] = fma2(exp22(mul2(dd, A2[s])), h[s], mul2(dx, Bv[s]));
+        if (r + 1 < kSelSeg) {
+          hist[r * 2 * nt + th.tid] = make_ulonglong2(h[0], h[1]);
+          hist[(r * 2 + 1) * nt + th.tid] = make_ulonglong2(h[2], h[3]);
+        }
+      };
+      if (!cut) {          // steps without a branch between them
+#pragma unroll
+        for (int r = 0; r < kSelSeg; ++r) step(r);
+      } else {
+#pragma unroll 1
+        for (int r = 0; r < kSelSeg; ++r) {
+          if (cut >> r & 1) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) h[s] = 0;
+          }
+          step(r);
         }
       }
     }
-#pragma unroll 1
-    for (int r = kSelSeg - 1; r >= 0; --r) {
-      const float4 d4 = *(const float4*)(s_d + r * CH + th.cl), g4 = *(const float4*)(s_go + r * CH + th.cl);
-      const float4 C4 = *(const float4*)(s_C + r * SP + 4 * th.sg);
-      const float d[4] = {d4.x, d4.y, d4.z, d4.w}, go[4] = {g4.x, g4.y, g4.z, g4.w};
-      const float Cv[4] = {C4.x, C4.y, C4.z, C4.w};
-      const bool cut = s_cut[r];
-      if (LOCAL) {
+    any_cut |= cut != 0;
+    // one step back from pre, the state before it; nothing passes a reset, an infinite state neither
+    const auto back = [&](int r, const f2* pre, bool here) {
+      f2 Cv[4];
+      const f2 dd = th.get2(s_d, r), gg = th.get2(s_go, r);
+      th.get_bc(s_C, r, Cv);
+      if constexpr (LOCAL) {
+        sumd = fma2(dd, pair(1.f, 1.f), sumd);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          sumd[c] += d[c];
+        for (int s = 0; s < 4; ++s) G[s] = mul2(exp22(mul2(dd, A2[s])), fma2(Cv[s], gg, G[s]));
+        if (here) {
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-            G[c][s] = cut ? 0.f : sel_exp2(d[c] * A2[c][s]) * fmaf(Cv[s], go[c], G[c][s]);
+          for (int s = 0; s < 4; ++s) G[s] = 0;
         }
-        any_cut |= cut;
-        continue;
-      }
-      const float4 x4 = *(const float4*)(s_x + r * CH + th.cl);
-      const float4 B4 = *(const float4*)(s_B + r * SP + 4 * th.sg);
-      const float dx[4] = {d4.x * x4.x, d4.y * x4.y, d4.z * x4.z, d4.w * x4.w}, Bv[4] = {B4.x, B4.y, B4.z, B4.w};
-      float bc[8] = {}, gb[4], wa[4], o[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 q = hist[(r * 4 + c) * nt + th.tid];
-        const float pre[4] = {q.x, q.y, q.z, q.w};
-        gb[c] = wa[c] = o[c] = 0.f;
+      } else {
+        f2 Bv[4], ag[4], w[4], bB[4], bC[4], gb2, wa2, o2;
+        const f2 dx = mul2(dd, th.get2(s_x, r));
+        th.get_bc(s_B, r, Bv);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const float a = sel_exp2(d[c] * A2[c][s]);
-          const float Gt = fmaf(Cv[s], go[c], G[c][s]);
-          o[c] = fmaf(Cv[s], h[c][s], o[c]);
-          bc[4 + s] = fmaf(go[c], h[c][s], bc[4 + s]);
-          bc[s] = fmaf(Gt, dx[c], bc[s]);
-          gb[c] = fmaf(Gt, Bv[s], gb[c]);
-          // nothing passes a reset, an infinite state neither
-          const float ag = cut ? 0.f : a * Gt, w = cut ? 0.f : ag * pre[s];
-          wa[c] = fmaf(w, A2[c][s], wa[c]);
-          dA[c][s] = fmaf(w, d[c], dA[c][s]);
-          G[c][s] = ag;
-          h[c][s] = pre[s];
+          const f2 Gt = fma2(Cv[s], gg, G[s]);
+          o2 = s ? fma2(Cv[s], h[s], o2) : mul2(Cv[s], h[s]);
+          bC[s] = mul2(gg, h[s]);
+          bB[s] = mul2(Gt, dx);
+          gb2 = s ? fma2(Gt, Bv[s], gb2) : mul2(Gt, Bv[s]);
+          ag[s] = mul2(exp22(mul2(dd, A2[s])), Gt);
+          w[s] = mul2(ag[s], pre[s]);
+          h[s] = pre[s];
+        }
+        if (here) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) ag[s] = w[s] = 0;
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          wa2 = s ? fma2(w[s], A2[s], wa2) : mul2(w[s], A2[s]);
+          dA[s] = fma2(w[s], dd, dA[s]);
+          G[s] = ag[s];
+        }
+        float vB[4], vC[4], gb[2], wa[2], o[2];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          float a, b;
+          split(bB[s], a, b);
+          vB[s] = a + b;
+          split(bC[s], a, b);
+          vC[s] = a + b;
+        }
+        th.sum_states(gb2, gb);
+        th.sum_states(wa2, wa);
+        th.sum_states(o2, o);
+        __syncwarp();         // every lane has read its row
+        if (th.owns()) {
+          th.put_sums(s_x, r, gb);
+          th.put_sums(s_d, r, wa);
+          th.put_sums(s_go, r, o);
+        }
+        // over the channels: lanes L, 2 L, .. apart; at last one of two lanes keeps dB, the other dC
+        constexpr unsigned all = 0xffffffffu;
+        if (CG >= 2) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            vB[s] += __shfl_xor_sync(all, vB[s + 2], L);
+            vC[s] += __shfl_xor_sync(all, vC[s + 2], L);
+          }
+        }
+        if (CG >= 4) {
+          vB[0] += __shfl_xor_sync(all, vB[1], 2 * L);
+          vC[0] += __shfl_xor_sync(all, vC[1], 2 * L);
+        }
+        float* q = red + (th.warp * kSelSeg + r) * 2 * SP + 4 * th.sg + th.sx;
+        if constexpr (CG >= 8) {
+          const bool up = th.lane & (4 * L);
+          float v = (up ? vC[0] : vB[0]) + __shfl_xor_sync(all, up ? vB[0] : vC[0], 4 * L);
+#pragma unroll
+          for (int i = 8 * L; i < 32; i *= 2) v += __shfl_xor_sync(all, v, i);
+          if (th.lane < 8 * L) q[up ? SP : 0] = v;
+        } else {
+          constexpr int n = CG >= 4 ? 1 : CG >= 2 ? 2 : 4;
+#pragma unroll
+          for (int s = 0; s < n; ++s) {
+            q[s] = vB[s];
+            q[SP + s] = vC[s];
+          }
         }
       }
-      sel_sum<L, 32, 8>(bc, th.lane);
-      if (sel_first<L, 32, 8>(th.lane)) {
-        constexpr int NB = CG >= 8 ? 1 : 8 / CG;
-        const int j = sel_owner<L, 32, 8>(th.lane);   // values 0..3 are dB, 4..7 dC
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          s_red[(th.warp * kSelSeg + r) * 2 * SP + ((j + i) & 4 ? SP : 0) + 4 * th.sg + ((j + i) & 3)] = bc[i];
+    };
+    const auto before = [&](int r, f2* pre) {
+      if (!LOCAL) {
+        const ulonglong2 q0 = hist[(r - 1) * 2 * nt + th.tid], q1 = hist[(r * 2 - 1) * nt + th.tid];
+        pre[0] = q0.x; pre[1] = q0.y; pre[2] = q1.x; pre[3] = q1.y;
       }
-      sel_sum<1, L, 4>(gb, th.lane);
-      sel_sum<1, L, 4>(wa, th.lane);
-      sel_sum<1, L, 4>(o, th.lane);
-      __syncwarp();
-      if (first) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int e = r * CH + th.cl + own + i;
-          const float xx = s_x[e], gg = s_go[e];
-          const float ddt = fmaf(gb[i], xx, wa[i] * kLn2) * s_sg[e];
-          s_x[e] = fmaf(gb[i], s_d[e], Do[i] * gg);
-          s_d[e] = ddt;
-          s_ds[e] *= fmaf(Do[i], xx, o[i]);
-          dDo[i] = fmaf(gg, xx, dDo[i]);
-          dbo[i] += ddt;
-        }
+    };
+    f2 pre[4];
+    if (!cut) {
+#pragma unroll 7
+      for (int r = kSelSeg - 1; r > 0; --r) {
+        before(r, pre);
+        back(r, pre, false);
+      }
+    } else {
+#pragma unroll 1
+      for (int r = kSelSeg - 1; r > 0; --r) {
+        before(r, pre);
+        back(r, pre, cut >> r & 1);
       }
     }
-    __syncthreads();
+    back(0, first, cut & 1);
+    if (k > 0) fetch(seg - kSelSeg);
+    __syncwarp();
     if (!LOCAL) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int r = th.row + i * ROWS, t = seg + r;
         if (r < kSelSeg && t < end) {
-          const int e = r * CH + 4 * th.col;
-          if (p.dx) sel_store4<T>(p.dx, t * p.dx_t + th.b * p.dx_b + n, p.vec, th.left, s_x + e);
-          if (p.ddt) sel_store4<T>(p.ddt, t * p.ddt_t + th.b * p.ddt_b + n, p.vec, th.left, s_d + e);
-          if (p.dgate) sel_store4<T>(p.dgate, t * p.du_t + th.b * p.du_b + n, p.vec, th.left, s_ds + e);
+          float gb[W], wa[W], o[W], vx[W], vz[W], vu[W];
+          th.get(s_x, r, gb);
+          th.get(s_d, r, wa);
+          th.get(s_go, r, o);
+#pragma unroll
+          for (int q = 0; q < W; ++q) {
+            vx[q] = fmaf(gb[q], d[i][q], Dv[q] * go[i][q]);
+            vz[q] = fmaf(gb[q], x[i][q], wa[q] * kLn2) * sig[i][q];
+            vu[q] = gs[i][q] * fmaf(Dv[q], x[i][q], o[q]);
+            dD[q] = fmaf(go[i][q], x[i][q], dD[q]);
+            db[q] += vz[q];
+          }
+          if (p.dx) sel_store<T, W>(pdx + i * ROWS * p.dx_t, th.how, th.left, vx);
+          if (p.ddt) sel_store<T, W>(pdz + i * ROWS * p.ddt_t, th.how, th.left, vz);
+          if (p.dgate) sel_store<T, W>(pdu + i * ROWS * p.du_t, th.how, th.left, vu);
         }
       }
-      if (p.dB || p.dC) write_bc(seg, min(kSelSeg, th.t1 - seg));
-      __syncthreads();
+      pdx -= kSelSeg * p.dx_t;
+      pdz -= kSelSeg * p.ddt_t;
+      pdu -= kSelSeg * p.du_t;
+      __syncwarp();
     }
+  }
+  if (bc && segs > 0) {
+    __syncthreads();
+    write_bc(th.t0, s_red + (REDS > 1 ? (place ^ 1) * RED : 0));
   }
   if (LOCAL) {
     th.store_state(p.loc, lead, G);
-    if (th.sg == 0)
+    if (th.sg == 0) {
+      float s[2];
+      split(sumd, s[0], s[1]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (th.cl + c < th.nn) p.sumd[lead * p.N + th.n0 + th.cl + c] = sumd[c];
+      for (int c = 0; c < 2; ++c)
+        if (th.cl + c < th.nn) p.sumd[lead * p.N + th.n0 + th.cl + c] = s[c];
+    }
     if (th.tid == 0 && th.tile == 0 && th.g == 0) p.cut[lead] = any_cut;
     return;
   }
   if (p.dh0 && th.chunk == 0) th.store_state(p.dh0, th.b, G);
   if (p.dA) th.store_state(p.dA, lead, dA);
-  if (first) {
+  // dD and db: over the lanes that have laid out the same channels
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (th.cl + own + i < th.nn) {
-        const size_t e = lead * p.N + th.n0 + th.cl + own + i;
-        if (p.dD) p.dD[e] = dDo[i];
-        if (p.db) p.db[e] = dbo[i];
-      }
+  for (int q = 0; q < W; ++q) {
+#pragma unroll
+    for (int i = Th::Q; i < 32; i *= 2) {
+      dD[q] += __shfl_xor_sync(0xffffffffu, dD[q], i);
+      db[q] += __shfl_xor_sync(0xffffffffu, db[q], i);
+    }
+    if (th.row == 0 && q < th.left) {
+      const size_t e = lead * p.N + th.n0 + th.col + q;
+      if (p.dD) p.dD[e] = dD[q];
+      if (p.db) p.db[e] = db[q];
+    }
   }
 }
 
@@ -689,7 +1025,7 @@ __global__ void __launch_bounds__(256) k_sel_step(const SelStep p) {
     if (act) {
       float sig;
       x = to_f(((const T*)p.x)[b * p.x_b + n]);
-      const float d = sel_delta(to_f(((const T*)p.dt)[b * p.dt_b + n]) + (p.bias ? p.bias[n] : 0.f), p.softplus, sig);
+      const float d = sel_delta<false>(to_f(((const T*)p.dt)[b * p.dt_b + n]) + (p.bias ? p.bias[n] : 0.f), p.softplus, sig);
       const T* Bp = (const T*)p.Bm + b * p.bm_b + (long long)g * p.S + 4 * sg;
       const T* Cp = (const T*)p.Cm + b * p.cm_b + (long long)g * p.S + 4 * sg;
 #pragma unroll
@@ -716,7 +1052,7 @@ __global__ void __launch_bounds__(256) k_sel_step(const SelStep p) {
       if (p.gate) {
         float s, so;
         const float u = to_f(((const T*)p.gate)[b * p.u_b + n]);
-        sigmoid_pair<Accurate<T>::value>(u, s, so);
+        sigmoid_pair<false>(u, s, so);
         y *= u * s;
       }
     }

@@ -2,7 +2,7 @@
 #include "selective_launch.cuh"
 
 namespace delrec {
-int sel_run_backward(int dtype, int L, int warps, const SelArgs& p, cudaStream_t st) {
-  return by_dtype(dtype, [&](auto t) { return sel_by_l<decltype(t), true>(L, warps, p, st); });
+int sel_run_backward(int dtype, int L, const SelArgs& p, cudaStream_t st) {
+  return by_dtype(dtype, [&](auto t) { return sel_by_l<decltype(t), true>(L, p, st); });
 }
 }  // namespace delrec

@@ -6,43 +6,43 @@
 
 namespace delrec {
 
-int sel_run_forward(int dtype, int L, int warps, const SelArgs& p, cudaStream_t st);
-int sel_run_backward(int dtype, int L, int warps, const SelArgs& p, cudaStream_t st);
+int sel_run_forward(int dtype, int L, const SelArgs& p, cudaStream_t st);
+int sel_run_backward(int dtype, int L, const SelArgs& p, cudaStream_t st);
 
 template <class T, int L, bool BWD, bool LOCAL>
-static int sel_start(int warps, const SelArgs& p, cudaStream_t st) {
+static int sel_start(const SelArgs& p, cudaStream_t st) {
   const long long grid = (long long)p.tiles * p.G * p.B * p.chunks;
   if (grid > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   if constexpr (BWD) {
     auto kern = k_sel_bwd<T, L, LOCAL>;
-    // always the most that any call asks of this kernel: the limit belongs to the kernel, and a call of
-    // another width from another host thread must not lower it
-    constexpr int most = sel_bwd_smem(L, 2 * (32 / L) * 4, 2, LOCAL);
-    if (most > 48 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    kern<<<(unsigned)grid, 32 * warps, sel_bwd_smem(L, p.CH, warps, LOCAL), st>>>(p);
+    constexpr int smem = sel_bwd_smem<T, L, LOCAL>();
+    if (smem > 48 * 1024) SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kern<<<(unsigned)grid, kSelThreads, smem, st>>>(p);
   } else {
-    k_sel_fwd<T, L, LOCAL><<<(unsigned)grid, 32 * warps, sel_fwd_smem(L, p.CH), st>>>(p);
+    constexpr int smem = sel_fwd_smem<T, L, LOCAL>();
+    static_assert(smem <= 48 * 1024, "needs the attribute");
+    k_sel_fwd<T, L, LOCAL><<<(unsigned)grid, kSelThreads, smem, st>>>(p);
   }
   SQ_LAUNCHED();
   return DELREC_OK;
 }
 // the chunks' maps, their join (where time is cut), and the pass itself
 template <class T, int L, bool BWD>
-static int sel_pass(int warps, const SelArgs& p, cudaStream_t st) {
+static int sel_pass(const SelArgs& p, cudaStream_t st) {
   if (p.chunks > 1) {
-    int rc = sel_start<T, L, BWD, true>(warps, p, st);
+    int rc = sel_start<T, L, BWD, true>(p, st);
     if (rc) return rc;
     const size_t all = (size_t)p.B * p.N * p.S;
-    k_sel_join<BWD><<<(unsigned)((all + 255) / 256), 256, 0, st>>>(p, BWD ? p.ghT : p.h0);
+    k_sel_join<BWD><<<(unsigned)((all + 63) / 64), 64, 0, st>>>(p, BWD ? p.ghT : p.h0);
     SQ_LAUNCHED();
   }
-  return sel_start<T, L, BWD, false>(warps, p, st);
+  return sel_start<T, L, BWD, false>(p, st);
 }
 template <class T, bool BWD, int L = 1>
-static int sel_by_l(int l, int warps, const SelArgs& p, cudaStream_t st) {
+static int sel_by_l(int l, const SelArgs& p, cudaStream_t st) {
   if constexpr (4 * L <= kSelMaxS) {
-    if (l != L) return sel_by_l<T, BWD, 2 * L>(l, warps, p, st);
-    return sel_pass<T, L, BWD>(warps, p, st);
+    if (l != L) return sel_by_l<T, BWD, 2 * L>(l, p, st);
+    return sel_pass<T, L, BWD>(p, st);
   }
   return DELREC_ERR_UNSUPPORTED;
 }

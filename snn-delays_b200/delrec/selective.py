@@ -31,7 +31,8 @@ def _struct(x, S, G, softplus, lengths, dims, gate, y, Bm, Cm, *tensors):
     for t in (x, dims, gate, y, Bm, Cm) + tensors:
         st += t.stride()[:2] if t is not None else (0, 0)
     wide = 1 if lengths is not None and lengths.dtype == torch.int64 else 0
-    return _lib.Selective(*x.shape, S, G, _lib.SEQ_DTYPES[x.dtype], 1 if softplus else 0, wide, *st)
+    return _lib.Selective(*x.shape, S, G, _lib.SEQ_DTYPES[x.dtype], 1 if softplus else 0, wide,
+                          1 if lengths is not None else 0, 0, *st)
 
 
 def _forward(x, dt, A, Bm, Cm, h0, D, gate, dt_bias, lengths, resets, softplus, train):
@@ -208,8 +209,8 @@ def selective_step(x, dt, A, B, C, state=None, *, D=None, gate=None, dt_bias=Non
     y = torch.empty(Bs, N, device=dev, dtype=x.dtype)
     nxt = torch.empty(Bs, N, S, device=dev) if out is None else out
     if Bs and N:
-        s = _lib.Selective(1, Bs, N, S, G, _lib.SEQ_DTYPES[x.dtype], 1 if softplus else 0, 0, 0, x.stride(0), 0,
-                           dt.stride(0), 0, gate.stride(0) if gate is not None else 0, 0, N, 0, B.stride(0), 0,
+        s = _lib.Selective(1, Bs, N, S, G, _lib.SEQ_DTYPES[x.dtype], 1 if softplus else 0, 0, 0, 0, 0, x.stride(0),
+                           0, dt.stride(0), 0, gate.stride(0) if gate is not None else 0, 0, N, 0, B.stride(0), 0,
                            C.stride(0))
         P = _lib.addr
         _lib.launch("delrec_selective_step", dev, ctypes.byref(s), x.data_ptr(), dt.data_ptr(), A.data_ptr(),
