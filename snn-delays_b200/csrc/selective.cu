@@ -22,6 +22,13 @@ static int sel_lanes(int S) {
   while (4 * L < S) L *= 2;
   return L;
 }
+// Lanes to a channel in the scan: a block's 256 / L channels are no more than a narrow group needs
+// (each lane then lays out fewer), up to the 8 lanes whose kernels fit the SM best.
+static int sel_scan_lanes(int S, int Dg) {
+  int L = sel_lanes(S);
+  while (L < 8 && 128 / L >= Dg) L *= 2;
+  return L;
+}
 
 struct SelShape {
   int L, tiles, chunks, steps;
@@ -32,8 +39,9 @@ struct SelShape {
 // four rounds uncut there is nothing to gain.
 static SelShape sel_shape(const delrec_selective* s, int slots, double more) {
   SelShape h{};
-  h.L = sel_lanes(s->S);
-  const int CH = 256 / h.L, Dg = s->N / s->G;
+  const int Dg = s->N / s->G;
+  h.L = sel_scan_lanes(s->S, Dg);
+  const int CH = 256 / h.L;
   h.tiles = (Dg + CH - 1) / CH;
   const long long base = (long long)h.tiles * s->G * s->B;
   // of a padded batch's k chunks some (k + 1) / 2 hold steps, and the other blocks leave at once
