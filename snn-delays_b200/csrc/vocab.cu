@@ -15,6 +15,8 @@ static int check_vocab(const delrec_vocab* s) {
   if (s->distill && (s->teacher_dtype < DELREC_F32 || s->teacher_dtype > DELREC_F16)) return DELREC_ERR_ARG;
   if (!s->distill && s->K != 1) return DELREC_ERR_ARG;
   if (!(s->temperature > 0.f) || !(s->temperature < 1e30f)) return DELREC_ERR_ARG;
+  // tiles of 256 x 128 at least, in up to 16 parts, are counted in 32 bits
+  if (((long long)s->T * s->B / 256 + 1) * (s->V / 128 + 1) > (1LL << 27)) return DELREC_ERR_UNSUPPORTED;
   if (s->D > kVocabMaxD || s->K > kVocabMaxK || s->V > (1 << 30) || (long long)s->T * s->B > (1 << 24))
     return DELREC_ERR_UNSUPPORTED;
   return DELREC_OK;
@@ -48,14 +50,20 @@ struct VocabKeep {
 };
 
 static int vocab_bn(int n) { return n <= 128 ? 128 : 256; }
-// Parts of a reduction of kb 64-blocks over `tiles` output tiles: as many as fill the SMs' waves best, each
-// part at least 8 blocks; a further part has to save 5 % (its sums cross the memory once more).
-static int vocab_splits(long long tiles, long long kb) {
+// Columns of a gradient's tile: 512 where they are there (the operands of a tile cross L2 half as often
+// again for twice the products), not for fp32, whose segments want two accumulators.
+static int vocab_bnd(int n, int pieces) { return pieces == 1 && n > 256 && (n + 511) / 512 * 512 - n < 256 ? 512 : vocab_bn(n); }
+// Parts of the reduction (kb 64-blocks) of a tm x tn grid of 256 x bn tiles: more fill the pairs of SMs
+// better and cross the memory more often.  In microseconds: 0.4 a 64-block (0.65 of 512 columns), some 5 TB/s for
+// the sums of the parts, written and read.
+static int vocab_splits(long long tm, long long tn, int bn, long long kb, int nprod) {
+  const int pairs = kSeqSMs / 2;
   int best = 1;
-  double cost = (double)((tiles + kSeqSMs - 1) / kSeqSMs);
-  for (int k = 2; k <= 16 && k * 8 <= kb; ++k) {
-    const double c = (double)((tiles * k + kSeqSMs - 1) / kSeqSMs) / k;
-    if (c < cost * 0.95) { cost = c; best = k; }
+  double cost = 0;
+  for (int k = 1; k <= 16 && (k == 1 || k * 8 <= kb); ++k) {
+    const long long waves = (tm * tn * k + pairs - 1) / pairs;
+    const double c = waves * ((bn == 512 ? 0.65 : 0.4) * nprod * ((kb + k - 1) / k) + 2) + (k > 1 ? (double)k * tm * 256 * tn * bn * 8 / 5e6 + 5 : 0);
+    if (k == 1 || c < cost) { cost = c; best = k; }
   }
   return best;
 }
@@ -71,14 +79,14 @@ constexpr size_t kVocabBudget = 256u << 20;   // bytes of G at once
 static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
   VocabShape h{};
   h.M = (long long)s->T * s->B;
-  h.Mp = (h.M + 127) / 128 * 128;
+  h.Mp = (h.M + 255) / 256 * 256;
   h.Dp = (s->D + 7) / 8 * 8;
   h.pieces = s->dtype == DELREC_F32 ? 3 : 1;
   h.esz = s->dtype == DELREC_F32 ? 4 : 2;
   h.x_piece = h.Mp * h.Dp;
   h.w_piece = (long long)s->V * h.Dp;
   h.bnv = vocab_bn(s->V);
-  h.bnd = vocab_bn(s->D);
+  h.bnd = vocab_bnd(s->D, h.pieces);
   VocabTake take;
   h.x = take((size_t)h.x_piece * h.pieces * 2);
   // whether W can be an operand as it lies is known at the call: room for its copy where it may be needed
@@ -96,8 +104,8 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
     h.count = (s->V + h.Vc - 1) / h.Vc;
     h.g_piece = h.Mp * h.Vc;
     const long long dtiles = (s->D + h.bnd - 1) / h.bnd;
-    h.dx_splits = vocab_splits((h.Mp / 128) * dtiles, std::min(h.Vc, s->V) / 64);
-    h.dw_splits = vocab_splits(((std::min(h.Vc, s->V) + 127) / 128) * dtiles, h.Mp / 64);
+    h.dx_splits = vocab_splits(h.Mp / 256, dtiles, h.bnd, std::min(h.Vc, s->V) / 64, h.pieces == 3 ? 6 : 1);
+    h.dw_splits = vocab_splits((std::min(h.Vc, s->V) + 255) / 256, dtiles, h.bnd, h.Mp / 64, h.pieces == 3 ? 6 : 1);
     h.db_runs = (int)std::max<long long>(1, std::min<long long>(64, h.M / 64));
     h.G = take((size_t)h.g_piece * h.pieces * 2);
     h.coef = take((size_t)h.M * 4);
@@ -204,10 +212,15 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   if (rc) return rc;
   rc = by_dtype(s->dtype, [&](auto t) {
     using E = decltype(t);
-    const size_t smem = ((size_t)(s->D + 3) / 4 * 4 + 2 * s->K) * 4;
-    const int nt = s->K == 1 ? 32 : 128;
-    if (!((uintptr_t)w & 15) && s->D % (16 / sizeof(E)) == 0) k_vocab_targets<E, true><<<a.M, nt, smem, st>>>(a);
-    else k_vocab_targets<E, false><<<a.M, nt, smem, st>>>(a);
+    const bool vec = !((uintptr_t)w & 15) && s->D % (16 / sizeof(E)) == 0;
+    if (s->K <= 4) {   // a warp to a row
+      if (vec) k_vocab_targets<E, true, 1><<<(a.M + 3) / 4, 128, 0, st>>>(a);
+      else k_vocab_targets<E, false, 1><<<(a.M + 3) / 4, 128, 0, st>>>(a);
+    } else {
+      const size_t smem = ((size_t)(s->D + 3) / 4 * 4 + 2 * s->K) * 4;
+      if (vec) k_vocab_targets<E, true, 4><<<a.M, 128, smem, st>>>(a);
+      else k_vocab_targets<E, false, 4><<<a.M, 128, smem, st>>>(a);
+    }
     SQ_LAUNCHED();
     return (int)DELREC_OK;
   });
@@ -219,7 +232,7 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   g.part = (float2*)(base + h.part); g.part_ld = h.Mp;
   g.bias = bias; g.bias_code = s->dtype; g.scale = a.scale;
   if ((rc = vg_logits(s->dtype == DELREC_F16, h.bnv, false, X, W, g, st))) return rc;
-  k_vocab_lse<<<(a.M + 31) / 32, 256, 0, st>>>(a, g.part, g.part_ld, (s->V + h.bnv - 1) / h.bnv * 2, each);
+  k_vocab_lse<<<(a.M + 31) / 32, 1024, 0, st>>>(a, g.part, g.part_ld, (s->V + h.bnv - 1) / h.bnv * 2, each);
   SQ_LAUNCHED();
   if (!each) {
     k_vocab_reduce<<<1, 1024, 0, st>>>(a, s->reduction == 1, out);

@@ -6,10 +6,15 @@
 //               type, from the row's log-sum-exp, for one piece of the vocabulary.
 //   dW = G^T x  and  dx += G W  for that piece (VG_OUT).
 //
-// Persistent: one CTA per SM walks 128 x BN output tiles.  One thread streams operand tiles with TMA into
-// a ring of shared-memory stages, one issues tcgen05.mma (M=128, N=BN, K=16) into one of two
-// accumulators in tensor memory, eight warps read the other one back, so the epilogue of a tile runs
-// under the next tile's products.  fp32 operands are three bf16 pieces each (an exact split) and six piece
+// Persistent: a pair of CTAs on two SMs walks 256 x BN output tiles (cta_group::2).  Each keeps 128 rows
+// of A and of the accumulators, and half of B's columns, which the tensor cores of both read: a 256 x 256
+// tile's operands then take 32 instead of 48 KB a SM and 64-block (8192 positions on 32768 tokens, 512
+// channels: the gradients' products 115 -> 99 us each).  The gradients' products take 512 columns to a
+// tile (BN = 512, one accumulator) where those are there: 24 KB for as much work (training pass of the
+// same 755 -> 718 us of backward).  In each CTA one thread streams operand tiles
+// with TMA (no multicast) into a ring of shared-memory stages; in the first one a thread issues tcgen05.mma (M=256, N=BN, K=16)
+// into one of two accumulators in tensor memory; eight warps of each read the other one back, so
+// the epilogue of a tile runs under the next tile's products.  fp32 operands are three bf16 pieces each (an exact split) and six piece
 // products, smallest first; 16-bit operands are taken as they are.  The tensor core's accumulator
 // truncates, so long fp32 reductions run in segments whose sums are added outside it.
 //
@@ -23,7 +28,8 @@
 namespace delrec {
 
 enum { VG_STATS = 0, VG_GRAD = 1, VG_OUT = 2 };
-constexpr int kVgThreads = 320;       // warps 0..7 epilogue, 8 TMA, 9 MMA
+constexpr int kVgEpi = 8;             // epilogue warps
+constexpr int kVgThreads = 32 * (kVgEpi + 2);   // then one for TMA, one for MMA
 constexpr int kVgMaxProd = 6;
 constexpr int kVgTimeout = 1 << 3;    // ST_TIMEOUT of the status word
 
@@ -56,18 +62,41 @@ struct VgArgs {
   const float* inv;
 };
 
-constexpr int vg_stages(int BN) { return BN == 256 ? 4 : 6; }
-constexpr size_t vg_smem(int BN) { return (size_t)vg_stages(BN) * (128 * 64 + BN * 64) * 2 + 1024; }
+constexpr int vg_stages(int BN) { return BN == 512 ? 4 : BN == 256 ? 6 : 8; }
+constexpr size_t vg_smem(int BN) { return (size_t)vg_stages(BN) * (128 * 64 + BN / 2 * 64) * 2 + 1024; }
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+// bar: an mbarrier of the pair's first CTA
+__device__ __forceinline__ void vg_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          dst),
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(dst),
       "l"((unsigned long long)map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void vg_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// the address of the same place in the pair's first CTA
+__device__ __forceinline__ uint32_t vg_first(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void vg_arrive(uint32_t bar) {   // a shared::cluster address
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void vg_mma(uint32_t tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(
+          tmem),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// arrives at this barrier of both CTAs once the products issued so far are done
+__device__ __forceinline__ void vg_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"((unsigned short)3)
+               : "memory");
+}
+__device__ __forceinline__ void vg_meet() {   // both CTAs of the pair
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Waits at most limit_ns; false when the time is up here or was elsewhere in the CTA.
 __device__ __forceinline__ bool vg_wait(uint32_t bar, uint32_t parity, long long limit_ns, volatile int* abort, int* status) {
@@ -135,10 +164,10 @@ __device__ __forceinline__ void vg_store_row(E* dst, int col, int N, const float
 
 // OUT: element type of VG_OUT's result
 template <int BN, bool AMN, bool BMN, int EPI, bool F16, class OUT>
-__global__ void __launch_bounds__(kVgThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
     k_vocab_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const VgArgs g) {
-  constexpr int STAGES = vg_stages(BN);
-  constexpr uint32_t A_BYTES = 128 * 64 * 2, B_BYTES = BN * 64 * 2;
+  constexpr int STAGES = vg_stages(BN), ACCS = BN == 512 ? 1 : 2;
+  constexpr uint32_t A_BYTES = 128 * 64 * 2, B_BYTES = BN / 2 * 64 * 2;
   extern __shared__ unsigned char dsm[];
   __shared__ __align__(8) uint64_t bars[2 * STAGES + 4];
   __shared__ uint32_t s_tmem;
@@ -148,6 +177,8 @@ __global__ void __launch_bounds__(kVgThreads, 1)
   const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]);
   const uint32_t acc_full = smem_u32(&bars[2 * STAGES]), acc_empty = smem_u32(&bars[2 * STAGES + 2]);
   volatile int* abort = &s_abort;
+  uint32_t rank;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -156,40 +187,46 @@ __global__ void __launch_bounds__(kVgThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(acc_full + 8 * s, 1);
-      mbar_init(acc_empty + 8 * s, 8);
+      mbar_init(acc_empty + 8 * s, 2 * kVgEpi);
     }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&ma) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&mb) : "memory");
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
-                 "r"((uint32_t)(2 * BN))
+  if (warp == kVgEpi + 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                 "r"((uint32_t)(ACCS * BN))
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  vg_meet();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
 
   const int rows = *g.rows;
   const int M = g.M < 0 ? rows : g.M, K = g.K < 0 ? rows : g.K;
-  const int tm = (M + 127) / 128, tn = (g.N + BN - 1) / BN;
+  const int tm = (M + 255) / 256, tn = (g.N + BN - 1) / BN;
   const int kb = (K + 63) / 64;
   const int seg = g.seg > 0 ? g.seg : max(1, (kb + g.splits - 1) / g.splits);   // 64-blocks of a segment
   const int nseg = (kb + seg - 1) / seg;
-  const long long items = (long long)tm * tn * g.splits;
+  // (the host has made sure that the items fit 32 bits)
+  const unsigned items = (unsigned)tm * tn * g.splits, w0 = blockIdx.x >> 1, dw = gridDim.x >> 1;
+  const auto tile_m = [&](unsigned w) { return (int)(w % (unsigned)tm); };
+  const auto tile_n = [&](unsigned w) { return (int)(w / (unsigned)tm % (unsigned)tn); };
+  const auto tile_s = [&](unsigned w) { return (int)(w / ((unsigned)tm * (unsigned)tn)); };
   // segments of part s of the reduction
-  const auto first_seg = [&](int s) { return (int)((long long)nseg * s / g.splits); };
+  const auto first_seg = [&](int s) { return (int)((unsigned)(nseg * s) / (unsigned)g.splits); };
 
-  if (warp == 8) {
+  if (warp == kVgEpi) {
     if (lane == 0) {
       unsigned it = 0;
       bool ok = true;
-      for (long long w = blockIdx.x; ok && w < items; w += gridDim.x) {
-        const int m0 = (int)(w % tm) * 128, n0 = (int)(w / tm % tn) * BN, sp = (int)(w / ((long long)tm * tn));
+      for (unsigned w = w0; ok && w < items; w += dw) {
+        const int m0 = tile_m(w) * 256 + (int)rank * 128, n0 = tile_n(w) * BN, sp = tile_s(w);
+        const int am = g.a_mn + m0, bm = g.b_mn + n0 + (int)rank * (BN < 256 ? BN / 2 : 128);
         const int s1 = first_seg(sp + 1);
         for (int s = first_seg(sp); ok && s < s1; ++s) {
           const int k0 = s * seg, k1 = min(kb, k0 + seg);
@@ -201,41 +238,46 @@ __global__ void __launch_bounds__(kVgThreads, 1)
                 ok = false;
                 break;
               }
-              const uint32_t bar = full0 + 8 * st, a = sA + st * A_BYTES, b = sB + st * B_BYTES;
-              mbar_expect_tx(bar, A_BYTES + B_BYTES);
-              const int ak = g.a_k + 64 * k, bk = g.b_k + 64 * k, am = g.a_mn + m0, bm = g.b_mn + n0;
+              const uint32_t bar = vg_first(full0 + 8 * st), a = sA + st * A_BYTES, b = sB + st * B_BYTES;
+              if (rank == 0) mbar_expect_tx(full0 + 8 * st, 2 * (A_BYTES + B_BYTES));
+              const int ak = g.a_k + 64 * k, bk = g.b_k + 64 * k;
               if (AMN) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) tma_load_3d(a + q * 8192, &ma, am + 64 * q, ak, za, bar);
+                for (int q = 0; q < 2; ++q) vg_load(a + q * 8192, &ma, am + 64 * q, ak, za, bar);
               } else {
-                tma_load_3d(a, &ma, ak, am, za, bar);
+                vg_load(a, &ma, ak, am, za, bar);
               }
+              // of each 256 columns a CTA holds 128
               if (BMN) {
 #pragma unroll
-                for (int q = 0; q < BN / 64; ++q) tma_load_3d(b + q * 8192, &mb, bm + 64 * q, bk, zb, bar);
+                for (int q = 0; q < BN / 128; ++q) vg_load(b + q * 8192, &mb, bm + q / 2 * 256 + q % 2 * 64, bk, zb, bar);
               } else {
-                tma_load_3d(b, &mb, bk, bm, zb, bar);
+                static_assert(BMN || BN <= 256, "one box");
+                vg_load(b, &mb, bk, bm, zb, bar);
               }
             }
           }
         }
       }
-      if (!ok)   // the copies in flight: those of the last STAGES rounds
+      if (!ok && rank == 0)   // the pair's copies in flight: those of the last STAGES rounds
         for (unsigned j = it > STAGES ? it - STAGES : 0; j < it; ++j)
           vg_drain(full0 + 8 * (j % STAGES), j / STAGES & 1u, g.spin_ns);
     }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = F16 ? umma_idesc_bf16(BN, AMN, BMN) & ~((1u << 7) | (1u << 10)) : umma_idesc_bf16(BN, AMN, BMN);
+  } else if (warp == kVgEpi + 1) {
+    if (lane == 0 && rank == 0) {
+      // as for a single CTA, with M = 256 and the element types
+      constexpr int MN = BN == 512 ? 256 : BN;
+      constexpr uint32_t bf16 = umma_idesc_bf16(MN, AMN, BMN) + ((uint32_t)(128 >> 4) << 24);
+      constexpr uint32_t idesc = F16 ? bf16 & ~((1u << 7) | (1u << 10)) : bf16;
       constexpr uint64_t astep = AMN ? (2048 >> 4) : (32 >> 4), bstep = BMN ? (2048 >> 4) : (32 >> 4);
       unsigned it = 0, acc = 0;
       bool ok = true;
-      for (long long w = blockIdx.x; ok && w < items; w += gridDim.x) {
-        const int sp = (int)(w / ((long long)tm * tn)), s1 = first_seg(sp + 1);
+      for (unsigned w = w0; ok && w < items; w += dw) {
+        const int sp = tile_s(w), s1 = first_seg(sp + 1);
         for (int s = first_seg(sp); ok && s < s1; ++s, ++acc) {
           const int n = (min(kb, (s + 1) * seg) - s * seg) * g.nprod;
-          const uint32_t d = tmem + (acc & 1) * BN;
-          if (!(ok = vg_wait(acc_empty + 8 * (acc & 1), (acc / 2 & 1u) ^ 1u, g.spin_ns, abort, g.status))) break;
+          const uint32_t d = tmem + (acc % ACCS) * BN;
+          if (!(ok = vg_wait(acc_empty + 8 * (acc % ACCS), (acc / ACCS & 1u) ^ 1u, g.spin_ns, abort, g.status))) break;
           tc_fence_after();
           for (int j = 0; j < n; ++j, ++it) {
             const int st = it % STAGES;
@@ -243,10 +285,13 @@ __global__ void __launch_bounds__(kVgThreads, 1)
             tc_fence_after();
             const uint64_t ad = umma_desc_sw128(sA + st * A_BYTES, AMN), bd = umma_desc_sw128(sB + st * B_BYTES, BMN);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_bf16(d, ad + astep * kk, bd + bstep * kk, idesc, j > 0 || kk > 0);
-            umma_commit(empty0 + 8 * st);
+            for (int kk = 0; kk < 4; ++kk) {
+              vg_mma(d, ad + astep * kk, bd + bstep * kk, idesc, j > 0 || kk > 0);
+              if (BN == 512) vg_mma(d + 256, ad + astep * kk, bd + (16384 >> 4) + bstep * kk, idesc, j > 0 || kk > 0);
+            }
+            vg_commit(empty0 + 8 * st);
           }
-          if (ok) umma_commit(acc_full + 8 * (acc & 1));
+          if (ok) vg_commit(acc_full + 8 * (acc % ACCS));
         }
       }
       if (!ok && it > 0) vg_drain(empty0 + 8 * ((it - 1) % STAGES), (it - 1) / STAGES & 1u, g.spin_ns);
@@ -258,17 +303,17 @@ __global__ void __launch_bounds__(kVgThreads, 1)
     const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16) + half * HC;
     unsigned acc = 0;
     bool ok = true;
-    for (long long w = blockIdx.x; ok && w < items; w += gridDim.x) {
-      const int m0 = (int)(w % tm) * 128, ct = (int)(w / tm % tn), n0 = ct * BN + half * HC;
-      const int sp = (int)(w / ((long long)tm * tn));
+    for (unsigned w = w0; ok && w < items; w += dw) {
+      const int m0 = tile_m(w) * 256 + (int)rank * 128, ct = tile_n(w), n0 = ct * BN + half * HC;
+      const int sp = tile_s(w);
       const int s0 = first_seg(sp), s1 = first_seg(sp + 1);
       const int m = m0 + q * 32 + lane;
       // a part without segments still writes its zeros
       for (int s = s0; ok && (s < s1 || s == s0); ++s) {
         const bool have = s < s1;
-        const uint32_t t = lane_base + (acc & 1) * BN;
+        const uint32_t t = lane_base + (acc % ACCS) * BN;
         if (have) {
-          ok = vg_wait(acc_full + 8 * (acc & 1), acc / 2 & 1u, g.spin_ns, abort, g.status);
+          ok = vg_wait(acc_full + 8 * (acc % ACCS), acc / ACCS & 1u, g.spin_ns, abort, g.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -293,10 +338,10 @@ __global__ void __launch_bounds__(kVgThreads, 1)
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = n + i < g.N ? v[i] : -INFINITY;
             }
-            float mx = v[0];
+            float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, v[i]);
-            mx = fmaxf(top, mx * g.scale);
+            for (int i = 4; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+            const float mx = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * g.scale);
             const float at = mx == -INFINITY ? 0.f : mx;
             float s4[4] = {sum * vg_exp2(top - at), 0.f, 0.f, 0.f};
 #pragma unroll
@@ -392,7 +437,7 @@ __global__ void __launch_bounds__(kVgThreads, 1)
         if (have) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) vg_arrive(acc_empty + 8 * (acc & 1));
+          if (lane == 0) vg_arrive(vg_first(acc_empty + 8 * (acc % ACCS)));
           ++acc;
         }
       }
@@ -401,9 +446,10 @@ __global__ void __launch_bounds__(kVgThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  vg_meet();
+  if (warp == kVgEpi + 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN)) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(ACCS * BN)) : "memory");
   }
 }
 

@@ -142,32 +142,41 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, l
   }
 }
 
-// The targets of packed row blockIdx.x: p, the sums of p over repeated indices, the targets' logits y
-// (dot products in float32) and h = sum p (log p - ln2 y).  One warp for K = 1, four else.
-template <class T, bool VEC>
+// The targets of a packed row: p, the sums of p over repeated indices, the targets' logits y (dot
+// products in float32) and h = sum p (log p - ln2 y).  W warps to a row: four, x staged as float32, or
+// one for up to four targets (8192 rows of one target: 17 us with a block to a row, 9 so).
+template <class T, bool VEC, int W>
 __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
   extern __shared__ float smf[];
-  __shared__ float s_red[4];
-  const int r = blockIdx.x;
-  if (r >= *a.rows) return;
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, W = nt / 32, K = a.K, D = a.D;
-  float* s_x = smf;                 // [D]
-  float* s_p = s_x + (D + 3) / 4 * 4;   // [K]
-  int* s_i = (int*)(s_p + K);       // [K]
+  __shared__ float s_red[4], s_few[W == 1 ? 32 : 1];
+  const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (r >= *a.rows) return;        // with W = 1 a whole warp: no block-wide barrier below
+  const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5, tid = W == 1 ? lane : threadIdx.x, K = a.K, D = a.D;
+  constexpr int nt = 32 * W;
+  float* s_x = smf;                                                          // [D], W = 4
+  float* s_p = W == 1 ? s_few + (threadIdx.x >> 5) * 8 : s_x + (D + 3) / 4 * 4;   // [K]
+  int* s_i = (int*)(s_p + (W == 1 ? 4 : K));                                 // [K]
+  const auto sync = [] {
+    if (W == 1) __syncwarp();
+    else __syncthreads();
+  };
   const int m = a.rowmap[r];
   const T* x = (const T*)a.x + m / a.B * a.x_t + m % a.B * a.x_b;
-  for (int d = tid; d < D; d += nt) s_x[d] = to_f(x[d]);
+  if (W > 1)
+    for (int d = tid; d < D; d += nt) s_x[d] = to_f(x[d]);
   const auto all = [&](float v, bool max) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       const float u = __shfl_xor_sync(0xffffffffu, v, o);
       v = max ? fmaxf(v, u) : v + u;
     }
-    __syncthreads();
-    if (lane == 0) s_red[warp] = v;
-    __syncthreads();
-    v = s_red[0];
-    for (int w = 1; w < W; ++w) v = max ? fmaxf(v, s_red[w]) : v + s_red[w];
+    if (W > 1) {
+      __syncthreads();
+      if (lane == 0) s_red[warp] = v;
+      __syncthreads();
+      v = s_red[0];
+      for (int w = 1; w < W; ++w) v = max ? fmaxf(v, s_red[w]) : v + s_red[w];
+    }
     return v;
   };
   float top = -INFINITY;
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
   } else if (tid == 0) {
     s_p[0] = 1.f;
   }
-  __syncthreads();
+  sync();
   if (a.p)
     for (int k = tid; k < K; k += nt) {
       float s = 0.f;
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
         }
       float xv[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) xv[i] = d + i < D ? s_x[d + i] : 0.f;
+      for (int i = 0; i < N; ++i) xv[i] = d + i < D ? (W == 1 ? to_f(x[d + i]) : s_x[d + i]) : 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (row[j]) {
@@ -259,31 +268,37 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
   if (tid == 0) a.h[r] = h;
 }
 
-// A row's log-sum-exp from its tiles' maxima and sums, and its loss.  Block: 32 rows by 8 runs of tiles.
-static __global__ void __launch_bounds__(256) k_vocab_lse(const VocabArgs a, const float2* __restrict__ part,
-                                                          long long ld, int tiles, float* each) {
-  __shared__ float2 s[8][32];
+// A row's log-sum-exp from its tiles' maxima and sums, and its loss.  Block: 32 rows by 32 runs of tiles.
+__device__ __forceinline__ void vocab_join(float& top, float& sum, float2 v) {
+  const float mx = fmaxf(top, v.x), at = mx == -INFINITY ? 0.f : mx;
+  sum = sum * exp2f(top - at) + v.y * exp2f(v.x - at);
+  top = mx;
+}
+static __global__ void __launch_bounds__(1024) k_vocab_lse(const VocabArgs a, const float2* __restrict__ part,
+                                                           long long ld, int tiles, float* each) {
+  __shared__ float2 s[32][33];
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
   const int rows = *a.rows, r = blockIdx.x * 32 + lane;
   if (blockIdx.x * 32 >= rows) return;
   float top = -INFINITY, sum = 0.f;
   if (r < rows)
-#pragma unroll 4
-    for (int t = run; t < tiles; t += 8) {
-      const float2 v = part[t * ld + r];
-      const float mx = fmaxf(top, v.x), at = mx == -INFINITY ? 0.f : mx;
-      sum = sum * exp2f(top - at) + v.y * exp2f(v.x - at);
-      top = mx;
+    for (int t0 = run; t0 < tiles; t0 += 32 * 8) {
+      float2 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = t0 + 32 * k < tiles ? part[(t0 + 32 * k) * ld + r] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) vocab_join(top, sum, v[k]);
     }
   s[run][lane] = make_float2(top, sum);
   __syncthreads();
-  if (run || r >= rows) return;
-  for (int k = 1; k < 8; ++k) {
-    const float2 v = s[k][lane];
-    const float mx = fmaxf(top, v.x), at = mx == -INFINITY ? 0.f : mx;
-    sum = sum * exp2f(top - at) + v.y * exp2f(v.x - at);
-    top = mx;
+  for (int k = 16; k; k >>= 1) {
+    if (run < k) {
+      vocab_join(top, sum, s[run + k][lane]);
+      s[run][lane] = make_float2(top, sum);
+    }
+    __syncthreads();
   }
+  if (run || r >= rows) return;
   const float lse = top + log2f(sum);
   a.lse[r] = lse;
   const float loss = a.tau * a.tau * fmaf(kLn2v, lse, a.h[r]);
@@ -315,11 +330,13 @@ static __global__ void __launch_bounds__(1024) k_vocab_coef(const VocabArgs a, i
   __shared__ float s_top[32];
   const int rows = *a.rows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float one = reduction == 0 ? 0.f : *g * a.tau / (reduction == 1 ? (float)max(rows, 1) : 1.f);
-  float top = 0.f;
-  for (int r = threadIdx.x; r < rows; r += 1024) {
-    const float c = fabsf(reduction == 0 ? g[a.rowmap[r]] * a.tau : one);
-    if (c < INFINITY) top = fmaxf(top, c);
-  }
+  float top = reduction != 0 && fabsf(one) < INFINITY ? fabsf(one) : 0.f;
+  if (reduction == 0)
+#pragma unroll 4
+    for (int r = threadIdx.x; r < rows; r += 1024) {
+      const float c = fabsf(g[a.rowmap[r]] * a.tau);
+      if (c < INFINITY) top = fmaxf(top, c);
+    }
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s_top[warp] = top;
@@ -329,6 +346,7 @@ static __global__ void __launch_bounds__(1024) k_vocab_coef(const VocabArgs a, i
   frexpf(top, &e);                                        // top = f 2^e, f in [0.5, 1)
   e = top > 0.f ? min(max(14 - e, -100), 120) : 0;
   const float up = ldexpf(1.f, e);
+#pragma unroll 4
   for (int r = threadIdx.x; r < rows; r += 1024) {
     const float c = reduction == 0 ? g[a.rowmap[r]] * a.tau : one, l = a.loss[r];
     coef[r] = l != l ? l : c * up;
