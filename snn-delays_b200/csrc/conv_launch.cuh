@@ -23,8 +23,7 @@ template <class T, bool BWD, int K = 1>
 static int conv_by_k(int k, int V, const ConvArgs& a, cudaStream_t st) {
   if constexpr (K <= kConvMaxK) {
     if (k != K) return conv_by_k<T, BWD, K + 1>(k, V, a, st);
-    constexpr int VW = BWD ? 4 : 16 / sizeof(T);
-    return V > 1 ? conv_start<T, K, VW, BWD>(a, st) : conv_start<T, K, 1, BWD>(a, st);
+    return V > 1 ? conv_start<T, K, 4, BWD>(a, st) : conv_start<T, K, 1, BWD>(a, st);
   }
   return DELREC_ERR_ARG;
 }

@@ -14,7 +14,7 @@ namespace delrec {
 
 enum { CONV_NONE = 0, CONV_SILU = 1 };
 constexpr int kConvMaxK = 8;
-constexpr int kConvAhead = 4;   // rows of x (and gy) on their way while one batch is worked on
+constexpr int kConvAhead = 4;   // rows of x (and gy) on their way together; eight 16-bit ones of x alone
 
 struct ConvArgs {
   int T, B, N, act, kind;       // kind of lengths: 0 int32, 1 int64, 2 one byte a row (0 or 1 steps)
@@ -46,8 +46,8 @@ __device__ __forceinline__ void conv_store(T* ptr, const float* v) {
 template <class T>
 __device__ __forceinline__ float silu(float p, float& d) {
   float s, o;
-  sigmoid_pair<Accurate<T>::value>(p, s, o);
-  d = s * (1.f + p * o);
+  sigmoid_pair<false>(p, s, o);   // (one ex2: |p| 2^-24 of it, also in float32)
+  d = s * fmaf(p, o, 1.f);
   return p * s;
 }
 
@@ -129,32 +129,39 @@ struct ConvThread {
 };
 
 template <class T, int K, int V>
-__global__ void __launch_bounds__(128) k_conv_fwd(const ConvArgs a) {
+__global__ void __launch_bounds__(128, K <= 4 ? 6 : 4) k_conv_fwd(const ConvArgs a) {
+  constexpr int AHEAD = sizeof(T) == 2 ? 2 * kConvAhead : kConvAhead;
   ConvThread<T, K, V> s(a);
   if (!s.init()) return;
   const int end = min(s.t1, s.len);
-  if (s.t0 <= s.len) s.fill();
-  for (int t = s.t0; t < end; t += kConvAhead) {
-    VecOf<T, V> in[kConvAhead];
+  const T* px = s.row(a.x, s.t0, a.x_t, a.x_b);
+  T* py = const_cast<T*>(s.row(a.y, s.t0, a.y_t, a.y_b));
+  using Row = VecOf<T, V>;
+  const auto one = [&](int t, const Row& in, T* to) {
+    float x[V], p[V];
+    unpack_vec<T, V>(in, x);
+    if (s.cut(t)) s.clear();
+    s.pre(x, p);
+    if (a.act == CONV_SILU) {
+      float d;
 #pragma unroll
-    for (int i = 0; i < kConvAhead; ++i)
-      if (t + i < end) in[i] = *(const VecOf<T, V>*)s.row(a.x, t + i, a.x_t, a.x_b);
-#pragma unroll
-    for (int i = 0; i < kConvAhead; ++i) {
-      if (t + i >= end) break;
-      float x[V], p[V];
-      unpack_vec<T, V>(in[i], x);
-      if (s.cut(t + i)) s.clear();
-      s.pre(x, p);
-      if (a.act == CONV_SILU) {
-        float d;
-#pragma unroll
-        for (int v = 0; v < V; ++v) p[v] = silu<T>(p[v], d);
-      }
-      conv_store<T, V>(const_cast<T*>(s.row(a.y, t + i, a.y_t, a.y_b)), p);
-      s.push(x);
+      for (int v = 0; v < V; ++v) p[v] = silu<T>(p[v], d);
     }
+    conv_store<T, V>(to, p);
+    s.push(x);
+  };
+  int t = s.t0;
+  if (t <= s.len) s.fill();
+  for (; t + AHEAD <= end; t += AHEAD) {
+    Row in[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) in[i] = *(const Row*)(px + i * a.x_t);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) one(t + i, in[i], py + i * a.y_t);
+    px += AHEAD * a.x_t;
+    py += AHEAD * a.y_t;
   }
+  for (; t < end; ++t, px += a.x_t, py += a.y_t) one(t, *(const Row*)px, py);
   const float zero[V] = {};
   for (int t = max(s.t0, end); t < s.t1; ++t) conv_store<T, V>(const_cast<T*>(s.row(a.y, t, a.y_t, a.y_b)), zero);
   // the chunk that holds the last row there is writes the state behind it (chunk 0 of an empty sequence)
@@ -191,60 +198,67 @@ __global__ void __launch_bounds__(128) k_conv_bwd(const ConvArgs a) {
     }
   };
   if (s.t0 <= s.len) {
+    const T *px = s.row(a.x, s.t0, a.x_t, a.x_b), *pg = a.gy ? s.row(a.gy, s.t0, a.gy_t, a.gy_b) : nullptr;
+    using Row = VecOf<T, V>;
     s.fill();
-    for (int t = s.t0; t < end; t += kConvAhead) {
-      VecOf<T, V> in[kConvAhead], gin[kConvAhead];
+    const auto one = [&](int t, const Row& in, const Row& gin) {
+      float x[V], g[V];
+      unpack_vec<T, V>(in, x);
+      unpack_vec<T, V>(gin, g);
+      since = min(since + 1, 1 << 30);
+      if (s.cut(t)) {
+        s.clear();
+        since = 0;
+      }
+      if (a.act == CONV_SILU) {
+        float p[V], d;
+        s.pre(x, p);
 #pragma unroll
-      for (int i = 0; i < kConvAhead; ++i)
-        if (t + i < end) {
-          in[i] = *(const VecOf<T, V>*)s.row(a.x, t + i, a.x_t, a.x_b);
-          if (a.gy) gin[i] = *(const VecOf<T, V>*)s.row(a.gy, t + i, a.gy_t, a.gy_b);
-          else gin[i] = VecOf<T, V>{};
+        for (int v = 0; v < V; ++v) {
+          silu<T>(p[v], d);
+          g[v] *= d;
         }
+      }
+#pragma unroll
+      for (int d = 0; d < K; ++d)
+        if (d <= since) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[d][v] = fmaf(s.w[K - 1 - d][v], g[v], acc[d][v]);
+        }
+      if (t < s.t1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          db[v] += g[v];
+          dw[K - 1][v] = fmaf(g[v], x[v], dw[K - 1][v]);
+#pragma unroll
+          for (int j = 0; j + 1 < K; ++j) dw[j][v] = fmaf(g[v], s.win[j][v], dw[j][v]);
+        }
+      }
+      emit(t - (K - 1), acc[K - 1]);
+      s.push(x);
+#pragma unroll
+      for (int d = K - 1; d > 0; --d)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[d][v] = acc[d - 1][v];
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[0][v] = 0.f;
+    };
+    int t = s.t0;
+    for (; t + kConvAhead <= end; t += kConvAhead) {
+      Row in[kConvAhead], gin[kConvAhead];
 #pragma unroll
       for (int i = 0; i < kConvAhead; ++i) {
-        if (t + i >= end) break;
-        float x[V], g[V];
-        unpack_vec<T, V>(in[i], x);
-        unpack_vec<T, V>(gin[i], g);
-        since = min(since + 1, 1 << 30);
-        if (s.cut(t + i)) {
-          s.clear();
-          since = 0;
-        }
-        if (a.act == CONV_SILU) {
-          float p[V], d;
-          s.pre(x, p);
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            silu<T>(p[v], d);
-            g[v] *= d;
-          }
-        }
-#pragma unroll
-        for (int d = 0; d < K; ++d)
-          if (d <= since) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[d][v] = fmaf(s.w[K - 1 - d][v], g[v], acc[d][v]);
-          }
-        if (t + i < s.t1) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            db[v] += g[v];
-            dw[K - 1][v] = fmaf(g[v], x[v], dw[K - 1][v]);
-#pragma unroll
-            for (int j = 0; j + 1 < K; ++j) dw[j][v] = fmaf(g[v], s.win[j][v], dw[j][v]);
-          }
-        }
-        emit(t + i - (K - 1), acc[K - 1]);
-        s.push(x);
-#pragma unroll
-        for (int d = K - 1; d > 0; --d)
-#pragma unroll
-          for (int v = 0; v < V; ++v) acc[d][v] = acc[d - 1][v];
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[0][v] = 0.f;
+        in[i] = *(const Row*)(px + i * a.x_t);
+        gin[i] = pg ? *(const Row*)(pg + i * a.gy_t) : Row{};
       }
+      px += kConvAhead * a.x_t;
+      if (pg) pg += kConvAhead * a.gy_t;
+#pragma unroll
+      for (int i = 0; i < kConvAhead; ++i) one(t + i, in[i], gin[i]);
+    }
+    for (; t < end; ++t, px += a.x_t) {
+      one(t, *(const Row*)px, pg ? *(const Row*)pg : Row{});
+      if (pg) pg += a.gy_t;
     }
     // acc[d] now belongs to position last - d + 1, last the last row walked; those of the new state
     // take its gradient

@@ -106,7 +106,7 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
     const long long dtiles = (s->D + h.bnd - 1) / h.bnd;
     h.dx_splits = vocab_splits(h.Mp / 256, dtiles, h.bnd, std::min(h.Vc, s->V) / 64, h.pieces == 3 ? 6 : 1);
     h.dw_splits = vocab_splits((std::min(h.Vc, s->V) + 255) / 256, dtiles, h.bnd, h.Mp / 64, h.pieces == 3 ? 6 : 1);
-    h.db_runs = (int)std::max<long long>(1, std::min<long long>(64, h.M / 64));
+    h.db_runs = (int)std::max<long long>(1, std::min<long long>(128, h.M / 32));
     h.G = take((size_t)h.g_piece * h.pieces * 2);
     h.coef = take((size_t)h.M * 4);
     h.inv = take(4);
@@ -310,9 +310,10 @@ int delrec_vocab_loss_backward(const delrec_vocab* s, const void* x, const void*
     }
     if (db) {
       float* part = (float*)(base + h.db);
-      const dim3 grid((n + 127) / 128, h.db_runs);
-      if (f16) k_vocab_db_part<__half><<<grid, 128, 0, st>>>(a.rows, (const __half*)(base + h.G), n, h.Vc, h.g_piece, h.pieces, part);
-      else k_vocab_db_part<__nv_bfloat16><<<grid, 128, 0, st>>>(a.rows, (const __nv_bfloat16*)(base + h.G), n, h.Vc, h.g_piece, h.pieces, part);
+      const dim3 grid((n + 1023) / 1024, h.db_runs);
+      if (f16) k_vocab_db_part<__half, 1><<<grid, 128, 0, st>>>(a.rows, (const __half*)(base + h.G), n, h.Vc, h.g_piece, part);
+      else if (h.pieces == 1) k_vocab_db_part<__nv_bfloat16, 1><<<grid, 128, 0, st>>>(a.rows, (const __nv_bfloat16*)(base + h.G), n, h.Vc, h.g_piece, part);
+      else k_vocab_db_part<__nv_bfloat16, 3><<<grid, 128, 0, st>>>(a.rows, (const __nv_bfloat16*)(base + h.G), n, h.Vc, h.g_piece, part);
       SQ_LAUNCHED();
       rc = by_dtype(s->dtype, [&](auto t) {
         using E = decltype(t);

@@ -371,21 +371,31 @@ __global__ void __launch_bounds__(256) k_vocab_patch(const VocabArgs a, const fl
   }
 }
 
-// column sums of a piece of G over runs of rows: part[run][column]; then db
-template <class E>
+// column sums of a piece of G over runs of rows: part[run][column]; then db.  Eight columns a thread (a
+// row's pitch is a multiple of 256).
+template <class E, int P>
 __global__ void __launch_bounds__(128) k_vocab_db_part(const int* __restrict__ rows, const E* __restrict__ G, int n,
-                                                       long long ld, long long piece, int pieces, float* part) {
-  const int c = blockIdx.x * 128 + threadIdx.x, run = blockIdx.y, runs = gridDim.y;
+                                                       long long ld, long long piece, float* part) {
+  const int c = (blockIdx.x * 128 + threadIdx.x) * 8, run = blockIdx.y, runs = gridDim.y;
   if (c >= n) return;
   const long long R = *rows, r0 = R * run / runs, r1 = R * (run + 1) / runs;
-  float s = 0.f;
-#pragma unroll 8
+  float s[8] = {};
+#pragma unroll 4
   for (long long r = r0; r < r1; ++r) {
-    float v = to_f(G[r * ld + c]);
-    for (int p = 1; p < pieces; ++p) v += to_f(G[p * piece + r * ld + c]);
-    s += v;
+    float v[8], f[8];
+    unpack_vec<E, 8>(*(const VecOf<E, 8>*)(G + r * ld + c), v);
+#pragma unroll
+    for (int p = 1; p < P; ++p) {
+      unpack_vec<E, 8>(*(const VecOf<E, 8>*)(G + p * piece + r * ld + c), f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += f[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] += v[k];
   }
-  part[(long long)run * n + c] = s;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (c + k < n) part[(long long)run * n + c + k] = s[k];
 }
 template <class T>
 __global__ void __launch_bounds__(256) k_vocab_db(const float* __restrict__ part, int n, int runs,
