@@ -20,6 +20,7 @@ from .dcls import Dcls1d
 from .delay_layers import axonal_recdel, common_recdel, synaptic_recdel
 from .linear import Linear, readout_time_sum
 from .neuron import BatchNorm1d, Dropout
+from .vocab_loss import linear_cross_entropy, linear_distill
 
 
 def _lif(config, step_mode=None):
@@ -129,6 +130,27 @@ class SNN(torch.nn.Module):
         for m in self.layers[:-1]:
             h = m(h)
         return readout_time_sum(h, last.weight, last.bias)
+
+    def _hidden(self, x, what):
+        """What the readout takes, for a loss that is fused with it."""
+        assert x.dim() == 3
+        if type(self.layers[-1]) is not Linear:
+            raise RuntimeError(f"delrec_b200: {what} needs a Linear readout")
+        for m in self.layers[:-1]:
+            x = m(x)
+        return x
+
+    def position_loss(self, x, target, **kw):
+        """Cross entropy of forward(x)[t, b] against target (T,B) at every position, without forming
+        the (T,B,output_size) readout (``vocab_loss.linear_cross_entropy``, which takes ``kw``)."""
+        h, last = self._hidden(x, "position_loss"), self.layers[-1]
+        return linear_cross_entropy(h, last.weight, target, last.bias, **kw)
+
+    def distill_loss(self, x, indices, logits, **kw):
+        """Distillation of forward(x) from a teacher's kept logits (T,B,K) at every position, without
+        forming the readout (``vocab_loss.linear_distill``, which takes ``kw``)."""
+        h, last = self._hidden(x, "distill_loss"), self.layers[-1]
+        return linear_distill(h, last.weight, indices, logits, last.bias, **kw)
 
     def init_weights(self):
         for m in self.layers:

@@ -17,6 +17,8 @@ import torch.nn.functional as F
 from . import functional as Fn
 from .block_norm import GATES, block_join, block_norm
 from .gated import gated_scan, gated_step
+from .selective import selective_scan, selective_step
+from .short_conv import ACTS, short_conv, short_conv_step
 
 
 class MemoryModule(torch.nn.Module):
@@ -196,6 +198,89 @@ class GatedIntegrator(MemoryModule):
 
     def extra_repr(self):
         return f"decay_input={self.decay_input}, step_mode={self.step_mode}, checkpoint8={self.checkpoint8}"
+
+
+class ShortConv(MemoryModule):
+    """A short causal convolution over time, one filter per channel (``short_conv.short_conv``),
+    as it stands in front of ``GatedIntegrator`` or ``SelectiveIntegrator``.
+
+    Multi-step mode: x (T,B,N) -> y (T,B,N) from zeros, or from the window of the call before with
+    ``keep_state=True``.  Single-step mode ('s'): x (B,N) -> y (B,N), the window moving on from call
+    to call until ``reset`` (``utils.reset_states``); no gradient passes.  ``v`` is the window
+    (K-1,B,N) in x's type."""
+
+    def __init__(self, num_features, kernel_size: int = 4, act: str = "silu", bias: bool = True, step_mode: str = "m",
+                 keep_state: bool = False):
+        super().__init__()
+        if step_mode not in ("m", "s"):
+            raise ValueError(f"step_mode must be 'm' or 's', got {step_mode!r}")
+        if act not in ACTS:
+            raise ValueError(f"act must be one of {sorted(ACTS)}, got {act!r}")
+        self.act, self.step_mode, self.keep_state = act, step_mode, keep_state
+        bound = kernel_size ** -0.5
+        self.weight = torch.nn.Parameter(torch.empty(num_features, kernel_size).uniform_(-bound, bound))
+        if bias:
+            self.bias = torch.nn.Parameter(torch.empty(num_features).uniform_(-bound, bound))
+        else:
+            self.register_parameter("bias", None)
+        self.register_memory("v", None)
+
+    def forward(self, x, lengths=None, resets=None):
+        if self.step_mode == "s":
+            if lengths is not None or resets is not None:
+                raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
+            y, self.v = short_conv_step(x, self.weight, self.bias, self.v, act=self.act)
+            return y
+        y, v = short_conv(x, self.weight, self.bias, self.v if self.keep_state else None, act=self.act,
+                          lengths=lengths, resets=resets)
+        if self.keep_state:
+            self.v = v.detach()
+        return y
+
+    def extra_repr(self):
+        n, k = self.weight.shape
+        return f"{n}, kernel_size={k}, act={self.act}, step_mode={self.step_mode}"
+
+
+class SelectiveIntegrator(MemoryModule):
+    """A recurrence of S states per channel whose step size, input and output weights depend on the
+    input (``selective.selective_scan``), where ``GatedIntegrator`` has one state and its gate.
+
+    forward(x, dt, B, C, gate=None): multi-step mode (T,B,N) .. -> y (T,B,N) from a zero state, or
+    from the state of the call before with ``keep_state=True``; single-step mode ('s') (B,N) .. ->
+    y (B,N), the state moving on from call to call until ``reset``; no gradient passes.  Learned: the
+    decay A = -exp(A_log) (N,S), the skip D (N) and the bias of dt (N), whose step sizes start
+    between ``dt_min`` and ``dt_max``.  ``v`` is the state (B,N,S) in float32."""
+
+    def __init__(self, num_features, num_states: int = 16, dt_min: float = 1e-3, dt_max: float = 0.1,
+                 step_mode: str = "m", keep_state: bool = False):
+        super().__init__()
+        if step_mode not in ("m", "s"):
+            raise ValueError(f"step_mode must be 'm' or 's', got {step_mode!r}")
+        self.step_mode, self.keep_state = step_mode, keep_state
+        rates = torch.arange(1, num_states + 1, dtype=torch.float32)
+        self.A_log = torch.nn.Parameter(torch.log(rates).repeat(num_features, 1))
+        self.D = torch.nn.Parameter(torch.ones(num_features))
+        step = torch.exp(torch.empty(num_features).uniform_(math.log(dt_min), math.log(dt_max)))
+        self.dt_bias = torch.nn.Parameter(step + torch.log(-torch.expm1(-step)))   # softplus of it is the step
+        self.register_memory("v", None)
+
+    def forward(self, x, dt, B, C, gate=None, lengths=None, resets=None):
+        A = -torch.exp(self.A_log)
+        if self.step_mode == "s":
+            if lengths is not None or resets is not None:
+                raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
+            y, self.v = selective_step(x, dt, A, B, C, self.v, D=self.D, gate=gate, dt_bias=self.dt_bias)
+            return y
+        y, v = selective_scan(x, dt, A, B, C, self.v if self.keep_state else None, D=self.D, gate=gate,
+                              dt_bias=self.dt_bias, lengths=lengths, resets=resets)
+        if self.keep_state:
+            self.v = v.detach()
+        return y
+
+    def extra_repr(self):
+        n, k = self.A_log.shape
+        return f"{n}, num_states={k}, step_mode={self.step_mode}"
 
 
 class BlockNorm(torch.nn.Module):
