@@ -16,6 +16,10 @@
 // decays is exp(A sum delta)), are joined in time order (k_sel_join), and then every chunk runs from
 // its own start.
 //
+// exp(delta A) is ex2((delta log2 e) A): the factor goes with delta, whose rounding differs from step to
+// step, not with A, whose rounding would pull every step of a state the same way (the state after 500
+// bf16 steps on average 7.9e-7 -> 3.6e-7 off).
+//
 // What bounds it: the exponentials, 16 a clock and SM (one a state forward, two backward), with the
 // issue slots close behind.  Sums and states are float32.
 #pragma once
@@ -80,6 +84,11 @@ __device__ __forceinline__ f2 exp22(f2 v) {
   split(v, a, b);
   return pair(sel_exp2(a), sel_exp2(b));
 }
+// exp(delta A) from d = delta log2(e).  ex2.approx is low by 2.1e-8 of its value on average (it cuts
+// off), and a state that lives for a thousand steps sees that a thousand times: the exponent takes
+// 2.1e-8 log2(e) more (a product and a sum cost what a product costs).  d = 0 still gives exactly 1.
+constexpr float kSelLow = 2.97e-8f;
+__device__ __forceinline__ f2 sel_decay2(f2 d, f2 A) { return exp22(fma2(d, A, pair(kSelLow, kSelLow))); }
 __device__ __forceinline__ float sel_rcp(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -88,13 +97,13 @@ __device__ __forceinline__ float sel_rcp(float v) {
 
 // delta and its derivative by dt.  softplus(z) = max(z, 0) + log1p(t), t = exp(-|z|), with log1p(t) =
 // 2 artanh(s), s = t / (2 + t) <= 1/3, by its series up to s^15 (what is left out is below 2^-28 of it).
-template <bool GRAD>
+template <class T, bool GRAD>
 __device__ __forceinline__ float sel_delta(float z, int softplus, float& d) {
   if (!softplus) {
     d = 1.f;
     return z;
   }
-  const float t = sel_exp2(fabsf(z) * -kLog2e), s = t * sel_rcp(2.f + t), q = s * s;
+  const float t = exp_neg_abs<Accurate<T>::value>(z), s = t * sel_rcp(2.f + t), q = s * s;
   if (GRAD) {
     const float r = sel_rcp(1.f + t);
     d = z >= 0.f ? r : t * r;
@@ -308,12 +317,6 @@ struct SelThread {
   __device__ __forceinline__ void store_state(float* base, size_t lead, const f2* h) const {
     write_states(states_at(base, lead), p.S % 4 == 0, h);
   }
-  __device__ __forceinline__ void load_decay(f2* A2) const {
-    load_state(p.A, 0, A2);
-    const f2 k = pair(kLog2e, kLog2e);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) A2[s] = mul2(A2[s], k);
-  }
   __device__ __forceinline__ void load_weights(const float* w, float* v) const {
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] = w && i < left ? w[n0 + col + i] : 0.f;
@@ -419,10 +422,10 @@ __global__ void __launch_bounds__(kSelThreads, L >= 4 ? 5 : 3) k_sel_fwd(const S
   float* s_x = s_d + Th::AR;
   float* s_o = s_x + Th::AR;
   const int end = min(th.t1, th.len);
-  f2 A2[4], h[4], sumd = 0;
+  f2 A[4], h[4], sumd = 0;
   float bias[W], Dv[W];
   bool any_cut = false;
-  th.load_decay(A2);
+  th.load_state(p.A, 0, A);
   th.load_weights(p.bias, bias);
   th.load_weights(p.D, Dv);
   if (LOCAL) th.load_state(nullptr, 0, h);
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(kSelThreads, L >= 4 ? 5 : 3) k_sel_fwd(const S
   T* py = th.at((T*)p.y, th.t0, p.y_t, p.y_b);
   float* pst = !LOCAL && p.states ? th.states_at(p.states, (size_t)(th.t0 / kSelSeg) * p.B + th.b) : nullptr;
   const bool four = p.S % 4 == 0;
-  typename Th::Raw rx[NI], rz[NI], ru[NI], cu[NI];
+  typename Th::Raw rx[NI], rz[NI], ru[NI], cx[NI], cu[NI];
   RawOf<T, 4> rB[Th::BCN], rC[Th::BCN];
   uint32_t rcut = 0;
   const auto fetch = [&](int seg) {
@@ -468,16 +471,21 @@ __global__ void __launch_bounds__(kSelThreads, L >= 4 ? 5 : 3) k_sel_fwd(const S
     for (int i = 0; i < NI; ++i) {
       const int r = th.row + i * ROWS;
       if (r < kSelSeg) {   // past the end: delta 0 leaves a state as it is
-        float x[W] = {}, d[W] = {}, z[W], sig;
+        float dx[W] = {}, d[W] = {}, x[W], z[W], sig;
         if (seg + r < end) {
           sel_floats<T, W>(rx[i], x);
           sel_floats<T, W>(rz[i], z);
 #pragma unroll
-          for (int k = 0; k < W; ++k) d[k] = k < th.left ? sel_delta<false>(z[k] + bias[k], p.softplus, sig) : 0.f;
+          for (int k = 0; k < W; ++k) {
+            d[k] = k < th.left ? sel_delta<T, false>(z[k] + bias[k], p.softplus, sig) : 0.f;
+            dx[k] = d[k] * x[k];
+            d[k] *= kLog2e;
+          }
         }
         th.put(s_d, r, d);
-        th.put(s_x, r, x);
+        th.put(s_x, r, dx);
       }
+      cx[i] = rx[i];
       cu[i] = ru[i];
     }
     th.put_bc(rB, s_B);
@@ -491,10 +499,10 @@ __global__ void __launch_bounds__(kSelThreads, L >= 4 ? 5 : 3) k_sel_fwd(const S
     any_cut |= cut != 0;
     const auto step = [&](int r) {
       f2 Bv[4], Cv[4];
-      const f2 d = th.get2(s_d, r), dx = mul2(d, th.get2(s_x, r));
+      const f2 d = th.get2(s_d, r), dx = th.get2(s_x, r);
       th.get_bc(s_B, r, Bv);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) h[s] = fma2(exp22(mul2(d, A2[s])), h[s], mul2(dx, Bv[s]));
+      for (int s = 0; s < 4; ++s) h[s] = fma2(sel_decay2(d, A[s]), h[s], mul2(dx, Bv[s]));
       if (LOCAL) {
         sumd = fma2(d, pair(1.f, 1.f), sumd);
       } else {
@@ -528,7 +536,7 @@ __global__ void __launch_bounds__(kSelThreads, L >= 4 ? 5 : 3) k_sel_fwd(const S
         if (r < kSelSeg && t < end) {
           float o[W], x[W];
           th.get(s_o, r, o);
-          th.get(s_x, r, x);
+          sel_floats<T, W>(cx[i], x);
 #pragma unroll
           for (int k = 0; k < W; ++k) o[k] = fmaf(Dv[k], x[k], o[k]);
           if (gate) {
@@ -574,7 +582,7 @@ __global__ void __launch_bounds__(64) k_sel_join(const SelArgs p, const float* _
   if (i >= all) return;
   const int b = (int)(i / row);
   const size_t ns = i - b * row, n = ns / p.S;
-  const float A2 = p.A[ns] * kLog2e;
+  const float A = p.A[ns];
   float h = start ? start[i] : 0.f;
   constexpr int U = 16;                 // chunks whose maps are on their way together
   for (int c0 = 0; c0 < p.chunks; c0 += U) {
@@ -593,7 +601,7 @@ __global__ void __launch_bounds__(64) k_sel_join(const SelArgs p, const float* _
       const int c = BACK ? p.chunks - 1 - (c0 + k) : c0 + k;
       if (c0 + k < p.chunks) {
         p.loc[((size_t)c * p.B + b) * row + ns] = h;
-        h = cut[k] ? loc[k] : fmaf(sel_exp2(A2 * d[k]), h, loc[k]);
+        h = cut[k] ? loc[k] : fmaf(sel_exp2(A * d[k]), h, loc[k]);
       }
     }
   }
@@ -625,10 +633,10 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
   float* s_x = s_go + AR;                                        // later sum G B; not in a LOCAL pass
   const int end = min(th.t1, th.len);
   const size_t lead = (size_t)th.chunk * p.B + th.b;
-  f2 A2[4], G[4], dA[4], sumd = 0;
+  f2 A[4], G[4], dA[4], sumd = 0;
   float bias[W], Dv[W], dD[W] = {}, db[W] = {};
   bool any_cut = false;
-  th.load_decay(A2);
+  th.load_state(p.A, 0, A);
   th.load_weights(p.bias, bias);
   th.load_weights(p.D, Dv);
 #pragma unroll
@@ -725,7 +733,7 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
           sel_floats<T, W>(rz[i], z);
           if (grad) sel_floats<T, W>(rg[i], go[i]);
 #pragma unroll
-          for (int q = 0; q < W; ++q) d[i][q] = q < th.left ? sel_delta<!LOCAL>(z[q] + bias[q], p.softplus, sig[i][q]) : 0.f;
+          for (int q = 0; q < W; ++q) d[i][q] = q < th.left ? sel_delta<T, !LOCAL>(z[q] + bias[q], p.softplus, sig[i][q]) : 0.f;
           if (gate) {
             sel_floats<T, W>(ru[i], u);
 #pragma unroll
@@ -737,9 +745,15 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
             }
           }
         }
-        th.put(s_d, r, d[i]);
+        float d2[W], dx[W];
+#pragma unroll
+        for (int q = 0; q < W; ++q) {
+          d2[q] = d[i][q] * kLog2e;
+          dx[q] = d[i][q] * x[i][q];
+        }
+        th.put(s_d, r, d2);
         th.put(s_go, r, go[i]);
-        if (!LOCAL) th.put(s_x, r, x[i]);
+        if (!LOCAL) th.put(s_x, r, dx);
       }
     }
     th.put_bc(rC, s_C);
@@ -755,10 +769,10 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
       for (int s = 0; s < 4; ++s) first[s] = h[s];
       const auto step = [&](int r) {
         f2 Bv[4];
-        const f2 dd = th.get2(s_d, r), dx = mul2(dd, th.get2(s_x, r));
+        const f2 dd = th.get2(s_d, r), dx = th.get2(s_x, r);
         th.get_bc(s_B, r, Bv);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) h[s] = fma2(exp22(mul2(dd, A2[s])), h[s], mul2(dx, Bv[s]));
+        for (int s = 0; s < 4; ++s) h[s] = fma2(sel_decay2(dd, A[s]), h[s], mul2(dx, Bv[s]));
         if (r + 1 < kSelSeg) {
           hist[r * 2 * nt + th.tid] = make_ulonglong2(h[0], h[1]);
           hist[(r * 2 + 1) * nt + th.tid] = make_ulonglong2(h[2], h[3]);
@@ -787,14 +801,14 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
       if constexpr (LOCAL) {
         sumd = fma2(dd, pair(1.f, 1.f), sumd);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) G[s] = mul2(exp22(mul2(dd, A2[s])), fma2(Cv[s], gg, G[s]));
+        for (int s = 0; s < 4; ++s) G[s] = mul2(sel_decay2(dd, A[s]), fma2(Cv[s], gg, G[s]));
         if (here) {
 #pragma unroll
           for (int s = 0; s < 4; ++s) G[s] = 0;
         }
       } else {
         f2 Bv[4], ag[4], w[4], bB[4], bC[4], gb2, wa2, o2;
-        const f2 dx = mul2(dd, th.get2(s_x, r));
+        const f2 dx = th.get2(s_x, r);
         th.get_bc(s_B, r, Bv);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -803,7 +817,7 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
           bC[s] = mul2(gg, h[s]);
           bB[s] = mul2(Gt, dx);
           gb2 = s ? fma2(Gt, Bv[s], gb2) : mul2(Gt, Bv[s]);
-          ag[s] = mul2(exp22(mul2(dd, A2[s])), Gt);
+          ag[s] = mul2(sel_decay2(dd, A[s]), Gt);
           w[s] = mul2(ag[s], pre[s]);
           h[s] = pre[s];
         }
@@ -813,7 +827,7 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          wa2 = s ? fma2(w[s], A2[s], wa2) : mul2(w[s], A2[s]);
+          wa2 = s ? fma2(w[s], A[s], wa2) : mul2(w[s], A[s]);
           dA[s] = fma2(w[s], dd, dA[s]);
           G[s] = ag[s];
         }
@@ -900,7 +914,7 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
 #pragma unroll
           for (int q = 0; q < W; ++q) {
             vx[q] = fmaf(gb[q], d[i][q], Dv[q] * go[i][q]);
-            vz[q] = fmaf(gb[q], x[i][q], wa[q] * kLn2) * sig[i][q];
+            vz[q] = fmaf(gb[q], x[i][q], wa[q]) * sig[i][q];
             vu[q] = gs[i][q] * fmaf(Dv[q], x[i][q], o[q]);
             dD[q] = fmaf(go[i][q], x[i][q], dD[q]);
             db[q] += vz[q];
@@ -933,7 +947,12 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
     return;
   }
   if (p.dh0 && th.chunk == 0) th.store_state(p.dh0, th.b, G);
-  if (p.dA) th.store_state(p.dA, lead, dA);
+  if (p.dA) {
+    const f2 ln2 = pair(kLn2, kLn2);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) dA[s] = mul2(dA[s], ln2);
+    th.store_state(p.dA, lead, dA);
+  }
   // dD and db: over the lanes that have laid out the same channels
 #pragma unroll
   for (int q = 0; q < W; ++q) {
@@ -1025,13 +1044,13 @@ __global__ void __launch_bounds__(256) k_sel_step(const SelStep p) {
     if (act) {
       float sig;
       x = to_f(((const T*)p.x)[b * p.x_b + n]);
-      const float d = sel_delta<false>(to_f(((const T*)p.dt)[b * p.dt_b + n]) + (p.bias ? p.bias[n] : 0.f), p.softplus, sig);
+      const float d = sel_delta<T, false>(to_f(((const T*)p.dt)[b * p.dt_b + n]) + (p.bias ? p.bias[n] : 0.f), p.softplus, sig);
       const T* Bp = (const T*)p.Bm + b * p.bm_b + (long long)g * p.S + 4 * sg;
       const T* Cp = (const T*)p.Cm + b * p.cm_b + (long long)g * p.S + 4 * sg;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
         if (4 * sg + s < p.S) {
-          h[s] = fmaf(sel_exp2(d * (p.A[(size_t)n * p.S + 4 * sg + s] * kLog2e)), h[s], d * x * to_f(Bp[s]));
+          h[s] = fmaf(sel_exp2(fmaf(d * kLog2e, p.A[(size_t)n * p.S + 4 * sg + s], kSelLow)), h[s], d * x * to_f(Bp[s]));
           o = fmaf(to_f(Cp[s]), h[s], o);
         }
     }
