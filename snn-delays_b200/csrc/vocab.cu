@@ -70,7 +70,7 @@ static int vocab_splits(long long tm, long long tn, int bn, long long kb, int np
 
 struct VocabShape {
   long long M, Mp, Dp, x_piece, w_piece, g_piece;
-  int pieces, esz, bnv, bnd, Vc, count;     // Vc columns in each of `count` pieces of the vocabulary
+  int pieces, gp, esz, bnv, bnd, Vc, count; // gp pieces of G; Vc columns in each of `count` pieces of the vocabulary
   int dx_splits, dw_splits, db_runs;
   bool w_direct;                            // W is an operand as it lies
   size_t x, w, part, flags, h, each, G, coef, inv, dx, dw, db, total;
@@ -82,6 +82,10 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
   h.Mp = (h.M + 255) / 256 * 256;
   h.Dp = (s->D + 7) / 8 * 8;
   h.pieces = s->dtype == DELREC_F32 ? 3 : 1;
+  // G of 16-bit operands is rounded to their type: 1.4 times the error that rounding the gradients makes.
+  // Of few rows, where its roundings do not average out and the products wait for W anyway, a second
+  // piece is kept.
+  h.gp = h.pieces == 3 ? 3 : h.M <= 512 ? 2 : 1;
   h.esz = s->dtype == DELREC_F32 ? 4 : 2;
   h.x_piece = h.Mp * h.Dp;
   h.w_piece = (long long)s->V * h.Dp;
@@ -98,16 +102,16 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
     h.flags = take(s->distill ? h.M : 0);
     h.h = take((size_t)h.M * 4);
   } else {
-    const long long fit = std::max<long long>(1024, (long long)(kVocabBudget / ((size_t)h.Mp * h.pieces * 2)));
+    const long long fit = std::max<long long>(512, (long long)(kVocabBudget / ((size_t)h.Mp * h.gp * 2)));
     h.count = (int)((s->V + fit - 1) / fit);
     h.Vc = (int)(((s->V + h.count - 1) / h.count + 255) / 256 * 256);
     h.count = (s->V + h.Vc - 1) / h.Vc;
     h.g_piece = h.Mp * h.Vc;
     const long long dtiles = (s->D + h.bnd - 1) / h.bnd;
-    h.dx_splits = vocab_splits(h.Mp / 256, dtiles, h.bnd, std::min(h.Vc, s->V) / 64, h.pieces == 3 ? 6 : 1);
-    h.dw_splits = vocab_splits((std::min(h.Vc, s->V) + 255) / 256, dtiles, h.bnd, h.Mp / 64, h.pieces == 3 ? 6 : 1);
+    h.dx_splits = vocab_splits(h.Mp / 256, dtiles, h.bnd, std::min(h.Vc, s->V) / 64, h.gp == 3 ? 6 : h.gp);
+    h.dw_splits = vocab_splits((std::min(h.Vc, s->V) + 255) / 256, dtiles, h.bnd, h.Mp / 64, h.gp == 3 ? 6 : h.gp);
     h.db_runs = (int)std::max<long long>(1, std::min<long long>(128, h.M / 32));
-    h.G = take((size_t)h.g_piece * h.pieces * 2);
+    h.G = take((size_t)h.g_piece * h.gp * 2);
     h.coef = take((size_t)h.M * 4);
     h.inv = take(4);
     h.dx = take((size_t)h.dx_splits * h.Mp * h.Dp * 4);
@@ -138,13 +142,14 @@ static VocabArgs vocab_args(const delrec_vocab* s, char* keep) {
   return a;
 }
 
-// the products of pieces, smallest first
-static void vg_products(VgArgs* g, int pieces) {
+// the products of pieces, smallest first: all six of fp32's, or each piece of A with a 16-bit B
+static void vg_products(VgArgs* g, int a_pieces, int b_pieces) {
   static const int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
-  g->nprod = pieces == 3 ? 6 : 1;
+  const bool six = a_pieces == 3 && b_pieces == 3;
+  g->nprod = six ? 6 : a_pieces;
   for (int i = 0; i < g->nprod; ++i) {
-    g->pa[i] = pieces == 3 ? pa[i] : 0;
-    g->pb[i] = pieces == 3 ? pb[i] : 0;
+    g->pa[i] = six ? pa[i] : a_pieces - 1 - i;
+    g->pb[i] = six ? pb[i] : 0;
   }
 }
 
@@ -227,8 +232,8 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   if (rc) return rc;
   VgArgs g{};
   g.rows = a.rows;
-  g.M = -1; g.K = s->D; g.N = s->V; g.splits = 1; g.status = a.status; g.spin_ns = 2000000000ll;
-  vg_products(&g, h.pieces);
+  g.M = -1; g.K = s->D; g.N = s->V; g.splits = 1; g.seg = h.pieces == 3 ? 2 : 0; g.status = a.status; g.spin_ns = 2000000000ll;
+  vg_products(&g, h.pieces, h.pieces);
   g.part = (float2*)(base + h.part); g.part_ld = h.Mp;
   g.bias = bias; g.bias_code = s->dtype; g.scale = a.scale;
   if ((rc = vg_logits(s->dtype == DELREC_F16, h.bnv, false, X, W, g, st))) return rc;
@@ -263,25 +268,26 @@ int delrec_vocab_loss_backward(const delrec_vocab* s, const void* x, const void*
   VgSide X, W;
   int rc = vocab_operands(s, h, a, x, w, base, &X, &W, st);
   if (rc) return rc;
-  const VgSide G{base + h.G, h.Vc, h.Mp, h.Vc, h.g_piece, h.pieces};
+  const VgSide G{base + h.G, h.Vc, h.Mp, h.Vc, h.g_piece, h.gp};
   const long long MK = (long long)a.M * a.K;
   for (int c = 0; c < h.count; ++c) {
     const int v0 = c * h.Vc, n = std::min(h.Vc, s->V - v0);
     VgArgs g{};
     g.rows = a.rows; g.status = a.status; g.spin_ns = 2000000000ll;
-    vg_products(&g, h.pieces);
+    vg_products(&g, h.gp, h.pieces);
     {   // G = c softmax(z), then c (softmax(z) - p) at the targets
       VgArgs q = g;
-      q.M = -1; q.K = s->D; q.N = n; q.splits = 1; q.b_mn = v0;
+      vg_products(&q, h.pieces, h.pieces);
+      q.M = -1; q.K = s->D; q.N = n; q.splits = 1; q.seg = h.pieces == 3 ? 2 : 0; q.b_mn = v0;
       q.bias = bias; q.bias_code = s->dtype; q.scale = a.scale;
-      q.lse = a.lse; q.coef = coef; q.G = base + h.G; q.g_ld = h.Vc; q.g_piece = h.g_piece; q.pieces = h.pieces;
+      q.lse = a.lse; q.coef = coef; q.G = base + h.G; q.g_ld = h.Vc; q.g_piece = h.g_piece; q.pieces = h.gp;
       if ((rc = vg_logits(f16, h.bnv, true, X, W, q, st))) return rc;
       const unsigned blocks = (unsigned)((MK + 255) / 256);
-      if (f16) k_vocab_patch<__half><<<blocks, 256, 0, st>>>(a, coef, v0, n, (__half*)(base + h.G), h.Vc, h.g_piece, h.pieces);
-      else k_vocab_patch<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, coef, v0, n, (__nv_bfloat16*)(base + h.G), h.Vc, h.g_piece, h.pieces);
+      if (f16) k_vocab_patch<__half><<<blocks, 256, 0, st>>>(a, coef, v0, n, (__half*)(base + h.G), h.Vc, h.g_piece, h.gp);
+      else k_vocab_patch<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, coef, v0, n, (__nv_bfloat16*)(base + h.G), h.Vc, h.g_piece, h.gp);
       SQ_LAUNCHED();
     }
-    const int seg = h.pieces == 3 ? 16 : 0;
+    const int seg = h.pieces == 3 ? 8 : 0;
     if (dw) {   // rows v0.. of G^T x
       VgArgs q = g;
       q.M = n; q.K = -1; q.N = s->D; q.splits = h.dw_splits; q.seg = seg; q.inv = inv;
@@ -311,9 +317,15 @@ int delrec_vocab_loss_backward(const delrec_vocab* s, const void* x, const void*
     if (db) {
       float* part = (float*)(base + h.db);
       const dim3 grid((n + 1023) / 1024, h.db_runs);
-      if (f16) k_vocab_db_part<__half, 1><<<grid, 128, 0, st>>>(a.rows, (const __half*)(base + h.G), n, h.Vc, h.g_piece, part);
-      else if (h.pieces == 1) k_vocab_db_part<__nv_bfloat16, 1><<<grid, 128, 0, st>>>(a.rows, (const __nv_bfloat16*)(base + h.G), n, h.Vc, h.g_piece, part);
-      else k_vocab_db_part<__nv_bfloat16, 3><<<grid, 128, 0, st>>>(a.rows, (const __nv_bfloat16*)(base + h.G), n, h.Vc, h.g_piece, part);
+      const auto sum = [&](auto e, auto pieces) {
+        using E = decltype(e);
+        k_vocab_db_part<E, decltype(pieces)::value><<<grid, 128, 0, st>>>(a.rows, (const E*)(base + h.G), n, h.Vc, h.g_piece, part);
+      };
+      using One = std::integral_constant<int, 1>;
+      using Two = std::integral_constant<int, 2>;
+      using Three = std::integral_constant<int, 3>;
+      if (f16) h.gp == 1 ? sum(__half(), One()) : sum(__half(), Two());
+      else h.gp == 1 ? sum(__nv_bfloat16(), One()) : h.gp == 2 ? sum(__nv_bfloat16(), Two()) : sum(__nv_bfloat16(), Three());
       SQ_LAUNCHED();
       rc = by_dtype(s->dtype, [&](auto t) {
         using E = decltype(t);

@@ -28,11 +28,11 @@ static bool vg_map(CUtensorMap* m, const VgSide& s, bool f16, int box_rows) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool AMN, bool BMN, int EPI, bool F16, class OUT>
+template <int BN, bool AMN, bool BMN, int EPI, bool F16, bool SEGS, class OUT>
 static int vg_start(const VgSide& A, const VgSide& B, const VgArgs& g, cudaStream_t st) {
   CUtensorMap ma, mb;
   if (!vg_map(&ma, A, F16, AMN ? 64 : 128) || !vg_map(&mb, B, F16, BMN ? 64 : BN / 2)) return DELREC_ERR_CUDA;
-  auto kern = k_vocab_gemm<BN, AMN, BMN, EPI, F16, OUT>;
+  auto kern = k_vocab_gemm<BN, AMN, BMN, EPI, F16, SEGS, OUT>;
   SQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)vg_smem(BN)));
   kern<<<kSeqSMs, kVgThreads, vg_smem(BN), st>>>(ma, mb, g);
   SQ_LAUNCHED();

@@ -9,8 +9,9 @@
 The (positions, vocabulary) logits live tile by tile in tensor memory; the backward pass forms
 their gradient for a piece of the vocabulary at a time, as the operand of the products for dx and
 dweight.  x, weight and bias are of one type, float32, bfloat16 or float16; sums are float32, and
-float32 operands keep float32 accuracy (three bf16 pieces each).  In a 16-bit type the logits'
-gradient is rounded to it once before the two products.  CUDA tensors only.
+float32 operands keep float32 accuracy (three bf16 pieces each).  In a 16-bit type, where there are
+more than 512 positions, the logits' gradient is rounded to it once before the two products.  CUDA
+tensors only.
 """
 
 from __future__ import annotations
@@ -60,7 +61,7 @@ class VocabLoss(torch.autograd.Function):
         out, keep = _forward(x, w, bias, index, logits, lengths, meta)
         ctx.save_for_backward(x, w, bias, keep)
         ctx.meta = meta
-        ctx.kinds = index.shape[-1] if meta[0] else 1, index.dtype, logits.dtype if logits is not None else None
+        ctx.kept = index.shape[-1] if meta[0] else 1
         return out
 
     @staticmethod
@@ -80,7 +81,7 @@ def _backward(ctx, g):
     dw = torch.empty_like(w) if need[1] else None
     db = torch.empty_like(bias) if bias is not None and need[2] else None
     if keep is not None:
-        s = _struct(x, w, ctx.kinds[0], distill, reduction, None, None, None, tau, ignore)
+        s = _struct(x, w, ctx.kept, distill, reduction, None, None, None, tau, ignore)
         lib, ref = _lib.lib(), ctypes.byref(s)
         nbytes = lib.delrec_vocab_loss_backward_workspace(ref)
         ws = _lib.scratch(nbytes, dev)
