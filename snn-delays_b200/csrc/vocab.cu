@@ -222,7 +222,7 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
       if (vec) k_vocab_targets<E, true, 1><<<(a.M + 3) / 4, 128, 0, st>>>(a);
       else k_vocab_targets<E, false, 1><<<(a.M + 3) / 4, 128, 0, st>>>(a);
     } else {
-      const size_t smem = ((size_t)(s->D + 3) / 4 * 4 + 2 * s->K) * 4;
+      const size_t smem = ((size_t)(s->D + 7) / 8 * 8 * sizeof(E) + 15) / 16 * 16 + (size_t)8 * s->K;
       if (vec) k_vocab_targets<E, true, 4><<<a.M, 128, smem, st>>>(a);
       else k_vocab_targets<E, false, 4><<<a.M, 128, smem, st>>>(a);
     }

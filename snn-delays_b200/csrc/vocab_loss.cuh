@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, l
 }
 
 // The targets of a packed row: p, the sums of p over repeated indices, the targets' logits y (dot
-// products in float32) and h = sum p (log p - ln2 y).  W warps to a row: four, x staged as float32, or
+// products in float32) and h = sum p (log p - ln2 y).  W warps to a row: four, x staged as it is (16
+// bytes a lane: laid out in float32 its reads took the time, 72 us for 4096 rows of 64 targets), or
 // one for up to four targets (8192 rows of one target: 17 us with a block to a row, 9 so).
 template <class T, bool VEC, int W>
 __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
@@ -153,8 +154,10 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
   if (r >= *a.rows) return;        // with W = 1 a whole warp: no block-wide barrier below
   const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5, tid = W == 1 ? lane : threadIdx.x, K = a.K, D = a.D;
   constexpr int nt = 32 * W;
-  float* s_x = smf;                                                          // [D], W = 4
-  float* s_p = W == 1 ? s_few + (threadIdx.x >> 5) * 8 : s_x + (D + 3) / 4 * 4;   // [K]
+  constexpr int N = 16 / sizeof(T);      // the same order of sums whatever the alignment
+  const int Dn = (D + N - 1) / N * N;
+  T* s_x = (T*)smf;                                                          // [Dn], W = 4
+  float* s_p = W == 1 ? s_few + (threadIdx.x >> 5) * 8 : (float*)(s_x + Dn);  // [K]
   int* s_i = (int*)(s_p + (W == 1 ? 4 : K));                                 // [K]
   const auto sync = [] {
     if (W == 1) __syncwarp();
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
   const int m = a.rowmap[r];
   const T* x = (const T*)a.x + m / a.B * a.x_t + m % a.B * a.x_b;
   if (W > 1)
-    for (int d = tid; d < D; d += nt) s_x[d] = to_f(x[d]);
+    for (int d = tid; d < Dn; d += nt) s_x[d] = d < D ? x[d] : from_f<T>(0.f);
   const auto all = [&](float v, bool max) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -215,6 +218,7 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
     for (int k = tid; k < K; k += nt) {
       float s = 0.f;
       const int i = s_i[k];
+#pragma unroll 4
       for (int j = 0; j < K; ++j) s += s_i[j] == i ? s_p[j] : 0.f;
       a.p[(size_t)r * K + k] = s;
     }
@@ -224,31 +228,30 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
     float dot[4] = {};
     const T* row[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) row[j] = k0 + j < K && s_i[k0 + j] >= 0 ? w + (size_t)s_i[k0 + j] * D : nullptr;
-    constexpr int N = 16 / sizeof(T);      // the same order of sums whatever the alignment
+    for (int j = 0; j < 4; ++j) row[j] = w + (size_t)max(s_i[min(k0 + j, K - 1)], 0) * D;   // (row 0: not used)
+#pragma unroll 2
     for (int d = lane * N; d < D; d += 32 * N) {
       VecOf<T, N> q[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (row[j]) {
-          if (VEC) {
-            q[j] = *(const VecOf<T, N>*)(row[j] + d);
-          } else {
+      for (int j = 0; j < 4; ++j) {
+        if (VEC) {
+          q[j] = *(const VecOf<T, N>*)(row[j] + d);
+        } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) q[j].v[i] = d + i < D ? row[j][d + i] : from_f<T>(0.f);
-          }
+          for (int i = 0; i < N; ++i) q[j].v[i] = d + i < D ? row[j][d + i] : from_f<T>(0.f);
         }
+      }
       float xv[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) xv[i] = d + i < D ? (W == 1 ? to_f(x[d + i]) : s_x[d + i]) : 0.f;
+      for (int i = 0; i < (W == 1 ? N : 0); ++i) xv[i] = d + i < D ? to_f(x[d + i]) : 0.f;
+      if (W > 1) unpack_vec<T, N>(*(const VecOf<T, N>*)(s_x + d), xv);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (row[j]) {
-          float f[N];
-          unpack_vec<T, N>(q[j], f);
+      for (int j = 0; j < 4; ++j) {
+        float f[N];
+        unpack_vec<T, N>(q[j], f);
 #pragma unroll
-          for (int i = 0; i < N; ++i) dot[j] = fmaf(xv[i], f[i], dot[j]);
-        }
+        for (int i = 0; i < N; ++i) dot[j] = fmaf(xv[i], f[i], dot[j]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
