@@ -49,6 +49,9 @@ struct VocabKeep {
   }
 };
 
+// Positions past which the packing's blocks find the rows before their own from counts of a kernel before
+// it: they read all positions before their own otherwise.
+constexpr int kVocabCount = 1 << 16;
 static int vocab_bn(int n) { return n <= 128 ? 128 : 256; }
 // Columns of a gradient's tile: 512 where they are there (the operands of a tile cross L2 half as often
 // again for twice the products), not for fp32, whose segments want two accumulators.
@@ -210,7 +213,12 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
     k_vocab_flags<<<(a.M + 7) / 8, 256, 0, st>>>(a);
     SQ_LAUNCHED();
   }
-  k_vocab_rows<<<(a.M + 1023) / 1024, 1024, 0, st>>>(a, each);
+  int* counts = a.M > kVocabCount ? (int*)a.h : nullptr;   // (the rows' h is written later)
+  if (counts) {
+    k_vocab_count<<<(a.M + 1023) / 1024, 1024, 0, st>>>(a, counts);
+    SQ_LAUNCHED();
+  }
+  k_vocab_rows<<<(a.M + 1023) / 1024, 1024, 0, st>>>(a, counts, each);
   SQ_LAUNCHED();
   VgSide X, W;
   int rc = vocab_operands(s, h, a, x, w, base, &X, &W, st);

@@ -62,14 +62,25 @@ __device__ __forceinline__ bool vocab_counts(const VocabArgs& a, int m) {
   if (a.distill) return a.flags[m];
   return vocab_live(a, m) && vocab_index(a, m) != a.ignore;
 }
-// Packs the rows that count, in order.  A block of 1024 counts those before its own by itself.
-// each (M) or NULL: the positions' losses, 0 where a position does not count.
-static __global__ void __launch_bounds__(1024) k_vocab_rows(const VocabArgs a, float* each) {
+// rows that count in each block of 1024
+static __global__ void __launch_bounds__(1024) k_vocab_count(const VocabArgs a, int* counts) {
+  const int m = blockIdx.x * 1024 + threadIdx.x;
+  const int n = __syncthreads_count(m < a.M && vocab_counts(a, m));
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+// Packs the rows that count, in order.  A block of 1024 counts those before its own by itself, from the
+// blocks' counts where those are given.  each (M) or NULL: the positions' losses, 0 where a position does
+// not count.
+static __global__ void __launch_bounds__(1024) k_vocab_rows(const VocabArgs a, const int* __restrict__ counts, float* each) {
   __shared__ int s_warp[32], s_before;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, first = blockIdx.x * 1024;
   int before = 0;
+  if (counts) {
+    for (int k = tid; k < (int)blockIdx.x; k += 1024) before += counts[k];
+  } else {
 #pragma unroll 4
-  for (int m = tid; m < first; m += 1024) before += vocab_counts(a, m);
+    for (int m = tid; m < first; m += 1024) before += vocab_counts(a, m);
+  }
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) s_warp[warp] = before;
   __syncthreads();
@@ -144,7 +155,7 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, l
 
 // The targets of a packed row: p, the sums of p over repeated indices, the targets' logits y (dot
 // products in float32) and h = sum p (log p - ln2 y).  W warps to a row: four, x staged as it is (16
-// bytes a lane: laid out in float32 its reads took the time, 72 us for 4096 rows of 64 targets), or
+// bytes a lane: laid out in float32 its reads took the time: 4096 rows of 64 targets 72 us, 54 so), or
 // one for up to four targets (8192 rows of one target: 17 us with a block to a row, 9 so).
 template <class T, bool VEC, int W>
 __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
@@ -186,7 +197,7 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
   for (int k = tid; k < K; k += nt) {
     const size_t e = (size_t)m * K + k;
     long long i = vocab_index(a, e);
-    float t = a.distill ? vocab_teacher(a, e) / a.tau : 0.f;
+    float t = a.distill ? vocab_teacher(a, e) : 0.f;
     if (a.distill && !vocab_kept(i, t)) {
       i = -1;
       t = -INFINITY;
@@ -199,14 +210,14 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
     top = fmaxf(top, t);
   }
   float h = 0.f;
-  if (a.distill) {
+  if (a.distill) {   // differences first: logits of the type's lowest value stay finite at any temperature
     top = all(top, true);
     float sum = 0.f;
-    for (int k = tid; k < K; k += nt) sum += s_i[k] == -1 ? 0.f : expf(s_p[k] - top);
+    for (int k = tid; k < K; k += nt) sum += s_i[k] == -1 ? 0.f : expf((s_p[k] - top) / a.tau);
     sum = all(sum, false);
     const float ls = logf(sum);
     for (int k = tid; k < K; k += nt) {
-      const float lp = s_p[k] - top - ls, p = s_i[k] == -1 ? 0.f : expf(lp);
+      const float lp = (s_p[k] - top) / a.tau - ls, p = s_i[k] == -1 ? 0.f : expf(lp);
       s_p[k] = p;
       if (p != 0.f) h = fmaf(p, lp, h);
     }
@@ -326,20 +337,30 @@ static __global__ void __launch_bounds__(1024) k_vocab_reduce(const VocabArgs a,
   }
 }
 
-// c_r = g tau (/ count) of each packed row, brought to at most 2^14 by one power of two, whose inverse is
-// *inv: G = c (q - p) then fits fp16 with its small entries.  A row with a NaN loss has NaN gradients.
+// c_r = g tau (/ count) of each packed row in G = c (q - p), times a power of two whose inverse goes into
+// *inv: at most 2^14, so that G fits fp16 with its small entries.  Where all rows share one c, c itself
+// goes into *inv: c (q - 1) of a small q would round alike in every row, up to half a step off in a 16-bit
+// type (8192 positions on 32768 tokens bf16: gradients 3.3e-3 -> 1.7e-3 off, as much as the result's own
+// rounding).  A row with a NaN loss has NaN gradients.
 static __global__ void __launch_bounds__(1024) k_vocab_coef(const VocabArgs a, int reduction, const float* __restrict__ g,
                                                             float* coef, float* inv) {
   __shared__ float s_top[32];
   const int rows = *a.rows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float one = reduction == 0 ? 0.f : *g * a.tau / (reduction == 1 ? (float)max(rows, 1) : 1.f);
-  float top = reduction != 0 && fabsf(one) < INFINITY ? fabsf(one) : 0.f;
-  if (reduction == 0)
+  if (reduction != 0) {
 #pragma unroll 4
     for (int r = threadIdx.x; r < rows; r += 1024) {
-      const float c = fabsf(g[a.rowmap[r]] * a.tau);
-      if (c < INFINITY) top = fmaxf(top, c);
+      const float l = a.loss[r];
+      coef[r] = l != l ? l : 16384.f;
     }
+    if (threadIdx.x == 0) *inv = *g * a.tau / (reduction == 1 ? (float)max(rows, 1) : 1.f) * (1.f / 16384.f);
+    return;
+  }
+  float top = 0.f;
+#pragma unroll 4
+  for (int r = threadIdx.x; r < rows; r += 1024) {
+    const float c = fabsf(g[a.rowmap[r]] * a.tau);
+    if (c < INFINITY) top = fmaxf(top, c);
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s_top[warp] = top;
@@ -351,7 +372,7 @@ static __global__ void __launch_bounds__(1024) k_vocab_coef(const VocabArgs a, i
   const float up = ldexpf(1.f, e);
 #pragma unroll 4
   for (int r = threadIdx.x; r < rows; r += 1024) {
-    const float c = reduction == 0 ? g[a.rowmap[r]] * a.tau : one, l = a.loss[r];
+    const float c = g[a.rowmap[r]] * a.tau, l = a.loss[r];
     coef[r] = l != l ? l : c * up;
   }
   if (threadIdx.x == 0) *inv = ldexpf(1.f, -e);

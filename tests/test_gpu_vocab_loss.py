@@ -235,3 +235,47 @@ def test_no_positions():
         dx, dw = torch.autograd.grad(loss, (x, w))
         assert loss.item() == 0 and dx.shape == x.shape and not dw.any()
         assert linear_cross_entropy(x, w, t, reduction="none").shape == shape
+
+
+@pytest.mark.parametrize("teacher", DTYPES)
+def test_teacher_logits_of_the_lowest_value(teacher):
+    """A mask of the type's lowest value keeps its entries: next to others they weigh nothing, alone they
+    weigh the same, and no temperature makes them infinite.  The same bits as with logits that mean it."""
+    d, grad = _make((3, 7, 24, 50, True, "none", None), torch.float32, 5, seed=11)
+    d["index"] = d["index"].clamp(min=0)
+    plain = torch.randn(3, 7, 5, generator=torch.Generator().manual_seed(3)).to(teacher)
+    plain[0, :, 1:4] = -1e4                # exp(-1e4 / 3) is 0
+    plain[1] = 0
+    lowest = plain.clone()
+    lowest[0, :, 1:4] = torch.finfo(teacher).min
+    lowest[1] = torch.finfo(teacher).min
+    for tau in (0.25, 1.0, 3.0):
+        out = []
+        for logits in (plain, lowest):
+            c = _cuda(dict(d, logits=logits))
+            leaves = [c[k].requires_grad_(True) for k in ("x", "w", "bias")]
+            loss = _call(c, tau)
+            out.append([loss] + list(torch.autograd.grad(loss, leaves, grad.cuda())))
+        assert all(torch.isfinite(v).all() for v in out[0])
+        assert all(torch.equal(u, v) for u, v in zip(*out))
+
+
+def test_many_positions():
+    """More positions than the packing counts by itself: the same bits as in two calls."""
+    from delrec.vocab_loss import linear_cross_entropy
+    g = torch.Generator().manual_seed(5)
+    M = 140001
+    x = torch.randn(M, 16, generator=g).to("cuda", torch.bfloat16).requires_grad_(True)
+    w = torch.randn(24, 16, generator=g).to("cuda", torch.bfloat16)
+    t = torch.randint(0, 24, (M,), generator=g)
+    t[torch.rand(M, generator=g) < 0.3] = -100
+    t[4096:9000] = -100
+    t = t.cuda()
+    loss = linear_cross_entropy(x, w, t, reduction="none")
+    dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    for part in (slice(0, 60000), slice(60000, 120000), slice(120000, M)):
+        y = x.detach()[part].clone().requires_grad_(True)
+        l = linear_cross_entropy(y, w, t[part], reduction="none")
+        assert torch.equal(l, loss[part])
+        assert torch.equal(torch.autograd.grad(l, y, torch.ones_like(l))[0], dx[part])
+    assert (dx[t == -100] == 0).all() and (loss[t == -100] == 0).all() and (loss[t >= 0] > 0).all()
