@@ -25,7 +25,7 @@ struct ConvAlign {
 };
 
 // Four channels to a thread: eight 16-bit ones take twice the registers, and a quarter of the warps
-// then fit an SM (T=250 B=256 N=512 K=4 bf16 forward 62 us, four 45 us).
+// then fit an SM (T=250 B=256 N=512 K=4 bf16 forward 62 us, four 41).
 static constexpr int kConvWidth = 4;
 // Chunks of time: threads of four channels for `per_sm` an SM, as many as fit at once, whose rows in
 // flight cover the memory's latency; at least 8 (K - 1) rows each, of which the rows in front of (and
@@ -68,6 +68,7 @@ int delrec_short_conv_forward(const delrec_conv* s, const void* x, const float* 
   al.add(y, s->y_t, s->y_b);
   al.add(state, 0, 0);
   al.add(next, 0, 0);
+  if (s->T == 1 && (uintptr_t)w % 16) al.ok = false;   // k_conv_step takes the filters in fours
   conv_shape(s, kConvFwd, &a);
   return conv_run_forward(s->dtype, s->K, al.ok ? al.V : 1, a, (cudaStream_t)stream);
 }

@@ -15,6 +15,7 @@ static int conv_start(const ConvArgs& a, cudaStream_t st) {
   const long long blocks = (threads + 127) / 128;
   if (blocks > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   if constexpr (BWD) k_conv_bwd<T, K, V><<<(unsigned)blocks, 128, 0, st>>>(a);
+  else if (a.T == 1 && !a.resets) k_conv_step<T, K, V><<<(unsigned)blocks, 128, 0, st>>>(a);
   else k_conv_fwd<T, K, V><<<(unsigned)blocks, 128, 0, st>>>(a);
   SQ_LAUNCHED();
   return DELREC_OK;
