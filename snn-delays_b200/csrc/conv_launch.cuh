@@ -2,6 +2,8 @@
 // translation units, so that they compile side by side).
 #pragma once
 
+#include <algorithm>
+
 #include "short_conv.cuh"
 
 namespace delrec {
@@ -11,11 +13,18 @@ int conv_run_backward(int dtype, int K, int V, const ConvArgs& a, cudaStream_t s
 
 template <class T, int K, int V, bool BWD>
 static int conv_start(const ConvArgs& a, cudaStream_t st) {
-  const long long threads = (long long)((a.N + V - 1) / V) * a.B * a.chunks;
-  const long long blocks = (threads + 127) / 128;
+  const long long cols = (a.N + V - 1) / V;
+  if constexpr (!BWD) {
+    if (a.T == 1 && !a.resets) {   // as many threads as run at once, or one to a sequence
+      const int step = (int)std::min<long long>(a.B, std::max<long long>(1, kSeqSMs * 1024LL / cols));
+      k_conv_step<T, K, V><<<(unsigned)((cols * step + 127) / 128), 128, 0, st>>>(a, step);
+      SQ_LAUNCHED();
+      return DELREC_OK;
+    }
+  }
+  const long long blocks = (cols * a.B * a.chunks + 127) / 128;
   if (blocks > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
   if constexpr (BWD) k_conv_bwd<T, K, V><<<(unsigned)blocks, 128, 0, st>>>(a);
-  else if (a.T == 1 && !a.resets) k_conv_step<T, K, V><<<(unsigned)blocks, 128, 0, st>>>(a);
   else k_conv_fwd<T, K, V><<<(unsigned)blocks, 128, 0, st>>>(a);
   SQ_LAUNCHED();
   return DELREC_OK;

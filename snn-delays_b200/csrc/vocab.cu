@@ -76,7 +76,7 @@ struct VocabShape {
   int pieces, gp, esz, bnv, bnd, Vc, count; // gp pieces of G; Vc columns in each of `count` pieces of the vocabulary
   int dx_splits, dw_splits, db_runs;
   bool w_direct;                            // W is an operand as it lies
-  size_t x, w, part, flags, h, each, G, coef, inv, dx, dw, db, total;
+  size_t x, w, part, flags, ticket, h, each, G, coef, inv, dx, dw, db, total;
 };
 constexpr size_t kVocabBudget = 256u << 20;   // bytes of G at once
 static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
@@ -103,6 +103,7 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
     const long long tiles = (s->V + h.bnv - 1) / h.bnv * 2;
     h.part = take((size_t)tiles * h.Mp * sizeof(float2));
     h.flags = take(s->distill ? h.M : 0);
+    h.ticket = take(4);
     h.h = take((size_t)h.M * 4);
   } else {
     const long long fit = std::max<long long>(512, (long long)(kVocabBudget / ((size_t)h.Mp * h.gp * 2)));
@@ -156,29 +157,30 @@ static void vg_products(VgArgs* g, int a_pieces, int b_pieces) {
   }
 }
 
-template <class T>
-static int vocab_pack_t(const T* src, long long st, long long sb, int B, const int* rows, const int* rowmap, long long n,
-                        int D, int Dp, long long piece, void* out, cudaStream_t stream) {
-  constexpr int W = 16 / sizeof(T);
-  const bool vec = !(((uintptr_t)src) & 15) && st % W == 0 && sb % W == 0;
-  const int grid = seq_grid((size_t)(rows ? (n + 63) / 64 * 64 : n) * (Dp / 8), 256, 16);
-  if (vec) k_vocab_pack<T, true><<<grid, 256, 0, stream>>>(src, st, sb, B, rows, rowmap, n, D, Dp, piece, out);
-  else k_vocab_pack<T, false><<<grid, 256, 0, stream>>>(src, st, sb, B, rows, rowmap, n, D, Dp, piece, out);
-  SQ_LAUNCHED();
-  return DELREC_OK;
+// rows of x (packed) or of W as operands
+static VocabPack vocab_pack_of(const delrec_vocab* s, const void* src, long long st, long long sb, int B, const int* rows,
+                               const int* rowmap, long long n, long long Dp, long long piece, void* out) {
+  VocabPack p{src, st, sb, n, piece, B, s->D, (int)Dp, 0, rows, rowmap, out};
+  const int W = s->dtype == DELREC_F32 ? 4 : 8;
+  p.vec = !((uintptr_t)src & 15) && st % W == 0 && sb % W == 0;
+  return p;
 }
-// x and (where it has to be) W as operands
-static int vocab_operands(const delrec_vocab* s, const VocabShape& h, const VocabArgs& a, const void* x, const void* w,
-                          char* ws, VgSide* X, VgSide* W, cudaStream_t st) {
-  *X = VgSide{ws + h.x, s->D, h.Mp, h.Dp, h.x_piece, h.pieces};
-  *W = VgSide{h.w_direct ? w : ws + h.w, s->D, s->V, h.Dp, h.w_piece, h.pieces};
+static int vocab_pack_run(const delrec_vocab* s, const VocabPack& p, cudaStream_t st) {
   return by_dtype(s->dtype, [&](auto t) {
-    using E = decltype(t);
-    int rc = vocab_pack_t<E>((const E*)x, s->x_t, s->x_b, s->B, a.rows, a.rowmap, h.M, s->D, (int)h.Dp, h.x_piece, ws + h.x, st);
-    if (rc == DELREC_OK && !h.w_direct)
-      rc = vocab_pack_t<E>((const E*)w, s->D, 0, 1, nullptr, nullptr, s->V, s->D, (int)h.Dp, h.w_piece, ws + h.w, st);
-    return rc;
+    k_vocab_pack<decltype(t)><<<seq_grid((size_t)(p.n + 63) / 64 * 64 * (p.Dp / 8), 256, 16), 256, 0, st>>>(p);
+    SQ_LAUNCHED();
+    return (int)DELREC_OK;
   });
+}
+static VocabPack vocab_x(const delrec_vocab* s, const VocabShape& h, const VocabArgs& a, char* ws, VgSide* X) {
+  *X = VgSide{ws + h.x, s->D, h.Mp, h.Dp, h.x_piece, h.pieces};
+  return vocab_pack_of(s, a.x, s->x_t, s->x_b, s->B, a.rows, a.rowmap, h.M, h.Dp, h.x_piece, ws + h.x);
+}
+// W as an operand: as it lies, or its copy
+static int vocab_w(const delrec_vocab* s, const VocabShape& h, const VocabArgs& a, char* ws, VgSide* W, cudaStream_t st) {
+  *W = VgSide{h.w_direct ? a.w : ws + h.w, s->D, s->V, h.Dp, h.w_piece, h.pieces};
+  if (h.w_direct) return DELREC_OK;
+  return vocab_pack_run(s, vocab_pack_of(s, a.w, s->D, 0, 1, nullptr, nullptr, s->V, h.Dp, h.w_piece, ws + h.w), st);
 }
 
 }  // namespace delrec
@@ -206,6 +208,7 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   a.x = x; a.w = w; a.bias = bias; a.index = index; a.logits = logits; a.lengths = lengths;
   a.flags = (uint8_t*)(base + h.flags);
   a.h = (float*)(base + h.h);
+  a.ticket = (int*)(base + h.ticket);
   if (!(a.status = status_word())) return DELREC_ERR_CUDA;
   const cudaStream_t st = (cudaStream_t)stream;
   float* each = s->reduction == 0 ? out : nullptr;
@@ -221,19 +224,17 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   k_vocab_rows<<<(a.M + 1023) / 1024, 1024, 0, st>>>(a, counts, each);
   SQ_LAUNCHED();
   VgSide X, W;
-  int rc = vocab_operands(s, h, a, x, w, base, &X, &W, st);
+  const VocabPack pack = vocab_x(s, h, a, base, &X);
+  int rc = vocab_w(s, h, a, base, &W, st);
   if (rc) return rc;
   rc = by_dtype(s->dtype, [&](auto t) {
     using E = decltype(t);
     const bool vec = !((uintptr_t)w & 15) && s->D % (16 / sizeof(E)) == 0;
-    if (s->K <= 4) {   // a warp to a row
-      if (vec) k_vocab_targets<E, true, 1><<<(a.M + 3) / 4, 128, 0, st>>>(a);
-      else k_vocab_targets<E, false, 1><<<(a.M + 3) / 4, 128, 0, st>>>(a);
-    } else {
-      const size_t smem = ((size_t)(s->D + 7) / 8 * 8 * sizeof(E) + 15) / 16 * 16 + (size_t)8 * s->K;
-      if (vec) k_vocab_targets<E, true, 4><<<a.M, 128, smem, st>>>(a);
-      else k_vocab_targets<E, false, 4><<<a.M, 128, smem, st>>>(a);
-    }
+    const int few = s->K <= 4, blocks = few ? (a.M + 3) / 4 : a.M;   // a warp to a row, or a block
+    const size_t smem = few ? 0 : ((size_t)(s->D + 7) / 8 * 8 * sizeof(E) + 15) / 16 * 16 + (size_t)8 * s->K;
+    void (*kern)(VocabArgs, int, VocabPack) = few ? (vec ? k_vocab_targets<E, true, 1> : k_vocab_targets<E, false, 1>)
+                                                  : (vec ? k_vocab_targets<E, true, 4> : k_vocab_targets<E, false, 4>);
+    kern<<<blocks + seq_grid((size_t)h.Mp * (h.Dp / 8), 128, 16), 128, smem, st>>>(a, blocks, pack);
     SQ_LAUNCHED();
     return (int)DELREC_OK;
   });
@@ -245,12 +246,9 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   g.part = (float2*)(base + h.part); g.part_ld = h.Mp;
   g.bias = bias; g.bias_code = s->dtype; g.scale = a.scale;
   if ((rc = vg_logits(s->dtype == DELREC_F16, h.bnv, false, X, W, g, st))) return rc;
-  k_vocab_lse<<<(a.M + 31) / 32, 1024, 0, st>>>(a, g.part, g.part_ld, (s->V + h.bnv - 1) / h.bnv * 2, each);
+  k_vocab_lse<<<(a.M + 31) / 32, 1024, 0, st>>>(a, g.part, g.part_ld, (s->V + h.bnv - 1) / h.bnv * 2, each,
+                                                  s->reduction == 1, each ? nullptr : out);
   SQ_LAUNCHED();
-  if (!each) {
-    k_vocab_reduce<<<1, 1024, 0, st>>>(a, s->reduction == 1, out);
-    SQ_LAUNCHED();
-  }
   return DELREC_OK;
 }
 
@@ -274,8 +272,8 @@ int delrec_vocab_loss_backward(const delrec_vocab* s, const void* x, const void*
   k_vocab_coef<<<1, 1024, 0, st>>>(a, s->reduction, g_out, coef, inv);
   SQ_LAUNCHED();
   VgSide X, W;
-  int rc = vocab_operands(s, h, a, x, w, base, &X, &W, st);
-  if (rc) return rc;
+  int rc = vocab_pack_run(s, vocab_x(s, h, a, base, &X), st);
+  if (rc || (rc = vocab_w(s, h, a, base, &W, st))) return rc;
   const VgSide G{base + h.G, h.Vc, h.Mp, h.Vc, h.g_piece, h.gp};
   const long long MK = (long long)a.M * a.K;
   for (int c = 0; c < h.count; ++c) {

@@ -28,6 +28,7 @@ struct VocabArgs {
   int *rows, *rowmap, *pos;        // count; position of each packed row; packed row of each position or -1
   int* idx;                        // (M, K) of packed rows; -1: left out or out of range
   float *p, *y, *h, *lse, *loss;   // p and y (M, K); h, lse, loss (M): of packed rows
+  int* ticket;                     // blocks that are done with their rows' losses
   int* status;
 };
 
@@ -105,19 +106,30 @@ static __global__ void __launch_bounds__(1024) k_vocab_rows(const VocabArgs a, c
     if (on) a.rowmap[at] = m;
     else if (each) each[m] = 0.f;
   }
-  if (tid == 0 && first + 1024 >= a.M) *a.rows = total;
+  if (tid == 0 && first + 1024 >= a.M) {
+    *a.rows = total;
+    *a.ticket = 0;
+  }
 }
 
 // Rows as tensor-core operands: out[piece][row][Dp], 16-bit types as they are, fp32 in three bf16 pieces
 // (v = p0 + p1 + p2 exactly).  rows NULL: n rows in place, else the packed rows of x and zero rows up to
 // the next 64.  A thread takes eight columns.
-template <class T, bool VEC>
-__global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, long long st, long long sb, int B,
-                                                    const int* __restrict__ rows, const int* __restrict__ rowmap,
-                                                    long long n, int D, int Dp, long long piece, void* out) {
+struct VocabPack {
+  const void* src;
+  long long st, sb, n, piece;
+  int B, D, Dp, vec;               // vec: 16 bytes of a row at a time
+  const int *rows, *rowmap;
+  void* out;
+};
+template <class T>
+__device__ __forceinline__ void vocab_pack(const VocabPack& k_, long long first, long long step) {
+  const T* src = (const T*)k_.src;
+  const int *rows = k_.rows, *rowmap = k_.rowmap, B = k_.B, D = k_.D, Dp = k_.Dp;
+  const long long n = k_.n, st = k_.st, sb = k_.sb, piece = k_.piece;
   const int cols = Dp / 8;
   const long long real = rows ? *rows : n, all = (rows ? (real + 63) / 64 * 64 : n) * cols;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+  for (long long i = first; i < all; i += step) {
     const long long r = i / cols;
     const int c = (int)(i % cols) * 8;
     float v[8];
@@ -126,7 +138,7 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, l
     if (r < real) {
       const long long m = rows ? rowmap[r] : r;
       const T* s = src + (rows ? m / B * st + m % B * sb : m * st) + c;
-      if (VEC && c + 8 <= D) {
+      if (k_.vec && c + 8 <= D) {
         constexpr int W = 16 / sizeof(T);
 #pragma unroll
         for (int k = 0; k < 8; k += W) unpack_vec<T, W>(*(const VecOf<T, W>*)(s + k), v + k);
@@ -137,7 +149,7 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, l
       }
     }
     using E = std::conditional_t<std::is_same_v<T, __half>, __half, __nv_bfloat16>;
-    E* o = (E*)out + r * Dp + c;
+    E* o = (E*)k_.out + r * Dp + c;
     constexpr int P = sizeof(T) == 4 ? 3 : 1;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -153,12 +165,22 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const T* __restrict__ src, l
   }
 }
 
+template <class T>
+__global__ void __launch_bounds__(256) k_vocab_pack(const VocabPack k) {
+  vocab_pack<T>(k, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
+}
+
 // The targets of a packed row: p, the sums of p over repeated indices, the targets' logits y (dot
 // products in float32) and h = sum p (log p - ln2 y).  W warps to a row: four, x staged as it is (16
 // bytes a lane: laid out in float32 its reads took the time: 4096 rows of 64 targets 72 us, 54 so), or
-// one for up to four targets (8192 rows of one target: 17 us with a block to a row, 9 so).
+// one for up to four targets (8192 rows of one target: 17 us with a block to a row, 9 so).  The blocks
+// from `blocks` on bring x into operands: both wait for the packed rows alone.
 template <class T, bool VEC, int W>
-__global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a) {
+__global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a, int blocks, const VocabPack pack) {
+  if ((int)blockIdx.x >= blocks) {
+    vocab_pack<T>(pack, (blockIdx.x - blocks) * 128LL + threadIdx.x, (gridDim.x - blocks) * 128LL);
+    return;
+  }
   extern __shared__ float smf[];
   __shared__ float s_red[4], s_few[W == 1 ? 32 : 1];
   const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
@@ -288,12 +310,15 @@ __device__ __forceinline__ void vocab_join(float& top, float& sum, float2 v) {
   sum = sum * exp2f(top - at) + v.y * exp2f(v.x - at);
   top = mx;
 }
+// out not NULL: the block that comes last adds the rows' losses up, in a fixed order (their mean: divided;
+// 0 of none).
 static __global__ void __launch_bounds__(1024) k_vocab_lse(const VocabArgs a, const float2* __restrict__ part,
-                                                           long long ld, int tiles, float* each) {
+                                                           long long ld, int tiles, float* each, int mean, float* out) {
   __shared__ float2 s[32][33];
+  __shared__ int s_last;
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
-  const int rows = *a.rows, r = blockIdx.x * 32 + lane;
-  if (blockIdx.x * 32 >= rows) return;
+  const int rows = *a.rows, r = blockIdx.x * 32 + lane, used = max((rows + 31) / 32, 1);
+  if ((int)blockIdx.x >= used) return;
   float top = -INFINITY, sum = 0.f;
   if (r < rows)
     for (int t0 = run; t0 < tiles; t0 += 32 * 8) {
@@ -312,27 +337,35 @@ static __global__ void __launch_bounds__(1024) k_vocab_lse(const VocabArgs a, co
     }
     __syncthreads();
   }
-  if (run || r >= rows) return;
-  const float lse = top + log2f(sum);
-  a.lse[r] = lse;
-  const float loss = a.tau * a.tau * fmaf(kLn2v, lse, a.h[r]);
-  a.loss[r] = loss;
-  if (each) each[a.rowmap[r]] = loss;
-}
-// the sum or the mean of the rows' losses (0 of none), in a fixed order
-static __global__ void __launch_bounds__(1024) k_vocab_reduce(const VocabArgs a, int mean, float* out) {
-  __shared__ double s[32];
-  const int rows = *a.rows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (run == 0) {
+    if (r < rows) {
+      const float lse = top + log2f(sum);
+      a.lse[r] = lse;
+      const float loss = a.tau * a.tau * fmaf(kLn2v, lse, a.h[r]);
+      a.loss[r] = loss;
+      if (each) each[a.rowmap[r]] = loss;
+    }
+    if (out) {
+      __threadfence();
+      __syncwarp();
+      if (lane == 0) s_last = atomicAdd(a.ticket, 1) == used - 1;
+    }
+  }
+  if (!out) return;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  double* total = (double*)s;
   double v = 0.0;
 #pragma unroll 4
-  for (int r = threadIdx.x; r < rows; r += 1024) v += a.loss[r];
+  for (int k = threadIdx.x; k < rows; k += 1024) v += __ldcg(a.loss + k);
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane == 0) s[warp] = v;
+  if (lane == 0) total[run] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
     v = 0.0;
-    for (int w = 0; w < 32; ++w) v += s[w];
+    for (int w = 0; w < 32; ++w) v += total[w];
     *out = (float)(mean && rows > 0 ? v / rows : v);
   }
 }

@@ -150,3 +150,24 @@ def test_one_of_two_gradients():
         ref = O.short_conv(**d, **(dict(gy=gy) if use == "y" else dict(gs=gs)))
         (dx,) = torch.autograd.grad(y if use == "y" else new, c["x"], (gy if use == "y" else gs).cuda())
         within(dx, ref["dx"], ref["e_dx"], "dx")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", range(1, 9))
+@pytest.mark.parametrize("N", [5, 12])
+def test_steps_of_every_filter(dtype, K, N):
+    """Two single steps have the bits of a walk over two rows, wherever the filter stands in memory."""
+    from delrec.short_conv import short_conv, short_conv_step
+    g = torch.Generator().manual_seed(K)
+    B = 7
+    x = torch.randn(2, B, N, generator=g).to("cuda", dtype)
+    w = torch.randn(N * K + 1, generator=g).cuda()[1:].view(N, K)
+    b = torch.randn(N, generator=g).cuda()
+    s = torch.randn(K - 1, B, N, generator=g).to("cuda", dtype)
+    want, last = short_conv(x, w, b, s)
+    for filt in (w, w.clone()):
+        out = s.clone()
+        for t in range(2):
+            y, out = short_conv_step(x[t], filt, b, out, out=out)
+            assert torch.equal(y, want[t])
+        assert torch.equal(out, last)
