@@ -235,18 +235,34 @@ int delrec_selective_step(const delrec_selective* s, const void* x, const void* 
   p.active = active; p.y = y; p.next = next;
   p.x_b = s->x_b; p.dt_b = s->dt_b; p.u_b = s->u_b; p.bm_b = s->bm_b; p.cm_b = s->cm_b;
   const cudaStream_t st = (cudaStream_t)stream;
-  const int L = sel_lanes(s->S);
+  p.Dg = s->N / s->G;
+  const SelAlign al(s);
+  p.bcvec = al.states(s, Bm, Cm);
+  const int L = sel_lanes(s->S), L8 = L >= 4 ? L / 2 : L;
+  const long long threads = kSeqSMs * 1024LL, NL = (long long)s->N * L8;
+  if (state && p.four && s->B * NL > threads) {   // more than run at once: eight states to a lane from S = 9 on
+    const int rows = (int)std::max<long long>(1, threads / NL);
+    const long long blocks = (rows * NL + 255) / 256;
+    if (blocks > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
+    return by_dtype(s->dtype, [&](auto t) {
+      using E = decltype(t);
+      void (*kern)(SelStep, int) = L == 1 ? k_sel_steps<E, 1, 4> : L == 2 ? k_sel_steps<E, 2, 4> : L == 4 ? k_sel_steps<E, 2, 8>
+                                 : L == 8 ? k_sel_steps<E, 4, 8> : L == 16 ? k_sel_steps<E, 8, 8> : k_sel_steps<E, 16, 8>;
+      kern<<<(unsigned)blocks, 256, 0, st>>>(p, rows);
+      SQ_LAUNCHED();
+      return (int)DELREC_OK;
+    });
+  }
   const long long blocks = ((long long)s->B * s->N * L + 255) / 256;
   if (blocks > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
-  const auto go = [&](auto t) {
+  return by_dtype(s->dtype, [&](auto t) {
     using E = decltype(t);
     void (*kern)(SelStep) = L == 1 ? k_sel_step<E, 1> : L == 2 ? k_sel_step<E, 2> : L == 4 ? k_sel_step<E, 4>
                           : L == 8 ? k_sel_step<E, 8> : L == 16 ? k_sel_step<E, 16> : k_sel_step<E, 32>;
     kern<<<(unsigned)blocks, 256, 0, st>>>(p);
     SQ_LAUNCHED();
     return (int)DELREC_OK;
-  };
-  return by_dtype(s->dtype, go);
+  });
 }
 
 }  // extern "C"

@@ -1005,9 +1005,11 @@ __global__ void __launch_bounds__(256) k_sel_bc(long long cols, int tiles, const
   }
 }
 
-// One time step: L lanes to a channel, four states a lane.  state and next (B,N,S) may be one tensor.
+// One time step: L lanes to a channel, four states a lane, everything that a lane reads on its way at once.
+// state and next (B,N,S) may be one tensor.
 struct SelStep {
-  int B, N, S, G, softplus, four;   // four: states in 16-byte accesses
+  int B, N, S, G, Dg, softplus;
+  int four, bcvec;                  // four: states in 16-byte accesses; bcvec: B and C in fours
   const void *x, *dt, *Bm, *Cm, *gate;
   const float *A, *D, *bias;
   const float* state;
@@ -1016,66 +1018,159 @@ struct SelStep {
   float* next;
   long long x_b, dt_b, u_b, bm_b, cm_b;
 };
-template <class T, int L>
-__global__ void __launch_bounds__(256) k_sel_step(const SelStep p) {
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  const long long ch = i / L;
-  const int sg = (int)(i % L);
-  const bool on = ch < (long long)p.B * p.N;
-  const int b = on ? (int)(ch / p.N) : 0, n = on ? (int)(ch % p.N) : 0, g = n / (p.N / p.G);
-  const bool act = on && (!p.active || p.active[b]);
-  const long long at = ch * p.S + 4 * sg;
-  float o = 0.f, x = 0.f;
-  if (on) {
-    float h[4] = {};
-    const bool four = p.four;
-    if (p.state) {
-      if (four) {
-        if (4 * sg < p.S) {
-          const float4 v = *(const float4*)(p.state + at);
-          h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
+// What a lane reads of a sequence besides its states, and what it makes of them.  Its quads of states are
+// 4 L apart, so that the lanes of a channel read whole sectors.
+template <class T, int L, int Q>
+struct SelLane {
+  float A[Q], Bv[Q], Cv[Q], x, z, u, D, bias;
+  const SelStep& p;
+  int n, g, s0;
+  __device__ __forceinline__ SelLane(const SelStep& p_, int n_, int s0_) : p(p_), n(n_), s0(s0_) {
+    g = p.G == 1 ? 0 : (unsigned)n / (unsigned)p.Dg;
+  }
+  static constexpr int off(int s) { return s / 4 * 4 * L + s % 4; }
+  __device__ __forceinline__ void weights(bool on) {
+    const float* Ap = p.A + (size_t)n * p.S + s0;
+#pragma unroll
+    for (int s = 0; s < Q; ++s) A[s] = on && s0 + off(s) < p.S ? Ap[off(s)] : 0.f;
+    D = on && p.D ? p.D[n] : 0.f;
+    bias = on && p.bias ? p.bias[n] : 0.f;
+  }
+  __device__ __forceinline__ void inputs(bool act, long long b) {
+    x = z = u = 0.f;
+#pragma unroll
+    for (int s = 0; s < Q; ++s) Bv[s] = Cv[s] = 0.f;
+    if (!act) return;            // what does not count is not read
+    x = to_f(((const T*)p.x)[b * p.x_b + n]);
+    z = to_f(((const T*)p.dt)[b * p.dt_b + n]);
+    if (p.gate) u = to_f(((const T*)p.gate)[b * p.u_b + n]);
+    const T *Bp = (const T*)p.Bm + b * p.bm_b + (long long)g * p.S + s0, *Cp = (const T*)p.Cm + b * p.cm_b + (long long)g * p.S + s0;
+#pragma unroll
+    for (int k = 0; k < Q; k += 4) {
+      if (p.bcvec) {
+        if (s0 + off(k) < p.S) {
+          unpack_vec<T, 4>(*(const VecOf<T, 4>*)(Bp + off(k)), Bv + k);
+          unpack_vec<T, 4>(*(const VecOf<T, 4>*)(Cp + off(k)), Cv + k);
         }
       } else {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          if (4 * sg + s < p.S) h[s] = p.state[at + s];
+        for (int s = k; s < k + 4; ++s)
+          if (s0 + off(s) < p.S) {
+            Bv[s] = to_f(Bp[off(s)]);
+            Cv[s] = to_f(Cp[off(s)]);
+          }
       }
-    }
-    if (act) {
-      float sig;
-      x = to_f(((const T*)p.x)[b * p.x_b + n]);
-      const float d = sel_delta<T, false>(to_f(((const T*)p.dt)[b * p.dt_b + n]) + (p.bias ? p.bias[n] : 0.f), p.softplus, sig);
-      const T* Bp = (const T*)p.Bm + b * p.bm_b + (long long)g * p.S + 4 * sg;
-      const T* Cp = (const T*)p.Cm + b * p.cm_b + (long long)g * p.S + 4 * sg;
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (4 * sg + s < p.S) {
-          h[s] = fmaf(sel_exp2(fmaf(d * kLog2e, p.A[(size_t)n * p.S + 4 * sg + s], kSelLow)), h[s], d * x * to_f(Bp[s]));
-          o = fmaf(to_f(Cp[s]), h[s], o);
-        }
-    }
-    if (four) {
-      if (4 * sg < p.S) *(float4*)(p.next + at) = f4(h);
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (4 * sg + s < p.S) p.next[at + s] = h[s];
     }
   }
+  __device__ __forceinline__ void load(const float* at, float* h) const {
 #pragma unroll
-  for (int k = 1; k < L; k *= 2) o += __shfl_xor_sync(0xffffffffu, o, k);
-  if (on && sg == 0) {
-    float y = 0.f;
-    if (act) {
-      y = fmaf(p.D ? p.D[n] : 0.f, x, o);
-      if (p.gate) {
-        float s, so;
-        const float u = to_f(((const T*)p.gate)[b * p.u_b + n]);
-        sigmoid_pair<false>(u, s, so);
-        y *= u * s;
+    for (int k = 0; k < Q; k += 4) {
+      if (p.four) {
+        if (s0 + off(k) < p.S) unpack_vec<float, 4>(*(const VecOf<float, 4>*)(at + off(k)), h + k);
+      } else {
+#pragma unroll
+        for (int s = k; s < k + 4; ++s)
+          if (s0 + off(s) < p.S) h[s] = at[off(s)];
       }
     }
-    ((T*)p.y)[ch] = from_f<T>(y);
+  }
+  // h <- the next states, written to `at`; the output to y
+  __device__ __forceinline__ void run(bool on, bool act, float* h, float* at, T* y) {
+    float sig, o = 0.f;
+    const float d = sel_delta<T, false>(z + bias, p.softplus, sig), e = d * kLog2e, dx = d * x;
+    if (act) {
+#pragma unroll
+      for (int s = 0; s < Q; ++s) {
+        h[s] = fmaf(sel_exp2(fmaf(e, A[s], kSelLow)), h[s], dx * Bv[s]);
+        o = fmaf(Cv[s], h[s], o);
+      }
+    }
+    if (on) {
+#pragma unroll
+      for (int k = 0; k < Q; k += 4) {
+        if (p.four) {
+          if (s0 + off(k) < p.S) *(float4*)(at + off(k)) = f4(h + k);
+        } else {
+#pragma unroll
+          for (int s = k; s < k + 4; ++s)
+            if (s0 + off(s) < p.S) at[off(s)] = h[s];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 1; j < L; j *= 2) o += __shfl_xor_sync(0xffffffffu, o, j);
+    if (on && s0 == 0) {
+      float v = fmaf(D, x, o);
+      if (p.gate) {
+        float s, so;
+        sigmoid_pair<false>(u, s, so);
+        v *= u * s;
+      }
+      *y = from_f<T>(act ? v : 0.f);
+    }
+  }
+};
+template <class T, int L>
+__global__ void __launch_bounds__(256) k_sel_step(const SelStep p) {
+  const long long i = blockIdx.x * 256LL + threadIdx.x, at = i / L;
+  const bool on = at < (long long)p.B * p.N;
+  const unsigned ch = on ? (unsigned)at : 0u;           // B N fits 31 bits
+  const int b = (int)(ch / (unsigned)p.N);
+  const bool act = on && (!p.active || p.active[b]);
+  SelLane<T, L, 4> t(p, (int)(ch - (unsigned)b * p.N), 4 * (int)(i % L));
+  const long long s = (long long)ch * p.S + t.s0;
+  float h[4] = {};
+  if (on && p.state) t.load(p.state + s, h);
+  t.inputs(act, b);
+  t.weights(act);
+  t.run(on, act, h, p.next + s, (T*)p.y + ch);
+}
+
+// The same where there are more sequences than threads: a lane (Q states) keeps its channel's weights and
+// takes every `rows`-th sequence, whose states are on their way to its own place in shared memory while it
+// works on the ones before (a lane per sequence has too few bytes in flight: 4096 x 512 x 16 states bf16 in
+// a graph 88 -> 61 us, 2048 x 700 x 24 fp32 120 -> 69, of 41 that the states take).
+constexpr int kSelStages = 3;
+__device__ __forceinline__ void cp_async16(void* smem, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <class T, int L, int Q>
+__global__ void __launch_bounds__(256, 4) k_sel_steps(const SelStep p, int rows) {
+  __shared__ float4 ring[kSelStages][Q / 4][256];
+  const long long i = blockIdx.x * 256LL + threadIdx.x, NL = (long long)p.N * L;
+  const bool there = i < NL * rows;
+  long long b = i / NL;
+  SelLane<T, L, Q> t(p, (int)(i % NL / L), 4 * (int)(i % L));
+  t.weights(there);
+  const auto place = [&](long long row) { return (row * p.N + t.n) * p.S + t.s0; };
+  const auto fetch = [&](int stage, long long row) {
+    if (there && row < p.B) {
+#pragma unroll
+      for (int k = 0; k < Q / 4; ++k)
+        if (t.s0 + 4 * L * k < p.S) cp_async16(&ring[stage][k][threadIdx.x], p.state + place(row) + 4 * L * k);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < kSelStages; ++j) fetch(j, b + (long long)j * rows);
+  int stage = 0;
+  for (int k = 0; k < p.B; k += min(rows, p.B - k), b += rows) {   // the same number of rounds in a whole warp
+    const bool on = there && b < p.B;
+    const bool act = on && (!p.active || p.active[b]);
+    t.inputs(act, b);
+    cp_async_wait<kSelStages - 1>();
+    float h[Q] = {};
+#pragma unroll
+    for (int q = 0; q < Q / 4; ++q)
+      if (t.s0 + 4 * L * q < p.S) unpack_vec<float, 4>(*(const VecOf<float, 4>*)&ring[stage][q][threadIdx.x], h + 4 * q);
+    t.run(on, act, h, p.next + place(b), (T*)p.y + b * p.N + t.n);
+    fetch(stage, b + (long long)kSelStages * rows);
+    stage = stage + 1 == kSelStages ? 0 : stage + 1;
   }
 }
 

@@ -192,3 +192,30 @@ def test_one_of_two_gradients_and_of_one_input():
             y, hT = _call(c)
             (v,) = torch.autograd.grad(y if use == "y" else hT, c[k], (gy if use == "y" else gh).cuda())
             within(v, ref[NAMES[k]], ref["e_" + NAMES[k]], f"{NAMES[k]} of {use}")
+
+
+@pytest.mark.parametrize("N,S,G,B", [(5, 4, 1, 31001), (512, 8, 1, 303), (700, 24, 2, 57), (40, 64, 4, 501), (33, 128, 3, 301),
+                                     (16, 12, 1, 5003), (6000, 16, 1, 31)])
+def test_step_of_many_sequences(N, S, G, B):
+    """More states than threads: the states of the same calls on few sequences, bit for bit, and their
+    outputs but for the order of a sum of S products."""
+    from delrec.selective import selective_step
+    g = torch.Generator().manual_seed(N)
+    rnd = lambda *s: torch.randn(*s, generator=g).cuda()   # noqa: E731
+    x, dt, gate = rnd(B, N), rnd(B, N), rnd(B, N)
+    A, Bm, C, D, bias = -rnd(N, S).abs(), rnd(B, G, S), rnd(B, G, S), rnd(N), rnd(N)
+    state = rnd(B, N, S)
+    active = (torch.rand(B, generator=g) < 0.8).cuda()
+    x[~active] = float("nan")               # what does not count is not read
+    kw = dict(D=D, dt_bias=bias)
+    few = max(1, B // 40)
+    parts = [selective_step(x[i:i + few], dt[i:i + few], A, Bm[i:i + few], C[i:i + few], state[i:i + few], gate=gate[i:i + few],
+                            active=active[i:i + few], **kw) for i in range(0, B, few)]
+    y, nxt = (torch.cat(v) for v in zip(*parts))
+    mag = (C.abs().repeat_interleave(N // G, 1) * nxt.abs()).sum(-1) + (D * x).abs()
+    tol = torch.where(active[:, None], (S + 2) * 2.0 ** -23 * mag * gate.abs(), torch.zeros_like(y))
+    for out in (None, state.clone()):
+        got, h = selective_step(x, dt, A, Bm, C, state if out is None else out, gate=gate, active=active, out=out, **kw)
+        assert torch.equal(h, nxt)
+        assert ((got - y).abs() <= tol).all()
+        assert torch.equal(h[~active], state[~active]) and (got[~active] == 0).all()
