@@ -82,7 +82,7 @@ __device__ __forceinline__ uint32_t vg_first(uint32_t addr) {
   return r;
 }
 __device__ __forceinline__ void vg_arrive(uint32_t bar) {   // a shared::cluster address
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void vg_mma(uint32_t tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
   asm volatile(
