@@ -7,12 +7,12 @@
 // A thread holds 2 channels x 4 states; L lanes (4 L >= S) share a channel's states, the other
 // 32 / L lane groups of a warp hold other channels.  The sums over states (y, dx, ddt) run over four
 // values in the thread and then over L lanes, those over channels (dB, dC) over two values and then
-// over 32 / L lanes: either way a lane hands on half of what it holds at each exchange.  A block walks kSelSeg steps at a time, whose
-// inputs it lays out in shared memory in float32; states stay in registers.
+// over 32 / L lanes: either way a lane hands on half of what it holds at each exchange.  A block walks
+// kSelSeg steps at a time, whose inputs it lays out in shared memory in float32; states stay in registers.
 //
 // The backward pass keeps the states before every kSelSeg-th step (written by the forward pass),
 // recomputes those in between into shared memory and walks the segment back.  Where the rows are
-// few, time is cut into chunks: their affine maps come first (k_sel_local; the product of a chunk's
+// few, time is cut into chunks: their affine maps come first (LOCAL passes; the product of a chunk's
 // decays is exp(A sum delta)), are joined in time order (k_sel_join), and then every chunk runs from
 // its own start.
 //
@@ -20,10 +20,17 @@
 // step, not with A, whose rounding would pull every step of a state the same way (the state after 500
 // bf16 steps on average 7.9e-7 -> 3.6e-7 off).
 //
-// What bounds it: the exponentials, 16 a clock and SM (one a state forward, two backward), with the
-// issue slots close behind.  Sums and states are float32.
+// What bounds it.  At T=250 B=256 N=512 S=16 fp32 the forward kernel takes FWD us (its bytes, the kept
+// states among them, 120; the exponentials, 16 a clock and SM, 116), the backward kernel BWD (180 and 233).
+// Both are held up by shared memory and by waiting: 21 and 67 wavefronts a warp, step and 256 states (a
+// 16-byte read by 32 lanes is four, however many of them read the same), 73 and 250 instructions, on 20 and
+// 12 warps an SM, as many as their registers allow.  Of four channels by four states to a thread (fewer
+// reads of B and C, 255 registers: 886 to 1090), the states or the decays of half a segment in registers
+// (862 to 1240) and keeping every other state (846 to 909) none was faster backward.  Sums and states are
+// float32.
 #pragma once
 
+#include "f32x2.cuh"
 #include "seq_common.cuh"
 
 namespace delrec {
@@ -61,24 +68,6 @@ __device__ __forceinline__ float sel_exp2(float v) {
   return r;
 }
 
-// Two floats in one register pair: sm_100 multiplies and adds them in one issue slot.
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pair(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void split(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ f2 exp22(f2 v) {
   float a, b;
   split(v, a, b);

@@ -24,6 +24,7 @@
 // Every wait is bounded: on expiry the CTA records ST_TIMEOUT, drains its copies and returns.
 #pragma once
 
+#include "f32x2.cuh"
 #include "seq_common.cuh"
 #include "tc_ptx.cuh"
 
@@ -175,6 +176,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
   __shared__ __align__(8) uint64_t bars[2 * STAGES + 4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ float4 s_bias[EPI == VG_OUT ? 1 : kVgEpi][8];   // 32 columns' bias of each epilogue warp
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (smem_u32(dsm) + 1023u) & ~1023u, sA = base, sB = base + STAGES * A_BYTES;
   const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]);
@@ -330,15 +332,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
           float top = -INFINITY, sum = 0.f;
           // 32 columns of the row
           const auto chunk = [&](int n, float* v) {
+            f2 w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pair(v[2 * i], v[2 * i + 1]);
             if (g.bias) {
               const float b = n + lane < g.N ? (g.bias_code == DELREC_F32 ? ((const float*)g.bias)[g.b_mn + n + lane]
                                                : F16 ? to_f(((const __half*)g.bias)[g.b_mn + n + lane])
                                                      : to_f(((const __nv_bfloat16*)g.bias)[g.b_mn + n + lane]))
                                              : 0.f;
+              __syncwarp();
+              ((float*)s_bias[warp])[lane] = b;
+              __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, b, i);
+              for (int i = 0; i < 8; ++i) {
+                const float4 b4 = s_bias[warp][i];
+                w[2 * i] = add2(w[2 * i], pair(b4.x, b4.y));
+                w[2 * i + 1] = add2(w[2 * i + 1], pair(b4.z, b4.w));
+              }
             }
+            const f2 scale = pair(g.scale, g.scale);
             if constexpr (EPI == VG_STATS) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) split(w[i], v[2 * i], v[2 * i + 1]);
               if (n + 32 > g.N) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = n + i < g.N ? v[i] : -INFINITY;
@@ -348,30 +363,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
               for (int i = 4; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
               const float mx = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * g.scale);
               const float at = mx == -INFINITY ? 0.f : mx;
-              float s4[4] = {sum * vg_exp2(top - at), 0.f, 0.f, 0.f};
+              const f2 low = pair(-at, -at);
+              f2 s2[2] = {pair(sum * vg_exp2(top - at), 0.f), pair(0.f, 0.f)};
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s4[i & 3] += vg_exp2(fmaf(v[i], g.scale, -at));
+              for (int i = 0; i < 16; ++i) {
+                float a, b;
+                split(fma2(pair(v[2 * i], v[2 * i + 1]), scale, low), a, b);
+                s2[i & 1] = add2(s2[i & 1], pair(vg_exp2(a), vg_exp2(b)));
+              }
+              float s4[4];
+              split(s2[0], s4[0], s4[1]);
+              split(s2[1], s4[2], s4[3]);
               sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
               top = mx;
             } else {
+              const f2 low = pair(-lse, -lse), c2 = pair(coef, coef);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = coef * vg_exp2(fmaf(v[i], g.scale, -lse));
+              for (int i = 0; i < 16; ++i) {
+                float a, b;
+                split(fma2(w[i], scale, low), a, b);
+                split(mul2(pair(vg_exp2(a), vg_exp2(b)), c2), v[2 * i], v[2 * i + 1]);
+              }
               if (n + 32 > g.N) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = n + i < g.N ? v[i] : 0.f;
               }
-              if (!in) {
+              if (m0 + q * 32 + 32 > M) {   // the last rows' tile
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                for (int i = 0; i < 32; ++i) v[i] = in ? v[i] : 0.f;
               }
               using E = std::conditional_t<F16, __half, __nv_bfloat16>;
-              E* dst = (E*)g.G + (long long)m * g.g_ld;
-              for (int pc = 0; pc < g.pieces; ++pc) {
-                vg_store_row<E, 32>(dst + pc * g.g_piece, n, (int)g.g_ld, v);
-                if (pc + 1 < g.pieces) {   // what the piece leaves
+              E* dst = (E*)g.G + (long long)m * g.g_ld + n;   // (a row's pitch is a multiple of 256)
+              for (int pc = 0;; ++pc) {
+                uint32_t h[16];
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) v[i] -= to_f(from_f<E>(v[i]));
-                }
+                for (int i = 0; i < 16; ++i) h[i] = vg_pack2<F16>(v[2 * i], v[2 * i + 1]);
+                vg_store32(dst, h);
+                vg_store32(dst + 16, h + 8);
+                if (pc + 1 == g.pieces) break;
+                dst += g.g_piece;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] -= to_f(from_f<E>(v[i]));   // what the piece leaves
               }
               __syncwarp();
             }
