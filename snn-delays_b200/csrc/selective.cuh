@@ -20,8 +20,8 @@
 // step, not with A, whose rounding would pull every step of a state the same way (the state after 500
 // bf16 steps on average 7.9e-7 -> 3.6e-7 off).
 //
-// What bounds it.  At T=250 B=256 N=512 S=16 fp32 the forward kernel takes FWD us (its bytes, the kept
-// states among them, 120; the exponentials, 16 a clock and SM, 116), the backward kernel BWD (180 and 233).
+// What bounds it.  At T=250 B=256 N=512 S=16 fp32 the forward kernel takes 300 us (its bytes, the kept
+// states among them, 120; the exponentials, 16 a clock and SM, 116), the backward kernel 850 (180 and 233).
 // Both are held up by shared memory and by waiting: 21 and 67 wavefronts a warp, step and 256 states (a
 // 16-byte read by 32 lanes is four, however many of them read the same), 73 and 250 instructions, on 20 and
 // 12 warps an SM, as many as their registers allow.  Of four channels by four states to a thread (fewer
