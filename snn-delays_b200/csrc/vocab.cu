@@ -73,10 +73,10 @@ static int vocab_splits(long long tm, long long tn, int bn, long long kb, int np
 
 struct VocabShape {
   long long M, Mp, Dp, x_piece, w_piece, g_piece;
-  int pieces, gp, esz, bnv, bnd, Vc, count; // gp pieces of G; Vc columns in each of `count` pieces of the vocabulary
+  int pieces, gp, bnv, bnd, Vc, count; // gp pieces of G; Vc columns in each of `count` pieces of the vocabulary
   int dx_splits, dw_splits, db_runs;
   bool w_direct;                            // W is an operand as it lies
-  size_t x, w, part, flags, ticket, h, each, G, coef, inv, dx, dw, db, total;
+  size_t x, w, part, flags, ticket, h, G, coef, inv, dx, dw, db, total;
 };
 constexpr size_t kVocabBudget = 256u << 20;   // bytes of G at once
 static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
@@ -89,7 +89,6 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
   // Of few rows, where its roundings do not average out and the products wait for W anyway, a second
   // piece is kept.
   h.gp = h.pieces == 3 ? 3 : h.M <= 512 ? 2 : 1;
-  h.esz = s->dtype == DELREC_F32 ? 4 : 2;
   h.x_piece = h.Mp * h.Dp;
   h.w_piece = (long long)s->V * h.Dp;
   h.bnv = vocab_bn(s->V);
