@@ -208,8 +208,9 @@ def vocab_loss(x, w, index, bias=None, logits=None, tau=1.0, ignore=-100, length
     b = torch.zeros(V, dtype=f) if bias is None else bias.double()
     z = (x2 @ w2.t() + b) / tau
     mag = (x2.abs() @ w2.abs().t() + b.abs()) / tau
-    # the tensor core's accumulator truncates, 2 u of the running sum per 16 products; a dot product of
-    # a target in fp32 adds as much (D / 32 terms a lane, then 5)
+    # the tensor core's accumulator truncates, 2 u of the running sum per 16 products; a target's logit is one
+    # of them and is allowed what a dot product of its own in fp32 would add (D / 32 terms a lane, then 5),
+    # the sum below counting the product's error twice as it is
     ez = (D / 16 + 12) * 2 * U * mag
     et = (D / 32 * 8 + 16) * U * mag
     lse = torch.logsumexp(z, 1)

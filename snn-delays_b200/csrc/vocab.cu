@@ -41,7 +41,7 @@ struct VocabKeep {
     rowmap = take(M * 4);
     pos = take(M * 4);
     idx = take(MK * 4);
-    p = take(s->distill ? MK * 4 : 0);
+    p = take(s->K > 1 ? MK * 4 : 0);
     y = take(MK * 4);
     lse = take(M * 4);
     loss = take(M * 4);
@@ -76,7 +76,7 @@ struct VocabShape {
   int pieces, gp, bnv, bnd, Vc, count; // gp pieces of G; Vc columns in each of `count` pieces of the vocabulary
   int dx_splits, dw_splits, db_runs;
   bool w_direct;                            // W is an operand as it lies
-  size_t x, w, part, flags, ticket, h, G, coef, inv, dx, dw, db, total;
+  size_t x, w, part, tab, flags, ticket, h, G, coef, inv, dx, dw, db, total;
 };
 constexpr size_t kVocabBudget = 256u << 20;   // bytes of G at once
 static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
@@ -101,6 +101,7 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
   if (!backward) {
     const long long tiles = (s->V + h.bnv - 1) / h.bnv * 2;
     h.part = take((size_t)tiles * h.Mp * sizeof(float2));
+    h.tab = take(s->K > 1 ? (size_t)tiles * h.Mp * 4 : 0);
     h.flags = take(s->distill ? h.M : 0);
     h.ticket = take(4);
     h.h = take((size_t)h.M * 4);
@@ -138,7 +139,7 @@ static VocabArgs vocab_args(const delrec_vocab* s, char* keep) {
   a.rowmap = (int*)(keep + k.rowmap);
   a.pos = (int*)(keep + k.pos);
   a.idx = (int*)(keep + k.idx);
-  a.p = s->distill ? (float*)(keep + k.p) : nullptr;
+  a.p = s->K > 1 ? (float*)(keep + k.p) : nullptr;
   a.y = (float*)(keep + k.y);
   a.lse = (float*)(keep + k.lse);
   a.loss = (float*)(keep + k.loss);
@@ -226,14 +227,14 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   const VocabPack pack = vocab_x(s, h, a, base, &X);
   int rc = vocab_w(s, h, a, base, &W, st);
   if (rc) return rc;
+  const int halves = (s->V + h.bnv - 1) / h.bnv * 2;
+  unsigned* tab = s->K > 1 ? (unsigned*)(base + h.tab) : nullptr;
   rc = by_dtype(s->dtype, [&](auto t) {
     using E = decltype(t);
-    const bool vec = !((uintptr_t)w & 15) && s->D % (16 / sizeof(E)) == 0;
-    const int few = s->K <= 4, blocks = few ? (a.M + 3) / 4 : a.M;   // a warp to a row, or a block
-    const size_t smem = few ? 0 : ((size_t)(s->D + 7) / 8 * 8 * sizeof(E) + 15) / 16 * 16 + (size_t)8 * s->K;
-    void (*kern)(VocabArgs, int, VocabPack) = few ? (vec ? k_vocab_targets<E, true, 1> : k_vocab_targets<E, false, 1>)
-                                                  : (vec ? k_vocab_targets<E, true, 4> : k_vocab_targets<E, false, 4>);
-    kern<<<blocks + seq_grid((size_t)h.Mp * (h.Dp / 8), 128, 16), 128, smem, st>>>(a, blocks, pack);
+    const int W = s->K == 1 ? 1 : s->K <= 32 ? 32 : 128, blocks = (a.M + 128 / W - 1) / (128 / W);
+    const size_t smem = W == 1 ? 0 : (size_t)(128 / W) * 4 * s->K * 4;
+    auto kern = W == 1 ? k_vocab_targets<E, 1> : W == 32 ? k_vocab_targets<E, 32> : k_vocab_targets<E, 128>;
+    kern<<<blocks + seq_grid((size_t)h.Mp * (h.Dp / 8), 128, 16), 128, smem, st>>>(a, blocks, pack, tab, h.Mp, halves, h.bnv / 2);
     SQ_LAUNCHED();
     return (int)DELREC_OK;
   });
@@ -243,10 +244,10 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   g.M = -1; g.K = s->D; g.N = s->V; g.splits = 1; g.seg = h.pieces == 3 ? 2 : 0; g.status = a.status; g.spin_ns = 2000000000ll;
   vg_products(&g, h.pieces, h.pieces);
   g.part = (float2*)(base + h.part); g.part_ld = h.Mp;
+  g.idx = a.idx; g.tab = tab; g.z = a.y; g.kept = s->K;
   g.bias = bias; g.bias_code = s->dtype; g.scale = a.scale;
   if ((rc = vg_logits(s->dtype == DELREC_F16, h.bnv, false, X, W, g, st))) return rc;
-  k_vocab_lse<<<(a.M + 31) / 32, 1024, 0, st>>>(a, g.part, g.part_ld, (s->V + h.bnv - 1) / h.bnv * 2, each,
-                                                  s->reduction == 1, each ? nullptr : out);
+  k_vocab_lse<<<(a.M + 31) / 32, 1024, 0, st>>>(a, g.part, g.part_ld, halves, each, s->reduction == 1, each ? nullptr : out);
   SQ_LAUNCHED();
   return DELREC_OK;
 }

@@ -2,8 +2,9 @@
 // follows them:
 //
 //   logits      z = x W^T (rows x vocabulary), never stored.  VG_STATS: each row's maximum and sum of
-//               exponentials over the tile's columns.  VG_GRAD: c_m softmax(z)_mv in the operands'
-//               type, from the row's log-sum-exp, for one piece of the vocabulary.
+//               exponentials over the tile's columns, and the logits of its targets.  VG_GRAD:
+//               c_m softmax(z)_mv in the operands' type, from the row's log-sum-exp, for one piece of the
+//               vocabulary.
 //   dW = G^T x  and  dx += G W  for that piece (VG_OUT).
 //
 // Persistent: a pair of CTAs on two SMs walks 256 x BN output tiles (cta_group::2).  Each keeps 128 rows
@@ -48,6 +49,12 @@ struct VgArgs {
   // VG_STATS: part[2 * column tile + half][row] = {max, sum}, in units of log2
   float2* part;
   long long part_ld;
+  // .. and the rows' targets: their columns in rising order (rows, kept), where a half tile's begin (see
+  // k_vocab_targets; NULL for kept = 1), their logits
+  const int* idx;
+  const unsigned* tab;
+  float* z;
+  int kept;
   const void* bias;             // of the columns (element type), NULL: 0
   int bias_code;                // its element type
   float scale;                  // log2(e) / temperature
@@ -314,6 +321,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
       const int sp = tile_s(w);
       const int s0 = first_seg(sp), s1 = first_seg(sp + 1);
       const int m = m0 + q * 32 + lane;
+      // the next target's column, its place in the row's list, and the target behind it
+      unsigned next = ~0u, after = ~0u;
+      int pos = 0;
+      const int* list = nullptr;
+      if (EPI == VG_STATS && m < M) {
+        list = g.idx + (long long)m * g.kept;
+        if (g.kept == 1) {
+          next = *list;
+        } else {
+          const unsigned t = g.tab[(2 * ct + half) * g.part_ld + m];
+          pos = t >> 8;
+          if ((t & 255) != 255) {
+            next = n0 + (t & 255);
+            if (pos + 1 < g.kept) after = list[pos + 1];
+          }
+        }
+      }
       // a part without segments still writes its zeros
       for (int s = s0; ok && (s < s1 || s == s0); ++s) {
         const bool have = s < s1;
@@ -358,6 +382,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = n + i < g.N ? v[i] : -INFINITY;
               }
+              unsigned at32;
+              while ((at32 = next - (unsigned)n) < 32u) {
+                float u[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) u[i] = at32 & 16 ? v[i + 16] : v[i];
+#pragma unroll
+                for (int o = 8; o; o >>= 1)
+#pragma unroll
+                  for (int i = 0; i < o; ++i) u[i] = at32 & o ? u[i + o] : u[i];
+                g.z[(long long)m * g.kept + pos] = u[0];
+                ++pos;
+                next = after;
+                after = pos + 1 < g.kept ? list[pos + 1] : ~0u;
+              }
+              __syncwarp();
               float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
               for (int i = 4; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);

@@ -6,7 +6,7 @@
 //   d loss_m / d z_v = tau (q_v - sum_{k: i_k = v} p_k)
 //
 // p = softmax(t / tau) over the K kept logits t of a teacher; the cross entropy is K = 1, p = 1,
-// tau = 1.  Logits are carried as y = z log2(e) / tau, sums in float32.
+// tau = 1.  Exponentials are of y = z log2(e) / tau, sums in float32.
 #pragma once
 
 #include "seq_common.cuh"
@@ -26,8 +26,8 @@ struct VocabArgs {
   const void *x, *w, *bias, *index, *logits, *lengths;
   uint8_t* flags;                  // (M) distillation: does the position count
   int *rows, *rowmap, *pos;        // count; position of each packed row; packed row of each position or -1
-  int* idx;                        // (M, K) of packed rows; -1: left out or out of range
-  float *p, *y, *h, *lse, *loss;   // p and y (M, K); h, lse, loss (M): of packed rows
+  int* idx;                        // (M, K) of packed rows: tokens in rising order, each once, then -1
+  float *p, *y, *h, *lse, *loss;   // p (NULL for K = 1: 1) and y (M, K): z, then log2 q; h, lse, loss (M): of packed rows
   int* ticket;                     // blocks that are done with their rows' losses
   int* status;
 };
@@ -170,138 +170,132 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const VocabPack k) {
   vocab_pack<T>(k, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
 }
 
-// The targets of a packed row: p, the sums of p over repeated indices, the targets' logits y (dot
-// products in float32) and h = sum p (log p - ln2 y).  W warps to a row: four, x staged as it is (16
-// bytes a lane: laid out in float32 its reads took the time: 4096 rows of 64 targets 72 us, 54 so), or
-// one for up to four targets (8192 rows of one target: 17 us with a block to a row, 9 so).  The blocks
-// from `blocks` on bring x into operands: both wait for the packed rows alone.
-template <class T, bool VEC, int W>
-__global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a, int blocks, const VocabPack pack) {
+// The targets of a packed row, W threads to it: their tokens in rising order, each once, with the sum of its
+// p (then -1), h = sum p log p, and where each half tile of the logits (`cols` columns) finds its first target:
+// tab[half][row] = place in the list << 8 | column, 255 without one.  Their logits come from the product that
+// makes the statistics: a dot product of its own is off by another rounding than the log-sum-exp (the tensor
+// core's accumulator truncates), and that difference is all there is of the loss of a target that is nearly
+// certain (z = 40 over 512 channels: -4e-5 of 0).  The blocks from `blocks` on bring x into operands:
+// both wait for the packed rows alone.
+template <class T, int W>
+__global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a, int blocks, const VocabPack pack, unsigned* tab,
+                                                       long long ld, int halves, int cols) {
   if ((int)blockIdx.x >= blocks) {
     vocab_pack<T>(pack, (blockIdx.x - blocks) * 128LL + threadIdx.x, (gridDim.x - blocks) * 128LL);
     return;
   }
-  extern __shared__ float smf[];
-  __shared__ float s_red[4], s_few[W == 1 ? 32 : 1];
-  const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (r >= *a.rows) return;        // with W = 1 a whole warp: no block-wide barrier below
-  const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5, tid = W == 1 ? lane : threadIdx.x, K = a.K, D = a.D;
-  constexpr int nt = 32 * W;
-  constexpr int N = 16 / sizeof(T);      // the same order of sums whatever the alignment
-  const int Dn = (D + N - 1) / N * N;
-  T* s_x = (T*)smf;                                                          // [Dn], W = 4
-  float* s_p = W == 1 ? s_few + (threadIdx.x >> 5) * 8 : (float*)(s_x + Dn);  // [K]
-  int* s_i = (int*)(s_p + (W == 1 ? 4 : K));                                 // [K]
-  const auto sync = [] {
-    if (W == 1) __syncwarp();
-    else __syncthreads();
-  };
-  const int m = a.rowmap[r];
-  const T* x = (const T*)a.x + m / a.B * a.x_t + m % a.B * a.x_b;
-  if (W > 1)
-    for (int d = tid; d < Dn; d += nt) s_x[d] = d < D ? x[d] : from_f<T>(0.f);
-  const auto all = [&](float v, bool max) {
+  const int r = blockIdx.x * (128 / W) + threadIdx.x / W;
+  if (r >= *a.rows) return;        // whole warps with W = 32, the whole block with W = 128
+  const int m = a.rowmap[r], K = a.K;
+  if constexpr (W == 1) {          // K = 1: p = 1
+    const long long i = vocab_index(a, m);
+    const bool in = i >= 0 && i < a.V, ok = in && (!a.distill || fabsf(vocab_teacher(a, m)) < INFINITY);
+    if (!in) atomicOr(a.status, kVocabIndexRange);
+    a.idx[r] = ok ? (int)i : -1;
+    if (!ok) a.y[r] = __int_as_float(0x7fc00000);
+  } else {
+    extern __shared__ int smi[];
+    __shared__ float s_red[4];
+    const int tid = threadIdx.x % W, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int* s_i = smi + threadIdx.x / W * 4 * K;       // [K] tokens; -1 left out, -2 out of range; later in rising order
+    float* s_p = (float*)(s_i + K);                 // [K]
+    int* s_u = s_i + 2 * K;                         // [K] the token where it stands first, else kNone
+    float* s_s = (float*)(s_i + 3 * K);             // [K] the sum of its p
+    constexpr int kNone = 0x7fffffff;
+    const auto sync = [] {
+      if (W == 32) __syncwarp();
+      else __syncthreads();
+    };
+    const auto all = [&](float v, bool max) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float u = __shfl_xor_sync(0xffffffffu, v, o);
-      v = max ? fmaxf(v, u) : v + u;
+      for (int o = 16; o; o >>= 1) {
+        const float u = __shfl_xor_sync(0xffffffffu, v, o);
+        v = max ? fmaxf(v, u) : v + u;
+      }
+      if (W > 32) {
+        __syncthreads();
+        if (lane == 0) s_red[warp] = v;
+        __syncthreads();
+        v = s_red[0];
+        for (int w = 1; w < 4; ++w) v = max ? fmaxf(v, s_red[w]) : v + s_red[w];
+      }
+      return v;
+    };
+    float top = -INFINITY, h = 0.f;
+    for (int k = tid; k < K; k += W) {
+      const size_t e = (size_t)m * K + k;
+      long long i = vocab_index(a, e);
+      float t = vocab_teacher(a, e);
+      if (!vocab_kept(i, t)) {
+        i = -1;
+        t = -INFINITY;
+      } else if (i >= a.V) {
+        atomicOr(a.status, kVocabIndexRange);
+        i = -2;
+        h = __int_as_float(0x7fc00000);
+      }
+      s_i[k] = (int)i;
+      s_p[k] = t;
+      top = fmaxf(top, t);
     }
-    if (W > 1) {
-      __syncthreads();
-      if (lane == 0) s_red[warp] = v;
-      __syncthreads();
-      v = s_red[0];
-      for (int w = 1; w < W; ++w) v = max ? fmaxf(v, s_red[w]) : v + s_red[w];
-    }
-    return v;
-  };
-  float top = -INFINITY;
-  for (int k = tid; k < K; k += nt) {
-    const size_t e = (size_t)m * K + k;
-    long long i = vocab_index(a, e);
-    float t = a.distill ? vocab_teacher(a, e) : 0.f;
-    if (a.distill && !vocab_kept(i, t)) {
-      i = -1;
-      t = -INFINITY;
-    } else if (i < 0 || i >= a.V) {
-      atomicOr(a.status, kVocabIndexRange);
-      i = -2;
-    }
-    s_i[k] = (int)i;
-    s_p[k] = t;
-    top = fmaxf(top, t);
-  }
-  float h = 0.f;
-  if (a.distill) {   // differences first: logits of the type's lowest value stay finite at any temperature
+    // differences first: logits of the type's lowest value stay finite at any temperature
     top = all(top, true);
     float sum = 0.f;
-    for (int k = tid; k < K; k += nt) sum += s_i[k] == -1 ? 0.f : expf((s_p[k] - top) / a.tau);
-    sum = all(sum, false);
-    const float ls = logf(sum);
-    for (int k = tid; k < K; k += nt) {
+    for (int k = tid; k < K; k += W) sum += s_i[k] == -1 ? 0.f : expf((s_p[k] - top) / a.tau);
+    const float ls = logf(all(sum, false));
+    for (int k = tid; k < K; k += W) {
       const float lp = (s_p[k] - top) / a.tau - ls, p = s_i[k] == -1 ? 0.f : expf(lp);
       s_p[k] = p;
       if (p != 0.f) h = fmaf(p, lp, h);
     }
-  } else if (tid == 0) {
-    s_p[0] = 1.f;
-  }
-  sync();
-  if (a.p)
-    for (int k = tid; k < K; k += nt) {
-      float s = 0.f;
+    h = all(h, false);
+    if (tid == 0) a.h[r] = h;
+    sync();
+    float own = 0.f;
+    for (int k = tid; k < K; k += W) {
       const int i = s_i[k];
+      float s = 0.f;
+      int first = K;
 #pragma unroll 4
-      for (int j = 0; j < K; ++j) s += s_i[j] == i ? s_p[j] : 0.f;
-      a.p[(size_t)r * K + k] = s;
-    }
-  // four targets at a time, their rows of W on the way together
-  const T* w = (const T*)a.w;
-  for (int k0 = warp * 4; k0 < K; k0 += W * 4) {
-    float dot[4] = {};
-    const T* row[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) row[j] = w + (size_t)max(s_i[min(k0 + j, K - 1)], 0) * D;   // (row 0: not used)
-#pragma unroll 2
-    for (int d = lane * N; d < D; d += 32 * N) {
-      VecOf<T, N> q[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (VEC) {
-          q[j] = *(const VecOf<T, N>*)(row[j] + d);
-        } else {
-#pragma unroll
-          for (int i = 0; i < N; ++i) q[j].v[i] = d + i < D ? row[j][d + i] : from_f<T>(0.f);
+      for (int j = K - 1; j >= 0; --j)
+        if (s_i[j] == i) {
+          s += s_p[j];
+          first = j;
         }
+      const bool on = i >= 0 && first == k;
+      s_u[k] = on ? i : kNone;
+      s_s[k] = s;
+      own += on;
+    }
+    const int n = (int)all(own, false);
+    sync();
+    for (int k = tid; k < K; k += W) {
+      const int i = s_u[k];
+      if (i != kNone) {
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < K; ++j) rank += s_u[j] < i;
+        s_i[rank] = i;
+        a.idx[(size_t)r * K + rank] = i;
+        a.p[(size_t)r * K + rank] = s_s[k];
       }
-      float xv[N];
-#pragma unroll
-      for (int i = 0; i < (W == 1 ? N : 0); ++i) xv[i] = d + i < D ? to_f(x[d + i]) : 0.f;
-      if (W > 1) unpack_vec<T, N>(*(const VecOf<T, N>*)(s_x + d), xv);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float f[N];
-        unpack_vec<T, N>(q[j], f);
-#pragma unroll
-        for (int i = 0; i < N; ++i) dot[j] = fmaf(xv[i], f[i], dot[j]);
+      if (k >= n) {
+        a.idx[(size_t)r * K + k] = -1;
+        a.p[(size_t)r * K + k] = a.y[(size_t)r * K + k] = 0.f;
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int o = 16; o; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-      if (lane == 0 && k0 + j < K) {
-        const int i = s_i[k0 + j];
-        float y = (dot[j] + (a.bias && i >= 0 ? to_f(((const T*)a.bias)[i]) : 0.f)) * a.scale;
-        if (i == -2) y = __int_as_float(0x7fc00000);
-        a.y[(size_t)r * K + k0 + j] = y;
-        a.idx[(size_t)r * K + k0 + j] = max(i, -1);
-        if (i == -2 || (i >= 0 && s_p[k0 + j] != 0.f)) h = fmaf(-kLn2v * s_p[k0 + j], y, h);
+    sync();
+    for (int t = tid; t < halves; t += W) {
+      int lo = 0, hi = n;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (s_i[mid] < t * cols) lo = mid + 1;
+        else hi = mid;
       }
+      const int off = lo < n ? s_i[lo] - t * cols : cols;
+      tab[t * ld + r] = (unsigned)lo << 8 | (off < cols ? off : 255);
     }
   }
-  h = all(h, false);
-  if (tid == 0) a.h[r] = h;
 }
 
 // A row's log-sum-exp from its tiles' maxima and sums, and its loss.  Block: 32 rows by 32 runs of tiles.
@@ -310,6 +304,8 @@ __device__ __forceinline__ void vocab_join(float& top, float& sum, float2 v) {
   sum = sum * exp2f(top - at) + v.y * exp2f(v.x - at);
   top = mx;
 }
+// The targets' logits in y become d = log2 q, from the row's maximum and sum themselves: a loss near 0 keeps
+// its sign, and is off by what the sum's 1 is off.  A warp to a row's targets.
 // out not NULL: the block that comes last adds the rows' losses up, in a fixed order (their mean: divided;
 // 0 of none).
 static __global__ void __launch_bounds__(1024) k_vocab_lse(const VocabArgs a, const float2* __restrict__ part,
@@ -337,21 +333,35 @@ static __global__ void __launch_bounds__(1024) k_vocab_lse(const VocabArgs a, co
     }
     __syncthreads();
   }
-  if (run == 0) {
-    if (r < rows) {
-      const float lse = top + log2f(sum);
-      a.lse[r] = lse;
-      const float loss = a.tau * a.tau * fmaf(kLn2v, lse, a.h[r]);
-      a.loss[r] = loss;
-      if (each) each[a.rowmap[r]] = loss;
+  const int mine = blockIdx.x * 32 + run;
+  if (mine < rows) {
+    top = s[0][run].x;
+    const float ls = log2f(s[0][run].y);
+    float dot = 0.f;
+    for (int k = lane; k < a.K; k += 32) {
+      const size_t e = (size_t)mine * a.K + k;
+      float d = fmaf(a.y[e], a.scale, -top) - ls;
+      d = d > 0.f ? 0.f : d;            // (NaN stays)
+      a.y[e] = d;
+      const float p = a.p ? a.p[e] : 1.f;
+      if (p != 0.f) dot = fmaf(p, d, dot);
     }
-    if (out) {
-      __threadfence();
-      __syncwarp();
-      if (lane == 0) s_last = atomicAdd(a.ticket, 1) == used - 1;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (lane == 0) {
+      a.lse[mine] = top + ls;
+      float loss = a.tau * a.tau * fmaf(-kLn2v, dot, a.p ? a.h[mine] : 0.f);
+      loss = loss < 0.f ? 0.f : loss;   // as the formula: p and q are distributions
+      a.loss[mine] = loss;
+      if (each) each[a.rowmap[mine]] = loss;
     }
   }
   if (!out) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(a.ticket, 1) == used - 1;
+  }
   __syncthreads();
   if (!s_last) return;
   __threadfence();
@@ -411,7 +421,7 @@ static __global__ void __launch_bounds__(1024) k_vocab_coef(const VocabArgs a, i
   if (threadIdx.x == 0) *inv = ldexpf(1.f, -e);
 }
 
-// the targets' entries of a piece of G: c (q - p), each rounded once; repeated indices write the same
+// the targets' entries of a piece of G: c (q - p), each rounded once; near q = p = 1 from what is left of them
 template <class E>
 __global__ void __launch_bounds__(256) k_vocab_patch(const VocabArgs a, const float* __restrict__ coef, int v0, int n,
                                                      E* G, long long ld, long long piece, int pieces) {
@@ -420,7 +430,8 @@ __global__ void __launch_bounds__(256) k_vocab_patch(const VocabArgs a, const fl
   if (r >= *a.rows) return;
   const int i = a.idx[e] - v0;
   if (i < 0 || i >= n) return;
-  float v = coef[r] * (exp2f(a.y[e] - a.lse[r]) - (a.p ? a.p[e] : 1.f));
+  const float d = a.y[e], t = a.p ? a.p[e] : 1.f;
+  float v = coef[r] * (t > 0.5f ? expm1f(kLn2v * d) + (1.f - t) : exp2f(d) - t);
   for (int p = 0; p < pieces; ++p) {
     const E q = from_f<E>(v);
     G[p * piece + r * ld + i] = q;
