@@ -78,6 +78,9 @@ __device__ __forceinline__ f2 exp22(f2 v) {
 // 2.1e-8 log2(e) more (a product and a sum cost what a product costs).  d = 0 still gives exactly 1.
 constexpr float kSelLow = 2.97e-8f;
 __device__ __forceinline__ f2 sel_decay2(f2 d, f2 A) { return exp22(fma2(d, A, pair(kSelLow, kSelLow))); }
+// A as the kernels take it: an infinite one is the largest number there is, whose decay over any step is the
+// same 0, so that delta = 0 (rows past the end, chunks without steps) leaves a state as it is: 0 A is not NaN.
+__device__ __forceinline__ float sel_finite(float A) { return fabsf(A) == INFINITY ? copysignf(3.402823466e38f, A) : A; }
 __device__ __forceinline__ float sel_rcp(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -303,6 +306,15 @@ struct SelThread {
       for (int s = 0; s < 4; ++s) h[s] = 0;
     }
   }
+  __device__ __forceinline__ void load_decays(f2* A) const {
+    load_state(p.A, 0, A);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float a, b;
+      split(A[s], a, b);
+      A[s] = pair(sel_finite(a), sel_finite(b));
+    }
+  }
   __device__ __forceinline__ void store_state(float* base, size_t lead, const f2* h) const {
     write_states(states_at(base, lead), p.S % 4 == 0, h);
   }
@@ -414,7 +426,7 @@ __global__ void __launch_bounds__(kSelThreads, L >= 4 ? 5 : 3) k_sel_fwd(const S
   f2 A[4], h[4], sumd = 0;
   float bias[W], Dv[W];
   bool any_cut = false;
-  th.load_state(p.A, 0, A);
+  th.load_decays(A);
   th.load_weights(p.bias, bias);
   th.load_weights(p.D, Dv);
   if (LOCAL) th.load_state(nullptr, 0, h);
@@ -571,7 +583,7 @@ __global__ void __launch_bounds__(64) k_sel_join(const SelArgs p, const float* _
   if (i >= all) return;
   const int b = (int)(i / row);
   const size_t ns = i - b * row, n = ns / p.S;
-  const float A = p.A[ns];
+  const float A = sel_finite(p.A[ns]);
   float h = start ? start[i] : 0.f;
   constexpr int U = 16;                 // chunks whose maps are on their way together
   for (int c0 = 0; c0 < p.chunks; c0 += U) {
@@ -625,7 +637,7 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
   f2 A[4], G[4], dA[4], sumd = 0;
   float bias[W], Dv[W], dD[W] = {}, db[W] = {};
   bool any_cut = false;
-  th.load_state(p.A, 0, A);
+  th.load_decays(A);
   th.load_weights(p.bias, bias);
   th.load_weights(p.D, Dv);
 #pragma unroll
@@ -1021,7 +1033,7 @@ struct SelLane {
   __device__ __forceinline__ void weights(bool on) {
     const float* Ap = p.A + (size_t)n * p.S + s0;
 #pragma unroll
-    for (int s = 0; s < Q; ++s) A[s] = on && s0 + off(s) < p.S ? Ap[off(s)] : 0.f;
+    for (int s = 0; s < Q; ++s) A[s] = on && s0 + off(s) < p.S ? sel_finite(Ap[off(s)]) : 0.f;
     D = on && p.D ? p.D[n] : 0.f;
     bias = on && p.bias ? p.bias[n] : 0.f;
   }

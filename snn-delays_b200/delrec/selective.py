@@ -164,7 +164,7 @@ def selective_scan(x, dt, A, B, C, h0=None, *, D=None, gate=None, dt_bias=None, 
     int64: sequence b has lengths[b] steps; later positions are not read, their y and gradients
     are 0, and hT is the state after the last step there is.  ``resets`` (T,B) bool: True drops the
     state before that step (sequences packed one after another).  A decay below 1.2e-38 counts as
-    0.  Strides of T and B are free; a strided channel (or group and state) dimension is copied.
+    0, and A = -inf is one of 0 at every step whose delta is not 0.  Strides of T and B are free; a strided channel (or group and state) dimension is copied.
 
     Gradients reach x, dt, A, B, C, h0, D, gate and dt_bias.  For the backward pass the inputs are
     kept, and the float32 state before every 8th step."""
