@@ -164,6 +164,30 @@ class BatchNorm1d(torch.nn.BatchNorm1d):
         return super().forward(x)
 
 
+# States of streaming modules.  Eagerly each call makes a new one, and who keeps the state before can go back to
+# it.  A call captured in a graph moves the state that there is on in place, so that every replay takes it further.
+
+
+def _captured(state):
+    return state is not None and torch.cuda.is_current_stream_capturing()
+
+
+def _kept(m):
+    """The state that a multi-step call of module ``m`` begins from (a copy where it will be written over: a backward
+    pass may want it)."""
+    v = m.v if m.keep_state else None
+    return v.clone() if _captured(v) else v
+
+
+def _keep(m, v):
+    """``v`` is the state behind a multi-step call."""
+    if m.keep_state:
+        if _captured(m.v):
+            m.v.copy_(v.detach())
+        else:
+            m.v = v.detach()
+
+
 class GatedIntegrator(MemoryModule):
     """A leaky integrator with a learned, input-dependent decay (``gated.gated_scan``), in
     place of ``LIFNode`` where no spikes are wanted: forward(z, f) with gate logits f.
@@ -171,7 +195,9 @@ class GatedIntegrator(MemoryModule):
     Multi-step mode: z (T,B,N), f (T,B,G) -> h (T,B,N) from a zero state, or from the state
     of the call before with ``keep_state=True``.  Single-step mode ('s'): z (B,N), f (B,G) ->
     h (B,N), the state moving on from call to call until ``reset`` (``utils.reset_states``);
-    no gradient passes.  ``v`` is the state (B,N) in float32."""
+    no gradient passes.  ``v`` is the state (B,N) in float32.  A call captured in a CUDA graph
+    moves the ``v`` that there is on in place, replay after replay (``v.zero_()`` starts it
+    again); without one it begins from zeros each time."""
 
     def __init__(self, decay_input: bool = True, step_mode: str = "m", keep_state: bool = False,
                  checkpoint8: bool = False):
@@ -188,12 +214,11 @@ class GatedIntegrator(MemoryModule):
         if self.step_mode == "s":
             if lengths is not None or resets is not None:
                 raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
-            h, self.v = gated_step(z, f, self.v, decay_input=self.decay_input)
+            h, self.v = gated_step(z, f, self.v, decay_input=self.decay_input, out=self.v if _captured(self.v) else None)
             return h
-        h, v = gated_scan(z, f, self.v if self.keep_state else None, lengths=lengths, resets=resets,
+        h, v = gated_scan(z, f, _kept(self), lengths=lengths, resets=resets,
                           decay_input=self.decay_input, checkpoint8=self.checkpoint8)
-        if self.keep_state:
-            self.v = v.detach()
+        _keep(self, v)
         return h
 
     def extra_repr(self):
@@ -207,7 +232,7 @@ class ShortConv(MemoryModule):
     Multi-step mode: x (T,B,N) -> y (T,B,N) from zeros, or from the window of the call before with
     ``keep_state=True``.  Single-step mode ('s'): x (B,N) -> y (B,N), the window moving on from call
     to call until ``reset`` (``utils.reset_states``); no gradient passes.  ``v`` is the window
-    (K-1,B,N) in x's type."""
+    (K-1,B,N) in x's type, in a CUDA graph as in ``GatedIntegrator``."""
 
     def __init__(self, num_features, kernel_size: int = 4, act: str = "silu", bias: bool = True, step_mode: str = "m",
                  keep_state: bool = False):
@@ -229,12 +254,10 @@ class ShortConv(MemoryModule):
         if self.step_mode == "s":
             if lengths is not None or resets is not None:
                 raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
-            y, self.v = short_conv_step(x, self.weight, self.bias, self.v, act=self.act)
+            y, self.v = short_conv_step(x, self.weight, self.bias, self.v, act=self.act, out=self.v if _captured(self.v) else None)
             return y
-        y, v = short_conv(x, self.weight, self.bias, self.v if self.keep_state else None, act=self.act,
-                          lengths=lengths, resets=resets)
-        if self.keep_state:
-            self.v = v.detach()
+        y, v = short_conv(x, self.weight, self.bias, _kept(self), act=self.act, lengths=lengths, resets=resets)
+        _keep(self, v)
         return y
 
     def extra_repr(self):
@@ -248,7 +271,8 @@ class SelectiveIntegrator(MemoryModule):
 
     forward(x, dt, B, C, gate=None): multi-step mode (T,B,N) .. -> y (T,B,N) from a zero state, or
     from the state of the call before with ``keep_state=True``; single-step mode ('s') (B,N) .. ->
-    y (B,N), the state moving on from call to call until ``reset``; no gradient passes.  Learned: the
+    y (B,N), the state moving on from call to call until ``reset``, in a CUDA graph as in
+    ``GatedIntegrator``; no gradient passes.  Learned: the
     decay A = -exp(A_log) (N,S), the skip D (N) and the bias of dt (N), whose step sizes start
     between ``dt_min`` and ``dt_max``.  ``v`` is the state (B,N,S) in float32."""
 
@@ -270,12 +294,12 @@ class SelectiveIntegrator(MemoryModule):
         if self.step_mode == "s":
             if lengths is not None or resets is not None:
                 raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
-            y, self.v = selective_step(x, dt, A, B, C, self.v, D=self.D, gate=gate, dt_bias=self.dt_bias)
+            y, self.v = selective_step(x, dt, A, B, C, self.v, D=self.D, gate=gate, dt_bias=self.dt_bias,
+                                       out=self.v if _captured(self.v) else None)
             return y
-        y, v = selective_scan(x, dt, A, B, C, self.v if self.keep_state else None, D=self.D, gate=gate,
-                              dt_bias=self.dt_bias, lengths=lengths, resets=resets)
-        if self.keep_state:
-            self.v = v.detach()
+        y, v = selective_scan(x, dt, A, B, C, _kept(self), D=self.D, gate=gate, dt_bias=self.dt_bias, lengths=lengths,
+                              resets=resets)
+        _keep(self, v)
         return y
 
     def extra_repr(self):
