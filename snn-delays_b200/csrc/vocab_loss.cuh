@@ -395,7 +395,8 @@ static __global__ void __launch_bounds__(1024) k_vocab_coef(const VocabArgs a, i
       const float l = a.loss[r];
       coef[r] = l != l ? l : 16384.f;
     }
-    if (threadIdx.x == 0) *inv = *g * a.tau / (reduction == 1 ? (float)max(rows, 1) : 1.f) * (1.f / 16384.f);
+    // (nothing counts: gradients of 0 whatever *g is)
+    if (threadIdx.x == 0) *inv = rows ? *g * a.tau / (reduction == 1 ? (float)rows : 1.f) * (1.f / 16384.f) : 0.f;
     return;
   }
   float top = 0.f;
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(256) k_vocab_planes(long long n, int D, const 
         v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
       }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] *= up;
+    for (int k = 0; k < 4; ++k) v[k] = r >= 0 ? v[k] * up : 0.f;   // 0 where a position does not count, also of an infinite up
     T* o = out + m * D + c;
     if (D % 4 == 0) {
       *(VecOf<T, 4>*)o = pack_vec<T, 4>(v);

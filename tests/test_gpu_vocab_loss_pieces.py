@@ -1,0 +1,125 @@
+"""The vocabulary losses past what one pass over the logits' gradient holds, against float64: several pieces of
+the vocabulary, more positions than keep a second piece of a 16-bit gradient, tiles of 512 columns, sums in parts."""
+
+import pytest
+import torch
+
+from sequence_cases import HALF, within
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+# positions (T, B), D, V, type, entries a teacher keeps (0: cross entropy), temperature, reduction, bias, lengths, least pieces
+CASES = [((100, 512), 264, 6007, BF16, 0, 1.0, "mean", True, False, 3), ((100, 512), 40, 6007, F16, 0, 1.0, "none", True, False, 3),
+         ((40, 512), 72, 5003, F32, 0, 1.0, "sum", True, False, 3), ((100, 512), 136, 6007, BF16, 7, 2.0, "mean", True, False, 3),
+         ((40, 512), 300, 4700, F32, 3, 0.5, "none", True, False, 3), ((64, 1024), 16, 5200, BF16, 0, 1.0, "mean", True, True, 3),
+         ((7, 100), 512, 3001, F16, 20, 1.0, "sum", False, False, 1), ((1, 600), 264, 2049, F32, 64, 2.0, "mean", True, False, 1),
+         ((3, 171), 512, 1500, BF16, 33, 1.0, "mean", True, False, 1), ((12, 300), 500, 999, BF16, 5, 1.0, "none", True, True, 1),
+         ((1, 513), 24, 260, F16, 4, 1.0, "mean", True, False, 1), ((9, 400), 513, 1111, F16, 1, 3.0, "sum", True, True, 1)]
+
+
+def _make(case, seed=0):
+    (T, B), D, V, dtype, K, tau, reduction, bias, ragged, _ = case
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")   # noqa: E731
+    d = dict(x=rnd(T, B, D).to(dtype), w=(rnd(V, D) * 2 * D ** -0.5).to(dtype), bias=rnd(V).to(dtype) if bias else None,
+             lengths=torch.randint(0, T + 1, (B,), generator=g, device="cuda") if ragged else None)
+    if K:
+        d["index"] = torch.randint(0, V, (T, B, K), generator=g, device="cuda")
+        d["logits"] = rnd(T, B, K) * 2
+        d["index"][torch.rand(T, B, K, generator=g, device="cuda") < 0.1] = -1
+    else:
+        d["index"] = torch.randint(0, V, (T, B), generator=g, device="cuda")
+        d["index"][torch.rand(T, B, generator=g, device="cuda") < 0.1] = -100
+    return d, rnd(T, B) if reduction == "none" else torch.tensor(1.7, device="cuda")
+
+
+def _reference(d, case, grad):
+    """loss, dx, dw, db in float64 and the bounds of fp32 arithmetic with G rounded to its type once, 4096 positions at a time
+    (as ``oracle.selective_oracle.vocab_loss`` has them for small sizes)."""
+    (T, B), D, V, dtype, K, tau, reduction, _, _, _ = case
+    f, M = torch.float64, T * B
+    half = HALF[dtype] if dtype != F32 else 4 * U
+    on = torch.ones(T, B, dtype=torch.bool, device="cuda")
+    if d["lengths"] is not None:
+        on &= torch.arange(T, device="cuda")[:, None] < d["lengths"][None]
+    idx = d["index"].reshape(M, -1)
+    on = on.flatten() & (idx >= 0).any(1)
+    rows = on.nonzero()[:, 0]
+    n = rows.numel()
+    w, b = d["w"].to(f), torch.zeros(V, dtype=f, device="cuda") if d["bias"] is None else d["bias"].to(f)
+    wa = w.abs()
+    share = n if reduction == "mean" else 1
+    loss, el = torch.zeros(M, dtype=f, device="cuda"), torch.zeros(M, dtype=f, device="cuda")
+    z0 = lambda *s: torch.zeros(*s, dtype=f, device="cuda")   # noqa: E731
+    r = dict(dx=z0(M, D), dw=z0(V, D), db=z0(V))
+    e = dict(dx=z0(M, D), dw=z0(V, D), db=z0(V))
+    c = (grad.reshape(M).to(f) if reduction == "none" else grad.to(f).expand(M) / share) * tau
+    top = c[rows].abs().max()
+    acc = lambda k: (k / 16 + 24) * 2 * U   # noqa: E731
+    for i in range(0, n, 4096):
+        at = rows[i:i + 4096]
+        x2, ii, cc = d["x"].reshape(M, D)[at].to(f), idx[at], c[at][:, None]
+        z = (x2 @ w.t() + b) / tau
+        mag = (x2.abs() @ wa.t() + b.abs()) / tau
+        ez = (D / 16 + 12) * 2 * U * mag
+        et = torch.maximum((D / 32 * 8 + 16) * U * mag, ez)     # a target's logit: a dot product of its own, or the tensor core's
+        lse = torch.logsumexp(z, 1)
+        elt = 2 * U * (z.abs() + lse.abs()[:, None]) + 100 * U + V / 2048 * U + ez
+        q = torch.exp(z - lse[:, None])
+        elt = elt + (q * elt).sum(1, keepdim=True)
+        kept = ii >= 0
+        t = d["logits"].reshape(M, K)[at].to(f) / tau if K else z0(len(at), 1)
+        lp = torch.log_softmax(torch.where(kept, t, torch.full_like(t, -float("inf"))), 1)
+        p, lp0, ii = torch.exp(lp), torch.where(kept, lp, torch.zeros_like(lp)), ii.clamp(min=0)
+        zt = torch.where(kept, z.gather(1, ii), torch.zeros_like(lp))
+        rp = (30 + 4 * t.abs().amax(1, keepdim=True) + 2 * lp0.abs()) * U if K else torch.zeros_like(lp)
+        loss[at] = tau * tau * ((p * (lp0 - zt)).sum(1) + lse)
+        el[at] = tau * tau * ((p * (rp * (1 + lp0.abs() + zt.abs()) + et.gather(1, ii) + (K + 8) * U * (lp0.abs() + zt.abs()))).sum(1)
+                              + (q * elt).sum(1) + 8 * U * lse.abs() + 110 * U)
+        P = torch.zeros_like(q).scatter_add_(1, ii, p)
+        eP = torch.zeros_like(q).scatter_add_(1, ii, p * (rp + (K + 2) * U))
+        G = cc * (q - P)
+        eG = cc.abs() * (q * (elt + et) + eP + 4 * U * (q + P))
+        eG = eG + half * (G.abs() + eG) + top * 2.0 ** -38
+        r["dx"][at], e["dx"][at] = G @ w, (eG + acc(V) * G.abs()) @ wa
+        r["dw"] += G.t() @ x2
+        e["dw"] += (eG + acc(n) * G.abs()).t() @ x2.abs()
+        r["db"] += G.sum(0)
+        e["db"] += (eG + (n / 128 + 140) * U * G.abs()).sum(0)      # 128 runs of n / 128 rows
+    if reduction == "none":
+        r["loss"], e["loss"] = loss.view(T, B), el.view(T, B)
+    else:
+        r["loss"], e["loss"] = loss.sum() / share, el.sum() / share + 4 * U * loss.abs().sum() / share
+    r["dx"], e["dx"] = r["dx"].view(T, B, D), e["dx"].view(T, B, D)
+    return r, e
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_against_float64(case):
+    from delrec import _lib
+    from delrec.vocab_loss import linear_cross_entropy, linear_distill
+    _, D, V, dtype, K, tau, reduction, bias, _, pieces = case
+    d, grad = _make(case)
+    r, e = _reference(d, case, grad)
+    leaves = {k: d[k].requires_grad_(True) for k in ("x", "w", "bias") if d[k] is not None}
+    if K:
+        loss = linear_distill(d["x"], d["w"], d["index"], d["logits"], d["bias"], temperature=tau, reduction=reduction,
+                              lengths=d["lengths"])
+    else:
+        loss = linear_cross_entropy(d["x"], d["w"], d["index"], d["bias"], reduction=reduction, lengths=d["lengths"])
+    within(loss, r["loss"], e["loss"], "loss")
+    before = _lib.launch_count()
+    grads = torch.autograd.grad(loss, list(leaves.values()), grad)
+    # a piece takes at most seven launches, all of them four more: as many pieces as are meant to be tested
+    assert _lib.launch_count() - before > 7 * (pieces - 1) + 4
+    for k, v in zip(leaves, grads):
+        name = {"x": "dx", "w": "dw", "bias": "db"}[k]
+        within(v, r[name], e[name], name)
+    again = torch.autograd.grad(linear_distill(d["x"], d["w"], d["index"], d["logits"], d["bias"], temperature=tau,
+                                               reduction=reduction, lengths=d["lengths"]) if K else
+                                linear_cross_entropy(d["x"], d["w"], d["index"], d["bias"], reduction=reduction,
+                                                     lengths=d["lengths"]), list(leaves.values()), grad)
+    for a, v in zip(again, grads):
+        assert torch.equal(a, v)
