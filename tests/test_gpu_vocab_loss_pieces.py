@@ -14,6 +14,7 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 CASES = [((100, 512), 264, 6007, BF16, 0, 1.0, "mean", True, False, 3), ((100, 512), 40, 6007, F16, 0, 1.0, "none", True, False, 3),
          ((40, 512), 72, 5003, F32, 0, 1.0, "sum", True, False, 3), ((100, 512), 136, 6007, BF16, 7, 2.0, "mean", True, False, 3),
          ((40, 512), 300, 4700, F32, 3, 0.5, "none", True, False, 3), ((64, 1024), 16, 5200, BF16, 0, 1.0, "mean", True, True, 3),
+         ((300, 1024), 16, 1100, BF16, 0, 1.0, "sum", True, True, 3),
          ((7, 100), 512, 3001, F16, 20, 1.0, "sum", False, False, 1), ((1, 600), 264, 2049, F32, 64, 2.0, "mean", True, False, 1),
          ((3, 171), 512, 1500, BF16, 33, 1.0, "mean", True, False, 1), ((12, 300), 500, 999, BF16, 5, 1.0, "none", True, True, 1),
          ((1, 513), 24, 260, F16, 4, 1.0, "mean", True, False, 1), ((9, 400), 513, 1111, F16, 1, 3.0, "sum", True, True, 1)]
@@ -112,7 +113,7 @@ def test_against_float64(case):
     within(loss, r["loss"], e["loss"], "loss")
     before = _lib.launch_count()
     grads = torch.autograd.grad(loss, list(leaves.values()), grad)
-    # a piece takes at most seven launches, all of them four more: as many pieces as are meant to be tested
+    # a piece takes six or seven launches, all of them three or four more: as many pieces as are meant to be tested
     assert _lib.launch_count() - before > 7 * (pieces - 1) + 4
     for k, v in zip(leaves, grads):
         name = {"x": "dx", "w": "dw", "bias": "db"}[k]
