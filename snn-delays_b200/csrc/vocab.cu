@@ -78,7 +78,10 @@ struct VocabShape {
   bool w_direct;                            // W is an operand as it lies
   size_t x, w, part, tab, flags, ticket, h, G, coef, inv, dx, dw, db, total;
 };
-constexpr size_t kVocabBudget = 256u << 20;   // bytes of G at once
+// Bytes of G at once, in whole tiles of 256 columns; 512 columns of all positions where those take more (past
+// 262144 positions of one 16-bit piece, 87381 of fp32): dx is read and written once a piece, so narrower ones would
+// be bound by it, and take less than x's operand and dx's sums from 512 features on.
+constexpr size_t kVocabBudget = 256u << 20;
 static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
   VocabShape h{};
   h.M = (long long)s->T * s->B;
@@ -106,7 +109,7 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
     h.ticket = take(4);
     h.h = take((size_t)h.M * 4);
   } else {
-    const long long fit = std::max<long long>(512, (long long)(kVocabBudget / ((size_t)h.Mp * h.gp * 2)));
+    const long long fit = std::max<long long>(512, (long long)(kVocabBudget / ((size_t)h.Mp * h.gp * 2)) / 256 * 256);
     h.count = (int)((s->V + fit - 1) / fit);
     h.Vc = (int)(((s->V + h.count - 1) / h.count + 255) / 256 * 256);
     h.count = (s->V + h.Vc - 1) / h.Vc;

@@ -200,3 +200,25 @@ def test_the_logits_gradient_stays_within_its_room():
     whole = 65536 * 65536 * 2
     assert lib.delrec_vocab_loss_backward_workspace(ctypes.byref(s)) < whole / 8
     assert lib.delrec_vocab_loss_forward_workspace(ctypes.byref(s)) < whole / 8
+
+
+def test_room_of_the_logits_gradient():
+    """256 MB of it, or 512 columns of all positions where those take more: what a backward pass takes besides is the same
+    for a vocabulary of one such piece and of many, but for the weight's operand and sums."""
+    from delrec import _lib
+    lib = _lib.lib()
+
+    def take(M, V, dtype):
+        s = _lib.Vocab(1, M, 8, V, 1, dtype, 0, 1, 0, 0, 0, 1, 1.0, 0, -100, 0, 8)
+        return lib.delrec_vocab_loss_backward_workspace(ctypes.byref(s))
+
+    for dtype, each in ((1, 2), (2, 2), (0, 6)):
+        for M in (600, 51200, 100000, 262144, 300000, 1 << 20):
+            Mp = (M + 255) // 256 * 256
+            room = max(256 << 20, 512 * Mp * each)
+            V = 64 * max(512, room // (Mp * each))       # many pieces of it
+            if (M // 256 + 1) * (V // 128 + 1) > 1 << 27:
+                continue
+            # x's operand, dx's and dweight's sums in up to 16 parts, dbias's runs, and the weight's operand
+            rest = Mp * 8 * (each + 16 * 4) + V * 8 * each + (room // (Mp * each) + 256) * (16 * 8 * 4 + 128 * 4) + Mp * 4 + 4096
+            assert 0 < take(M, V, dtype) <= room + rest, (dtype, M)
