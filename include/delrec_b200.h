@@ -414,7 +414,7 @@ typedef struct delrec_selective {
   int32_t softplus;
   int32_t lengths_wide;  /* lengths are int64 */
   int32_t ragged;        /* there are lengths (a hint: how time is cut; the same in every call of a pass) */
-  int32_t reserved;
+  int32_t no_bc;         /* backward: neither dB nor dC is wanted; their partial sums then take no workspace */
   int64_t x_t, x_b, dt_t, dt_b, u_t, u_b, y_t, y_b;             /* x, dt, gate, y */
   int64_t bm_t, bm_b, cm_t, cm_b;                               /* Bm, Cm */
   int64_t gy_t, gy_b, dx_t, dx_b, ddt_t, ddt_b, du_t, du_b;     /* gradients of y, x, dt, gate */

@@ -32,6 +32,7 @@ static int sel_scan_lanes(int S, int Dg) {
 
 struct SelShape {
   int L, tiles, chunks, steps;
+  int parts;                      // tiles of a backward launch
 };
 // Time is cut into chunks of at least 64 steps where that fills the SMs better: `slots` blocks run at
 // once, so c chunks take ceil(blocks c / slots) / c of a sequence's time, and the maps that go before
@@ -58,6 +59,14 @@ static SelShape sel_shape(const delrec_selective* s, int slots, double more) {
     }
   h.steps = ((s->T + chunks - 1) / chunks + kSelSeg - 1) / kSelSeg * kSelSeg;
   h.chunks = (s->T + h.steps - 1) / h.steps;
+  // Sums of dB and dC wait in one place a tile of channels: (tiles, T, B, G, S) floats twice.  Where those are more
+  // than the states kept for the pass (S > 64: 8 channels to a tile; SelThread::PARTS), a launch takes a part of the tiles and the next
+  // one adds to its sums, if each still fills the GPU eight times (N = 2048, S = 128, T = 64, B = 256: 4.4 -> 2.2 GB,
+  // 10.3 -> 10.5 ms; as few places as fill the GPU, 14 of 256: 0.6 GB, 11.0 ms).
+  const long long full = (8LL * slots + (long long)s->G * s->B - 1) / ((long long)s->G * s->B);
+  h.parts = (int)std::min<long long>(h.tiles, std::max<long long>(full, (Dg + 15) / 16));
+  const int launches = (h.tiles + h.parts - 1) / h.parts;
+  h.parts = (h.tiles + launches - 1) / launches;
   return h;
 }
 static SelShape sel_fwd_shape(const delrec_selective* s) { return sel_shape(s, kSeqSMs * 5, 0.6); }
@@ -88,7 +97,7 @@ static SelPlan sel_bwd_plan(const delrec_selective* s) {
   const SelShape h = sel_bwd_shape(s);
   SelPlan w;
   w.chunks(s, h);
-  const size_t rows = (size_t)h.chunks * s->B, bc = (size_t)h.tiles * s->T * s->B * s->G * s->S;
+  const size_t rows = (size_t)h.chunks * s->B, bc = s->no_bc ? 0 : (size_t)h.parts * s->T * s->B * s->G * s->S;
   w.dA = w.take(rows * s->N * s->S * 4);
   w.dD = w.take(rows * s->N * 4);
   w.db = w.take(rows * s->N * 4);
@@ -116,7 +125,7 @@ static SelArgs sel_args(const delrec_selective* s, const SelShape& h, const SelP
   SelArgs p{};
   p.T = s->T; p.B = s->B; p.N = s->N; p.S = s->S; p.G = s->G; p.Dg = s->N / s->G;
   p.softplus = s->softplus; p.wide = s->lengths_wide;
-  p.chunks = h.chunks; p.steps = h.steps; p.tiles = h.tiles;
+  p.chunks = h.chunks; p.steps = h.steps; p.tiles = h.tiles; p.parts = h.parts;
   p.x_t = s->x_t; p.x_b = s->x_b; p.dt_t = s->dt_t; p.dt_b = s->dt_b; p.u_t = s->u_t; p.u_b = s->u_b;
   p.y_t = s->y_t; p.y_b = s->y_b; p.bm_t = s->bm_t; p.bm_b = s->bm_b; p.cm_t = s->cm_t; p.cm_b = s->cm_b;
   p.gy_t = s->gy_t; p.gy_b = s->gy_b; p.dx_t = s->dx_t; p.dx_b = s->dx_b; p.ddt_t = s->ddt_t; p.ddt_b = s->ddt_b;
@@ -172,7 +181,7 @@ int delrec_selective_backward(const delrec_selective* s, const void* x, const vo
                               void* dgate, float* ddt_bias, float* dh0, void* ws, size_t wsb, void* stream) {
   const int rc = check_selective(s);
   if (rc) return rc;
-  if (!x || !dt || !A || !Bm || !Cm || !states || (dgate && !gate)) return DELREC_ERR_ARG;
+  if (!x || !dt || !A || !Bm || !Cm || !states || (dgate && !gate) || (s->no_bc && (dB || dC))) return DELREC_ERR_ARG;
   if (s->S % 4 == 0 && (((uintptr_t)dh0) & 15)) return DELREC_ERR_ARG;
   const SelShape h = sel_bwd_shape(s);
   const SelPlan w = sel_bwd_plan(s);
@@ -187,6 +196,7 @@ int delrec_selective_backward(const delrec_selective* s, const void* x, const vo
   p.db = ddt_bias ? (float*)(base + w.db) : nullptr;
   p.dB = dB ? (float*)(base + w.dB) : nullptr;
   p.dC = dC ? (float*)(base + w.dC) : nullptr;
+  if (!dB && !dC) p.parts = p.tiles;
   SelAlign al(s);
   al.add(x, s->x_t, s->x_b);
   al.add(dt, s->dt_t, s->dt_b);
@@ -214,7 +224,7 @@ int delrec_selective_backward(const delrec_selective* s, const void* x, const vo
     if (blocks > 0x7fffffffLL) return DELREC_ERR_UNSUPPORTED;
     return by_dtype(s->dtype, [&](auto t) {
       using E = decltype(t);
-      k_sel_bc<E><<<(unsigned)blocks, 256, 0, st>>>(cols, h.tiles, p.dB, p.dC, (E*)dB, (E*)dC);
+      k_sel_bc<E><<<(unsigned)blocks, 256, 0, st>>>(cols, h.parts, p.dB, p.dC, (E*)dB, (E*)dC);
       SQ_LAUNCHED();
       return (int)DELREC_OK;
     });

@@ -42,7 +42,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct SelArgs {
   int T, B, N, S, G, Dg;          // Dg = N / G channels to a group
   int softplus, wide, vec, bcvec; // vec: rows of x, dt, gate, y and their gradients in fours, twos or ones; bcvec: B and C in fours
-  int chunks, steps, tiles;       // chunks of `steps` rows; tiles of channels to a group
+  int chunks, steps, tiles;       // chunks of `steps` rows; tiles of channels to a group in this launch
+  int parts;                      // tiles of a backward launch
+  int tile0, add;                 // the first tile; add: dB and dC hold the sums of the launches before
   const void *x, *dt, *Bm, *Cm, *gate;
   const float *A, *D, *bias, *h0;
   const void* lengths;
@@ -58,7 +60,7 @@ struct SelArgs {
   const float* ghT;
   void *dx, *ddt, *dgate;
   float *dh0, *dA, *dD, *db;      // dA (chunks * B, N, S), dD, db (chunks * B, N): partial sums
-  float *dB, *dC;                 // (tiles, T, B, G, S): partial sums
+  float *dB, *dC;                 // (tiles of a launch, T, B, G, S): partial sums
   long long gy_t, gy_b, dx_t, dx_b, ddt_t, ddt_b, du_t, du_b;
 };
 
@@ -200,6 +202,7 @@ struct SelThread {
   static constexpr int CG = 32 / L;            // pairs of channels in a warp
   static constexpr int CW = 2 * CG;            // channels of a warp
   static constexpr int CH = kSelWarps * CW;    // channels of a block
+  static constexpr bool PARTS = BWD && L > 16; // the tiles may take several launches (see sel_shape)
   static constexpr int SP = 4 * L;             // padded states
   static constexpr int W = CW < 4 ? 2 : 4;     // channels that a lane lays out
   static constexpr int Q = CW / W;             // lanes to a row
@@ -234,7 +237,7 @@ struct SelThread {
     i /= p.G;
     b = (int)(i % p.B);
     chunk = (int)(i / p.B);
-    const int c0 = tile * CH + warp * CW;
+    const int c0 = ((PARTS ? p.tile0 : 0) + tile) * CH + warp * CW;
     n0 = g * p.Dg + c0;
     nn = max(0, min(CW, p.Dg - c0));
     t0 = chunk * p.steps;
@@ -677,7 +680,13 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
 #pragma unroll
           for (int w = 0; w < kSelWarps; ++w) v += red[w * kSelSeg * 2 * SP + e];
         float* dst = q < SP ? p.dB : p.dC;
-        if (dst) dst[bc_0 + t * bc_t + s] = v;
+        if (dst) {
+          dst += bc_0 + t * bc_t + s;
+          // one block adds to a place in a launch: no order of atomics, and no wait for what is there (T=250 B=32
+          // N=2048 S=128 in three launches 5461 us, with a read 9742)
+          if (Th::PARTS && p.add) atomicAdd(dst, v);
+          else *dst = v;
+        }
       }
     }
   };
@@ -988,7 +997,7 @@ static __global__ void __launch_bounds__(1024) k_sel_sum(long long cols, long lo
     out[j] = t;
   }
 }
-// dB and dC (T,B,G,S) from their partial sums, one to a tile of channels
+// dB and dC (T,B,G,S) from their partial sums, one to a tile of channels of a launch
 template <class T>
 __global__ void __launch_bounds__(256) k_sel_bc(long long cols, int tiles, const float* __restrict__ dB,
                                                 const float* __restrict__ dC, T* __restrict__ oB, T* __restrict__ oC) {

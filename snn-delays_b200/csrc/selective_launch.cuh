@@ -36,7 +36,18 @@ static int sel_pass(const SelArgs& p, cudaStream_t st) {
     k_sel_join<BWD><<<(unsigned)((all + 63) / 64), 64, 0, st>>>(p, BWD ? p.ghT : p.h0);
     SQ_LAUNCHED();
   }
-  return sel_start<T, L, BWD, false>(p, st);
+  if constexpr (BWD) {   // `parts` tiles of channels a launch, each after the one before
+    SelArgs q = p;
+    for (q.tile0 = 0; q.tile0 < p.tiles; q.tile0 += p.parts) {
+      q.tiles = std::min(p.parts, p.tiles - q.tile0);
+      q.add = q.tile0 > 0;
+      const int rc = sel_start<T, L, true, false>(q, st);
+      if (rc) return rc;
+    }
+    return DELREC_OK;
+  } else {
+    return sel_start<T, L, false, false>(p, st);
+  }
 }
 template <class T, bool BWD, int L = 1>
 static int sel_by_l(int l, const SelArgs& p, cudaStream_t st) {

@@ -68,7 +68,7 @@ class Conv(ctypes.Structure):
 
 class Selective(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("T", "B", "N", "S", "G", "dtype", "softplus", "lengths_wide", "ragged",
-                                              "reserved")] \
+                                              "no_bc")] \
         + _i64("x_t", "x_b", "dt_t", "dt_b", "u_t", "u_b", "y_t", "y_b", "bm_t", "bm_b", "cm_t", "cm_b", "gy_t",
                "gy_b", "dx_t", "dx_b", "ddt_t", "ddt_b", "du_t", "du_b")
 

@@ -95,6 +95,7 @@ def _backward(ctx, gy, ghT):
         if ghT is not None:
             ghT = ghT.contiguous()
         s = _struct(x, S, G, ctx.softplus, lengths, dt, gate, None, Bm, Cm, gy, dx, ddt, dgate)
+        s.no_bc = 1 if dB is None and dC is None else 0
         nbytes = _lib.lib().delrec_selective_backward_workspace(ctypes.byref(s))
         ws = _lib.scratch(nbytes, dev)
         P = _lib.addr
@@ -167,7 +168,9 @@ def selective_scan(x, dt, A, B, C, h0=None, *, D=None, gate=None, dt_bias=None, 
     0, and A = -inf is one of 0 at every step whose delta is not 0.  Strides of T and B are free; a strided channel (or group and state) dimension is copied.
 
     Gradients reach x, dt, A, B, C, h0, D, gate and dt_bias.  For the backward pass the inputs are
-    kept, and the float32 state before every 8th step."""
+    kept, and the float32 state before every 8th step.  Where B or C learns, sums over channels take
+    twice (T,B,G,S) float32 while it runs, for each tile of 8 (S > 64) to 256 (S <= 4) channels
+    of a group, but no more than those states take where that fills the GPU."""
     G, S = _check(x, dt, A, B, C, D, gate, dt_bias, h0, "h0", 3)
     T, Bs, _ = x.shape
     if lengths is not None:

@@ -53,6 +53,41 @@ def test_a_decay_of_minus_infinity_drops_the_state(T, B, N, S, lengths, dtype):
         assert ((hT[b] - want).abs()[hit] <= (32 * 2.0 ** -24 * want.abs())[hit] + 2.0 ** -140).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,B,N,S,G,launches", [(2, 900, 60, 128, 1, 2), (2, 1800, 40, 128, 2, 2), (9, 1800, 20, 70, 1, 2),
+                                                (1, 4000, 33, 100, 1, 2), (1, 4000, 33, 40, 1, 1)])
+def test_sums_over_many_tiles_of_channels(T, B, N, S, G, launches, dtype):
+    """More tiles of channels than dB and dC have places for their sums: two launches add them up."""
+    from delrec import _lib
+    from delrec.selective import selective_scan
+    from oracle import selective_oracle as O
+    g = torch.Generator().manual_seed(6)
+    rnd = lambda *s: torch.randn(*s, generator=g)   # noqa: E731
+    d = dict(x=rnd(T, B, N).to(dtype), dt=(rnd(T, B, N) - 2).to(dtype), A=-rnd(N, S).abs() - 0.1, Bm=rnd(T, B, G, S).to(dtype),
+             Cm=rnd(T, B, G, S).to(dtype), D=rnd(N), lengths=torch.randint(0, T + 1, (B,), generator=g))
+    gy, gh = rnd(T, B, N).to(dtype), rnd(B, N, S)
+    ref = O.selective(**d, gy=gy, ghT=gh)
+    c = {k: v.cuda() for k, v in d.items()}
+    leaves = ["x", "dt", "A", "Bm", "Cm", "D"]
+    for k in leaves:
+        c[k].requires_grad_(True)
+    y, hT = selective_scan(c["x"], c["dt"], c["A"], c["Bm"], c["Cm"], D=c["D"], lengths=c["lengths"])
+    before = _lib.launch_count()
+    grads = torch.autograd.grad((y, hT), [c[k] for k in leaves], (gy.cuda(), gh.cuda()), retain_graph=True)
+    assert _lib.launch_count() - before == launches + 3        # sums of dA, dD; dB and dC
+    for k, v in zip(leaves, grads):
+        name = dict(x="dx", dt="ddt", A="dA", Bm="dB", Cm="dC", D="dD")[k]
+        within(v, ref[name], ref["e_" + name], name)
+    # one of the two, and neither: the same numbers, and one launch for neither
+    (dB,) = torch.autograd.grad((y, hT), c["Bm"], (gy.cuda(), gh.cuda()), retain_graph=True)
+    assert torch.equal(dB, grads[3])
+    y, hT = selective_scan(c["x"], c["dt"].detach(), c["A"].detach(), c["Bm"].detach(), c["Cm"].detach(), D=c["D"].detach(),
+                           lengths=c["lengths"])
+    before = _lib.launch_count()
+    (dx,) = torch.autograd.grad((y, hT), c["x"], (gy.cuda(), gh.cuda()))
+    assert _lib.launch_count() - before == 1 and torch.equal(dx, grads[0])
+
+
 @pytest.mark.parametrize("B", [2, 9000])
 def test_a_step_with_a_decay_of_minus_infinity(B):
     """Also where there are more sequences than threads."""

@@ -222,3 +222,26 @@ def test_room_of_the_logits_gradient():
             # x's operand, dx's and dweight's sums in up to 16 parts, dbias's runs, and the weight's operand
             rest = Mp * 8 * (each + 16 * 4) + V * 8 * each + (room // (Mp * each) + 256) * (16 * 8 * 4 + 128 * 4) + Mp * 4 + 4096
             assert 0 < take(M, V, dtype) <= room + rest, (dtype, M)
+
+
+def test_room_of_the_scans_sums():
+    """dB and dC have a place for their sums to each tile of channels, but no more than one to 16 channels where that fills
+    the GPU eight times, and none where neither is wanted."""
+    from delrec import _lib
+    lib, p = _lib.lib(), ctypes.c_void_p(4096)
+
+    def take(T, B, N, S, G=1, no_bc=0):
+        s = _lib.Selective(T, B, N, S, G, 0, 1, 0, 0, no_bc)
+        return lib.delrec_selective_backward_workspace(ctypes.byref(s))
+
+    for T, B, N, S, G, places in ((250, 256, 2048, 128, 1, 128), (250, 256, 512, 16, 1, 8), (9, 4000, 64, 100, 1, 4),
+                                  (64, 600, 64, 128, 1, 8), (100, 256, 4096, 64, 4, 64)):
+        none = take(T, B, N, S, G, 1)
+        # dA, dD and dbias to each sequence and chunk (one chunk here)
+        assert B * N * (S + 2) * 4 <= none <= B * N * (S + 2) * 4 + 4096
+        assert take(T, B, N, S, G) - none <= 2 * places * T * B * G * S * 4 + 1024
+    s = _lib.Selective(4, 2, 8, 16, 1, 0, 1, 0, 0, 1)
+    need = take(4, 2, 8, 16)
+    for dB, dC in ((p, None), (None, p)):
+        assert lib.delrec_selective_backward(ctypes.byref(s), p, p, p, p, p, *(None,) * 5, p, p, None, p, p, p, dB, dC, None, None,
+                                             None, None, p, need, None) == 1
