@@ -76,7 +76,7 @@ class Selective(ctypes.Structure):
 class Vocab(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("T", "B", "D", "V", "K", "dtype", "distill", "reduction", "lengths_wide",
                                               "index_wide", "teacher_dtype", "w_aligned")] \
-        + [("temperature", ctypes.c_float), ("reserved", ctypes.c_int32)] + _i64("ignore_index", "x_t", "x_b")
+        + [("temperature", ctypes.c_float), ("split", ctypes.c_int32)] + _i64("ignore_index", "x_t", "x_b")
 
 
 _P = ctypes.c_void_p

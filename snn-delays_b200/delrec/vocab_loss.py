@@ -10,8 +10,10 @@ The (positions, vocabulary) logits live tile by tile in tensor memory; the backw
 their gradient for a piece of the vocabulary at a time, as the operand of the products for dx and
 dweight.  x, weight and bias are of one type, float32, bfloat16 or float16; sums are float32, and
 float32 operands keep float32 accuracy (three bf16 pieces each).  In a 16-bit type, where there are
-more than 512 positions, the logits' gradient is rounded to it once before the two products.  CUDA
-tensors only.
+more than 512 positions, the logits' gradient is rounded to it once before the two products: the
+gradients are then off by up to 1.4 times what their own rounding makes.  ``split=True`` keeps it in
+two pieces, as few positions do: no more off than from a float32 one, for half to four fifths of the
+training pass's time again.  CUDA tensors only.
 """
 
 from __future__ import annotations
@@ -28,23 +30,24 @@ REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_FEATURES, MAX_KEPT, MAX_POSITIONS, MAX_VOCABULARY = 8192, 1024, 1 << 24, 1 << 30
 
 
-def _struct(x, w, K, distill, reduction, lengths, index, logits, tau, ignore):
+def _struct(x, w, K, distill, reduction, lengths, index, logits, tau, ignore, split):
     T, B, D = x.shape
     wide = lambda t: 1 if t is not None and t.dtype == torch.int64 else 0   # noqa: E731
     return _lib.Vocab(T, B, D, w.shape[0], K, _lib.SEQ_DTYPES[x.dtype], distill, reduction, wide(lengths), wide(index),
                       _lib.SEQ_DTYPES[logits.dtype] if logits is not None else 0,
-                      1 if w.data_ptr() % 16 == 0 else 0, tau, 0, ignore, x.stride(0), x.stride(1))
+                      1 if w.data_ptr() % 16 == 0 else 0, tau, split, ignore, x.stride(0), x.stride(1))
 
 
 def _forward(x, w, bias, index, logits, lengths, meta):
     """(loss, what the backward pass takes over)"""
-    distill, reduction, tau, ignore = meta
+    distill, reduction, tau, ignore, split = meta
     T, B, _ = x.shape
     dev = x.device
     out = torch.empty((T, B) if reduction == 0 else (), device=dev)
     if not (T and B):
         return out.zero_(), None
-    s = _struct(x, w, index.shape[-1] if distill else 1, distill, reduction, lengths, index, logits, tau, ignore)
+    s = _struct(x, w, index.shape[-1] if distill else 1, distill, reduction, lengths, index, logits, tau, ignore,
+                split)
     lib, ref = _lib.lib(), ctypes.byref(s)
     nkeep, nbytes = lib.delrec_vocab_loss_keep(ref), lib.delrec_vocab_loss_forward_workspace(ref)
     keep, ws = _lib.scratch(nkeep, dev), _lib.scratch(nbytes, dev)
@@ -74,14 +77,14 @@ def _backward(ctx, g):
     if g is None:
         return (None,) * 7
     x, w, bias, keep = ctx.saved_tensors
-    distill, reduction, tau, ignore = ctx.meta
+    distill, reduction, tau, ignore, split = ctx.meta
     need = ctx.needs_input_grad
     dev = x.device
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
     dw = torch.empty_like(w) if need[1] else None
     db = torch.empty_like(bias) if bias is not None and need[2] else None
     if keep is not None:
-        s = _struct(x, w, ctx.kept, distill, reduction, None, None, None, tau, ignore)
+        s = _struct(x, w, ctx.kept, distill, reduction, None, None, None, tau, ignore, split)
         lib, ref = _lib.lib(), ctypes.byref(s)
         nbytes = lib.delrec_vocab_loss_backward_workspace(ref)
         ws = _lib.scratch(nbytes, dev)
@@ -145,7 +148,8 @@ def _run(x, w, bias, index, logits, lengths, meta, lead):
     return out.view(lead) if meta[1] == 0 else out
 
 
-def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, reduction="mean", lengths=None):
+def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, reduction="mean", lengths=None,
+                         split=False):
     """Softmax cross entropy of x weight^T + bias against ``target``, in float32.
 
     x (T,B,D) or (.., D), weight (V,D), bias (V); target int32 / int64 of x's leading shape.  Positions
@@ -153,20 +157,22 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, red
     ``lengths`` (B,) int32 / int64 (x (T,B,D)), where neither x nor target is read.  ``reduction``:
     "mean" over the positions that count (0 where none does), "sum", or "none" (losses of the leading
     shape).  Any other target outside the vocabulary makes its loss, and the gradients, NaN and sets a
-    bit of ``_lib.status()``.  Gradients reach x, weight and bias."""
+    bit of ``_lib.status()``.  Gradients reach x, weight and bias; ``split``: how they are rounded in a
+    16-bit type (above)."""
     lead = _check(x, weight, bias, reduction, lengths)
     if target.shape != lead or target.dtype not in (torch.int32, torch.int64) or target.device != x.device:
         raise RuntimeError(f"delrec_b200: target must be int32 or int64 {tuple(lead)} on {x.device}")
     ignore = int(ignore_index)
     if not -(1 << 63) <= ignore < 1 << 63:
         raise RuntimeError(f"delrec_b200: ignore_index {ignore} is past 64 bits")
-    return _run(x, weight, bias, target, None, lengths, (0, REDUCTIONS[reduction], 1.0, ignore), lead)
+    return _run(x, weight, bias, target, None, lengths, (0, REDUCTIONS[reduction], 1.0, ignore, 1 if split else 0), lead)
 
 
-def linear_distill(x, weight, indices, logits, bias=None, *, temperature=1.0, reduction="mean", lengths=None):
+def linear_distill(x, weight, indices, logits, bias=None, *, temperature=1.0, reduction="mean", lengths=None,
+                   split=False):
     """Distillation of x weight^T + bias from a teacher's K kept logits a position, in float32.
 
-    x, weight, bias, ``reduction``, ``lengths`` as in ``linear_cross_entropy``.  indices (.., K) int32 /
+    x, weight, bias, ``reduction``, ``lengths``, ``split`` as in ``linear_cross_entropy``.  indices (.., K) int32 /
     int64 and logits (.., K) float32, bfloat16 or float16, K from 1 to 1024: the teacher's distribution
     is p = softmax(logits / temperature) over them, the student's q = softmax(z / temperature) over the
     whole vocabulary, loss = temperature^2 sum_k p_k (log p_k - log q[indices_k]).  An entry with a
@@ -187,4 +193,5 @@ def linear_distill(x, weight, indices, logits, bias=None, *, temperature=1.0, re
     tau = float(temperature)
     if not 0.0 < tau < 1e30:
         raise RuntimeError(f"delrec_b200: temperature must be positive, got {temperature}")
-    return _run(x, weight, bias, indices, logits, lengths, (1, REDUCTIONS[reduction], tau, 0), lead)
+    return _run(x, weight, bias, indices, logits, lengths, (1, REDUCTIONS[reduction], tau, 0, 1 if split else 0),
+                lead)

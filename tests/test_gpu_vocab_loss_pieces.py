@@ -36,12 +36,13 @@ def _make(case, seed=0):
     return d, rnd(T, B) if reduction == "none" else torch.tensor(1.7, device="cuda")
 
 
-def _reference(d, case, grad):
-    """loss, dx, dw, db in float64 and the bounds of fp32 arithmetic with G rounded to its type once, 4096 positions at a time
+def _reference(d, case, grad, split=False):
+    """loss, dx, dw, db in float64 and the bounds of fp32 arithmetic with G rounded to its type once (split: and what that
+    leaves, once), 4096 positions at a time
     (as ``oracle.selective_oracle.vocab_loss`` has them for small sizes)."""
     (T, B), D, V, dtype, K, tau, reduction, _, _, _ = case
     f, M = torch.float64, T * B
-    half = HALF[dtype] if dtype != F32 else 4 * U
+    half = 4 * U if dtype == F32 else HALF[dtype] ** 2 if split else HALF[dtype]
     on = torch.ones(T, B, dtype=torch.bool, device="cuda")
     if d["lengths"] is not None:
         on &= torch.arange(T, device="cuda")[:, None] < d["lengths"][None]
@@ -97,19 +98,23 @@ def _reference(d, case, grad):
     return r, e
 
 
+def _loss(d, case, **kw):
+    from delrec.vocab_loss import linear_cross_entropy, linear_distill
+    _, _, _, _, K, tau, reduction, _, _, _ = case
+    if K:
+        return linear_distill(d["x"], d["w"], d["index"], d["logits"], d["bias"], temperature=tau, reduction=reduction,
+                              lengths=d["lengths"], **kw)
+    return linear_cross_entropy(d["x"], d["w"], d["index"], d["bias"], reduction=reduction, lengths=d["lengths"], **kw)
+
+
 @pytest.mark.parametrize("case", CASES)
 def test_against_float64(case):
     from delrec import _lib
-    from delrec.vocab_loss import linear_cross_entropy, linear_distill
-    _, D, V, dtype, K, tau, reduction, bias, _, pieces = case
+    pieces = case[-1]
     d, grad = _make(case)
     r, e = _reference(d, case, grad)
     leaves = {k: d[k].requires_grad_(True) for k in ("x", "w", "bias") if d[k] is not None}
-    if K:
-        loss = linear_distill(d["x"], d["w"], d["index"], d["logits"], d["bias"], temperature=tau, reduction=reduction,
-                              lengths=d["lengths"])
-    else:
-        loss = linear_cross_entropy(d["x"], d["w"], d["index"], d["bias"], reduction=reduction, lengths=d["lengths"])
+    loss = _loss(d, case)
     within(loss, r["loss"], e["loss"], "loss")
     before = _lib.launch_count()
     grads = torch.autograd.grad(loss, list(leaves.values()), grad)
@@ -118,9 +123,36 @@ def test_against_float64(case):
     for k, v in zip(leaves, grads):
         name = {"x": "dx", "w": "dw", "bias": "db"}[k]
         within(v, r[name], e[name], name)
-    again = torch.autograd.grad(linear_distill(d["x"], d["w"], d["index"], d["logits"], d["bias"], temperature=tau,
-                                               reduction=reduction, lengths=d["lengths"]) if K else
-                                linear_cross_entropy(d["x"], d["w"], d["index"], d["bias"], reduction=reduction,
-                                                     lengths=d["lengths"]), list(leaves.values()), grad)
-    for a, v in zip(again, grads):
+    for a, v in zip(torch.autograd.grad(_loss(d, case), list(leaves.values()), grad), grads):
         assert torch.equal(a, v)
+
+
+@pytest.mark.parametrize("case", [c for c in CASES if c[3] != F32])
+def test_split_gradient_against_float64(case):
+    """Two pieces of a 16-bit gradient: what its rounding adds is squared."""
+    d, grad = _make(case, 1)
+    r, e = _reference(d, case, grad, True)
+    leaves = {k: d[k].requires_grad_(True) for k in ("x", "w", "bias") if d[k] is not None}
+    loss = _loss(d, case, split=True)
+    assert torch.equal(loss, _loss(d, case))
+    for k, v in zip(leaves, torch.autograd.grad(loss, list(leaves.values()), grad)):
+        name = {"x": "dx", "w": "dw", "bias": "db"}[k]
+        within(v, r[name], e[name], name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("positions", [512, 513])
+def test_error_of_a_distillation(positions, dtype):
+    """Root mean square errors: with two pieces (``split``, or up to 512 positions) that of rounding the result, at most one
+    half step evenly (HALF / sqrt(3) of an entry), with one piece as much again at random from the targets' entries."""
+    case = ((1, positions), 512, 4000, dtype, 64, 2.0, "mean", False, False, 1)
+    d, grad = _make(case, 2)
+    r, _ = _reference(d, case, grad)
+    leaves = [d[k].requires_grad_(True) for k in ("x", "w")]
+    for split in (False, True):
+        got = torch.autograd.grad(_loss(d, case, split=split), leaves, grad)
+        for v, name in zip(got, ("dx", "dw")):
+            ref = r[name]
+            err = ((v.double() - ref).pow(2).mean() / ref.pow(2).mean()).sqrt().item()
+            one = HALF[dtype] * 3 ** -0.5
+            assert err <= (1.02 if split or positions <= 512 else 1.5) * one, (name, split, err / one)
