@@ -42,7 +42,7 @@ struct VgArgs {
   int M, K;                     // output rows and reduction length; -1: *rows
   int N;                        // output columns
   int nprod, pa[kVgMaxProd], pb[kVgMaxProd];
-  int a_mn, b_mn, a_k, b_k;     // where the operands start
+  int b_mn, b_k;                // where B starts
   int splits, seg;              // reduction in `splits` parts of whole segments of `seg` 64-blocks (0: one per part)
   int* status;
   long long spin_ns;
@@ -238,7 +238,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
       bool ok = true;
       for (unsigned w = w0; ok && w < items; w += dw) {
         const int m0 = tile_m(w) * 256 + (int)rank * 128, n0 = tile_n(w) * BN, sp = tile_s(w);
-        const int am = g.a_mn + m0, bm = g.b_mn + n0 + (int)rank * (BN < 256 ? BN / 2 : 128);
+        const int bm = g.b_mn + n0 + (int)rank * (BN < 256 ? BN / 2 : 128);
         const int s1 = first_seg(sp + 1);
         for (int s = first_seg(sp); ok && s < s1; ++s) {
           const int k0 = s * seg, k1 = min(kb, k0 + seg);
@@ -252,12 +252,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVgThreads, 1)
               }
               const uint32_t bar = vg_first(full0 + 8 * st), a = sA + st * A_BYTES, b = sB + st * B_BYTES;
               if (rank == 0) mbar_expect_tx(full0 + 8 * st, 2 * (A_BYTES + B_BYTES));
-              const int ak = g.a_k + 64 * k, bk = g.b_k + 64 * k;
+              const int ak = 64 * k, bk = g.b_k + 64 * k;
               if (AMN) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) vg_load(a + q * 8192, &ma, am + 64 * q, ak, za, bar);
+                for (int q = 0; q < 2; ++q) vg_load(a + q * 8192, &ma, m0 + 64 * q, ak, za, bar);
               } else {
-                vg_load(a, &ma, ak, am, za, bar);
+                vg_load(a, &ma, ak, m0, za, bar);
               }
               // of each 256 columns a CTA holds 128
               if (BMN) {
