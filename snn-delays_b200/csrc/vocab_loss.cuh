@@ -350,8 +350,7 @@ static __global__ void __launch_bounds__(1024) k_vocab_lse(const VocabArgs a, co
     for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     if (lane == 0) {
       a.lse[mine] = top + ls;
-      float loss = a.tau * a.tau * fmaf(-kLn2v, dot, a.p ? a.h[mine] : 0.f);
-      loss = loss < 0.f ? 0.f : loss;   // as the formula: p and q are distributions
+      const float loss = a.tau * a.tau * fmaf(-kLn2v, dot, a.p ? a.h[mine] : 0.f);
       a.loss[mine] = loss;
       if (each) each[a.rowmap[mine]] = loss;
     }

@@ -140,6 +140,25 @@ def test_split_gradient_against_float64(case):
         within(v, r[name], e[name], name)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [1, 5, 129, 900])
+@pytest.mark.parametrize("K", [1, 2, 8, 9, 31, 32, 33, 128, 129, 1000, 1024])
+def test_lists_of_every_length(K, V, dtype):
+    """Lists longer and shorter than the vocabulary, most of them with tokens that stand many times."""
+    case = ((1, 37), 40, V, dtype, K, 2.0, "none", True, False, 1)
+    d, grad = _make(case, 3)
+    d["index"][0, 0, 3:] = -1              # a position of three entries at most, one of a single token, one of none
+    d["index"][0, 1] = V - 1
+    d["index"][0, 2] = -1
+    r, e = _reference(d, case, grad)
+    leaves = {k: d[k].requires_grad_(True) for k in ("x", "w", "bias")}
+    loss = _loss(d, case)
+    within(loss, r["loss"], e["loss"], "loss")
+    for k, v in zip(leaves, torch.autograd.grad(loss, list(leaves.values()), grad)):
+        name = {"x": "dx", "w": "dw", "bias": "db"}[k]
+        within(v, r[name], e[name], name)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("positions", [512, 513])
 def test_error_of_a_distillation(positions, dtype):
