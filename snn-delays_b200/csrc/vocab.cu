@@ -105,7 +105,7 @@ static VocabShape vocab_shape(const delrec_vocab* s, bool backward) {
   if (!backward) {
     const long long tiles = (s->V + h.bnv - 1) / h.bnv * 2;
     h.part = take((size_t)tiles * h.Mp * sizeof(float2));
-    h.tab = take(s->K > 1 ? (size_t)tiles * h.Mp * 4 : 0);
+    h.tab = take(s->K > kVgFew ? (size_t)tiles * h.Mp * 4 : 0);
     h.flags = take(s->distill ? h.M : 0);
     h.ticket = take(4);
     h.h = take((size_t)h.M * 4);
@@ -232,13 +232,15 @@ int delrec_vocab_loss_forward(const delrec_vocab* s, const void* x, const void* 
   int rc = vocab_w(s, h, a, base, &W, st);
   if (rc) return rc;
   const int halves = (s->V + h.bnv - 1) / h.bnv * 2;
-  unsigned* tab = s->K > 1 ? (unsigned*)(base + h.tab) : nullptr;
+  unsigned* tab = s->K > kVgFew ? (unsigned*)(base + h.tab) : nullptr;
   rc = by_dtype(s->dtype, [&](auto t) {
     using E = decltype(t);
     const int W = s->K == 1 ? 1 : s->K <= 32 ? 32 : 128, blocks = (a.M + 128 / W - 1) / (128 / W);
-    const size_t smem = W == 1 ? 0 : (size_t)(128 / W) * 4 * s->K * 4;
+    int P = 128;
+    while (P < s->K) P *= 2;
+    const size_t smem = W == 128 ? (size_t)P * 16 : 0;
     auto kern = W == 1 ? k_vocab_targets<E, 1> : W == 32 ? k_vocab_targets<E, 32> : k_vocab_targets<E, 128>;
-    kern<<<blocks + seq_grid((size_t)h.Mp * (h.Dp / 8), 128, 16), 128, smem, st>>>(a, blocks, pack, tab, h.Mp, halves, h.bnv / 2);
+    kern<<<blocks + seq_grid((size_t)h.Mp * (h.Dp / 8), 128, 16), 128, smem, st>>>(a, blocks, pack, tab, h.Mp, halves, h.bnv / 2, P);
     SQ_LAUNCHED();
     return (int)DELREC_OK;
   });

@@ -170,16 +170,52 @@ __global__ void __launch_bounds__(256) k_vocab_pack(const VocabPack k) {
   vocab_pack<T>(k, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
 }
 
-// The targets of a packed row, W threads to it: their tokens in rising order, each once, with the sum of its
-// p (then -1), h = sum p log p, and where each half tile of the logits (`cols` columns) finds its first target:
-// tab[half][row] = place in the list << 8 | column, 255 without one.  Their logits come from the product that
-// makes the statistics: a dot product of its own is off by another rounding than the log-sum-exp (the tensor
-// core's accumulator truncates), and that difference is all there is of the loss of a target that is nearly
-// certain (z = 40 over 512 channels: -4e-5 of 0).  The blocks from `blocks` on bring x into operands:
-// both wait for the packed rows alone.
+// entry e of a teacher's lists, `there` if it is one: its token and logit, kVocabNone and -inf where it is left out,
+// kVocabNone and bad where its index is past the vocabulary
+constexpr int kVocabNone = 0x7fffffff;
+__device__ __forceinline__ int vocab_entry(const VocabArgs& a, size_t e, bool there, float& t, bool& bad) {
+  t = -INFINITY;
+  if (!there) return kVocabNone;
+  const long long i = vocab_index(a, e);
+  const float v = vocab_teacher(a, e);
+  if (!vocab_kept(i, v)) return kVocabNone;
+  t = v;
+  if (i < a.V) return (int)i;
+  atomicOr(a.status, kVocabIndexRange);
+  bad = true;
+  return kVocabNone;
+}
+// where each half tile of `cols` columns finds its first of the n tokens of a rising list, by `step` threads
+__device__ __forceinline__ void vocab_halves(const int* list, int n, int first, int step, unsigned* tab, long long ld, int halves,
+                                             int cols) {
+  for (int t = first; t < halves; t += step) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (list[mid] < t * cols) lo = mid + 1;
+      else hi = mid;
+    }
+    const int off = lo < n ? list[lo] - t * cols : cols;
+    tab[t * ld] = (unsigned)lo << 8 | (off < cols ? off : 255);
+  }
+}
+
+// The targets of a packed row: their tokens in rising order, each once, with the sum of its p (then -1), h = sum p log p,
+// and where each half tile of the logits (`cols` columns) finds its first target: tab[half][row] = place in the list << 8 |
+// column, 255 without one (tab NULL: not wanted).  Differences of a teacher's logits are taken first: those of the
+// type's lowest value stay finite at any temperature.
+//
+// Their logits come from the product that makes the statistics: a dot product of its own is off by another rounding
+// than the log-sum-exp (the tensor core's accumulator truncates), and that difference is all there is of the loss of a
+// target that is nearly certain (z = 40 over 512 channels: -4e-5 of 0).  It was slower, too: 4096 rows of 64 targets, 512
+// channels, bf16, 54 us of a forward pass of 171, now 154; of 1024 targets 1573, now 414.
+//
+// W threads to a row: one for one target; a warp, an entry to a lane, up to 32 (sorted by counting, K steps: 4096 rows of
+// four 22 us of the small pass, 26 by the block's way); else a block, by a bitonic sort of P places (K's power of two, 128
+// at least).  The blocks from `blocks` on bring x into operands: both wait for the packed rows alone.
 template <class T, int W>
 __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a, int blocks, const VocabPack pack, unsigned* tab,
-                                                       long long ld, int halves, int cols) {
+                                                       long long ld, int halves, int cols, int P) {
   if ((int)blockIdx.x >= blocks) {
     vocab_pack<T>(pack, (blockIdx.x - blocks) * 128LL + threadIdx.x, (gridDim.x - blocks) * 128LL);
     return;
@@ -193,108 +229,147 @@ __global__ void __launch_bounds__(128) k_vocab_targets(const VocabArgs a, int bl
     if (!in) atomicOr(a.status, kVocabIndexRange);
     a.idx[r] = ok ? (int)i : -1;
     if (!ok) a.y[r] = __int_as_float(0x7fc00000);
-  } else {
-    extern __shared__ int smi[];
-    __shared__ float s_red[4];
-    const int tid = threadIdx.x % W, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int* s_i = smi + threadIdx.x / W * 4 * K;       // [K] tokens; -1 left out, -2 out of range; later in rising order
-    float* s_p = (float*)(s_i + K);                 // [K]
-    int* s_u = s_i + 2 * K;                         // [K] the token where it stands first, else kNone
-    float* s_s = (float*)(s_i + 3 * K);             // [K] the sum of its p
-    constexpr int kNone = 0x7fffffff;
-    const auto sync = [] {
-      if (W == 32) __syncwarp();
-      else __syncthreads();
+  } else if constexpr (W == 32) {  // an entry to a lane
+    __shared__ int s_few[4][32];
+    constexpr unsigned full = 0xffffffffu;
+    const int lane = threadIdx.x & 31;
+    const auto all = [&](float v, bool max) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        const float u = __shfl_xor_sync(full, v, o);
+        v = max ? fmaxf(v, u) : v + u;
+      }
+      return v;
     };
+    bool bad = false;
+    float t;
+    const int i = vocab_entry(a, (size_t)m * K + lane, lane < K, t, bad);
+    const float top = all(t, true), sum = all(t == -INFINITY ? 0.f : expf((t - top) / a.tau), false);
+    const float lp = (t - top) / a.tau - logf(sum), p = t == -INFINITY ? 0.f : expf(lp);
+    const float h = all(bad ? __int_as_float(0x7fc00000) : p != 0.f ? p * lp : 0.f, false);
+    if (lane == 0) a.h[r] = h;
+    float s = 0.f;
+    int first = 32, rank = 0;
+    for (int j = K - 1; j >= 0; --j) {
+      const float q = __shfl_sync(full, p, j);
+      if (__shfl_sync(full, i, j) == i) {
+        s += q;
+        first = j;
+      }
+    }
+    const bool on = i != kVocabNone && first == lane;
+    const int u = on ? i : kVocabNone, n = __popc(__ballot_sync(full, on));
+    for (int j = 0; j < K; ++j) rank += __shfl_sync(full, u, j) < i;
+    const size_t e = (size_t)r * K;
+    if (on) {
+      a.idx[e + rank] = i;
+      a.p[e + rank] = s;
+    }
+    if (lane >= n && lane < K) {
+      a.idx[e + lane] = -1;
+      a.p[e + lane] = a.y[e + lane] = 0.f;
+    }
+    if (!tab) return;
+    int* s_i = s_few[threadIdx.x >> 5];
+    if (on) s_i[rank] = i;
+    __syncwarp();
+    vocab_halves(s_i, n, lane, 32, tab + r, ld, halves, cols);
+  } else {
+    extern __shared__ unsigned long long s_key[];    // [P] token and place, in rising order
+    __shared__ float s_red[4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float* s_p = (float*)(s_key + P);                // [P]
+    int* s_i = (int*)(s_p + P);                      // [P] the tokens, each once
+    const auto token = [&](int e) { return (int)(s_key[e] >> 10); };
     const auto all = [&](float v, bool max) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) {
         const float u = __shfl_xor_sync(0xffffffffu, v, o);
         v = max ? fmaxf(v, u) : v + u;
       }
-      if (W > 32) {
-        __syncthreads();
-        if (lane == 0) s_red[warp] = v;
-        __syncthreads();
-        v = s_red[0];
-        for (int w = 1; w < 4; ++w) v = max ? fmaxf(v, s_red[w]) : v + s_red[w];
-      }
+      __syncthreads();
+      if (lane == 0) s_red[warp] = v;
+      __syncthreads();
+      v = s_red[0];
+      for (int w = 1; w < 4; ++w) v = max ? fmaxf(v, s_red[w]) : v + s_red[w];
       return v;
     };
     float top = -INFINITY, h = 0.f;
-    for (int k = tid; k < K; k += W) {
-      const size_t e = (size_t)m * K + k;
-      long long i = vocab_index(a, e);
-      float t = vocab_teacher(a, e);
-      if (!vocab_kept(i, t)) {
-        i = -1;
-        t = -INFINITY;
-      } else if (i >= a.V) {
-        atomicOr(a.status, kVocabIndexRange);
-        i = -2;
-        h = __int_as_float(0x7fc00000);
-      }
-      s_i[k] = (int)i;
+    for (int k = tid; k < P; k += W) {
+      bool bad = false;
+      float t;
+      const int i = vocab_entry(a, (size_t)m * K + k, k < K, t, bad);
+      if (bad) h = __int_as_float(0x7fc00000);
+      s_key[k] = (unsigned long long)i << 10 | k;
       s_p[k] = t;
       top = fmaxf(top, t);
     }
-    // differences first: logits of the type's lowest value stay finite at any temperature
     top = all(top, true);
     float sum = 0.f;
-    for (int k = tid; k < K; k += W) sum += s_i[k] == -1 ? 0.f : expf((s_p[k] - top) / a.tau);
+    for (int k = tid; k < K; k += W) sum += s_p[k] == -INFINITY ? 0.f : expf((s_p[k] - top) / a.tau);
     const float ls = logf(all(sum, false));
     for (int k = tid; k < K; k += W) {
-      const float lp = (s_p[k] - top) / a.tau - ls, p = s_i[k] == -1 ? 0.f : expf(lp);
+      const float lp = (s_p[k] - top) / a.tau - ls, p = s_p[k] == -INFINITY ? 0.f : expf(lp);
       s_p[k] = p;
       if (p != 0.f) h = fmaf(p, lp, h);
     }
     h = all(h, false);
     if (tid == 0) a.h[r] = h;
-    sync();
-    float own = 0.f;
-    for (int k = tid; k < K; k += W) {
-      const int i = s_i[k];
-      float s = 0.f;
-      int first = K;
-#pragma unroll 4
-      for (int j = K - 1; j >= 0; --j)
-        if (s_i[j] == i) {
-          s += s_p[j];
-          first = j;
+    __syncthreads();
+    for (int size = 2; size <= P; size *= 2)         // bitonic sort
+      for (int step = size / 2; step; step /= 2) {
+        for (int j = tid; j < P / 2; j += W) {
+          const int lo = 2 * j - (j & (step - 1)), hi = lo + step;
+          const unsigned long long u = s_key[lo], v = s_key[hi];
+          if ((u > v) == !(lo & size)) {
+            s_key[lo] = v;
+            s_key[hi] = u;
+          }
         }
-      const bool on = i >= 0 && first == k;
-      s_u[k] = on ? i : kNone;
-      s_s[k] = s;
-      own += on;
-    }
-    const int n = (int)all(own, false);
-    sync();
-    for (int k = tid; k < K; k += W) {
-      const int i = s_u[k];
-      if (i != kNone) {
-        int rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < K; ++j) rank += s_u[j] < i;
-        s_i[rank] = i;
-        a.idx[(size_t)r * K + rank] = i;
-        a.p[(size_t)r * K + rank] = s_s[k];
+        __syncthreads();
       }
-      if (k >= n) {
-        a.idx[(size_t)r * K + k] = -1;
-        a.p[(size_t)r * K + k] = a.y[(size_t)r * K + k] = 0.f;
-      }
+    // a thread's stretch of the sorted list: its tokens that stand there first, behind those of the threads before
+    const int C = P / W, e0 = tid * C;
+    int before = e0 ? token(e0 - 1) : kVocabNone, own = 0;
+    for (int e = e0; e < e0 + C; ++e) {
+      const int i = token(e);
+      own += i != kVocabNone && i != before;
+      before = i;
     }
-    sync();
-    for (int t = tid; t < halves; t += W) {
-      int lo = 0, hi = n;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (s_i[mid] < t * cols) lo = mid + 1;
-        else hi = mid;
-      }
-      const int off = lo < n ? s_i[lo] - t * cols : cols;
-      tab[t * ld + r] = (unsigned)lo << 8 | (off < cols ? off : 255);
+    int at = own, n = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int u = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += u;
     }
+    __syncthreads();
+    if (lane == 31) s_red[warp] = __int_as_float(at);
+    __syncthreads();
+    at -= own;
+    for (int w = 0; w < 4; ++w) {
+      const int u = __float_as_int(s_red[w]);
+      at += w < warp ? u : 0;
+      n += u;
+    }
+    before = e0 ? token(e0 - 1) : kVocabNone;
+    for (int e = e0; e < e0 + C; ++e) {
+      const int i = token(e);
+      if (i != kVocabNone && i != before) {
+        float s = 0.f;
+        for (int j = e; j < P && token(j) == i; ++j) s += s_p[s_key[j] & 1023];
+        s_i[at] = i;
+        a.idx[(size_t)r * K + at] = i;
+        a.p[(size_t)r * K + at] = s;
+        ++at;
+      }
+      before = i;
+    }
+    for (int k = n + tid; k < K; k += W) {
+      a.idx[(size_t)r * K + k] = -1;
+      a.p[(size_t)r * K + k] = a.y[(size_t)r * K + k] = 0.f;
+    }
+    __syncthreads();
+    vocab_halves(s_i, n, tid, W, tab + r, ld, halves, cols);
   }
 }
 
