@@ -605,7 +605,8 @@ __global__ void __launch_bounds__(64) k_sel_join(const SelArgs p, const float* _
       const int c = BACK ? p.chunks - 1 - (c0 + k) : c0 + k;
       if (c0 + k < p.chunks) {
         p.loc[((size_t)c * p.B + b) * row + ns] = h;
-        h = cut[k] ? loc[k] : fmaf(sel_exp2(A * d[k]), h, loc[k]);
+        // (0 stays 0 also where a chunk grows past the largest float)
+        h = cut[k] || h == 0.f ? loc[k] : fmaf(sel_exp2(A * d[k]), h, loc[k]);
       }
     }
   }

@@ -99,3 +99,37 @@ def test_a_step_with_a_decay_of_minus_infinity(B):
     ys, hs = selective_scan(d["x"], d["dt"], d["A"], d["Bm"], d["Cm"], d["h0"], D=d["D"], gate=d["gate"], dt_bias=d["dt_bias"])
     assert torch.isfinite(y).all() and torch.equal(h, hs)
     torch.testing.assert_close(y, ys[0], rtol=2.0 ** -18, atol=2.0 ** -18)     # the order of a sum of eight
+
+
+@pytest.mark.parametrize("back", [False, True])
+def test_growth_past_the_largest_number_of_a_state_that_is_zero(back):
+    """A chunk of time may grow by more than a float holds; a state (or gradient) of 0 in front of it stays 0."""
+    from delrec.selective import selective_scan
+    T, N, S = 1024, 4, 4
+    g = torch.Generator().manual_seed(8)
+    rnd = lambda *s: torch.randn(*s, generator=g).cuda()   # noqa: E731
+    dt, A = torch.ones(T, 1, N, device="cuda"), torch.full((N, S), 2.0, device="cuda")
+    bm, cm, x = rnd(T, 1, S), rnd(T, 1, S), rnd(T, 1, N)
+    gy = torch.ones(T, 1, N, device="cuda")
+    if back:                               # only the first steps are looked at
+        gy[10:] = 0
+        x[10:] = 0
+        bm[:] = 0
+    else:
+        x[:-10] = 0
+    x.requires_grad_(True)
+    y, hT = selective_scan(x, dt, A, bm, cm, softplus=False)
+    (dx,) = torch.autograd.grad(y, x, gy)
+    # the steps that matter alone, uncut
+    part = slice(0, 10) if back else slice(T - 10, T)
+    xs = x.detach()[part].clone().requires_grad_(True)
+    ys, hs = selective_scan(xs, dt[part], A, bm[part], cm[part], softplus=False)
+    (ds,) = torch.autograd.grad(ys, xs, gy[part])
+    # (of steps that reach states a thousand steps on, e^2000 larger, dx is infinite by the formula, too)
+    assert torch.isfinite(y).all() and torch.isfinite(dx[part]).all()
+    # the sums cut in other places
+    torch.testing.assert_close(y[part], ys, rtol=2.0 ** -18, atol=0)
+    torch.testing.assert_close(dx[part], ds, rtol=2.0 ** -18, atol=0)
+    if not back:
+        torch.testing.assert_close(hT, hs, rtol=2.0 ** -18, atol=0)
+        assert (y[:-10] == 0).all()
