@@ -415,17 +415,19 @@ static __global__ void __launch_bounds__(1024) k_vocab_lse(const VocabArgs a, co
     float dot = 0.f;
     for (int k = lane; k < a.K; k += 32) {
       const size_t e = (size_t)mine * a.K + k;
-      float d = fmaf(a.y[e], a.scale, -top) - ls;
+      const float z = a.y[e];
+      float d = fmaf(z, a.scale, -top) - ls;
       d = d > 0.f ? 0.f : d;            // (NaN stays)
       a.y[e] = d;
       const float p = a.p ? a.p[e] : 1.f;
-      if (p != 0.f) dot = fmaf(p, d, dot);
+      // a logit that a mask made the type's lowest value has no z log2(e), but a loss
+      if (p != 0.f) dot = fmaf(p, d == -INFINITY && z > -INFINITY ? z / a.tau : kLn2v * d, dot);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     if (lane == 0) {
       a.lse[mine] = top + ls;
-      const float loss = a.tau * a.tau * fmaf(-kLn2v, dot, a.p ? a.h[mine] : 0.f);
+      const float loss = a.tau * a.tau * ((a.p ? a.h[mine] : 0.f) - dot);
       a.loss[mine] = loss;
       if (each) each[a.rowmap[mine]] = loss;
     }
