@@ -462,7 +462,7 @@ typedef struct delrec_vocab {
   int32_t index_wide;        /* index is int64 */
   int32_t teacher_dtype;     /* of logits */
   int32_t w_aligned;         /* W is 16-byte aligned */
-  float temperature;         /* tau > 0; 1 for the cross entropy */
+  float temperature;         /* tau, 1e-6 to 1e6; 1 for the cross entropy */
   int32_t split;             /* backward: the logits' gradient of a 16-bit type in two pieces of it, also past 512 positions */
   int64_t ignore_index;
   int64_t x_t, x_b;

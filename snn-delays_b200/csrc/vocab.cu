@@ -14,7 +14,7 @@ static int check_vocab(const delrec_vocab* s) {
   if (s->dtype < DELREC_F32 || s->dtype > DELREC_F16 || s->reduction < 0 || s->reduction > 2) return DELREC_ERR_ARG;
   if (s->distill && (s->teacher_dtype < DELREC_F32 || s->teacher_dtype > DELREC_F16)) return DELREC_ERR_ARG;
   if (!s->distill && s->K != 1) return DELREC_ERR_ARG;
-  if (!(s->temperature > 0.f) || !(s->temperature < 1e30f)) return DELREC_ERR_ARG;
+  if (!(s->temperature > 0.99e-6f) || !(s->temperature < 1.01e6f)) return DELREC_ERR_ARG;   // 1e-6 to 1e6
   // tiles of 256 x 128 at least, in up to 16 parts, are counted in 32 bits
   if (((long long)s->T * s->B / 256 + 1) * (s->V / 128 + 1) > (1LL << 27)) return DELREC_ERR_UNSUPPORTED;
   if (s->D > kVocabMaxD || s->K > kVocabMaxK || s->V > (1 << 30) || (long long)s->T * s->B > (1 << 24))

@@ -27,6 +27,9 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+# An exponent z log2(e) / temperature is off by 2^-24 of itself: past 2^31 its power of two is no float any more.  The
+# loss is good to some temperature^2 2^-20.
+MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-6, 1e6
 MAX_FEATURES, MAX_KEPT, MAX_POSITIONS, MAX_VOCABULARY = 8192, 1024, 1 << 24, 1 << 30
 
 
@@ -175,9 +178,9 @@ def linear_distill(x, weight, indices, logits, bias=None, *, temperature=1.0, re
     x, weight, bias, ``reduction``, ``lengths``, ``split`` as in ``linear_cross_entropy``.  indices (.., K) int32 /
     int64 and logits (.., K) float32, bfloat16 or float16, K from 1 to 1024: the teacher's distribution
     is p = softmax(logits / temperature) over them, the student's q = softmax(z / temperature) over the
-    whole vocabulary, loss = temperature^2 sum_k p_k (log p_k - log q[indices_k]).  An entry with a
-    negative index or a logit of -inf is left out; a position that keeps none does not count.  An
-    index that stands twice counts twice.  An index past the vocabulary makes its loss, and the gradients,
+    whole vocabulary, loss = temperature^2 sum_k p_k (log p_k - log q[indices_k]), temperature from
+    1e-6 to 1e6.  An entry with a negative index or a logit of -inf is left out; a position that keeps
+    none does not count.  An index that stands twice counts twice.  An index past the vocabulary makes its loss, and the gradients,
     NaN and sets a bit of ``_lib.status()``.  Gradients reach x, weight and bias, not the teacher."""
     lead = _check(x, weight, bias, reduction, lengths)
     ishape = indices.shape
@@ -191,7 +194,7 @@ def linear_distill(x, weight, indices, logits, bias=None, *, temperature=1.0, re
     if torch.is_grad_enabled() and logits.requires_grad:
         raise RuntimeError("delrec_b200: no gradient passes to the teacher's logits; detach them")
     tau = float(temperature)
-    if not 0.0 < tau < 1e30:
-        raise RuntimeError(f"delrec_b200: temperature must be positive, got {temperature}")
+    if not MIN_TEMPERATURE <= tau <= MAX_TEMPERATURE:
+        raise RuntimeError(f"delrec_b200: temperature must be from {MIN_TEMPERATURE} to {MAX_TEMPERATURE}, got {temperature}")
     return _run(x, weight, bias, indices, logits, lengths, (1, REDUCTIONS[reduction], tau, 0, 1 if split else 0),
                 lead)

@@ -1,4 +1,4 @@
-"""Tokens masked through the bias, by -inf or by the type's lowest value."""
+"""Tokens masked through the bias, by -inf or by the type's lowest value, and temperatures at their limits."""
 
 import pytest
 import torch
@@ -75,3 +75,25 @@ def test_a_masked_target(K, dtype):
         assert all(torch.isfinite(v).all() for v in grads)
         # the position's share of its target is all that reaches bias[0]: q - p = -1 / K there
         assert abs(grads[2][0].item() + 1 / max(K, 1)) <= HALF[dtype] + 4 * U
+
+
+def test_temperatures_at_their_limits():
+    """From 1e-6 to 1e6, against float64; past those refused."""
+    from delrec.vocab_loss import linear_distill
+    x, w, b, _, live, t = _inputs(torch.float32)
+    logits = torch.randn(70, 3, generator=torch.Generator().manual_seed(3)).cuda()
+    idx = torch.stack([t, live[:70], live[70:140]], 1)
+    z = x.detach().double() @ w.detach().double().t() + b.double()
+    for tau in (1e-6, 1e-3, 1e3, 1e6):
+        loss = linear_distill(x, w, idx, logits, b, temperature=tau, reduction="none")
+        lp = torch.log_softmax(logits.double() / tau, 1)
+        want = tau * tau * (lp.exp() * (torch.where(lp > -1e300, lp, 0.0) - torch.log_softmax(z / tau, 1).gather(1, idx))).sum(1)
+        # logits of magnitudes below 30 (15 of them at most twice over): (D / 16 + 12) 2 u of them twice, times tau; sums and p
+        # 300 u of log 300, times tau^2; an exponent's rounding in p, |t| u / tau of an entry whose log q is |z| / tau
+        bound = U * (tau * 30 * 30 * 2 + 16 * 30 + tau * tau * 300 * 6)
+        assert ((loss.double() - want).abs() <= bound + 4 * U * want.abs()).all(), tau
+        dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+        assert torch.isfinite(dx).all()
+    for tau in (0.9e-6, 1.1e6, 1e-300, 1e29):
+        with pytest.raises(RuntimeError, match="temperature"):
+            linear_distill(x, w, idx, logits, b, temperature=tau)
