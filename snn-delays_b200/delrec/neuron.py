@@ -168,21 +168,29 @@ class BatchNorm1d(torch.nn.BatchNorm1d):
 # it.  A call captured in a graph moves the state that there is on in place, so that every replay takes it further.
 
 
-def _captured(state):
-    return state is not None and torch.cuda.is_current_stream_capturing()
+def _captured(m):
+    """Is a call of module ``m`` captured that moves a state on?  The state then lives as long as the module does,
+    also after ``reset``: replays write to it."""
+    if m.v is None or not torch.cuda.is_current_stream_capturing():
+        return False
+    held = m.__dict__.setdefault("_captured_states", [])
+    if not any(v is m.v for v in held):
+        held.append(m.v)
+    return True
 
 
 def _kept(m):
     """The state that a multi-step call of module ``m`` begins from (a copy where it will be written over: a backward
     pass may want it)."""
-    v = m.v if m.keep_state else None
-    return v.clone() if _captured(v) else v
+    if not m.keep_state:
+        return None
+    return m.v.clone() if _captured(m) else m.v
 
 
 def _keep(m, v):
     """``v`` is the state behind a multi-step call."""
     if m.keep_state:
-        if _captured(m.v):
+        if _captured(m):
             m.v.copy_(v.detach())
         else:
             m.v = v.detach()
@@ -214,7 +222,7 @@ class GatedIntegrator(MemoryModule):
         if self.step_mode == "s":
             if lengths is not None or resets is not None:
                 raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
-            h, self.v = gated_step(z, f, self.v, decay_input=self.decay_input, out=self.v if _captured(self.v) else None)
+            h, self.v = gated_step(z, f, self.v, decay_input=self.decay_input, out=self.v if _captured(self) else None)
             return h
         h, v = gated_scan(z, f, _kept(self), lengths=lengths, resets=resets,
                           decay_input=self.decay_input, checkpoint8=self.checkpoint8)
@@ -254,7 +262,7 @@ class ShortConv(MemoryModule):
         if self.step_mode == "s":
             if lengths is not None or resets is not None:
                 raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
-            y, self.v = short_conv_step(x, self.weight, self.bias, self.v, act=self.act, out=self.v if _captured(self.v) else None)
+            y, self.v = short_conv_step(x, self.weight, self.bias, self.v, act=self.act, out=self.v if _captured(self) else None)
             return y
         y, v = short_conv(x, self.weight, self.bias, _kept(self), act=self.act, lengths=lengths, resets=resets)
         _keep(self, v)
@@ -295,7 +303,7 @@ class SelectiveIntegrator(MemoryModule):
             if lengths is not None or resets is not None:
                 raise RuntimeError("delrec_b200: lengths and resets are for the multi-step mode")
             y, self.v = selective_step(x, dt, A, B, C, self.v, D=self.D, gate=gate, dt_bias=self.dt_bias,
-                                       out=self.v if _captured(self.v) else None)
+                                       out=self.v if _captured(self) else None)
             return y
         y, v = selective_scan(x, dt, A, B, C, _kept(self), D=self.D, gate=gate, dt_bias=self.dt_bias, lengths=lengths,
                               resets=resets)

@@ -124,3 +124,26 @@ def test_replays_of_a_captured_piece_go_on(kind, train):
             for a, b in zip(out, want[k]):
                 assert torch.equal(a, b), k
         assert torch.equal(m.v, last)
+
+
+@pytest.mark.parametrize("kind", ["conv", "scan", "gated"])
+def test_a_captured_state_outlives_a_reset(kind):
+    """Replays go on writing to the state of the capture: no one else is given its memory."""
+    m, seq = _modules(kind)
+    with torch.no_grad():
+        m(*(v[0] for v in seq))
+        size, dtype = m.v.numel() * m.v.element_size(), torch.uint8
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            y = m(*(v[1] for v in seq))
+        graph.replay()
+        torch.cuda.synchronize()
+        m.reset()
+        m(*(v[0] for v in seq))            # and a state of its own behind a call
+        m.reset()
+        others = [torch.full((size,), 77, dtype=dtype, device="cuda") for _ in range(64)]
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all((v == 77).all() for v in others) and torch.isfinite(y).all()
