@@ -28,6 +28,11 @@
 // reads of B and C, 255 registers: 886 to 1090), the states or the decays of half a segment in registers
 // (862 to 1240) and keeping every other state (846 to 909) none was faster backward.  Sums and states are
 // float32.
+//
+// A lane holds four states whether they are there or not, and a power of two of lanes a channel: the time goes in
+// steps at S = 4, 8, 16, .. (that fp32 case, forward and backward: S = 1 to 4 215 and 740 us, 5 to 8 230 and 655, 9 to 16
+// 270 and 830, 17 to 32 550 and 1750, 33 to 64 1130 and 4560).  S <= 4 is slower backward than 8: k_sel_bwd<float, 1>
+// has 255 registers and spills 172 bytes.
 #pragma once
 
 #include "f32x2.cuh"
@@ -80,9 +85,13 @@ __device__ __forceinline__ f2 exp22(f2 v) {
 // 2.1e-8 log2(e) more (a product and a sum cost what a product costs).  d = 0 still gives exactly 1.
 constexpr float kSelLow = 2.97e-8f;
 __device__ __forceinline__ f2 sel_decay2(f2 d, f2 A) { return exp22(fma2(d, A, pair(kSelLow, kSelLow))); }
-// A as the kernels take it: an infinite one is the largest number there is, whose decay over any step is the
-// same 0, so that delta = 0 (rows past the end, chunks without steps) leaves a state as it is: 0 A is not NaN.
-__device__ __forceinline__ float sel_finite(float A) { return fabsf(A) == INFINITY ? copysignf(3.402823466e38f, A) : A; }
+// A as the kernels take it: -inf is the lowest number there is, whose decay over any step is the same 0, so that
+// delta = 0 (rows past the end, chunks without steps) leaves a state as it is: 0 A is not NaN.  (A NaN stays one.)
+__device__ __forceinline__ float sel_finite(float A) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(A), "f"(-3.402823466e38f));
+  return r;
+}
 __device__ __forceinline__ float sel_rcp(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
