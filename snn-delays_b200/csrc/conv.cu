@@ -25,7 +25,9 @@ struct ConvAlign {
 };
 
 // Four channels to a thread: eight 16-bit ones take twice the registers, and a quarter of the warps
-// then fit an SM (T=250 B=256 N=512 K=4 bf16 forward 62 us, four 41).
+// then fit an SM (T=250 B=256 N=512 K=4 bf16 forward 62 us, four 41).  One to a thread where N is no multiple of
+// four or a tensor lies odd: the same with N=510, 56 us forward and 121 backward instead of 42 and 90 (fp32 73 and 137
+// instead of 53 and 135).
 static constexpr int kConvWidth = 4;
 // Chunks of time: threads of four channels for `per_sm` an SM, as many as fit at once, whose rows in
 // flight cover the memory's latency; at least 8 (K - 1) rows each, of which the rows in front of (and

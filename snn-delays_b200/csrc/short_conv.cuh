@@ -5,7 +5,11 @@
 // x_{-1} .. x_{-(K-1)} come from a state (K-1,B,N); a reset at t drops what lies before t.  A
 // thread owns V neighbouring channels of one sequence and walks a chunk of time with the window
 // (and, in the backward pass, the K partial sums of dx) in registers, so each tensor crosses the
-// memory once apart from the K - 1 rows in front of (and behind) a chunk.  Memory bounds both passes.
+// memory once apart from the K - 1 rows in front of (and behind) a chunk.
+//
+// What bounds it: latency, of loads that come a batch at a time to 13 to 18 warps an SM, and of the resets, a byte
+// a row read within the row's work.  T=250 B=256 N=512 K=4 bf16: forward 42 us at 2.2 TB/s and 46 % of the issue
+// slots, backward 77 us at 2.3 TB/s and 56 %; T=1021 B=24 N=700 K=3 fp32 with resets 25 and 42 us at 2.2 to 2.8 TB/s.
 #pragma once
 
 #include "seq_common.cuh"
