@@ -207,8 +207,8 @@ __device__ __forceinline__ void vocab_halves(const int* list, int n, int first, 
 //
 // Their logits come from the product that makes the statistics: a dot product of its own is off by another rounding
 // than the log-sum-exp (the tensor core's accumulator truncates), and that difference is all there is of the loss of a
-// target that is nearly certain (z = 40 over 512 channels: -4e-5 of 0).  It was slower, too: 4096 rows of 64 targets, 512
-// channels, bf16, 54 us of a forward pass of 171, now 154; of 1024 targets 1573, now 414.
+// target that is nearly certain (z = 40 over 512 channels: -4e-5 of 0).  It takes longer, too (4096 rows on 32768 tokens, 512
+// channels, bf16, forward: 64 targets 171 us instead of 154, 1024 targets 1573 instead of 414).
 //
 // W threads to a row: one for one target; a warp, an entry to a lane, up to 32 (sorted by counting, K steps: 4096 rows of
 // four 22 us of the small pass, 26 by the block's way); else a block, by a bitonic sort of P places (K's power of two, 128
