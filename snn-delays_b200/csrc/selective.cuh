@@ -989,22 +989,22 @@ __global__ void __launch_bounds__(kSelThreads, L == 4 || L == 8 ? 3 : 2) k_sel_b
   }
 }
 
-// out[j] = sum over parts of part[k][j], in order.  Block: 32 columns by 32 runs of parts.
+// out[j] = sum over parts of part[k][j], in order and in 64 bits.  Block: 32 columns by 32 runs of parts.
 static __global__ void __launch_bounds__(1024) k_sel_sum(long long cols, long long parts, const float* __restrict__ part,
                                                   float* __restrict__ out) {
-  __shared__ float sum[32][33];
+  __shared__ double sum[32][33];
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
   const long long j = blockIdx.x * 32LL + lane;
   const long long p0 = parts * run / 32, p1 = parts * (run + 1) / 32;
-  float s = 0.f;
+  double s = 0.0;
   if (j < cols)
     for (long long q = p0; q < p1; ++q) s += part[q * cols + j];
   sum[run][lane] = s;
   __syncthreads();
   if (run == 0 && j < cols) {
-    float t = 0.f;
+    double t = 0.0;
     for (int r = 0; r < 32; ++r) t += sum[r][lane];
-    out[j] = t;
+    out[j] = (float)t;
   }
 }
 // dB and dC (T,B,G,S) from their partial sums, one to a tile of channels of a launch

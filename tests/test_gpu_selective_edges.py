@@ -133,3 +133,25 @@ def test_growth_past_the_largest_number_of_a_state_that_is_zero(back):
     if not back:
         torch.testing.assert_close(hT, hs, rtol=2.0 ** -18, atol=0)
         assert (y[:-10] == 0).all()
+
+
+@pytest.mark.parametrize("B,N", [(4096, 8), (3001, 37)])
+def test_parameter_gradients_are_rounded_once_over_sequences(B, N):
+    """A sequence's sums for D and dt_bias are 8 + k 2^-20, exact in 24 bits; over the sequences they are added in 64."""
+    from delrec.selective import selective_scan
+    g = torch.Generator().manual_seed(0)
+    x = torch.ones(8, B, N)
+    x[0] += torch.randint(0, 1 << 19, (B, N), generator=g).float() * 2.0 ** -20
+    xc = x.cuda()
+    D, bias = torch.zeros(N, device="cuda", requires_grad=True), torch.zeros(N, device="cuda", requires_grad=True)
+    A = torch.zeros(N, 1, device="cuda")
+    ones = torch.ones(8, B, 1, device="cuda")
+    last = torch.zeros(8, B, 1, device="cuda")
+    last[7] = 1.0
+    # without decay and with C = 1 at the last step alone, y_7 = sum of delta x + D x: d y_7 / d delta_t = x_t
+    y, _ = selective_scan(xc, torch.zeros(8, B, N, device="cuda"), A, ones, last, D=D, dt_bias=bias, softplus=False)
+    want = x.double().sum((0, 1)).float()
+    assert torch.equal(torch.autograd.grad(y, D, torch.ones_like(y), retain_graph=True)[0].cpu(), want)
+    gy = torch.zeros_like(y)
+    gy[7] = 1.0
+    assert torch.equal(torch.autograd.grad(y, bias, gy)[0].cpu(), want)
